@@ -109,7 +109,8 @@ def source_hash():
 # turned the two row sums into packed operations with op_sel lane swaps, and waves of that kernel that shared their CU with the persistent
 # MFMA / LDS-transpose weight-gradient kernel returned a wrong sum c1 in ~2 % of the rows (tools/replay_bisect.py), the
 # scalar code never does.  tests/test_kernel_resources.py fails the CPU suite if a packed FP32 instruction reappears in any kernel.
-HIPCC_FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fno-slp-vectorize', '-fno-vectorize']
+# -packed-fp32-ops takes the instructions away from the back end as well, which can still form them from scalar code.
+HIPCC_FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fno-slp-vectorize', '-fno-vectorize', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 EXTRA_FLAGS = os.environ.get('TFPP_BUILD_FLAGS', '').split()  # experiments only (build(force=True)); the product build has none
 HASH_PATH = LIB_PATH + '.srchash'  # written by build() next to the library (reading the embedded hash would dlopen the old binary)
 
