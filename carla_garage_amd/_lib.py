@@ -14,10 +14,10 @@ ROOT = os.path.dirname(PKG_DIR)
 HEADER = os.path.join(ROOT, 'include', 'tfpp.h')
 CSRC = os.path.join(PKG_DIR, 'csrc')
 LIB_PATH = os.path.join(PKG_DIR, 'libtfpp_hip.so')
-SOURCES = ['gemm_kernels.hip', 'gemm_glds.hip', 'gemm_wgrad_glds.hip', 'attention_kernels.hip', 'conv3x3_halo.hip', 'wgrad3x3_halo.hip', 'pointwise_kernels.hip', 'norm_kernels.hip', 'bn_rows_kernels.hip', 'misc_kernels.hip', 'lidar_kernels.hip', 'swin_kernels.hip', 'bev_kernels.hip', 'head_kernels.hip', 'augment_kernels.hip']
+SOURCES = ['gemm_kernels.hip', 'gemm_glds.hip', 'gemm_wgrad_glds.hip', 'attention_kernels.hip', 'conv3x3_halo.hip', 'wgrad3x3_halo.hip', 'pointwise_kernels.hip', 'norm_kernels.hip', 'bn_rows_kernels.hip', 'misc_kernels.hip', 'lidar_kernels.hip', 'swin_kernels.hip', 'bev_kernels.hip', 'head_kernels.hip', 'augment_kernels.hip', 'grad_clip.hip']
 
 F32, BF16 = 0, 1
-ABI_VERSION = 8  # include/tfpp.h TFPP_ABI_VERSION
+ABI_VERSION = 9  # include/tfpp.h TFPP_ABI_VERSION
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_GELU, ACT_TANH = 0, 1, 2, 3, 4
 EINVAL = -1000
 
@@ -237,8 +237,8 @@ class _Lib:
     mine = [ctypes.sizeof(ConvParams), ctypes.sizeof(WgradParams), ctypes.sizeof(BgemmParams), ctypes.sizeof(PackDesc),
             ctypes.sizeof(AttnParams)]
     mine.append(ctypes.sizeof(BnRows))
-    if n != 6 or list(sizes[:6]) != mine:
-      raise TfppError(f'struct layout mismatch: library {list(sizes[:6])} vs ctypes {mine}')
+    if n != len(mine) or list(sizes[:n]) != mine:
+      raise TfppError(f'struct layout mismatch: library {list(sizes[:n])} vs ctypes {mine}')
     if self._dll.tfpp_version() != ABI_VERSION:
       raise TfppError(f'ABI version mismatch: library {self._dll.tfpp_version()}, binding {ABI_VERSION} (include/tfpp.h TFPP_ABI_VERSION: bumped with every signature change)')
     got = ctypes.c_uint64(0)

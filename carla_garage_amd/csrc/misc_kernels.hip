@@ -571,9 +571,10 @@ extern "C" int tfpp_sum_f32(const float* x, float* out, int64_t n, void* stream)
 // ---------------------------------------------------------------------------------------------------------------
 __global__ void adamw_amsgrad_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
                                      float* __restrict__ vmax, long n, float lr, float beta1, float beta2, float eps, float wd_all, float bc1,
-                                     float bc2_sqrt, float grad_scale, const unsigned* __restrict__ no_decay) {
+                                     float bc2_sqrt, float grad_scale, const unsigned* __restrict__ no_decay, const float* __restrict__ grad_coef) {
   // no_decay (nullable): one bit per group of 4 consecutive elements of the arena (every parameter starts on a multiple of 4): set = this
   // parameter is in the weight_decay = 0 group of create_optimizer_groups (model.py:556-632: biases, norms, embeddings, queries)
+  if (grad_coef) grad_scale *= *grad_coef;  // clipping coefficient of tfpp_grad_clip
   long i = ((long)blockIdx.x * blockDim.x + threadIdx.x) * 4;
   const long stride = (long)gridDim.x * blockDim.x * 4;
   for (; i < n; i += stride) {
@@ -609,11 +610,11 @@ __global__ void adamw_amsgrad_kernel(float* __restrict__ p, const float* __restr
 }
 
 static int launch_adamw(float* p, const float* g, float* m, float* v, float* vmax, int64_t n, float lr, float beta1, float beta2, float eps,
-                        float weight_decay, int step, float grad_scale, const unsigned* no_decay, void* stream);
+                        float weight_decay, int step, float grad_scale, const unsigned* no_decay, const float* grad_coef, void* stream);
 
 extern "C" int tfpp_adamw_amsgrad(float* p, const float* g, float* m, float* v, float* vmax, int64_t n, float lr, float beta1, float beta2,
                                   float eps, float weight_decay, int step, float grad_scale, void* stream) {
-  return launch_adamw(p, g, m, v, vmax, n, lr, beta1, beta2, eps, weight_decay, step, grad_scale, nullptr, stream);
+  return launch_adamw(p, g, m, v, vmax, n, lr, beta1, beta2, eps, weight_decay, step, grad_scale, nullptr, nullptr, stream);
 }
 
 // Two parameter groups (team_code/train.py:522-523, use_optim_groups): elements whose bit in no_decay_bits (one bit per 4 elements, p must be the
@@ -621,11 +622,18 @@ extern "C" int tfpp_adamw_amsgrad(float* p, const float* g, float* m, float* v, 
 extern "C" int tfpp_adamw_amsgrad_groups(float* p, const float* g, float* m, float* v, float* vmax, int64_t n, float lr, float beta1, float beta2,
                                          float eps, float weight_decay, int step, float grad_scale, const uint32_t* no_decay_bits, void* stream) {
   if (!no_decay_bits) return TFPP_EINVAL;
-  return launch_adamw(p, g, m, v, vmax, n, lr, beta1, beta2, eps, weight_decay, step, grad_scale, no_decay_bits, stream);
+  return launch_adamw(p, g, m, v, vmax, n, lr, beta1, beta2, eps, weight_decay, step, grad_scale, no_decay_bits, nullptr, stream);
+}
+
+extern "C" int tfpp_adamw_amsgrad_clipped(float* p, const float* g, float* m, float* v, float* vmax, int64_t n, float lr, float beta1, float beta2,
+                                          float eps, float weight_decay, int step, float grad_scale, const uint32_t* no_decay_bits,
+                                          const float* grad_coef, void* stream) {
+  if (!grad_coef) return TFPP_EINVAL;
+  return launch_adamw(p, g, m, v, vmax, n, lr, beta1, beta2, eps, weight_decay, step, grad_scale, no_decay_bits, grad_coef, stream);
 }
 
 static int launch_adamw(float* p, const float* g, float* m, float* v, float* vmax, int64_t n, float lr, float beta1, float beta2, float eps,
-                        float weight_decay, int step, float grad_scale, const unsigned* no_decay, void* stream) {
+                        float weight_decay, int step, float grad_scale, const unsigned* no_decay, const float* grad_coef, void* stream) {
   if (!p || !g || !m || !v || !vmax || step < 1) return TFPP_EINVAL;
   if (((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v | (uintptr_t)vmax) & 15) return TFPP_EINVAL;
   const float bc1 = 1.f - powf(beta1, (float)step);
@@ -634,7 +642,7 @@ static int launch_adamw(float* p, const float* g, float* m, float* v, float* vma
   if (blocks > 16384) blocks = 16384;
   if (blocks < 1) blocks = 1;
   hipLaunchKernelGGL(adamw_amsgrad_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p, g, m, v, vmax, (long)n, lr, beta1, beta2,
-                     eps, weight_decay, bc1, bc2_sqrt, grad_scale, no_decay);
+                     eps, weight_decay, bc1, bc2_sqrt, grad_scale, no_decay, grad_coef);
   TFPP_CHECK_LAUNCH();
   return 0;
 }

@@ -1199,9 +1199,13 @@ def bce_logits_loss(logit, y, loss_out, weight=1.0, dlogit=None):
   lib.tfpp_bce_logits_loss(ptr(_chk(logit)), logit.shape[1], ptr(y), weight, ptr(loss_out), ptr(dlogit), logit.shape[0], stream())
 
 
-def adamw_amsgrad(p, g, m, v, vmax, lr, beta1, beta2, eps, weight_decay, step, grad_scale=1.0, no_decay_bits=None):
+def adamw_amsgrad(p, g, m, v, vmax, lr, beta1, beta2, eps, weight_decay, step, grad_scale=1.0, no_decay_bits=None, grad_coef=None):
   """no_decay_bits (int32 device tensor from no_decay_bitmask; p must start at the arena's first element): the weight_decay = 0 group of
-  create_optimizer_groups."""
+  create_optimizer_groups.  grad_coef (fp32 device scalar, GradClip.coef): also multiplies the gradient."""
+  if grad_coef is not None:
+    lib.tfpp_adamw_amsgrad_clipped(ptr(p), ptr(g), ptr(m), ptr(v), ptr(vmax), p.numel(), lr, beta1, beta2, eps, weight_decay, step, grad_scale,
+                                   ptr(no_decay_bits), ptr(grad_coef), stream())
+    return
   if no_decay_bits is not None:
     lib.tfpp_adamw_amsgrad_groups(ptr(p), ptr(g), ptr(m), ptr(v), ptr(vmax), p.numel(), lr, beta1, beta2, eps, weight_decay, step, grad_scale,
                                   ptr(no_decay_bits), stream())
@@ -1223,3 +1227,117 @@ def no_decay_bitmask(slices, no_decay_ids, total):
       bits[off // 4:(off + n + 3) // 4] = True
   words = np.packbits(bits.reshape(-1, 32), axis=1, bitorder='little').view('<u4').reshape(-1)
   return words.astype(np.uint32).view(np.int32)
+
+
+# ------------------------------------------------------------------------------------------------ gradient norm and clipping
+def one_device(*tensors):
+  """Device of the given tensors (None: left out); they have to share it.  Launches go to ITS current stream, whatever device is current."""
+  dev = None
+  for t in tensors:
+    if t is None:
+      continue
+    if not t.is_cuda:
+      raise ValueError('HIP ops need device tensors')
+    if dev is None:
+      dev = t.device
+    elif t.device != dev:
+      raise ValueError(f'tensors on different devices: {dev} and {t.device}')
+  return dev
+
+
+def is_dense(t):
+  """Do the elements of ``t`` fill one gap-free span of memory (in any order of its dimensions)?"""
+  want = 1
+  for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+    if st != want:
+      return t.numel() <= 1
+    want *= n
+  return True
+
+
+def _same_order(a, b):
+  return a.shape == b.shape and all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
+
+
+_GRAD_TYPES = (torch.float32, torch.bfloat16)
+
+
+class GradClip:
+  """Norm of the gradients ``tensors`` taken together, and their clipping (train.py:900-906: unscale, ``clip_grad_norm_``), in two launches for
+  any number of tensors.  fp32 or bf16, dense in memory; ``out`` (same shapes and dimension order, fp32 or bf16) receives the clipped
+  gradients, ``out=None`` clips in place.  The object holds the tensors and a table of their addresses in device memory: it is made once for
+  gradients that stay where they are (a gradient arena; a captured step) and again when they move -- never inside a capture, the table is a
+  host-to-device copy.  Results are bit-reproducible."""
+
+  def __init__(self, tensors, out=None):
+    import numpy as np
+    self.tensors = list(tensors)
+    self.out = self.tensors if out is None else list(out)
+    if len(self.out) != len(self.tensors):
+      raise ValueError(f'{len(self.tensors)} gradients, {len(self.out)} outputs')
+    if not self.tensors:
+      raise ValueError('GradClip needs at least one tensor')
+    self.device = one_device(*self.tensors, *self.out)
+    for g, o in zip(self.tensors, self.out):
+      if g.dtype not in _GRAD_TYPES or o.dtype not in _GRAD_TYPES:
+        raise TypeError(f'gradients are fp32 or bf16, got {g.dtype} -> {o.dtype}')
+      if not (g.is_contiguous() or is_dense(g)) or (o is not g and not _same_order(g, o)):
+        raise ValueError('gradients are dense in memory, and their outputs lie in the same order')
+    if torch.cuda.is_current_stream_capturing():
+      raise RuntimeError('GradClip is made before hipGraph capture: its table is copied from the host')
+    i64a = lambda it: np.fromiter(it, np.int64, len(self.tensors))
+    n, src, dst = i64a(t.numel() for t in self.tensors), i64a(t.data_ptr() for t in self.tensors), i64a(t.data_ptr() for t in self.out)
+    ss, ds = i64a(t.element_size() for t in self.tensors), i64a(t.element_size() for t in self.out)
+    some = n > 0
+    n, src, dst, ss, ds = n[some], src[some], dst[some], ss[some], ds[some]
+    # what is written may overlap nothing else; what is only read may repeat
+    apart = (src != dst) | (ss != ds)
+    lo = np.concatenate([dst, src[apart]])
+    hi = np.concatenate([dst + n * ds, (src + n * ss)[apart]])
+    written = np.arange(lo.size) < dst.size
+    order = np.argsort(lo, kind='stable')
+    lo, hi, written = lo[order], hi[order], written[order]
+    end, end_out = np.maximum.accumulate(np.concatenate([[0], hi]))[:-1], np.maximum.accumulate(np.concatenate([[0], np.where(written, hi, 0)]))[:-1]
+    if (lo < np.where(written, end, end_out)).any():
+      raise ValueError('the same memory is given twice: a clipped gradient may not overlap another one')
+    chunk = lib.raw('tfpp_grad_clip_chunk')()
+    per = (n + chunk - 1) // chunk
+    which = np.repeat(np.arange(n.size), per)
+    off = (np.arange(which.size) - np.repeat(np.cumsum(per) - per, per)) * chunk
+    table = np.empty(which.size, dtype=[('src', '<i8'), ('dst', '<i8'), ('n', '<i4'), ('flags', '<i4')])
+    table['src'], table['dst'], table['n'] = src[which] + off * ss[which], dst[which] + off * ds[which], np.minimum(n[which] - off, chunk)
+    table['flags'] = ((ss == 2) * 1 + (ds == 2) * 2 + ((src | dst) % 16 == 0) * 4)[which]
+    self.chunks = int(which.size)
+    if self.chunks >= 1 << 31:
+      raise ValueError('too many elements')
+    self.table = torch.from_numpy(table.view(np.uint8)).to(self.device)  # (pageable memory: the copy has completed when this returns)
+    self._partials = lib.raw('tfpp_grad_clip_partials')(self.chunks)
+
+  def _run(self, max_norm, norm_type, grad_scale, apply):
+    kind = {2: 2, 1: 1, float('inf'): 0}.get(float(norm_type))
+    if kind is None:
+      raise ValueError(f'norm_type is 1, 2 or inf, got {norm_type}')
+    if not float(max_norm) >= 0.0:
+      raise ValueError(f'max_norm is not negative, got {max_norm}')
+    with torch.cuda.device(self.device):
+      # scratch of this call alone (captured graphs keep theirs in the graph's own pool): nothing is shared between streams or graphs
+      buf = torch.empty(self._partials + 1, device=self.device, dtype=torch.float64)
+      res = buf[self._partials:].view(torch.float32)
+      if lib.profiler is not None:
+        lib.profiler.tag('grad_clip', 0.0, float(sum(t.numel() * t.element_size() * (2 + apply) for t in self.tensors)))
+      lib.tfpp_grad_clip(ptr(self.table) if self.chunks else None, self.chunks, ptr(buf), min(float(max_norm), 3.4e38), kind, float(grad_scale), ptr(res), int(apply), stream())
+    return res
+
+  def norm(self, norm_type=2.0, grad_scale=1.0):
+    """|| grad_scale * g || over all tensors: fp32 device scalar."""
+    return self._run(float('inf'), norm_type, grad_scale, False)[0]
+
+  def coef(self, max_norm, norm_type=2.0, grad_scale=1.0):
+    """(norm, min(1, max_norm / (norm + 1e-6))) as fp32 device scalars; the gradients are only read (adamw_amsgrad takes the coefficient)."""
+    res = self._run(max_norm, norm_type, grad_scale, False)
+    return res[0], res[1]
+
+  def clip_(self, max_norm, norm_type=2.0, grad_scale=1.0):
+    """out = g * grad_scale * min(1, max_norm / (norm + 1e-6)); returns the norm of grad_scale * g (fp32 device scalar).  As torch's
+    ``clip_grad_norm_``: a NaN norm makes every output NaN, an infinite one makes finite gradients zero."""
+    return self._run(max_norm, norm_type, grad_scale, True)[0]

@@ -16,6 +16,22 @@ from . import ops
 from .engine import F32
 
 
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+  """``torch.nn.utils.clip_grad_norm_`` (team_code/train.py:904-906) over the fused kernels: two launches for any number of gradients (ops.GradClip).
+  norm_type 1, 2 or inf.  Returns the norm before clipping (fp32 device scalar); the gradients are scaled in place.  As torch's, it reads the
+  norm on the host before it scales when ``error_if_nonfinite`` is set, and the gradients are then left as they were."""
+  grads = [p.grad for p in ([parameters] if isinstance(parameters, torch.Tensor) else parameters) if p.grad is not None]
+  if not grads:
+    return torch.tensor(0.0)
+  plan = ops.GradClip(grads)
+  if error_if_nonfinite:
+    norm = plan.norm(norm_type)
+    if not bool(torch.isfinite(norm)):
+      raise RuntimeError(f'The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped')
+  return plan.clip_(max_norm, norm_type)
+
+
 class FlatAdamW(torch.optim.Optimizer):
 
   def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=True, **unused):

@@ -20,9 +20,12 @@ from .losses import fused_losses, normalized_loss_weights, active_losses
 
 class Trainer:
 
-  def __init__(self, model, lr=3e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, process_group=None, use_graph=False, lazy_state=False):
+  def __init__(self, model, lr=3e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, process_group=None, use_graph=False, lazy_state=False,
+               max_grad_norm=None):
     """lazy_state: allocate the three optimizer-state arenas on the first optimizer launch (the drop-in path of dropin.py owns a Trainer
-    for its flat arenas and gradient exchange; the 1.4 GB of AdamW state is only needed when the fused optimizer is the one stepping)."""
+    for its flat arenas and gradient exchange; the 1.4 GB of AdamW state is only needed when the fused optimizer is the one stepping).
+    max_grad_norm: clip the (averaged) gradients to this Euclidean norm in front of the update, as train.py:900-906 does with use_grad_clip; the
+    coefficient goes into the optimizer kernel, so clipping costs one read of the arena.  self.grad_norm is the norm of the last step."""
     self.model = model
     prev = model.__dict__.get('_trainer')
     if prev is not None and prev is not self:
@@ -31,6 +34,7 @@ class Trainer:
     self.detached = False
     self._lazy_state = lazy_state
     self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay  # lr is read at every step: schedulers just set it
+    self.max_grad_norm, self.grad_norm, self._clip = max_grad_norm, None, None
     self.pg = process_group
     self.world = dist.get_world_size(process_group) if (dist.is_available() and dist.is_initialized()) else 1
     self.step_count = 0
@@ -209,7 +213,7 @@ class Trainer:
         i += 1
     return out
 
-  def _optimizer(self, step, grad_scale=None, upto=None, lo=0):
+  def _optimizer(self, step, grad_scale=None, upto=None, lo=0, grad_coef=None):
     """grad_scale: None = 1 / world (the arena holds the SUM over the ranks); the drop-in path passes 1.0 (already averaged).
     upto / lo: only the elements lo .. upto-1 of the arena (finish_step updates bucket after bucket as the all-reduces land)."""
     self._alloc_state()
@@ -221,7 +225,7 @@ class Trainer:
       bits = bits[lo // 128:]
     ops.adamw_amsgrad(self.flat_param[sl], self.eng.flat_grad[sl], self.exp_avg[sl], self.exp_avg_sq[sl], self.max_exp_avg_sq[sl], self.lr, self.betas[0],
                       self.betas[1], self.eps, self.weight_decay, step, grad_scale=1.0 / self.world if grad_scale is None else grad_scale,
-                      no_decay_bits=bits)
+                      no_decay_bits=bits, grad_coef=grad_coef)
 
   def train_step(self, batch):
     """batch: dict with rgb, lidar_bev, target_point, ego_vel, command and the *_label tensors (reference layouts).
@@ -260,6 +264,12 @@ class Trainer:
       buckets.raise_if_timed_out()  # a signal wait of an EARLIER step gave up (on any rank): stop before this step's gradients are averaged in
       self.agree_on_layout()
     works = buckets.exchange(self.eng.flat_grad, program, self.pg) if self.exchange else []
+    if getattr(self, 'max_grad_norm', None) is not None:  # the norm needs every bucket: no update before the last one has landed
+      for work in works:
+        if work is not None:
+          work.wait()
+      self._optimizer(self.step_count, grad_coef=self._clip_coef())
+      return
     if not works:
       self._optimizer(self.step_count)
       return
@@ -268,6 +278,13 @@ class Trainer:
         continue
       work.wait()
       self._optimizer(self.step_count, lo=lo, upto=hi)
+
+  def _clip_coef(self):
+    """Device scalar min(1, max_grad_norm / (norm + 1e-6)) of the averaged gradients in the arena (the padding between parameters is zero)."""
+    if self._clip is None or self._clip.tensors[0] is not self.eng.flat_grad:  # (first step, or the arena moved)
+      self._clip = ops.GradClip([self.eng.flat_grad])
+    self.grad_norm, coef = self._clip.coef(self.max_grad_norm, grad_scale=1.0 / self.world)
+    return coef
 
   # ---------------------------------------------------------------------------------------------- checkpoint / resume
   def _arena_slices(self):

@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define TFPP_ABI_VERSION 8
+#define TFPP_ABI_VERSION 9
 #define TFPP_EINVAL (-1000)
 #define TFPP_F32 0
 #define TFPP_BF16 1
@@ -655,6 +655,26 @@ int tfpp_adamw_amsgrad(float* p, const float* g, float* m, float* v, float* vmax
  * one bit per 4 consecutive elements of the arena starting at p (every parameter starts on a multiple of 4); set = weight_decay 0. */
 int tfpp_adamw_amsgrad_groups(float* p, const float* g, float* m, float* v, float* vmax, int64_t n, float lr, float beta1, float beta2,
                               float eps, float weight_decay, int step, float grad_scale, const uint32_t* no_decay_bits, void* stream);
+/* The same (no_decay_bits may be null), with the gradient also multiplied by *grad_coef, the clipping coefficient tfpp_grad_clip left in device
+ * memory: clipping without a pass of its own over the gradients. */
+int tfpp_adamw_amsgrad_clipped(float* p, const float* g, float* m, float* v, float* vmax, int64_t n, float lr, float beta1, float beta2,
+                               float eps, float weight_decay, int step, float grad_scale, const uint32_t* no_decay_bits, const float* grad_coef,
+                               void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Norm of the gradients of any number of tensors and their clipping (train.py:900-906).  norm_coef[0] = ||grad_scale g||_p (norm_type 2, 1, or 0 for
+ * the largest magnitude), norm_coef[1] = min(1, max_norm / (norm + 1e-6)); with apply != 0 also dst = grad_scale * norm_coef[1] * src.
+ * table: `chunks` entries in device memory, each at most tfpp_grad_clip_chunk() elements; flags: 1 src is bf16, 2 dst is bf16 (else fp32), 4 src and
+ * dst are 16-byte aligned.  src == dst clips in place.  ws: tfpp_grad_clip_partials(chunks) doubles, any content.  Fixed summation order. */
+typedef struct tfpp_grad_chunk {
+  const void* src;
+  void* dst;
+  int32_t n, flags;
+} tfpp_grad_chunk;
+int tfpp_grad_clip(const tfpp_grad_chunk* table, int chunks, double* ws, float max_norm, int norm_type, float grad_scale, float* norm_coef, int apply,
+                   void* stream);
+int tfpp_grad_clip_chunk(void);              /* returns the count (not an error code) */
+int tfpp_grad_clip_partials(int chunks);     /* returns the count (not an error code) */
 
 #ifdef __cplusplus
 }
