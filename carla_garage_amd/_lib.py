@@ -14,7 +14,7 @@ ROOT = os.path.dirname(PKG_DIR)
 HEADER = os.path.join(ROOT, 'include', 'tfpp.h')
 CSRC = os.path.join(PKG_DIR, 'csrc')
 LIB_PATH = os.path.join(PKG_DIR, 'libtfpp_hip.so')
-SOURCES = ['gemm_kernels.hip', 'gemm_glds.hip', 'gemm_wgrad_glds.hip', 'attention_kernels.hip', 'conv3x3_halo.hip', 'wgrad3x3_halo.hip', 'pointwise_kernels.hip', 'norm_kernels.hip', 'bn_rows_kernels.hip', 'misc_kernels.hip', 'lidar_kernels.hip', 'swin_kernels.hip', 'bev_kernels.hip', 'head_kernels.hip', 'augment_kernels.hip', 'grad_clip.hip']
+SOURCES = ['gemm_kernels.hip', 'gemm_glds.hip', 'gemm_wgrad_glds.hip', 'attention_kernels.hip', 'conv3x3_halo.hip', 'wgrad3x3_halo.hip', 'pointwise_kernels.hip', 'norm_kernels.hip', 'bn_rows_kernels.hip', 'misc_kernels.hip', 'lidar_kernels.hip', 'swin_kernels.hip', 'bev_kernels.hip', 'head_kernels.hip', 'augment_kernels.hip', 'grad_clip.hip', 'block_norm.hip']
 
 F32, BF16 = 0, 1
 ABI_VERSION = 9  # include/tfpp.h TFPP_ABI_VERSION
@@ -63,6 +63,13 @@ class AttnParams(ctypes.Structure):
 class PackDesc(ctypes.Structure):
   _fields_ = [('src', vp), ('dst', vp), ('row_map', vp), ('col_map', vp), ('total', i64), ('in_ld', i64), ('out_ld', i64),
               ('blk_start', i64), ('kind', i32), ('dtype', i32), ('a', i32 * 8)]
+
+
+class BlockNormParams(ctypes.Structure):
+  _fields_ = [(n, vp) for n in ('x', 'a', 'gate', 'post_w', 'post_b', 'pre_w', 'pre_b', 'scale', 'y', 'h', 'stat', 'dy', 'dh', 'dx', 'da', 'dgate', 'dpost_w',
+                                'dpost_b', 'dpre_w', 'dpre_b', 'dscale', 'partial')] + \
+      [(n, i64) for n in ('ld_x', 'ld_a', 'ld_g', 'ld_dy', 'ld_dh')] + \
+      [(n, i32) for n in ('B', 'T', 'C', 'layer', 'post', 'pre', 'gate_mode', 'gate_act', 'accumulate')] + [('alpha', f32), ('eps', f32)]
 
 
 _CTYPE = {'int': i32, 'int32_t': i32, 'int64_t': i64, 'uint64_t': ctypes.c_uint64, 'uint32_t': ctypes.c_uint32, 'float': f32, 'double': ctypes.c_double}
@@ -237,6 +244,7 @@ class _Lib:
     mine = [ctypes.sizeof(ConvParams), ctypes.sizeof(WgradParams), ctypes.sizeof(BgemmParams), ctypes.sizeof(PackDesc),
             ctypes.sizeof(AttnParams)]
     mine.append(ctypes.sizeof(BnRows))
+    mine.append(ctypes.sizeof(BlockNormParams))
     if n != len(mine) or list(sizes[:n]) != mine:
       raise TfppError(f'struct layout mismatch: library {list(sizes[:n])} vs ctypes {mine}')
     if self._dll.tfpp_version() != ABI_VERSION:

@@ -665,14 +665,15 @@ extern "C" int tfpp_source_hash(uint64_t* out) {
 }
 
 extern "C" int tfpp_struct_sizes(int* out, int n) {
-  if (!out || n < 6) return TFPP_EINVAL;
+  if (!out || n < 7) return TFPP_EINVAL;
   out[0] = (int)sizeof(tfpp_conv_params);
   out[1] = (int)sizeof(tfpp_wgrad_params);
   out[2] = (int)sizeof(tfpp_bgemm_params);
   out[3] = (int)sizeof(tfpp_pack_desc);
   out[4] = (int)sizeof(tfpp_attn_params);
   out[5] = (int)sizeof(tfpp_bn_rows);
-  return 6;
+  out[6] = (int)sizeof(tfpp_block_norm_params);
+  return 7;
 }
 
 // order-independent 64-bit hash of a buffer (debugging aid: which tensor differs between two replays of one hipGraph?)

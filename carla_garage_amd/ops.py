@@ -5,7 +5,7 @@ import ctypes
 
 import torch
 
-from ._lib import (lib, ConvParams, WgradParams, BgemmParams, PackDesc, AttnParams, BnRows, F32, BF16, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_GELU,
+from ._lib import (lib, ConvParams, WgradParams, BgemmParams, PackDesc, AttnParams, BnRows, BlockNormParams, F32, BF16, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_GELU,
                    ACT_TANH)
 
 import os as _os
@@ -1341,3 +1341,162 @@ class GradClip:
     """out = g * grad_scale * min(1, max_norm / (norm + 1e-6)); returns the norm of grad_scale * g (fp32 device scalar).  As torch's
     ``clip_grad_norm_``: a NaN norm makes every output NaN, an infinite one makes finite gradients zero."""
     return self._run(max_norm, norm_type, grad_scale, True)[0]
+
+
+# ------------------------------------------------------------------------------------------------ norms, gate and residual between two blocks
+def _row_view(t, shape, name):
+  """(tensor, row stride) of [..., C] rows that lie at one stride from each other (a packed tensor, a column slice of a wider one)."""
+  if tuple(t.shape) != tuple(shape):
+    raise ValueError(f'{name} has shape {tuple(t.shape)}, expected {tuple(shape)}')
+  c = shape[-1]
+  if t.stride(-1) != 1 and c != 1:
+    raise ValueError(f'{name}: channels have to be contiguous')
+  ld, n = None, 1
+  for d in range(t.dim() - 2, -1, -1):
+    if t.shape[d] == 1:
+      continue
+    if ld is None:
+      ld = t.stride(d)
+    elif t.stride(d) != ld * n:
+      raise ValueError(f'{name}: rows do not lie at one stride (shape {tuple(t.shape)}, strides {t.stride()})')
+    n *= t.shape[d]
+  ld = c if ld is None else ld
+  if ld < c and n > 1:
+    raise ValueError(f'{name}: rows overlap (strides {t.stride()})')
+  return ld
+
+
+def _channel_param(t, c, dev, name):
+  if t is None:
+    return
+  if t.dtype != torch.float32 or t.numel() != c or not t.is_contiguous() or t.device != dev:
+    raise ValueError(f'{name}: {c} contiguous fp32 values on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}')
+
+
+class BlockNormContext:
+  """What block_norm_bwd needs of its forward pass: the inputs (read again, not copied) and four statistics a row."""
+  __slots__ = ('x', 'a', 'gate', 'stat', 'opt', 'params', 'mode', 'lds', 'shape')
+
+
+_BLOCK_NORM_SUMS = {'pre_weight': ('dpre_w', 1), 'pre_bias': ('dpre_b', 2), 'post_weight': ('dpost_w', 4), 'post_bias': ('dpost_b', 8), 'scale': ('dscale', 16)}
+
+
+def _block_norm_params(ctx):
+  p = BlockNormParams()
+  B, T, C = ctx.shape
+  p.x, p.a, p.gate = ctx.x.data_ptr(), ctx.a.data_ptr(), ptr(ctx.gate)
+  p.post_w, p.post_b, p.pre_w, p.pre_b, p.scale = (ptr(ctx.params[n]) for n in ('post_weight', 'post_bias', 'pre_weight', 'pre_bias', 'scale'))
+  p.ld_x, p.ld_a, p.ld_g = ctx.lds
+  p.B, p.T, p.C, p.gate_mode = B, T, C, ctx.mode
+  p.layer, p.post, p.pre, p.gate_act, p.alpha, p.eps = ctx.opt
+  p.stat = ptr(ctx.stat)
+  return p
+
+
+def block_norm_fwd(x, a, *, kind='layer', post=True, pre=True, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, gate=None, gate_act=ACT_NONE,
+                   scale=None, alpha=1.0, eps=1e-5, save=True):
+  """From the residual stream ``x`` and a block's result ``a`` (both [..., C], fp32 or bf16; C <= 4096) to the next block's input, in one launch:
+    n = post(a)    y = alpha x + scale * gate_act(gate) * n    h = pre(y)        -> (y, h, context)
+  kind 'layer' | 'rms'; ``post`` / ``pre`` False: without that norm (h is None without ``pre``).  Weights, biases and ``scale``: [C] fp32 or None.
+  ``gate``: None, the shape of x (per token), or [B, C] for x [B, ..., C] (per sample), in x's type; gate_act ACT_NONE / ACT_SIGMOID / ACT_TANH.
+  h is the norm of y before y is rounded to its type.  The context (save=True) refers to x, a and gate: block_norm_bwd reads them again, so they
+  may not change in between."""
+  if kind not in ('layer', 'rms'):
+    raise ValueError(f"kind is 'layer' or 'rms', got {kind!r}")
+  if gate_act not in (ACT_NONE, ACT_SIGMOID, ACT_TANH):
+    raise ValueError('gate_act is ACT_NONE, ACT_SIGMOID or ACT_TANH')
+  dev = one_device(x, a, gate)
+  if x.dtype not in (torch.float32, torch.bfloat16) or a.dtype != x.dtype or (gate is not None and gate.dtype != x.dtype):
+    raise TypeError(f'x, a and gate share one type, fp32 or bf16: got {x.dtype}, {a.dtype}, {gate.dtype if gate is not None else None}')
+  if x.dim() < 1 or not 1 <= x.shape[-1] <= 4096:
+    raise ValueError(f'block_norm_fwd: 1 to 4096 channels, got shape {tuple(x.shape)}')
+  C = x.shape[-1]
+  rows = x.numel() // C
+  ctx = BlockNormContext()
+  ctx.params = dict(post_weight=post_weight, post_bias=post_bias, pre_weight=pre_weight, pre_bias=pre_bias, scale=scale)
+  for n, t in ctx.params.items():
+    _channel_param(t, C, dev, n)
+  if (not post and (post_weight is not None or post_bias is not None)) or (not pre and (pre_weight is not None or pre_bias is not None)):
+    raise ValueError('parameters of a norm that is switched off')
+  ld_x, ld_a, ld_g = _row_view(x, x.shape, 'x'), _row_view(a, x.shape, 'a'), 0
+  ctx.mode, B, T = 0, 1, rows
+  if gate is not None:
+    if gate.shape == x.shape:
+      ctx.mode, ld_g = 2, _row_view(gate, x.shape, 'gate')
+    elif x.dim() >= 2 and tuple(gate.shape) == (x.shape[0], C):
+      ld_g = _row_view(gate, gate.shape, 'gate')
+      B = x.shape[0]
+      T = rows // B if B else 0
+      ctx.mode = 1
+      if T == 1:  # one token a sample: per sample IS per token, without a workgroup for each sample
+        ctx.mode, B, T = 2, 1, rows
+    else:
+      raise ValueError(f'gate has shape {tuple(gate.shape)}, expected {tuple(x.shape)} or {(x.shape[0], C)}')
+  if rows > 0x7fffffff or (ctx.mode == 1 and B > 65530):
+    raise ValueError(f'block_norm_fwd: too many rows ({rows}) or samples ({B})')
+  ctx.x, ctx.a, ctx.gate, ctx.lds, ctx.shape = x, a, gate, (ld_x, ld_a, ld_g), (B, T, C)
+  ctx.opt = (int(kind == 'layer'), int(post), int(pre), gate_act, float(alpha), float(eps))
+  with torch.cuda.device(dev):
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    h = torch.empty(x.shape, device=dev, dtype=x.dtype) if pre else None
+    ctx.stat = torch.empty((max(rows, 1), 4), device=dev, dtype=torch.float32) if save else None
+    if rows:
+      p = _block_norm_params(ctx)
+      p.y, p.h = y.data_ptr(), ptr(h)
+      if lib.profiler is not None:
+        lib.profiler.tag('block_norm_fwd', 0.0, float(rows * C * x.element_size() * (3 + pre + (ctx.mode == 2))))
+      lib.tfpp_block_norm_fwd(ctypes.byref(p), dt(x), stream())
+  return y, h, (ctx if save else None)
+
+
+def block_norm_bwd(dy, dh, ctx, into=None):
+  """Gradients of block_norm_fwd: dict with x, a, gate, scale, post_weight, post_bias, pre_weight, pre_bias (None for what the forward call did not
+  have).  dy / dh: gradients of y / h, either may be None.  ``into``: {name: fp32 [C] tensor} the parameter gradients are ADDED to (the gradient
+  arena); the others are returned in new tensors.  Column sums are added in a fixed order."""
+  B, T, C = ctx.shape
+  x, dev = ctx.x, ctx.x.device
+  into = dict(into or {})
+  if dy is None and dh is None:
+    raise ValueError('block_norm_bwd: neither dy nor dh')
+  if dh is not None and not ctx.opt[2]:
+    raise ValueError('block_norm_bwd: dh given, but the forward pass had no pre-norm')
+  names = [n for n, t in ctx.params.items() if t is not None]
+  for n, t in into.items():
+    if n not in names:
+      raise ValueError(f'block_norm_bwd: the forward pass had no {n}')
+    _channel_param(t, C, dev, n)
+  one_device(x, dy, dh)
+  lds = []
+  for n, t in (('dy', dy), ('dh', dh)):
+    if t is not None and t.dtype != x.dtype:
+      raise TypeError(f'{n} is {t.dtype}, expected {x.dtype}')
+    lds.append(_row_view(t, x.shape, n) if t is not None else 0)
+  rows = B * T
+  with torch.cuda.device(dev):
+    out = {n: None for n in ('x', 'a', 'gate', 'scale', 'post_weight', 'post_bias', 'pre_weight', 'pre_bias')}
+    out['x'], out['a'] = torch.empty(x.shape, device=dev, dtype=x.dtype), torch.empty(x.shape, device=dev, dtype=x.dtype)
+    if ctx.gate is not None:
+      out['gate'] = torch.empty(ctx.gate.shape, device=dev, dtype=x.dtype)
+    fresh = torch.empty((len(names), C), device=dev, dtype=torch.float32)
+    for n, t in zip(names, fresh):
+      out[n] = into.get(n, t)
+    if rows == 0:  # no rows: every sum is empty
+      if fresh.numel():
+        zero_(fresh)
+      if out['gate'] is not None and out['gate'].numel():
+        zero_(out['gate'])
+    else:
+      p = _block_norm_params(ctx)
+      n_part = ctypes.c_int64()
+      lib.tfpp_block_norm_bwd_partial_floats(ctypes.byref(p), ctypes.addressof(n_part))
+      partial = torch.empty(n_part.value, device=dev, dtype=torch.float32)
+      p.dy, p.dh, p.ld_dy, p.ld_dh = ptr(dy), ptr(dh), lds[0], lds[1]
+      p.dx, p.da, p.dgate, p.partial = out['x'].data_ptr(), out['a'].data_ptr(), ptr(out['gate']), partial.data_ptr()
+      for n in names:
+        field, bit = _BLOCK_NORM_SUMS[n]
+        setattr(p, field, out[n].data_ptr())
+        p.accumulate |= bit if n in into else 0
+      if lib.profiler is not None:
+        lib.profiler.tag('block_norm_bwd', 0.0, float(rows * C * x.element_size() * (4 + (dy is not None) + (dh is not None) + 2 * (ctx.mode == 2))))
+      lib.tfpp_block_norm_bwd(ctypes.byref(p), dt(x), stream())
+  return out

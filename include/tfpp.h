@@ -676,6 +676,29 @@ int tfpp_grad_clip(const tfpp_grad_chunk* table, int chunks, double* ws, float m
 int tfpp_grad_clip_chunk(void);              /* returns the count (not an error code) */
 int tfpp_grad_clip_partials(int chunks);     /* returns the count (not an error code) */
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Between two blocks of a residual network: n = post(a), y = alpha x + scale * act(gate) * n, h = pre(y).  Rows [B, T, C] of `dtype`, row strides in
+ * elements (ld_*; y, h, dx, da and a per-token dgate are packed), fp32 parameters (null weight: 1, null bias: 0, null scale: 1).
+ * layer: LayerNorm, else RMS.  gate_mode 0 none, 1 one row per sample [B, C], 2 one per token; gate_act TFPP_ACT_NONE / SIGMOID / TANH.
+ * stat: 4 floats a row (mean, rstd of post; mean, rstd of pre; 16-byte aligned), written by forward when given, read by backward.  Backward takes the
+ * forward's x, a, gate and recomputes the rest; dy or dh may be null (not both; dh needs pre).  Parameter gradients (each nullable) are stored, or
+ * added to their destination where a bit of accumulate is set: 1 dpre_w, 2 dpre_b, 4 dpost_w, 8 dpost_b, 16 dscale.  C <= 4096.  partial: tfpp_block_norm_bwd_partial_floats. */
+typedef struct {
+  const void *x, *a, *gate;
+  const float *post_w, *post_b, *pre_w, *pre_b, *scale;
+  void *y, *h;
+  float* stat;
+  const void *dy, *dh;
+  void *dx, *da, *dgate;
+  float *dpost_w, *dpost_b, *dpre_w, *dpre_b, *dscale, *partial;
+  int64_t ld_x, ld_a, ld_g, ld_dy, ld_dh;
+  int B, T, C, layer, post, pre, gate_mode, gate_act, accumulate;
+  float alpha, eps;
+} tfpp_block_norm_params;
+int tfpp_block_norm_fwd(const tfpp_block_norm_params* p, int dtype, void* stream);
+int tfpp_block_norm_bwd(const tfpp_block_norm_params* p, int dtype, void* stream);
+int tfpp_block_norm_bwd_partial_floats(const tfpp_block_norm_params* p, int64_t* out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,5 @@
 """GPU tests of the transformer-block operators (-m gpu) against plain implementations in 64 bits: gradient norm and clipping (ops.GradClip,
-optim.clip_grad_norm_, Trainer's max_grad_norm).
+optim.clip_grad_norm_, Trainer's max_grad_norm), block norms (ops.block_norm_fwd / _bwd), differential attention (ops.diff_attn_fwd / _bwd).
 
 Tolerances are componentwise: half a step of the output's type relative to the value, plus K fp32 roundings (2^-24 each) of the same
 formula evaluated with absolute values -- a running error bound; K counts the roundings on the longest path of one output."""
@@ -203,3 +203,217 @@ def test_adamw_takes_the_clipping_coefficient(ops):
     res.append((p, m, v))
   for a, b, k in zip(res[0], res[1], (8, 8, 16)):  # (the coefficient is rounded into the product in another place: a few roundings of each value)
     within('adamw', a, b.double(), k * U[F32] * b.abs() + (1e-2 * 16 * U[F32] if a is res[0][0] else 0.0))
+
+
+# ------------------------------------------------------------------------------------------------ block norms
+def norm_oracle(x, a, kind, o, gate, act, alpha, eps, dy=None, dh=None, mags=False):
+  """fp64; with ``mags`` the same formulas over absolute values (running error magnitudes).  gate broadcast to x's shape by the caller."""
+  A = torch.abs if mags else (lambda z: z)
+  sub = (lambda p, q: p + q) if mags else (lambda p, q: p - q)
+  mean_abs = lambda z: A(z).amax(-1, keepdim=True) if mags else z.mean(-1, keepdim=True)
+  layer = kind == 'layer'
+
+  def stats(z, true):
+    zc = true - true.mean(-1, keepdim=True) if layer else true
+    r = 1.0 / torch.sqrt(zc.pow(2).mean(-1, keepdim=True) + eps)
+    n = zc * r
+    return n, r, ((sub(A(z), mean_abs(z)) if layer else A(z)) * r if mags else n)
+
+  g = None if gate is None else {0: lambda z: z, 2: torch.sigmoid, 4: torch.tanh}[act](gate)
+  w = lambda k, none: torch.full((x.shape[-1],), none, dtype=torch.float64, device=DEV) if o.get(k) is None else o[k].double()
+  sc, gg = w('scale', 1.0), (torch.ones_like(x) if g is None else g)
+  res = {}
+  if o.get('post', True):
+    an, ar, am = stats(a, a)
+    n, nm = an * w('post_weight', 1.0) + w('post_bias', 0.0), A(am) * A(w('post_weight', 1.0)) + A(w('post_bias', 0.0))
+  else:
+    an, ar, n, nm = a, None, a, A(a)
+    am = A(a)
+  y = alpha * x + sc * gg * n
+  ym = A(alpha * x) + A(sc) * A(gg) * nm
+  res['y'] = ym if mags else y
+  if o.get('pre', True):
+    yn, yr, yhm = stats(ym, y)
+    res['h'] = (A(yhm) * A(w('pre_weight', 1.0)) + A(w('pre_bias', 0.0))) if mags else yn * w('pre_weight', 1.0) + w('pre_bias', 0.0)
+  if dy is None and dh is None:
+    return res
+  d = torch.zeros_like(x) if dy is None else A(dy)
+
+  def back(dz, zn, zm, r):
+    zz = zm if mags else zn
+    m1 = A(dz).mean(-1, keepdim=True) if layer else 0.0
+    return r * sub(sub(A(dz), m1), A(zz) * (A(dz) * A(zz)).mean(-1, keepdim=True)) if mags else r * (dz - (dz.mean(-1, keepdim=True) if layer else 0.0) - zn * (dz * zn).mean(-1, keepdim=True))
+
+  if dh is not None:
+    d = d + back(dh * w('pre_weight', 1.0), yn, yhm, yr)
+    res['pre_weight'] = (A(dh) * (A(yhm) if mags else yn)).flatten(0, -2).sum(0)
+    res['pre_bias'] = A(dh).flatten(0, -2).sum(0)
+  elif o.get('pre', True):
+    res['pre_weight'] = res['pre_bias'] = torch.zeros(x.shape[-1], dtype=torch.float64, device=DEV)
+  res['x'] = A(alpha * d)
+  dn = d * A(sc) * A(gg)
+  if g is not None:
+    slope = {0: lambda z: torch.ones_like(z), 2: lambda z: z * (1 - z), 4: lambda z: (1 - z * z) if not mags else (1 + z * z)}[act](gg)
+    res['gate'] = d * A(sc) * (nm if mags else n) * slope
+  res['scale'] = (d * A(gg) * (nm if mags else n)).flatten(0, -2).sum(0)
+  if o.get('post', True):
+    res['a'] = back(dn * A(w('post_weight', 1.0)), an, am, ar)
+    res['post_weight'], res['post_bias'] = (dn * (A(am) if mags else an)).flatten(0, -2).sum(0), dn.flatten(0, -2).sum(0)
+  else:
+    res['a'] = dn
+  return res
+
+
+# longest path of one output: row sums of <= 8 serial + 6 shuffle + 3 wave additions, twice in each of four norms (statistics, sums of the backward),
+# the exponential of the gate (<= 16 roundings for |gate| < 8) and ~16 pointwise steps; column sums add their own serial length (below)
+K_NORM = 4 * 2 * 17 + 16 + 16
+
+
+def run_norm(ops, shape, dtype, kind, gate_kind, act=2, seed=0, alpha=1.0, strides=False, **o):
+  C = shape[-1]
+  wide = lambda *s, **k: randn(*s[:-1], s[-1] + 24, **k)[..., 8:8 + s[-1]] if strides else randn(*s, **k)
+  x, a = wide(*shape, dtype=dtype, seed=seed + 1, std=2.0), wide(*shape, dtype=dtype, seed=seed + 2, std=0.5, mean=0.2)
+  gate = None
+  if gate_kind == 'token':
+    gate = wide(*shape, dtype=dtype, seed=seed + 3)
+  elif gate_kind == 'sample':
+    gate = randn(shape[0], C, dtype=dtype, seed=seed + 3)
+  dy, dh = wide(*shape, dtype=dtype, seed=seed + 4), wide(*shape, dtype=dtype, seed=seed + 5)
+  y, h, ctx = ops.block_norm_fwd(x, a, kind=kind, gate=gate, gate_act=act if gate is not None else 0, alpha=alpha, **o)
+  use_dh = dh if o.get('pre', True) else None
+  into = {n: torch.ones(C, device=DEV) for n in ('scale', 'post_weight') if o.get(n) is not None}
+  gr = ops.block_norm_bwd(dy, use_dh, ctx, into=into)
+  full = None if gate is None else (gate.double().view(shape[0], *([1] * (len(shape) - 2)), C).expand(*shape) if gate_kind == 'sample' else gate.double())
+  args = (kind, o, full, act if gate is not None else 0, alpha, 1e-5)
+  dh64 = None if use_dh is None else dh.double()
+  want = norm_oracle(x.double(), a.double(), *args, dy=dy.double(), dh=dh64)
+  mag = norm_oracle(x.double(), a.double(), *args, dy=dy.double(), dh=dh64, mags=True)
+  rows = x.numel() // C
+  got = dict(gr, y=y, h=h)
+  for n, g in got.items():
+    if g is None or n not in want:
+      assert g is None or n in ('gate',), n
+      continue
+    w, m = want[n], mag[n]
+    if n == 'gate' and gate_kind == 'sample':
+      w, m = (z.reshape(shape[0], -1, C).sum(1) for z in (w, m))
+    k = K_NORM
+    if n in ('scale', 'post_weight', 'post_bias', 'pre_weight', 'pre_bias') or (n == 'gate' and gate_kind == 'sample'):
+      k += min(rows, 4 + rows // 512 + 600)  # serial additions of one workgroup's rows and of one slice of the partials
+    if n in into:
+      w, m = w + 1.0, m + 1.0
+    within(n, g, w.view(g.shape), (U[g.dtype] * w.abs() + k * U[F32] * m).view(g.shape))
+
+
+def full_params(C, layer, seed=60):
+  o = dict(scale=randn(C, seed=seed, std=0.3, mean=0.5), post_weight=randn(C, seed=seed + 1, std=0.2, mean=1.0), pre_weight=randn(C, seed=seed + 2, std=0.2, mean=1.0))
+  if layer:
+    o.update(post_bias=randn(C, seed=seed + 3, std=0.2), pre_bias=randn(C, seed=seed + 4, std=0.2))
+  return o
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('kind', ['layer', 'rms'])
+@pytest.mark.parametrize('gate', ['none', 'sample', 'token'])
+@pytest.mark.parametrize('shape', [(1, 1, 8), (2, 3, 27), (3, 50, 72), (12, 20, 576), (2, 129, 1512), (1, 40, 2048), (2, 9, 4096), (1, 3, 4095)], ids=str)
+def test_block_norm_forward_and_gradients(ops, shape, gate, kind, dtype):
+  run_norm(ops, shape, dtype, kind, gate, **full_params(shape[-1], kind == 'layer'))
+
+
+@pytest.mark.parametrize('o', [dict(post=False), dict(pre=False), dict(post=False, pre=False), dict()], ids=['no-post', 'no-pre', 'neither', 'no-parameters'])
+@pytest.mark.parametrize('act', [0, 4])
+def test_block_norm_parts(ops, o, act):
+  run_norm(ops, (4, 33, 216), BF16, 'layer', 'token', act=act, alpha=0.7, **o)
+  run_norm(ops, (4, 33, 216), F32, 'rms', 'sample', act=act, alpha=0.7, **o)
+
+
+def test_block_norm_slices_of_wider_rows(ops):
+  run_norm(ops, (3, 20, 64), BF16, 'layer', 'token', strides=True, **full_params(64, True))
+  run_norm(ops, (3, 20, 61), F32, 'rms', 'none', strides=True, **full_params(61, False))
+
+
+def test_block_norm_one_gradient_only(ops):
+  """dh alone (the residual stream ends here) and dy alone equal the pair with zeros in the other place."""
+  o = full_params(96, True)
+  x, a, g = randn(2, 10, 96, dtype=BF16, seed=70), randn(2, 10, 96, dtype=BF16, seed=71), randn(2, 96, dtype=BF16, seed=72)
+  _, _, ctx = ops.block_norm_fwd(x, a, gate=g, gate_act=2, **o)
+  d, z = randn(2, 10, 96, dtype=BF16, seed=73), torch.zeros(2, 10, 96, dtype=BF16, device=DEV)
+  for one, two in (((d, None), (d, z)), ((None, d), (z, d))):
+    p, q = ops.block_norm_bwd(*one, ctx), ops.block_norm_bwd(*two, ctx)
+    for n in p:
+      assert (p[n] is None and q[n] is None) or torch.equal(p[n], q[n]), n
+
+
+def test_block_norm_gradient_against_differences(ops):
+  """Directional derivatives of the 64-bit forward by central differences (step 1e-5: truncation ~1e-10 of the third derivative)."""
+  C = 48
+  o = full_params(C, True)
+  x, a, g = randn(2, 5, C, seed=80), randn(2, 5, C, seed=81), randn(2, 5, C, seed=82)
+  dy, dh = randn(2, 5, C, seed=83).double(), randn(2, 5, C, seed=84).double()
+  _, _, ctx = ops.block_norm_fwd(x, a, gate=g, gate_act=2, **o)
+  gr = ops.block_norm_bwd(dy.float(), dh.float(), ctx)
+  base = dict(x=x, a=a, gate=g, **o)
+
+  def loss(v):
+    r = norm_oracle(v['x'], v['a'], 'layer', {k: v[k] for k in o}, v['gate'], 2, 1.0, 1e-5)
+    return (r['y'] * dy).sum() + (r['h'] * dh).sum()
+
+  for n in base:
+    direction = randn(*base[n].shape, seed=90).double()
+    v = {k: t.double() for k, t in base.items()}
+    e = 1e-5
+    num = (loss({**v, n: v[n] + e * direction}) - loss({**v, n: v[n] - e * direction})) / (2 * e)
+    want = (gr[n].double() * direction).sum()
+    # each gradient element is within K_NORM fp32 roundings of magnitudes below ~50 here
+    assert abs(float(num - want)) <= K_NORM * U[F32] * 50 * float(direction.abs().sum()) + 1e-6 * abs(float(num)), (n, float(num), float(want))
+
+
+def test_block_norm_constant_rows_are_exact_zeros(ops):
+  x = torch.zeros(1, 4, 64, device=DEV)
+  y, h, ctx = ops.block_norm_fwd(x, torch.full_like(x, 3.0))
+  assert not y.any() and not h.any()
+  gr = ops.block_norm_bwd(torch.ones_like(x), torch.ones_like(x), ctx)
+  assert all(torch.isfinite(t).all() for t in gr.values() if t is not None)
+
+
+def test_block_norm_empty_and_refusals(ops):
+  e = torch.empty(0, 5, 32, device=DEV)
+  y, h, ctx = ops.block_norm_fwd(e, e, scale=torch.ones(32, device=DEV))
+  assert y.shape == e.shape and not ops.block_norm_bwd(e, e, ctx)['scale'].any()
+  x = randn(2, 3, 32)
+  bad = [dict(x=x.half(), a=x.half()), dict(a=x.bfloat16()), dict(a=x[:, :2]), dict(x=x.cpu(), a=x.cpu()), dict(kind='batch'), dict(gate=x[0]), dict(gate=x, gate_act=1),
+         dict(scale=torch.ones(31, device=DEV)), dict(scale=torch.ones(32, device=DEV, dtype=BF16)), dict(pre=False, pre_weight=torch.ones(32, device=DEV)),
+         dict(x=randn(1, 4097), a=randn(1, 4097)), dict(x=randn(2, 32, 3).transpose(1, 2)), dict(x=randn(32).expand(2, 3, 32))]
+  for kw in bad:
+    kw = {'x': x, 'a': x, **kw}
+    with pytest.raises((ValueError, TypeError)):
+      ops.block_norm_fwd(kw.pop('x'), kw.pop('a'), **kw)
+  _, _, ctx = ops.block_norm_fwd(x, x, pre=False)
+  for args in ((None, None), (x, x), (x.bfloat16(), None), (x[:1], None)):
+    with pytest.raises((ValueError, TypeError)):
+      ops.block_norm_bwd(*args, ctx)
+  with pytest.raises(ValueError):
+    ops.block_norm_bwd(x, None, ctx, into=dict(scale=torch.zeros(32, device=DEV)))
+
+
+def test_block_norm_captured(ops):
+  o = full_params(576, True)
+  x, a, g = (randn(2, 40, 576, dtype=BF16, seed=100 + i) for i in range(3))
+  dy, dh = randn(2, 40, 576, dtype=BF16, seed=110), randn(2, 40, 576, dtype=BF16, seed=111)
+
+  def step():
+    y, h, ctx = ops.block_norm_fwd(x, a, gate=g, gate_act=2, **o)
+    return [y, h] + [t for t in ops.block_norm_bwd(dy, dh, ctx).values() if t is not None]
+
+  step()
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    outs = step()
+  for k in range(3):
+    x.copy_(randn(2, 40, 576, dtype=BF16, seed=120 + k))
+    want = step()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(outs, want))
