@@ -14,7 +14,7 @@ ROOT = os.path.dirname(PKG_DIR)
 HEADER = os.path.join(ROOT, 'include', 'tfpp.h')
 CSRC = os.path.join(PKG_DIR, 'csrc')
 LIB_PATH = os.path.join(PKG_DIR, 'libtfpp_hip.so')
-SOURCES = ['gemm_kernels.hip', 'gemm_glds.hip', 'gemm_wgrad_glds.hip', 'attention_kernels.hip', 'conv3x3_halo.hip', 'wgrad3x3_halo.hip', 'pointwise_kernels.hip', 'norm_kernels.hip', 'bn_rows_kernels.hip', 'misc_kernels.hip', 'lidar_kernels.hip', 'swin_kernels.hip', 'bev_kernels.hip', 'head_kernels.hip', 'augment_kernels.hip', 'grad_clip.hip', 'block_norm.hip']
+SOURCES = ['gemm_kernels.hip', 'gemm_glds.hip', 'gemm_wgrad_glds.hip', 'attention_kernels.hip', 'conv3x3_halo.hip', 'wgrad3x3_halo.hip', 'pointwise_kernels.hip', 'norm_kernels.hip', 'bn_rows_kernels.hip', 'misc_kernels.hip', 'lidar_kernels.hip', 'swin_kernels.hip', 'bev_kernels.hip', 'head_kernels.hip', 'augment_kernels.hip', 'grad_clip.hip', 'block_norm.hip', 'diff_attention.hip']
 
 F32, BF16 = 0, 1
 ABI_VERSION = 9  # include/tfpp.h TFPP_ABI_VERSION
@@ -70,6 +70,14 @@ class BlockNormParams(ctypes.Structure):
                                 'dpost_b', 'dpre_w', 'dpre_b', 'dscale', 'partial')] + \
       [(n, i64) for n in ('ld_x', 'ld_a', 'ld_g', 'ld_dy', 'ld_dh')] + \
       [(n, i32) for n in ('B', 'T', 'C', 'layer', 'post', 'pre', 'gate_mode', 'gate_act', 'accumulate')] + [('alpha', f32), ('eps', f32)]
+
+
+class DiffAttnParams(ctypes.Structure):
+  _fields_ = [(n, vp) for n in ('q', 'k', 'v', 'lam', 'norm_w', 'out', 'o1', 'o2', 'lse', 'kv_len', 'q_start', 'key_mask', 'dout', 'd_o', 'delta', 'partial', 'dlam',
+                                'dnorm_w', 'dq_out', 'dk_out', 'dv_out')] + \
+      [('ld_mask', i64), ('q_s', i64 * 4), ('k_s', i64 * 4), ('v_s', i64 * 3), ('o_s', i64 * 3), ('do_s', i64 * 3), ('dq_s', i64 * 4), ('dk_s', i64 * 4), ('dv_s', i64 * 3)] + \
+      [(n, i32) for n in ('B', 'H', 'Hkv', 'Tq', 'Tk', 'd', 'dv', 'n_lam', 'norm', 'norm_w_bf16', 'causal', 'q_start_all', 'out_vec', 'dq_vec', 'dk_vec', 'dv_vec')] + \
+      [('scale', f32), ('out_scale', f32), ('eps', f32)]
 
 
 _CTYPE = {'int': i32, 'int32_t': i32, 'int64_t': i64, 'uint64_t': ctypes.c_uint64, 'uint32_t': ctypes.c_uint32, 'float': f32, 'double': ctypes.c_double}
@@ -245,6 +253,7 @@ class _Lib:
             ctypes.sizeof(AttnParams)]
     mine.append(ctypes.sizeof(BnRows))
     mine.append(ctypes.sizeof(BlockNormParams))
+    mine.append(ctypes.sizeof(DiffAttnParams))
     if n != len(mine) or list(sizes[:n]) != mine:
       raise TfppError(f'struct layout mismatch: library {list(sizes[:n])} vs ctypes {mine}')
     if self._dll.tfpp_version() != ABI_VERSION:

@@ -1,0 +1,1000 @@
+// Differential attention: the difference of two softmax maps with a learned weight, and the norm of each head's result.
+//   P_i = softmax(scale Q_i K_i^T) (i = 1, 2)      O = (P_1 - lambda P_2) V      out = out_scale * w * O / sqrt(mean(O^2) + eps)
+// Q [B, Tq, H, 2, d], K [B, Tk, Hkv, 2, d], V [B, Tk, Hkv, dv] with any strides but a contiguous last dimension; H / Hkv query heads share a key /
+// value head; d <= 128, dv <= 256.  Keys are left out by kv_len (per sequence), key_mask (per key) and causality (key <= q_start + query); a query
+// that sees no key gives zeros and takes no part in any gradient.  Left-out keys are never read: what lies there (NaN included) has no effect.
+//
+// All products are 32 x 32 x 16 MFMA tiles (bf16; fp32 runs the same code on eight 32 x 32 x 2 each).  Every score tile is computed transposed to
+// where it is contracted next, so that its C fragment IS the B operand of the following product and never leaves the registers:
+//   C layout: lane l, register r hold (row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32);  registers 8 t .. 8 t + 7 are the eight contraction
+//   slots of lane l for rows 16 t .. 16 t + 15 once both operands label slot e of half l / 32 as row 16 t + 8 (e / 4) + 4 (l / 32) + e % 4.
+// The other operand is read in that labelling from an LDS image [row][channel] by two ds_read_b64_tr_b16 (bf16) or eight scalar reads (fp32).
+// Images hold 16-byte chunks, chunk c of row r at r * NC + (c ^ swizzle(r)): row reads (32 rows, one chunk) and transpose reads (4 rows x 64
+// bytes) are both free of bank conflicts.  They are filled by buffer loads into LDS (16 bytes a lane, no registers), one tile ahead of the products,
+// where rows are 16-byte aligned, else element by element.
+#include <cmath>
+
+#include "common.h"
+#include "../../include/tfpp.h"
+
+namespace {
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float NO_MAX = -1.0e30f;     // running maximum before the first visible key: finite, so that -inf scores give exp2(-inf) = 0
+constexpr float MAX_SLACK = 8.f;       // the running maximum follows once it is 2^8 behind: probabilities stay below 256, exact in fp32 / bf16 range
+constexpr int QB = 128;                // queries (keys) of a workgroup in the backward passes, 32 per wave
+
+template <typename T> struct Frag8;
+template <> struct Frag8<bf16_t> { uint4 v; };
+template <> struct Frag8<float> { float v[8]; };
+
+__device__ __forceinline__ void mma(const Frag8<bf16_t>& a, const Frag8<bf16_t>& b, f32x16_t& c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a.v), __builtin_bit_cast(bf16x8_t, b.v), c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(const Frag8<float>& a, const Frag8<float>& b, f32x16_t& c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
+}
+// C registers 8 t .. 8 t + 7 as an operand.  bf16: one rounding (2^-9 relative) of each probability / score gradient, as its partner operand has
+__device__ __forceinline__ void to_frag(const f32x16_t& c, int t, Frag8<bf16_t>& f) {
+  f.v = make_uint4(f2bf_pack2(c[8 * t], c[8 * t + 1]), f2bf_pack2(c[8 * t + 2], c[8 * t + 3]), f2bf_pack2(c[8 * t + 4], c[8 * t + 5]),
+                   f2bf_pack2(c[8 * t + 6], c[8 * t + 7]));
+}
+__device__ __forceinline__ void to_frag(const f32x16_t& c, int t, Frag8<float>& f) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f.v[e] = c[8 * t + e];
+}
+
+__device__ __forceinline__ unsigned long long low_bits(int n) { return n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1ull); }
+constexpr int pow2_at_least(int n) { return n <= 1 ? 1 : 2 * pow2_at_least((n + 1) / 2); }
+
+// LDS image of rows with 32 * CB channels (NC 16-byte chunks a row, a power of two)
+template <typename T, int CB> struct Img {
+  static constexpr int VEC = ElemTraits<T>::VEC, USED = 32 * CB / VEC, NC = pow2_at_least(USED);
+  static constexpr int ROW_BYTES = NC * 16;
+  __device__ static __forceinline__ int swizzle(int r) {
+    if constexpr (NC >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (NC == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+  }
+  __device__ static __forceinline__ int off(int r, int c) { return (r * NC + (c ^ swizzle(r))) * 16; }
+  // operand of 32 rows x 16 channels (channels 16 ks ..): lane l has row l % 32, channels 16 ks + 8 (l / 32) ..
+  __device__ static __forceinline__ void rows(const unsigned char* img, int row, int ks, int half, Frag8<T>& f) {
+    if constexpr (sizeof(T) == 2) {
+      f.v = *reinterpret_cast<const uint4*>(img + off(row, 2 * ks + half));
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(img + off(row, 4 * ks + 2 * half)), b = *reinterpret_cast<const float4*>(img + off(row, 4 * ks + 2 * half + 1));
+      f.v[0] = a.x; f.v[1] = a.y; f.v[2] = a.z; f.v[3] = a.w; f.v[4] = b.x; f.v[5] = b.y; f.v[6] = b.z; f.v[7] = b.w;
+    }
+  }
+  // operand of 32 channels (32 cb ..) x 16 rows (row0 ..), contraction over rows in the C fragments' labelling
+  __device__ static __forceinline__ void cols(const unsigned char* img, int row0, int cb, int lane, Frag8<T>& f) {
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, r = row0 + 4 * half + (i >> 2), c = cb * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(img + off(r, c) + sub));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(img + off(r + 8, c) + sub));
+      const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+      f.v = make_uint4(a.x, a.y, b.x, b.y);
+    } else {
+      const int m = cb * 32 + (lane & 31);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int r = row0 + 8 * (e >> 2) + 4 * half + (e & 3);
+        f.v[e] = *reinterpret_cast<const float*>(img + off(r, m >> 2) + (m & 3) * 4);
+      }
+    }
+  }
+  // fill ROWS rows: row r comes from base + r * ld (n channels), zeros where its bit in `valid` is not set and behind channel n.  VECTOR: buffer loads
+  // into LDS, one 32-bit offset a lane (64 rows stay below 2 GB: checked by the launcher); a chunk that is left out gets an offset behind the
+  // descriptor's range, for which the hardware returns zeros without touching memory.
+  template <int ROWS, bool VECTOR, int NT> __device__ static __forceinline__ void fill(unsigned char* img, const T* __restrict__ base, long ld, int n, unsigned long long valid, int tid) {
+    constexpr int SLOTS = ROWS * NC;
+    if constexpr (VECTOR) {
+      static_assert(NT % NC == 0 && SLOTS % 64 == 0, "a thread keeps its position in the row");
+      const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+      const int ldb = (int)ld * (int)sizeof(T), r0 = tid / NC, rowb = r0 * ldb;
+      const bool all = (valid & low_bits(ROWS)) == low_bits(ROWS);
+#pragma unroll
+      for (int u = 0; u * NT < SLOTS; ++u) {
+        if (u * NT + wave * 64 < SLOTS) {
+          const int r = r0 + u * (NT / NC), c = (tid % NC) ^ swizzle(r);
+          bool ok = c * VEC < n;
+          if (!all) ok = ok && ((valid >> r) & 1ull);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t*)(img + (u * NT + wave * 64) * 16), 16, ok ? rowb + c * 16 : (int)0x80000000, u * (NT / NC) * ldb, 0, 0);
+        }
+      }
+    } else {
+      for (int i = tid; i < ROWS * 32 * CB; i += NT) {
+        const int r = i / (32 * CB), c = i % (32 * CB);
+        T v = ElemTraits<T>::from_f(0.f);
+        if (c < n && ((valid >> r) & 1ull)) v = base[(long)r * ld + c];
+        *reinterpret_cast<T*>(img + off(r, c / VEC) + (c % VEC) * sizeof(T)) = v;
+      }
+    }
+  }
+};
+
+// operand straight from global memory: 8 channels (c ..) of one row, zeros behind channel n or where the row is left out
+template <typename T, bool VECTOR> __device__ __forceinline__ void load_frag(const T* __restrict__ row, int c, int n, bool ok, Frag8<T>& f) {
+  if constexpr (VECTOR) {
+    if constexpr (sizeof(T) == 2) {
+      f.v = ok && c < n ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 a = ok && c + e < n ? *reinterpret_cast<const float4*>(row + c + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        f.v[e] = a.x; f.v[e + 1] = a.y; f.v[e + 2] = a.z; f.v[e + 3] = a.w;
+      }
+    }
+  } else if constexpr (sizeof(T) == 2) {
+    unsigned u[4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const unsigned lo = ok && c + e < n ? row[c + e] : 0, hi = ok && c + e + 1 < n ? row[c + e + 1] : 0;
+      u[e / 2] = lo | hi << 16;
+    }
+    f.v = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = ok && c + e < n ? row[c + e] : 0.f;
+  }
+}
+
+// four consecutive channels c .. of a row with n channels
+template <typename T> __device__ __forceinline__ void store4(T* __restrict__ row, int c, int n, bool vec, float a, float b, float e, float f) {
+  if (vec && c + 3 < n) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + c) = make_uint2(f2bf_pack2(a, b), f2bf_pack2(e, f));
+    else *reinterpret_cast<float4*>(row + c) = make_float4(a, b, e, f);
+  } else {
+    if (c < n) row[c] = ElemTraits<T>::from_f(a);
+    if (c + 1 < n) row[c + 1] = ElemTraits<T>::from_f(b);
+    if (c + 2 < n) row[c + 2] = ElemTraits<T>::from_f(e);
+    if (c + 3 < n) row[c + 3] = ElemTraits<T>::from_f(f);
+  }
+}
+
+__device__ __forceinline__ float norm_weight(const tfpp_diff_attn_params& p, int c) {
+  return !p.norm_w ? 1.f : (p.norm_w_bf16 ? bf2f(((const bf16_t*)p.norm_w)[c]) : ((const float*)p.norm_w)[c]);
+}
+
+// workgroup -> (tile, batch x head).  Workgroups go round the 8 XCDs in turn: all tiles of one key / value head stay on one XCD (its K and V
+// are read from that XCD's L2) where the heads divide evenly.
+__device__ __forceinline__ void place(int heads, int tiles, int& bh, int& tile) {
+  const int id = blockIdx.x;
+  if (heads % 8 == 0) {
+    bh = (id % 8) + 8 * ((id / 8) / tiles);
+    tile = (id / 8) % tiles;
+  } else {
+    bh = id / tiles;
+    tile = id % tiles;
+  }
+}
+
+struct Seq {  // what a sequence's queries may see
+  int len, start;  // keys 0 .. len - 1; query i sees key j <= start + i (causal)
+};
+__device__ __forceinline__ Seq sequence(const tfpp_diff_attn_params& p, int b) {
+  Seq s;
+  s.len = p.Tk;
+  if (p.kv_len) {
+    const int n = p.kv_len[b];
+    s.len = n < 0 ? 0 : (n < p.Tk ? n : p.Tk);
+  }
+  s.start = p.q_start ? p.q_start[b] : p.q_start_all;
+  return s;
+}
+// bit i: key j0 + i exists and is not left out
+__device__ __forceinline__ unsigned long long key_bits(const tfpp_diff_attn_params& p, int b, int j0, int len, int lane) {
+  const int j = j0 + lane;
+  bool ok = j < len;
+  if (p.key_mask && ok) ok = p.key_mask[(long)b * p.ld_mask + j] != 0;
+  return __ballot(ok);
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// forward.  Workgroup = (batch, head, 128 queries), wave = 32 queries, lane l and l + 32 = one query.  S_i^T = K_i Q_i^T (keys x queries), running
+// maximum and sum per query, O_i^T += V^T P_i^T: both maps share every V operand.  O_1 and O_2 are kept apart to the end because their sums are
+// not known before; one pass, 4 d + 4 dv flop a pair.  Wide heads (SPLIT): O_1 and O_2 of 32 queries do not fit one wave's registers, so two waves
+// share the queries, one map each, and meet in LDS at the end.
+template <typename T, int NB> constexpr bool fwd_split() { return NB >= (sizeof(T) == 2 ? 8 : 5); }
+template <typename T, int NB> constexpr int fwd_threads() { return fwd_split<T, NB>() && sizeof(T) == 2 ? 512 : 256; }
+template <typename T, int NB> constexpr int fwd_queries() { return fwd_threads<T, NB>() / (fwd_split<T, NB>() ? 4 : 2); }
+template <typename T, int NB> constexpr int fwd_lds() { return 2 * key_tile<T>() * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES); }
+
+template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_threads<T, NB>()), (fwd_threads<T, NB>() == 512 || NB <= (sizeof(T) == 2 ? 4 : 2) ? 2 : 1)) void diff_attn_fwd_kernel(tfpp_diff_attn_params p) {
+  constexpr int KT = key_tile<T>(), CD = (NB + 1) / 2, NT = fwd_threads<T, NB>(), MAPS = fwd_split<T, NB>() ? 1 : 2, QB = fwd_queries<T, NB>();
+  typedef Img<T, CD> ImgK;
+  typedef Img<T, NB> ImgV;
+  constexpr int K_BYTES = KT * ImgK::ROW_BYTES, V_BYTES = KT * ImgV::ROW_BYTES, BUF = 2 * K_BYTES + V_BYTES;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int tiles = (p.Tq + QB - 1) / QB;
+  int bh, tile;
+  place(p.B * p.H, tiles, bh, tile);
+  if (p.causal) tile = tiles - 1 - tile;  // the longest rows first
+  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
+  const Seq sq = sequence(p, b);
+  const int map0 = MAPS == 1 ? wave & 1 : 0;  // this wave's (first) map
+  const int w0 = tile * QB + (MAPS == 1 ? wave >> 1 : wave) * 32, qi = w0 + (lane & 31), qc = qi < p.Tq ? qi : p.Tq - 1;
+  const T* kb = (const T*)p.k + (long)b * p.k_s[0] + (long)hk * p.k_s[2];
+  const T* vb = (const T*)p.v + (long)b * p.v_s[0] + (long)hk * p.v_s[2];
+  constexpr bool HOLD = sizeof(T) == 2 ? VECTOR || NB < 8 : NB < 5;  // wide fp32 heads do not fit the registers: Q is read again for every tile
+  const T* qrow = (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2];
+  Frag8<T> q[MAPS][HOLD ? NB : 1];
+  if constexpr (HOLD)
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i)
+#pragma unroll
+      for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(qrow + (long)(map0 + i) * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][ks]);
+  const int last = tile * QB + QB < p.Tq ? tile * QB + QB : p.Tq;  // causal: the workgroup's last query bounds its keys
+  int end = sq.len;
+  if (p.causal) end = sq.start + last < end ? sq.start + last : end;
+  const int steps = end > 0 ? (end + KT - 1) / KT : 0;
+  const float c = p.scale * LOG2E;
+
+  f32x16_t o[MAPS][NB];
+#pragma unroll
+  for (int i = 0; i < MAPS; ++i)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][n][r] = 0.f;
+  float m[MAPS], l[MAPS];  // m: both halves of a query agree; l: this half's keys
+
+#pragma unroll
+  for (int i = 0; i < MAPS; ++i) m[i] = NO_MAX, l[i] = 0.f;
+
+  auto fill = [&](int step, unsigned long long bits) {
+    unsigned char* buf = smem + (step & 1) * BUF;
+    const long j0 = (long)step * KT;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, bits, tid);
+    ImgV::template fill<KT, VECTOR, NT>(buf + 2 * K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, bits, tid);
+  };
+  unsigned long long bits = 0;
+  if (steps > 0) {
+    bits = key_bits(p, b, 0, sq.len, lane);
+    fill(0, bits);
+  }
+  for (int s = 0; s < steps; ++s) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // image s is complete, and every wave is past its reads of image s - 1
+    const unsigned long long cur = bits;
+    if (s + 1 < steps) {
+      bits = key_bits(p, b, (s + 1) * KT, sq.len, lane);
+      fill(s + 1, bits);
+    }
+    const int j0 = s * KT;
+    const int seen = p.causal ? sq.start + w0 + 32 - j0 : KT;  // keys of this tile that the wave's last query sees
+    if (seen <= 0 || cur == 0) continue;
+    const bool masked = (cur & low_bits(KT)) != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
+    const unsigned long long mine = p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur;
+    const unsigned char* buf = smem + (s & 1) * BUF;
+#pragma unroll 1
+    for (int kb32 = 0; kb32 < KT / 32; ++kb32) {
+      f32x16_t sc[MAPS];
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[i][r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < NB; ++ks) {
+          Frag8<T> a;
+          ImgK::rows(buf + (map0 + i) * K_BYTES, kb32 * 32 + (lane & 31), ks, half, a);
+          if constexpr (!HOLD) load_frag<T, VECTOR>(qrow + (long)(map0 + i) * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][0]);
+          mma(a, q[i][HOLD ? ks : 0], sc[i]);
+        }
+      }
+      if (masked) {
+        const unsigned vis = (unsigned)(mine >> (kb32 * 32)) >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool keep = (vis >> (8 * (r >> 2) + (r & 3))) & 1u;
+#pragma unroll
+          for (int i = 0; i < MAPS; ++i) sc[i][r] = keep ? sc[i][r] : -INFINITY;
+        }
+      }
+      float mx[MAPS];
+      bool grew = false;
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i) {
+        mx[i] = sc[i][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx[i] = fmaxf(mx[i], sc[i][r]);
+        mx[i] *= c;
+        grew = grew || mx[i] > m[i] + MAX_SLACK;
+      }
+      if (__any(grew)) {
+#pragma unroll
+        for (int i = 0; i < MAPS; ++i) {
+          const float to = fmaxf(m[i], fmaxf(mx[i], other_half(mx[i])));
+          const float f = exp2f(m[i] - to);
+          m[i] = to;
+          l[i] *= f;
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][n][r] *= f;
+        }
+      }
+      Frag8<T> pf[MAPS][2];
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          sc[i][r] = __builtin_amdgcn_exp2f(fmaf(sc[i][r], c, -m[i]));
+          l[i] += sc[i][r];
+        }
+        to_frag(sc[i], 0, pf[i][0]);
+        to_frag(sc[i], 1, pf[i][1]);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          Frag8<T> v;
+          ImgV::cols(buf + 2 * K_BYTES, kb32 * 32 + 16 * t, n, lane, v);
+#pragma unroll
+          for (int i = 0; i < MAPS; ++i) mma(v, pf[i][t], o[i][n]);
+        }
+    }
+  }
+
+  const float lam = p.lam[p.n_lam > 1 ? h : 0];
+  const long row = ((long)b * p.H + h) * p.Tq + qi;
+  const bool live = qi < p.Tq;
+  const int dvs = (p.dv + 7) & ~7;
+#pragma unroll
+  for (int i = 0; i < MAPS; ++i) {
+    l[i] += other_half(l[i]);
+    const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);  // no visible key: zeros; NaN stays
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][n][r] *= inv;
+    // log2 of the sum; +inf for a query without keys: exp2(score - inf) = 0 in the backward passes
+    if (p.lse && live && half == 0) p.lse[(long)(map0 + i) * p.B * p.H * p.Tq + row] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
+    if (p.o1 && live) {
+      T* to = (T*)(map0 + i ? p.o2 : p.o1) + row * dvs;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          store4<T>(to, n * 32 + 8 * g + 4 * half, dvs, true, o[i][n][4 * g], o[i][n][4 * g + 1], o[i][n][4 * g + 2], o[i][n][4 * g + 3]);
+    }
+  }
+  if constexpr (MAPS == 1) {  // O_2 of the odd waves to the even ones, in the registers' own order
+    static_assert(fwd_lds<T, NB>() >= 4 * NB * 16 * 64 * 4, "the exchange fits the images' LDS");
+    float* x = reinterpret_cast<float*>(smem) + (wave >> 1) * (NB * 16 * 64) + lane;
+    __syncthreads();  // every wave is past its last image
+    if (map0)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[(n * 16 + r) * 64] = o[0][n][r];
+    __syncthreads();
+    if (map0) return;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[0][n][r] -= lam * x[(n * 16 + r) * 64];
+  } else {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[0][n][r] -= lam * o[MAPS - 1][n][r];
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ss += o[0][n][r] * o[0][n][r];
+  float f = p.out_scale;
+  if (p.norm) {
+    ss += other_half(ss);
+    f *= 1.f / sqrtf(ss / (float)p.dv + p.eps);
+  }
+  if (live) {
+    T* out = (T*)p.out + (long)b * p.o_s[0] + (long)qi * p.o_s[1] + (long)h * p.o_s[2];
+    const bool vec = p.out_vec;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        __builtin_amdgcn_sched_barrier(0);  // (the weights of all channels at once would not fit the registers)
+        const int ch = n * 32 + 8 * g + 4 * half;
+        if (ch >= p.dv) continue;
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = p.norm && ch + e < p.dv ? f * norm_weight(p, ch + e) : f;
+        store4<T>(out, ch, p.dv, vec, o[0][n][4 * g] * w[0], o[0][n][4 * g + 1] * w[1], o[0][n][4 * g + 2] * w[2], o[0][n][4 * g + 3] * w[3]);
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// backward, in three launches and a sum (nothing is accumulated by atomics: the same bits from run to run).  With u = out_scale w dout:
+//   r = 1 / sqrt(mean(O^2) + eps)      dO = r u - O r^3 mean(u O)  (without the norm: dO = u)     dw = sum out_scale dout O r     dlambda = - sum dO . O_2
+//   dP = dO V^T      delta_i = dO . O_i      dS_1 = P_1 (dP - delta_1)      dS_2 = -lambda P_2 (dP - delta_2)
+//   dQ_i = scale dS_i K_i      dK_i = scale dS_i^T Q_i      dV = (P_1 - lambda P_2)^T dO
+// 1. diff_attn_bwd_rows_kernel: dO (rounded once: it is an MFMA operand twice), delta_i from that rounded dO -- so that the rows of dS still sum to
+//    zero -- and partial sums of dw, dlambda from the unrounded one.  Bounded by HBM.
+// grid (blocks, H); LPR lanes a row, 4 channels a lane
+template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_kernel(tfpp_diff_attn_params p, int lpr) {
+  __shared__ float sm[256 * 5];
+  const int h = blockIdx.y, lane = threadIdx.x & 63, c0 = (lane % lpr) * 4, dvs = (p.dv + 7) & ~7;
+  const int rpw = 64 / lpr, slots = (int)gridDim.x * 4 * rpw;
+  const long rows = (long)p.B * p.Tq;
+  const float lam = p.lam[p.n_lam > 1 ? h : 0];
+  float w[4], dw[4] = {0.f, 0.f, 0.f, 0.f}, dl = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = c0 + e < p.dv ? p.out_scale * (p.norm ? norm_weight(p, c0 + e) : 1.f) : 0.f;
+  const long first = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * rpw + lane / lpr;
+  const long rounds = (rows + slots - 1) / slots;
+  for (long k = 0; k < rounds; ++k) {  // (the same number of rounds in every lane: the shuffles below need them all)
+    const long n = first + k * slots;
+    const bool live = n < rows;
+    const int b = live ? (int)(n / p.Tq) : 0, t = live ? (int)(n % p.Tq) : 0;
+    const long row = ((long)b * p.H + h) * p.Tq + t;
+    const T* dout = (const T*)p.dout + (long)b * p.do_s[0] + (long)t * p.do_s[1] + (long)h * p.do_s[2];
+    float g[4], o1[4], o2[4], s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool in = live && c0 + e < p.dv;
+      g[e] = in ? ElemTraits<T>::to_f(dout[c0 + e]) : 0.f;
+      o1[e] = in ? ElemTraits<T>::to_f(((const T*)p.o1)[row * dvs + c0 + e]) : 0.f;
+      o2[e] = in ? ElemTraits<T>::to_f(((const T*)p.o2)[row * dvs + c0 + e]) : 0.f;
+      const float o = o1[e] - lam * o2[e];
+      s[0] += o * o;
+      s[1] += w[e] * g[e] * o;
+    }
+    float r = 1.f, f = 0.f;
+    if (p.norm) {
+      for (int x = 1; x < lpr; x <<= 1) {
+        s[0] += __shfl_xor(s[0], x, 64);
+        s[1] += __shfl_xor(s[1], x, 64);
+      }
+      r = 1.f / sqrtf(s[0] / (float)p.dv + p.eps);  // (eps > 0: checked by the launcher)
+      f = r * r * r * s[1] / (float)p.dv;
+    }
+    float d[4], t1 = 0.f, t2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float o = o1[e] - lam * o2[e];
+      dw[e] += p.out_scale * g[e] * o * r;
+      d[e] = r * w[e] * g[e] - o * f;
+      dl -= d[e] * o2[e];
+      const float dr = ElemTraits<T>::to_f(ElemTraits<T>::from_f(d[e]));
+      t1 += dr * o1[e];
+      t2 += dr * o2[e];
+    }
+    for (int x = 1; x < lpr; x <<= 1) {
+      t1 += __shfl_xor(t1, x, 64);
+      t2 += __shfl_xor(t2, x, 64);
+    }
+    if (live) {
+      if (c0 < dvs) store4<T>((T*)p.d_o + row * dvs, c0, dvs, true, d[0], d[1], d[2], d[3]);
+      if (c0 == 0) {
+        p.delta[row] = t1;
+        p.delta[(long)p.B * p.H * p.Tq + row] = t2;
+      }
+    }
+  }
+  // partial row (block, head): dlambda, then dw
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sm[e * 256 + threadIdx.x] = dw[e];
+  sm[4 * 256 + threadIdx.x] = dl;
+  __syncthreads();
+  float* out = p.partial + ((long)blockIdx.x * p.H + h) * (1 + p.dv);
+  if (threadIdx.x == 0) {
+    float a = 0.f;
+    for (int i = 0; i < 256; ++i) a += sm[4 * 256 + i];
+    out[0] = a;
+  }
+  for (int c = threadIdx.x; c < p.dv; c += 256) {
+    float a = 0.f;
+    for (int i = c >> 2; i < 256; i += lpr) a += sm[(c & 3) * 256 + i];
+    out[1 + c] = a;
+  }
+}
+
+// dlambda (blocks 0 .. n_lam - 1) and dw (the blocks behind): one value per workgroup, fixed order
+template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_kernel(tfpp_diff_attn_params p, int blocks) {
+  __shared__ float sm[4];
+  const int x = blockIdx.x, pitch = 1 + p.dv;
+  const bool is_lam = x < p.n_lam;
+  const int c = is_lam ? 0 : 1 + x - p.n_lam;
+  float s = 0.f;
+  if (is_lam && p.n_lam > 1)
+    for (int i = threadIdx.x; i < blocks; i += 256) s += p.partial[((long)i * p.H + x) * pitch];
+  else
+    for (int i = threadIdx.x; i < blocks * p.H; i += 256) s += p.partial[(long)i * pitch + c];
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = (sm[0] + sm[1]) + (sm[2] + sm[3]);
+  if (is_lam) p.dlam[x] = s;
+  else if (p.norm_w_bf16) ((bf16_t*)p.dnorm_w)[c - 1] = f2bf(s);
+  else ((float*)p.dnorm_w)[c - 1] = s;
+}
+
+// 2. dQ.  Workgroup = (batch, head, 128 queries), wave = 32 queries, as the forward pass: S_i^T = K_i Q_i^T, dP^T = V dO^T (keys x queries),
+//    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.
+template <typename T, int NB> constexpr int dq_lds() { return 2 * 32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES); }
+
+template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB <= (sizeof(T) == 2 ? 4 : 2) ? 2 : 1)) void diff_attn_bwd_dq_kernel(tfpp_diff_attn_params p) {
+  constexpr int KT = 32, NT = 256, CD = (NB + 1) / 2;
+  typedef Img<T, CD> ImgK;
+  typedef Img<T, NB> ImgV;
+  constexpr int K_BYTES = KT * ImgK::ROW_BYTES, V_BYTES = KT * ImgV::ROW_BYTES, BUF = 2 * K_BYTES + V_BYTES;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int tiles = (p.Tq + QB - 1) / QB;
+  int bh, tile;
+  place(p.B * p.H, tiles, bh, tile);
+  if (p.causal) tile = tiles - 1 - tile;
+  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv), dvs = (p.dv + 7) & ~7;
+  const Seq sq = sequence(p, b);
+  const int w0 = tile * QB + wave * 32, qi = w0 + (lane & 31), qc = qi < p.Tq ? qi : p.Tq - 1;
+  const long row = ((long)b * p.H + h) * p.Tq + qc, rows = (long)p.B * p.H * p.Tq;
+  const T* kb = (const T*)p.k + (long)b * p.k_s[0] + (long)hk * p.k_s[2];
+  const T* vb = (const T*)p.v + (long)b * p.v_s[0] + (long)hk * p.v_s[2];
+  constexpr bool HOLD = sizeof(T) == 2 || NB < 5;  // wide fp32 heads do not fit the registers: Q and dO are read again for every tile
+  const T* qrow = (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2];
+  Frag8<T> q[2][HOLD ? NB : 1], dof[HOLD ? 2 * NB : 1];
+  if constexpr (HOLD)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][ks]);
+  if constexpr (HOLD)
+#pragma unroll
+    for (int ks = 0; ks < 2 * NB; ++ks) load_frag<T, true>((const T*)p.d_o + row * dvs, ks * 16 + half * 8, dvs, true, dof[ks]);
+  const float lse[2] = {p.lse[row], p.lse[rows + row]}, delta[2] = {p.delta[row], p.delta[rows + row]};
+  const float lam = p.lam[p.n_lam > 1 ? h : 0], c = p.scale * LOG2E;
+  const int last = tile * QB + QB < p.Tq ? tile * QB + QB : p.Tq;
+  int end = sq.len;
+  if (p.causal) end = sq.start + last < end ? sq.start + last : end;
+  const int steps = end > 0 ? (end + KT - 1) / KT : 0;
+  f32x16_t dq[2][CD];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int n = 0; n < CD; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[i][n][r] = 0.f;
+  auto fill = [&](int step, unsigned long long bits) {
+    unsigned char* buf = smem + (step & 1) * BUF;
+    const long j0 = (long)step * KT;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, bits, tid);
+    ImgV::template fill<KT, VECTOR, NT>(buf + 2 * K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, bits, tid);
+  };
+  unsigned long long bits = 0;
+  if (steps > 0) {
+    bits = key_bits(p, b, 0, sq.len, lane);
+    fill(0, bits);
+  }
+  for (int s = 0; s < steps; ++s) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const unsigned long long cur = bits & low_bits(KT);
+    if (s + 1 < steps) {
+      bits = key_bits(p, b, (s + 1) * KT, sq.len, lane);
+      fill(s + 1, bits);
+    }
+    const int j0 = s * KT;
+    if ((p.causal && sq.start + w0 + 32 - j0 <= 0) || cur == 0) continue;
+    const bool masked = cur != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
+    const unsigned vis = (unsigned)(p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur) >> (4 * half);
+    const unsigned char* buf = smem + (s & 1) * BUF;
+    f32x16_t sc[2], dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[0][r] = sc[1][r] = dp[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int ks = 0; ks < NB; ++ks) {
+        Frag8<T> a;
+        ImgK::rows(buf + i * K_BYTES, lane & 31, ks, half, a);
+        if constexpr (!HOLD) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][0]);
+        mma(a, q[i][HOLD ? ks : 0], sc[i]);
+      }
+#pragma unroll
+    for (int ks = 0; ks < 2 * NB; ++ks) {
+      Frag8<T> a;
+      ImgV::rows(buf + 2 * K_BYTES, lane & 31, ks, half, a);
+      if constexpr (!HOLD) load_frag<T, true>((const T*)p.d_o + row * dvs, ks * 16 + half * 8, dvs, true, dof[0]);
+      mma(a, dof[HOLD ? ks : 0], dp);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float p0 = __builtin_amdgcn_exp2f(fmaf(sc[0][r], c, -lse[0])), p1 = __builtin_amdgcn_exp2f(fmaf(sc[1][r], c, -lse[1]));
+      if (masked) {
+        const bool keep = (vis >> (8 * (r >> 2) + (r & 3))) & 1u;
+        p0 = keep ? p0 : 0.f;
+        p1 = keep ? p1 : 0.f;
+      }
+      sc[0][r] = p0 * (dp[r] - delta[0]);
+      sc[1][r] = p1 * (dp[r] - delta[1]) * -lam;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Frag8<T> ds;
+        to_frag(sc[i], t, ds);
+#pragma unroll
+        for (int n = 0; n < CD; ++n) {
+          Frag8<T> a;
+          ImgK::cols(buf + i * K_BYTES, 16 * t, n, lane, a);
+          mma(a, ds, dq[i][n]);
+        }
+      }
+  }
+  if (qi < p.Tq) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      T* out = (T*)p.dq_out + (long)b * p.dq_s[0] + (long)qi * p.dq_s[1] + (long)h * p.dq_s[2] + (long)i * p.dq_s[3];
+#pragma unroll
+      for (int n = 0; n < CD; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          store4<T>(out, n * 32 + 8 * g + 4 * half, p.d, p.dq_vec, p.scale * dq[i][n][4 * g], p.scale * dq[i][n][4 * g + 1], p.scale * dq[i][n][4 * g + 2],
+                    p.scale * dq[i][n][4 * g + 3]);
+    }
+  }
+}
+
+// 3. dK, dV.  Workgroup = (batch, key / value head, 128 keys), wave = 32 keys, lane l and l + 32 = one key: S_i = Q_i K_i^T and dP = dO V^T
+//    (queries x keys), dV^T += dO^T (P_1 - lambda P_2), dK_i^T += Q_i^T dS_i, over all queries of all heads that share the key / value head.
+//    Wide heads: the accumulators of all three do not fit one wave's registers, so dK_1, dK_2 (PART_DK, the map in the grid's y) and dV (PART_DV) are
+//    separate workgroups; S and dP are computed again (3 / 2 of the flop).
+enum { PART_ALL, PART_DK, PART_DV };
+template <typename T, int NB> constexpr bool dkv_split() { return NB >= (sizeof(T) == 2 ? 5 : 4); }
+template <typename T, int NB> constexpr int dkv_lds() { return 2 * (32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + 4 * 32 * 4); }
+
+template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds__(256, (PART == PART_ALL ? NB <= (sizeof(T) == 2 ? 2 : 1) : NB <= (sizeof(T) == 2 ? 5 : 4)) ? 2 : 1) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
+  constexpr int QT = 32, NT = 256, MAPS = PART == PART_DK ? 1 : 2, CD = (NB + 1) / 2;
+  typedef Img<T, CD> ImgQ;
+  typedef Img<T, NB> ImgO;
+  constexpr int Q_BYTES = QT * ImgQ::ROW_BYTES, O_BYTES = QT * ImgO::ROW_BYTES, BUF = 2 * Q_BYTES + O_BYTES + 4 * QT * 4;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int tiles = (p.Tk + QB - 1) / QB, group = p.H / p.Hkv;
+  int bh, tile;
+  place(p.B * p.Hkv, tiles, bh, tile);
+  const int b = bh / p.Hkv, hk = bh % p.Hkv, dvs = (p.dv + 7) & ~7;
+  const Seq sq = sequence(p, b);
+  const int w0 = tile * QB + wave * 32, kj = w0 + (lane & 31);
+  bool seen = kj < sq.len;
+  if (seen && p.key_mask) seen = p.key_mask[(long)b * p.ld_mask + kj] != 0;
+  const int kc = kj < p.Tk ? kj : p.Tk - 1;
+  constexpr bool HOLD = sizeof(T) == 2 || NB < 4, WANT_DK = PART != PART_DV, WANT_DV = PART != PART_DK;
+  const int map0 = PART == PART_DK ? (int)blockIdx.y : 0;  // wide fp32 heads do not fit the registers: K and V are read again for every tile
+  const T* krow = (const T*)p.k + (long)b * p.k_s[0] + (long)kc * p.k_s[1] + (long)hk * p.k_s[2];
+  const T* vrow = (const T*)p.v + (long)b * p.v_s[0] + (long)kc * p.v_s[1] + (long)hk * p.v_s[2];
+  Frag8<T> k[MAPS][HOLD ? NB : 1], v[HOLD && WANT_DK ? 2 * NB : 1];
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i)
+#pragma unroll
+      for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, seen, k[i][ks]);
+    if constexpr (WANT_DK)
+#pragma unroll
+      for (int ks = 0; ks < 2 * NB; ++ks) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, seen, v[ks]);
+  }
+  f32x16_t dk[WANT_DK ? MAPS : 1][CD], dv[WANT_DV ? NB : 1];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+#pragma unroll
+    for (int n = 0; n < CD; ++n)
+#pragma unroll
+      for (int i = 0; i < (WANT_DK ? MAPS : 1); ++i) dk[i][n][r] = 0.f;
+#pragma unroll
+    for (int n = 0; n < (WANT_DV ? NB : 1); ++n) dv[n][r] = 0.f;
+  }
+  const float c = p.scale * LOG2E;
+  const long rows = (long)p.B * p.H * p.Tq;
+  // causal: query i sees the workgroup's first key from i = first key - start on
+  int q_lo = 0;
+  if (p.causal && tile * QB > sq.start) q_lo = (tile * QB - sq.start) / QT * QT;
+  const bool any = tile * QB < sq.len && q_lo < p.Tq;
+  const int per = any ? (p.Tq - q_lo + QT - 1) / QT : 0, steps = per * group;
+
+  auto fill = [&](int step) {
+    unsigned char* buf = smem + (step & 1) * BUF;
+    const int h = hk * group + step / per, q0 = q_lo + step % per * QT;
+    const unsigned long long bits = low_bits(p.Tq - q0);
+    const T* qb = (const T*)p.q + (long)b * p.q_s[0] + (long)q0 * p.q_s[1] + (long)h * p.q_s[2];
+    const long row = ((long)b * p.H + h) * p.Tq + q0;
+#pragma unroll
+    for (int i = map0; i < map0 + MAPS; ++i) ImgQ::template fill<QT, VECTOR, NT>(buf + i * Q_BYTES, qb + i * p.q_s[3], p.q_s[1], p.d, bits, tid);
+    ImgO::template fill<QT, true, NT>(buf + 2 * Q_BYTES, (const T*)p.d_o + row * dvs, dvs, dvs, bits, tid);
+    if (tid < 4 * QT) {  // lse_1, lse_2, delta_1, delta_2 of the tile; queries behind the last: +inf, so that P = 0
+      const int a = tid / QT, t = tid % QT;
+      const bool in = q0 + t < p.Tq;
+      const float* src = a < 2 ? p.lse : p.delta;
+      reinterpret_cast<float*>(buf + 2 * Q_BYTES + O_BYTES)[tid] = in ? src[(a & 1) * rows + row + t] : (a < 2 ? INFINITY : 0.f);
+    }
+  };
+  if (steps > 0) fill(0);
+  for (int s = 0; s < steps; ++s) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (s + 1 < steps) fill(s + 1);
+    const int h = hk * group + s / per, q0 = q_lo + s % per * QT;
+    if (p.causal && sq.start + q0 + QT - 1 < w0) continue;  // no query of the tile sees a key of this wave
+    const bool diag = p.causal && sq.start + q0 < w0 + 31;
+    const float lam = p.lam[p.n_lam > 1 ? h : 0];
+    const unsigned char* buf = smem + (s & 1) * BUF;
+    const float* st = reinterpret_cast<const float*>(buf + 2 * Q_BYTES + O_BYTES);
+    f32x16_t sc[MAPS], dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dp[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i) sc[i][r] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i)
+#pragma unroll
+      for (int ks = 0; ks < NB; ++ks) {
+        Frag8<T> a;
+        ImgQ::rows(buf + (map0 + i) * Q_BYTES, lane & 31, ks, half, a);
+        if constexpr (!HOLD) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, seen, k[i][0]);
+        mma(a, k[i][HOLD ? ks : 0], sc[i]);
+      }
+    if constexpr (WANT_DK)
+#pragma unroll
+      for (int ks = 0; ks < 2 * NB; ++ks) {
+        Frag8<T> a;
+        ImgO::rows(buf + 2 * Q_BYTES, lane & 31, ks, half, a);
+        if constexpr (!HOLD) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, seen, v[0]);
+        mma(a, v[HOLD ? ks : 0], dp);
+      }
+    f32x16_t pd;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int t0 = 8 * g + 4 * half;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pd[4 * g + e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i) {
+        const int map = map0 + i;
+        const float4 l4 = *reinterpret_cast<const float4*>(st + map * QT + t0), d4 = *reinterpret_cast<const float4*>(st + (2 + map) * QT + t0);
+        const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w}, sign = map ? -lam : 1.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          float pr = __builtin_amdgcn_exp2f(fmaf(sc[i][r], c, -ls[e]));
+          pr = seen && (!diag || kj <= sq.start + q0 + t0 + e) ? sign * pr : 0.f;
+          pd[r] += pr;
+          sc[i][r] = pr * (dp[r] - de[e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      Frag8<T> f;
+      if constexpr (WANT_DV) {
+        to_frag(pd, t, f);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          Frag8<T> a;
+          ImgO::cols(buf + 2 * Q_BYTES, 16 * t, n, lane, a);
+          mma(a, f, dv[n]);
+        }
+      }
+      if constexpr (WANT_DK)
+#pragma unroll
+        for (int i = 0; i < MAPS; ++i) {
+          to_frag(sc[i], t, f);
+#pragma unroll
+          for (int n = 0; n < CD; ++n) {
+            Frag8<T> a;
+            ImgQ::cols(buf + (map0 + i) * Q_BYTES, 16 * t, n, lane, a);
+            mma(a, f, dk[i][n]);
+          }
+        }
+    }
+  }
+  if (kj >= p.Tk) return;  // (keys that nobody sees get zeros)
+  if constexpr (WANT_DV) {
+    T* out = (T*)p.dv_out + (long)b * p.dv_s[0] + (long)kj * p.dv_s[1] + (long)hk * p.dv_s[2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        store4<T>(out, n * 32 + 8 * g + 4 * half, p.dv, p.dv_vec, dv[n][4 * g], dv[n][4 * g + 1], dv[n][4 * g + 2], dv[n][4 * g + 3]);
+  }
+  if constexpr (WANT_DK)
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) {
+      T* out = (T*)p.dk_out + (long)b * p.dk_s[0] + (long)kj * p.dk_s[1] + (long)hk * p.dk_s[2] + (long)(map0 + i) * p.dk_s[3];
+#pragma unroll
+      for (int n = 0; n < CD; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          store4<T>(out, n * 32 + 8 * g + 4 * half, p.d, p.dk_vec, p.scale * dk[i][n][4 * g], p.scale * dk[i][n][4 * g + 1], p.scale * dk[i][n][4 * g + 2],
+                    p.scale * dk[i][n][4 * g + 3]);
+    }
+}
+
+// lambda[h] = exp(lq1 . lk1) - exp(lq2 . lk2) + init of the four learned vectors of a head (one wave a head), and its gradient
+__device__ __forceinline__ float vec_at(const void* p, long i, int is_bf16) { return is_bf16 ? bf2f(((const bf16_t*)p)[i]) : ((const float*)p)[i]; }
+__device__ __forceinline__ void exps(const void* q1, const void* k1, const void* q2, const void* k2, int h, int d, int is_bf16, float& e1, float& e2) {
+  float s1 = 0.f, s2 = 0.f;
+  for (int i = threadIdx.x; i < d; i += 64) {
+    const long n = (long)h * d + i;
+    s1 += vec_at(q1, n, is_bf16) * vec_at(k1, n, is_bf16);
+    s2 += vec_at(q2, n, is_bf16) * vec_at(k2, n, is_bf16);
+  }
+  e1 = expf(wave_sum(s1));
+  e2 = expf(wave_sum(s2));
+}
+__global__ __launch_bounds__(64) void diff_lambda_fwd_kernel(const void* q1, const void* k1, const void* q2, const void* k2, float init, float* lam, int d, int is_bf16) {
+  float e1, e2;
+  exps(q1, k1, q2, k2, blockIdx.x, d, is_bf16, e1, e2);
+  if (threadIdx.x == 0) lam[blockIdx.x] = e1 - e2 + init;
+}
+template <typename T> __global__ __launch_bounds__(64) void diff_lambda_bwd_kernel(const float* dlam, const T* q1, const T* k1, const T* q2, const T* k2, T* dq1, T* dk1, T* dq2,
+                                                                                 T* dk2, int d) {
+  typedef ElemTraits<T> E;
+  float e1, e2;
+  exps(q1, k1, q2, k2, blockIdx.x, d, E::DT == TFPP_BF16, e1, e2);
+  const float g1 = dlam[blockIdx.x] * e1, g2 = -dlam[blockIdx.x] * e2;
+  for (int i = threadIdx.x; i < d; i += 64) {
+    const long n = (long)blockIdx.x * d + i;
+    dq1[n] = E::from_f(g1 * E::to_f(k1[n]));
+    dk1[n] = E::from_f(g1 * E::to_f(q1[n]));
+    dq2[n] = E::from_f(g2 * E::to_f(k2[n]));
+    dk2[n] = E::from_f(g2 * E::to_f(q2[n]));
+  }
+}
+
+bool strides_vec(const int64_t* s, int n, int vec) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] % vec) return false;
+  return true;
+}
+bool valid(const tfpp_diff_attn_params& p, int dtype) {
+  return (dtype == TFPP_F32 || dtype == TFPP_BF16) && p.q && p.k && p.v && p.lam && p.B >= 1 && p.H >= 1 && p.Hkv >= 1 && p.H % p.Hkv == 0 && p.Tq >= 1 && p.Tk >= 1 &&
+         p.d >= 1 && p.d <= 128 && p.dv >= 1 && p.dv <= 256 && (p.n_lam == 1 || p.n_lam == p.H) && p.scale > 0.f && std::isfinite(p.scale) && (!p.norm || p.eps > 0.f) &&
+         p.Tq < (1 << 30) && p.Tk < (1 << 30) && (long)p.B * p.H < (1l << 24);
+}
+// Can q, k, v be read 16 bytes at a time?
+bool vector_rows(const tfpp_diff_attn_params& p, int vec) {
+  const int64_t far = (1 << 24) * (int64_t)vec / 16;  // 16 MB from token to token: a tile's offsets fit 32 bits
+  return p.d % vec == 0 && p.dv % vec == 0 && p.q_s[1] <= far && p.k_s[1] <= far && p.v_s[1] <= far && !(((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15) && strides_vec(p.q_s, 4, vec) && strides_vec(p.k_s, 4, vec) &&
+         strides_vec(p.v_s, 3, vec);
+}
+// 32 / 16-byte channel quads of an output
+bool quad(const void* ptr, const int64_t* s, int n, int esz) { return !((uintptr_t)ptr & (4 * esz - 1)) && strides_vec(s, n, 4); }
+
+template <typename K> int lds_limit(K* kernel, int bytes, unsigned long long* done) {
+  if (bytes > 64 * 1024 && tfpp_first_use_on_this_device(done)) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) {
+      *done = 0;
+      return -(int)e;
+    }
+  }
+  return 0;
+}
+
+template <typename K> int start(K* kernel, dim3 grid, int threads, int lds, unsigned long long* done, const tfpp_diff_attn_params& p, hipStream_t st) {
+  const int rc = lds_limit(kernel, lds, done);
+  if (rc) return rc;
+  hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, st, p);
+  TFPP_CHECK_LAUNCH();
+  return 0;
+}
+
+enum { STEP_FWD, STEP_DQ, STEP_DKV };
+template <typename T, int NB, bool VECTOR> int launch(const tfpp_diff_attn_params& p, int step, hipStream_t st) {
+  static unsigned long long done[4] = {0, 0, 0, 0};
+  const int qb = step == STEP_FWD ? fwd_queries<T, NB>() : QB;
+  const long tiles = ((step == STEP_DKV ? p.Tk : p.Tq) + qb - 1) / qb, n = tiles * p.B * (step == STEP_DKV ? p.Hkv : p.H);
+  if (n > 0x7fffffffl) return TFPP_EINVAL;
+  const dim3 grid((unsigned)n);
+  if (step == STEP_FWD) return start(diff_attn_fwd_kernel<T, NB, VECTOR>, grid, fwd_threads<T, NB>(), fwd_lds<T, NB>(), &done[0], p, st);
+  if (step == STEP_DQ) return start(diff_attn_bwd_dq_kernel<T, NB, VECTOR>, grid, 256, dq_lds<T, NB>(), &done[1], p, st);
+  if constexpr (dkv_split<T, NB>()) {
+    const int rc = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DK>, dim3((unsigned)n, 2), 256, dkv_lds<T, NB>(), &done[2], p, st);
+    return rc ? rc : start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DV>, grid, 256, dkv_lds<T, NB>(), &done[3], p, st);
+  } else {
+    return start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_ALL>, grid, 256, dkv_lds<T, NB>(), &done[2], p, st);
+  }
+}
+// channels are padded to 16 NB / 32 NB: the width classes of the fusion transformers' heads (d 9, 27, 72) and the powers of two
+template <typename T> int dispatch(const tfpp_diff_attn_params& p, int step, hipStream_t st) {
+  const bool v = vector_rows(p, ElemTraits<T>::VEC);
+  const int need = (p.d + 15) / 16 > (p.dv + 31) / 32 ? (p.d + 15) / 16 : (p.dv + 31) / 32;
+#define DA_GO(NB) (v ? launch<T, NB, true>(p, step, st) : launch<T, NB, false>(p, step, st))
+  if (need <= 1) return DA_GO(1);
+  if (need <= 2) return DA_GO(2);
+  if (need <= 4) return DA_GO(4);
+  if (need <= 5) return DA_GO(5);
+  return DA_GO(8);
+#undef DA_GO
+}
+int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass for each head: 64 rows each at least, about 1024 in all
+  const long rows = (long)p.B * p.Tq;
+  long n = 1024 / p.H > 1 ? 1024 / p.H : 1;
+  if (n > (rows + 63) / 64) n = (rows + 63) / 64;
+  return (int)n;
+}
+}  // namespace
+
+extern "C" int tfpp_diff_attn_fwd(const tfpp_diff_attn_params* pp, int dtype, void* stream) {
+  if (!pp || !valid(*pp, dtype) || !pp->out || (pp->o1 != nullptr) != (pp->o2 != nullptr)) return TFPP_EINVAL;
+  tfpp_diff_attn_params p = *pp;
+  p.out_vec = quad(p.out, p.o_s, 3, dtype == TFPP_F32 ? 4 : 2);
+  return dtype == TFPP_F32 ? dispatch<float>(p, STEP_FWD, (hipStream_t)stream) : dispatch<bf16_t>(p, STEP_FWD, (hipStream_t)stream);
+}
+
+extern "C" int tfpp_diff_attn_bwd_partial_floats(const tfpp_diff_attn_params* p, int64_t* out) {
+  if (!p || !out || p->B < 1 || p->H < 1 || p->Tq < 1 || p->dv < 1) return TFPP_EINVAL;
+  *out = (int64_t)row_blocks(*p) * p->H * (1 + p->dv);
+  return 0;
+}
+
+extern "C" int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* pp, int dtype, void* stream) {
+  if (!pp || !valid(*pp, dtype)) return TFPP_EINVAL;
+  tfpp_diff_attn_params p = *pp;
+  if (!p.dout || !p.o1 || !p.o2 || !p.lse || !p.d_o || !p.delta || !p.partial || !p.dlam || !p.dq_out || !p.dk_out || !p.dv_out || (p.norm_w && !p.dnorm_w)) return TFPP_EINVAL;
+  if (p.H > 65535 || (((uintptr_t)p.o1 | (uintptr_t)p.o2 | (uintptr_t)p.d_o) & 15)) return TFPP_EINVAL;
+  const int esz = dtype == TFPP_F32 ? 4 : 2;
+  p.dq_vec = quad(p.dq_out, p.dq_s, 4, esz);
+  p.dk_vec = quad(p.dk_out, p.dk_s, 4, esz);
+  p.dv_vec = quad(p.dv_out, p.dv_s, 3, esz);
+  hipStream_t st = (hipStream_t)stream;
+  const int blocks = row_blocks(p);
+  int lpr = 1;
+  while (lpr * 4 < ((p.dv + 7) & ~7)) lpr <<= 1;
+  const dim3 sums(p.n_lam + (p.norm_w ? p.dv : 0));
+  if (dtype == TFPP_F32) {
+    hipLaunchKernelGGL(diff_attn_bwd_rows_kernel<float>, dim3(blocks, p.H), dim3(256), 0, st, p, lpr);
+    hipLaunchKernelGGL(diff_attn_bwd_sum_kernel<float>, sums, dim3(256), 0, st, p, blocks);
+  } else {
+    hipLaunchKernelGGL(diff_attn_bwd_rows_kernel<bf16_t>, dim3(blocks, p.H), dim3(256), 0, st, p, lpr);
+    hipLaunchKernelGGL(diff_attn_bwd_sum_kernel<bf16_t>, sums, dim3(256), 0, st, p, blocks);
+  }
+  TFPP_CHECK_LAUNCH();
+  for (int step : {STEP_DQ, STEP_DKV}) {
+    const int rc = dtype == TFPP_F32 ? dispatch<float>(p, step, st) : dispatch<bf16_t>(p, step, st);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
+extern "C" int tfpp_diff_lambda(const void* lq1, const void* lk1, const void* lq2, const void* lk2, float init, float* lam, int n, int d, int dtype, void* stream) {
+  if (!lq1 || !lk1 || !lq2 || !lk2 || !lam || n < 1 || d < 1 || (dtype != TFPP_F32 && dtype != TFPP_BF16)) return TFPP_EINVAL;
+  hipLaunchKernelGGL(diff_lambda_fwd_kernel, dim3(n), dim3(64), 0, (hipStream_t)stream, lq1, lk1, lq2, lk2, init, lam, d, dtype == TFPP_BF16);
+  TFPP_CHECK_LAUNCH();
+  return 0;
+}
+
+extern "C" int tfpp_diff_lambda_bwd(const float* dlam, const void* lq1, const void* lk1, const void* lq2, const void* lk2, void* dlq1, void* dlk1, void* dlq2, void* dlk2, int n,
+                                    int d, int dtype, void* stream) {
+  if (!dlam || !lq1 || !lk1 || !lq2 || !lk2 || !dlq1 || !dlk1 || !dlq2 || !dlk2 || n < 1 || d < 1 || (dtype != TFPP_F32 && dtype != TFPP_BF16)) return TFPP_EINVAL;
+  if (dtype == TFPP_F32)
+    hipLaunchKernelGGL(diff_lambda_bwd_kernel<float>, dim3(n), dim3(64), 0, (hipStream_t)stream, dlam, (const float*)lq1, (const float*)lk1, (const float*)lq2,
+                       (const float*)lk2, (float*)dlq1, (float*)dlk1, (float*)dlq2, (float*)dlk2, d);
+  else
+    hipLaunchKernelGGL(diff_lambda_bwd_kernel<bf16_t>, dim3(n), dim3(64), 0, (hipStream_t)stream, dlam, (const bf16_t*)lq1, (const bf16_t*)lk1, (const bf16_t*)lq2,
+                       (const bf16_t*)lk2, (bf16_t*)dlq1, (bf16_t*)dlk1, (bf16_t*)dlq2, (bf16_t*)dlk2, d);
+  TFPP_CHECK_LAUNCH();
+  return 0;
+}

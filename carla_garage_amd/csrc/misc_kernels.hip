@@ -665,7 +665,7 @@ extern "C" int tfpp_source_hash(uint64_t* out) {
 }
 
 extern "C" int tfpp_struct_sizes(int* out, int n) {
-  if (!out || n < 7) return TFPP_EINVAL;
+  if (!out || n < 8) return TFPP_EINVAL;
   out[0] = (int)sizeof(tfpp_conv_params);
   out[1] = (int)sizeof(tfpp_wgrad_params);
   out[2] = (int)sizeof(tfpp_bgemm_params);
@@ -673,7 +673,8 @@ extern "C" int tfpp_struct_sizes(int* out, int n) {
   out[4] = (int)sizeof(tfpp_attn_params);
   out[5] = (int)sizeof(tfpp_bn_rows);
   out[6] = (int)sizeof(tfpp_block_norm_params);
-  return 7;
+  out[7] = (int)sizeof(tfpp_diff_attn_params);
+  return 8;
 }
 
 // order-independent 64-bit hash of a buffer (debugging aid: which tensor differs between two replays of one hipGraph?)

@@ -5,7 +5,7 @@ import ctypes
 
 import torch
 
-from ._lib import (lib, ConvParams, WgradParams, BgemmParams, PackDesc, AttnParams, BnRows, BlockNormParams, F32, BF16, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_GELU,
+from ._lib import (lib, ConvParams, WgradParams, BgemmParams, PackDesc, AttnParams, BnRows, BlockNormParams, DiffAttnParams, F32, BF16, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_GELU,
                    ACT_TANH)
 
 import os as _os
@@ -1500,3 +1500,206 @@ def block_norm_bwd(dy, dh, ctx, into=None):
         lib.profiler.tag('block_norm_bwd', 0.0, float(rows * C * x.element_size() * (4 + (dy is not None) + (dh is not None) + 2 * (ctx.mode == 2))))
       lib.tfpp_block_norm_bwd(ctypes.byref(p), dt(x), stream())
   return out
+
+
+# ------------------------------------------------------------------------------------------------ differential attention
+def diff_lambda(lq1, lk1, lq2, lk2, init):
+  """lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + init of learned vectors [n, d] (or [d]: one lambda for all heads), fp32 or bf16 -> fp32 [n]."""
+  n, d = _lambda_vectors(lq1, lk1, lq2, lk2)
+  with torch.cuda.device(lq1.device):
+    lam = torch.empty(n, device=lq1.device, dtype=torch.float32)
+    lib.tfpp_diff_lambda(ptr(lq1), ptr(lk1), ptr(lq2), ptr(lk2), float(init), ptr(lam), n, d, dt(lq1), stream())
+  return lam
+
+
+def diff_lambda_bwd(dlam, lq1, lk1, lq2, lk2):
+  """Gradients of the four vectors from that of lambda ([n] fp32)."""
+  n, d = _lambda_vectors(lq1, lk1, lq2, lk2)
+  one_device(lq1, dlam)
+  if dlam.dtype != torch.float32 or dlam.numel() != n or not dlam.is_contiguous():
+    raise ValueError(f'dlam: {n} contiguous fp32 values, got {dlam.dtype} {tuple(dlam.shape)}')
+  with torch.cuda.device(lq1.device):
+    out = [torch.empty_like(t) for t in (lq1, lk1, lq2, lk2)]
+    lib.tfpp_diff_lambda_bwd(ptr(dlam), ptr(lq1), ptr(lk1), ptr(lq2), ptr(lk2), *[ptr(t) for t in out], n, d, dt(lq1), stream())
+  return out
+
+
+def _lambda_vectors(*ts):
+  one_device(*ts)
+  t = ts[0]
+  if t.dtype not in (torch.float32, torch.bfloat16):
+    raise TypeError(f'lambda vectors are fp32 or bf16, got {t.dtype}')
+  if t.dim() not in (1, 2) or t.numel() == 0 or any(x.shape != t.shape or x.dtype != t.dtype or not x.is_contiguous() for x in ts):
+    raise ValueError('lambda vectors: four contiguous tensors of one type and shape, [n, d] or [d]')
+  return (1, t.shape[0]) if t.dim() == 1 else tuple(t.shape)
+
+
+class DiffAttnContext:
+  """What diff_attn_bwd needs of its forward pass: P_1 V, P_2 V, the rows' log-sums and the options."""
+  __slots__ = ('o1', 'o2', 'lse', 'norm_weight', 'opt', 'kv_len', 'q_start', 'key_mask', 'shape')
+
+
+def _last_contiguous(t, name, dims):
+  if t.dim() != dims:
+    raise ValueError(f'{name} has {t.dim()} dimensions, expected {dims}')
+  if t.shape[-1] > 1 and t.stride(-1) != 1:
+    raise ValueError(f'{name}: the last dimension has to be contiguous')
+  return t.stride()[:-1]
+
+
+def _disjoint(t, name):
+  """Outputs: no element of ``t`` may share memory with another one (expanded tensors, overlapping windows)."""
+  want = 1
+  for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+    if st < want:
+      raise ValueError(f'{name}: elements overlap in memory (strides {t.stride()})')
+    want = st * n
+
+
+def _int_rows(t, n, dev, name):
+  if t is not None and (t.dtype != torch.int32 or t.numel() != n or t.dim() != 1 or not t.is_contiguous() or t.device != dev):
+    raise ValueError(f'{name}: {n} contiguous int32 values on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}')
+
+
+def _diff_attn_check(q, k, v, lam):
+  dev = one_device(q, k, v, lam)
+  if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    raise TypeError(f'q, k and v share one type, fp32 or bf16: got {q.dtype}, {k.dtype}, {v.dtype}')
+  qs, ks, vs = _last_contiguous(q, 'q', 5), _last_contiguous(k, 'k', 5), _last_contiguous(v, 'v', 4)
+  B, Tq, H, two, d = q.shape
+  Tk, Hkv, dv = k.shape[1], k.shape[2], v.shape[3]
+  if two != 2 or tuple(k.shape) != (B, Tk, Hkv, 2, d) or tuple(v.shape) != (B, Tk, Hkv, dv):
+    raise ValueError(f'shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: expected [B, Tq, H, 2, d], [B, Tk, Hkv, 2, d], [B, Tk, Hkv, dv]')
+  if not (1 <= d <= 128 and 1 <= dv <= 256):
+    raise ValueError(f'differential attention: d 1 to 128 and dv 1 to 256, got d = {d}, dv = {dv}')
+  if H < 1 or Hkv < 1 or H % Hkv:
+    raise ValueError(f'{H} query heads over {Hkv} key / value heads')
+  if max(Tq, Tk) >= 1 << 30 or B * H >= 1 << 24:
+    raise ValueError('differential attention: too many tokens or heads')
+  if lam.dtype != torch.float32 or lam.numel() not in (1, H) or not lam.is_contiguous():
+    raise ValueError(f'lam: 1 or {H} contiguous fp32 values, got {lam.dtype} {tuple(lam.shape)}')
+  return dev, qs, ks, vs, (B, Tq, Tk, H, Hkv, d, dv)
+
+
+def _diff_attn_params(q, k, v, lam, qs, ks, vs, shape, norm_weight, key_mask, kv_len, q_start, opt):
+  p = DiffAttnParams()
+  p.B, p.Tq, p.Tk, p.H, p.Hkv, p.d, p.dv = shape
+  p.q, p.k, p.v, p.lam, p.n_lam = q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), lam.numel()
+  p.q_s[:], p.k_s[:], p.v_s[:] = qs, ks, vs
+  p.scale, p.causal, p.norm, p.eps, p.out_scale, p.q_start_all = opt
+  p.norm_w, p.norm_w_bf16 = ptr(norm_weight), int(norm_weight is not None and norm_weight.dtype == torch.bfloat16)
+  p.kv_len, p.q_start, p.key_mask = ptr(kv_len), ptr(q_start), ptr(key_mask)
+  p.ld_mask = key_mask.stride(0) if key_mask is not None else 0
+  return p
+
+
+def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_len=None, key_mask=None, norm=True, norm_weight=None, norm_eps=1e-5, out_scale=1.0,
+                  save=False, out=None):
+  """Differential attention: P_i = softmax(scale q_i k_i^T) for the two halves of every head, O = (P_1 - lam P_2) v, each head's result normalised:
+  out = out_scale * norm_weight * O / sqrt(mean(O^2) + norm_eps)   (norm=False: out_scale * O).    -> (out [B, Tq, H, dv], context or None)
+    q [B, Tq, H, 2, d], k [B, Tk, Hkv, 2, d], v [B, Tk, Hkv, dv]: fp32 or bf16, d <= 128, dv <= 256, H a multiple of Hkv (query head h reads head
+    h // (H // Hkv)); any strides with a contiguous last dimension (slices of a fused projection, [B, H, T, ...] caches seen through permute).
+    lam: fp32 [H] or [1].  norm_weight: [dv], fp32 or bf16, or None.  scale > 0, default d ** -0.5.
+  Which keys a query sees: kv_len (int32 [B] on the device) leaves out keys >= kv_len[b]; key_mask (bool or uint8 [B, Tk]) those where it is 0; causal
+  those with key > q_start + query, q_start an int, int32 [B] on the device, or None for Tk - Tq.  k and v of keys left out by kv_len or key_mask are
+  not read and may hold anything; the other values have to be finite.  A query that sees no key gives zeros.
+  New tokens against a cache: q [B, 1, ...], k and v the whole cache, kv_len the tokens it holds (the new ones among them); for several new tokens
+  causal=True and q_start = kv_len - Tq.
+  save=True keeps what diff_attn_bwd needs.  ``out``: written in place of a new tensor, any strides that do not overlap."""
+  dev, qs, ks, vs, shape = _diff_attn_check(q, k, v, lam)
+  B, Tq, Tk, H, Hkv, d, dv = shape
+  if norm_weight is not None and (norm_weight.dtype not in (torch.float32, torch.bfloat16) or norm_weight.numel() != dv or not norm_weight.is_contiguous() or
+                                  norm_weight.device != dev or not norm):
+    raise ValueError(f'norm_weight: {dv} contiguous fp32 or bf16 values on {dev}, with norm=True')
+  scale = d ** -0.5 if scale is None else float(scale)
+  if not 0.0 < scale < float('inf'):
+    raise ValueError(f'scale has to be positive and finite, got {scale}')
+  if norm and not norm_eps > 0.0:
+    raise ValueError(f'norm_eps has to be positive, got {norm_eps}')
+  _int_rows(kv_len, B, dev, 'kv_len')
+  start_all, start_t = Tk - Tq, None
+  if torch.is_tensor(q_start):
+    _int_rows(q_start, B, dev, 'q_start')
+    start_t = q_start
+  elif q_start is not None:
+    start_all = int(q_start)
+    if abs(start_all) >= 1 << 30:
+      raise ValueError(f'q_start out of range: {start_all}')
+  if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != (B, Tk) or (Tk > 1 and key_mask.stride(1) != 1) or
+                               key_mask.device != dev):
+    raise ValueError(f'key_mask: bool or uint8 {(B, Tk)} on {dev} with contiguous rows, got {key_mask.dtype} {tuple(key_mask.shape)}')
+  with torch.cuda.device(dev):
+    if out is None:
+      out = torch.empty((B, Tq, H, dv), device=dev, dtype=q.dtype)
+    else:
+      if tuple(out.shape) != (B, Tq, H, dv) or out.dtype != q.dtype or out.device != dev:
+        raise ValueError(f'out: {q.dtype} {(B, Tq, H, dv)} on {dev}, got {out.dtype} {tuple(out.shape)}')
+      _disjoint(out, 'out')
+    os_ = _last_contiguous(out, 'out', 4)
+    ctx = None
+    if save:
+      ctx = DiffAttnContext()
+      dvs = pad_to(dv, 8)
+      ctx.o1, ctx.o2 = (torch.empty((B, H, Tq, dvs), device=dev, dtype=q.dtype) for _ in range(2))
+      ctx.lse = torch.empty((2, B, H, Tq), device=dev, dtype=torch.float32)
+      ctx.norm_weight, ctx.opt, ctx.shape = norm_weight, (scale, int(causal), int(norm), float(norm_eps), float(out_scale), start_all), shape
+      ctx.kv_len, ctx.q_start, ctx.key_mask = kv_len, start_t, key_mask
+    if B == 0 or Tq == 0:
+      return out, ctx
+    if Tk == 0:
+      out.zero_()
+      return out, ctx
+    p = _diff_attn_params(q, k, v, lam, qs, ks, vs, shape, norm_weight, key_mask, kv_len, start_t, (scale, int(causal), int(norm), norm_eps, out_scale, start_all))
+    p.out = out.data_ptr()
+    p.o_s[:] = os_
+    if save:
+      p.o1, p.o2, p.lse = ctx.o1.data_ptr(), ctx.o2.data_ptr(), ctx.lse.data_ptr()
+    if lib.profiler is not None:
+      lib.profiler.tag(f'diff_attn_fwd<{"f32" if q.dtype == torch.float32 else "bf16"}>', float(B * H * Tq * Tk * (4 * d + 4 * dv)))
+    lib.tfpp_diff_attn_fwd(ctypes.byref(p), dt(q), stream())
+  return out, ctx
+
+
+def diff_attn_bwd(dout, q, k, v, lam, ctx, dq=None, dk=None, dv=None):
+  """(dq, dk, dv, dlam, dnorm_weight) of diff_attn_fwd(q, k, v, lam, ..., save=True); kv_len, q_start and key_mask may not change in between.
+  dq / dk / dv: tensors (views of a fused gradient, any strides that do not overlap) to be written in place of new ones.  dlam has lam's shape (summed over
+  the heads when lam is one value), dnorm_weight the weight's type, None without one.  Nothing is added atomically: bit-reproducible."""
+  dev, qs, ks, vs, shape = _diff_attn_check(q, k, v, lam)
+  if ctx.shape != shape or ctx.o1.dtype != q.dtype:
+    raise ValueError(f'the context belongs to another forward pass: {ctx.shape} {ctx.o1.dtype}, now {shape} {q.dtype}')
+  B, Tq, Tk, H, Hkv, d, dvn = shape
+  if tuple(dout.shape) != (B, Tq, H, dvn) or dout.dtype != q.dtype or dout.device != dev:
+    raise ValueError(f'dout: {q.dtype} {(B, Tq, H, dvn)} on {dev}, got {dout.dtype} {tuple(dout.shape)}')
+  dos = _last_contiguous(dout, 'dout', 4)
+  with torch.cuda.device(dev):
+    outs = []
+    for n, t, like in (('dq', dq, q), ('dk', dk, k), ('dv', dv, v)):
+      if t is None:
+        t = torch.empty(like.shape, device=dev, dtype=q.dtype)
+      else:
+        if t.shape != like.shape or t.dtype != q.dtype or t.device != dev:
+          raise ValueError(f'{n}: {q.dtype} {tuple(like.shape)} on {dev}, got {t.dtype} {tuple(t.shape)}')
+        _disjoint(t, n)
+      outs.append(t)
+    strides = [_last_contiguous(t, n, dims) for n, t, dims in zip(('dq', 'dk', 'dv'), outs, (5, 5, 4))]
+    w = ctx.norm_weight
+    dlam, dw = torch.empty(lam.shape, device=dev, dtype=torch.float32), (torch.empty_like(w) if w is not None else None)
+    if B == 0 or Tq == 0 or Tk == 0:  # no pair of a query and a key: nothing has a gradient
+      for t in outs + [dlam] + ([dw] if dw is not None else []):
+        t.zero_()
+      return (*outs, dlam, dw)
+    p = _diff_attn_params(q, k, v, lam, qs, ks, vs, shape, w, ctx.key_mask, ctx.kv_len, ctx.q_start, ctx.opt)
+    n_part = ctypes.c_int64()
+    lib.tfpp_diff_attn_bwd_partial_floats(ctypes.byref(p), ctypes.addressof(n_part))
+    # scratch of this call alone: captured graphs keep theirs in the graph's own pool
+    d_o = torch.empty_like(ctx.o1)
+    delta = torch.empty_like(ctx.lse)
+    partial = torch.empty(n_part.value, device=dev, dtype=torch.float32)
+    p.o1, p.o2, p.lse, p.dout = ctx.o1.data_ptr(), ctx.o2.data_ptr(), ctx.lse.data_ptr(), dout.data_ptr()
+    p.d_o, p.delta, p.partial, p.dlam, p.dnorm_w = d_o.data_ptr(), delta.data_ptr(), partial.data_ptr(), dlam.data_ptr(), ptr(dw)
+    p.dq_out, p.dk_out, p.dv_out = (t.data_ptr() for t in outs)
+    p.do_s[:], p.dq_s[:], p.dk_s[:], p.dv_s[:] = dos, *strides
+    if lib.profiler is not None:
+      lib.profiler.tag(f'diff_attn_bwd<{"f32" if q.dtype == torch.float32 else "bf16"}>', float(B * H * Tq * Tk * (16 * d + 6 * dvn)))
+    lib.tfpp_diff_attn_bwd(ctypes.byref(p), dt(q), stream())
+  return (*outs, dlam, dw)

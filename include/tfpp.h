@@ -699,6 +699,42 @@ int tfpp_block_norm_fwd(const tfpp_block_norm_params* p, int dtype, void* stream
 int tfpp_block_norm_bwd(const tfpp_block_norm_params* p, int dtype, void* stream);
 int tfpp_block_norm_bwd_partial_floats(const tfpp_block_norm_params* p, int64_t* out);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Differential attention: P_i = softmax(scale Q_i K_i^T), i = 1, 2;  O = (P_1 - lam P_2) V;  out = out_scale * norm_w * O / sqrt(mean(O^2) + eps)
+ * (norm = 0: out = out_scale * O).  Element (b, t, h, i, c) of q lies at b q_s[0] + t q_s[1] + h q_s[2] + i q_s[3] + c, and so on: strides in
+ * elements, the last dimension contiguous.  H is a multiple of Hkv: query head h reads key / value head h / (H / Hkv).  d <= 128, dv <= 256.
+ * lam: n_lam = H (or 1) fp32 values.  kv_len (nullable): valid keys of each sequence; key_mask (nullable, [B] rows of pitch ld_mask): 0 leaves a key
+ * out; causal: key j is seen by query i when j <= q_start[b] + i (q_start null: q_start_all).  K and V of keys left out by kv_len or key_mask are
+ * not read.  A query without keys: out = 0.
+ * Forward for training also writes o1, o2 ([B, H, Tq, dv rounded up to 8], P_i V in `dtype`) and lse ([2, B, H, Tq], log2).  Backward reads them, dout
+ * and the inputs, and writes d_o (layout of o1), delta (layout of lse), partial (tfpp_diff_attn_bwd_partial_floats): scratch; dlam [n_lam], dnorm_w
+ * (type of norm_w), and the gradients dq_out, dk_out, dv_out with their own strides.  Fixed summation order throughout. */
+typedef struct {
+  const void *q, *k, *v;
+  const float* lam;
+  const void* norm_w;
+  void* out;
+  void *o1, *o2;
+  float* lse;
+  const int32_t *kv_len, *q_start;
+  const uint8_t* key_mask;
+  const void* dout;
+  void *d_o;
+  float *delta, *partial, *dlam;
+  void *dnorm_w, *dq_out, *dk_out, *dv_out;
+  int64_t ld_mask, q_s[4], k_s[4], v_s[3], o_s[3], do_s[3], dq_s[4], dk_s[4], dv_s[3];
+  int B, H, Hkv, Tq, Tk, d, dv, n_lam, norm, norm_w_bf16, causal, q_start_all;
+  int out_vec, dq_vec, dk_vec, dv_vec; /* set by the library */
+  float scale, out_scale, eps;
+} tfpp_diff_attn_params;
+int tfpp_diff_attn_fwd(const tfpp_diff_attn_params* p, int dtype, void* stream);
+int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* p, int dtype, void* stream);
+int tfpp_diff_attn_bwd_partial_floats(const tfpp_diff_attn_params* p, int64_t* out);
+/* lam[i] = exp(lq1[i] . lk1[i]) - exp(lq2[i] . lk2[i]) + init over n vectors of d values each, and the gradients of the vectors (stored). */
+int tfpp_diff_lambda(const void* lq1, const void* lk1, const void* lq2, const void* lk2, float init, float* lam, int n, int d, int dtype, void* stream);
+int tfpp_diff_lambda_bwd(const float* dlam, const void* lq1, const void* lk1, const void* lq2, const void* lk2, void* dlq1, void* dlk1, void* dlq2,
+                         void* dlk2, int n, int d, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -417,3 +417,393 @@ def test_block_norm_captured(ops):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(outs, want))
+
+
+# ------------------------------------------------------------------------------------------------ differential attention
+E32 = 2.0 ** -24
+
+
+def attn_visible(B, Tq, Tk, causal=False, kv_len=None, key_mask=None, q_start=None):
+  """[B, Tq, Tk] bool."""
+  j = torch.arange(Tk, device=DEV)
+  keep = torch.ones(B, Tq, Tk, dtype=torch.bool, device=DEV)
+  if kv_len is not None:
+    keep &= (j < kv_len[:, None])[:, None]
+  if key_mask is not None:
+    keep &= (key_mask != 0)[:, None]
+  if causal:
+    start = torch.full((B,), Tk - Tq, device=DEV) if q_start is None else (q_start if torch.is_tensor(q_start) else torch.full((B,), q_start, device=DEV))
+    keep &= j <= (start[:, None] + torch.arange(Tq, device=DEV))[..., None]
+  return keep
+
+
+def attn_oracle(q, k, v, lam, keep, dout=None, scale=None, norm=True, w=None, eps=1e-5, c=1.0):
+  """{name: (value, allowed error)} in 64 bits.  Errors: first-order propagation of every rounding of the kernels, worst case: U of the storage type for
+  P, O_i, dO, dS, P_1 - lam P_2 and the result; 2^-24 times the length of a sum for fp32 accumulation; the scores' error enters P relatively."""
+  u = U[q.dtype]
+  ut = u if q.dtype == BF16 else 0.0  # fp32 operands are not rounded on their way into a product
+  B, Tq, H, _, d = q.shape
+  Tk, Hkv, dv = k.shape[1], k.shape[2], v.shape[3]
+  scale = d ** -0.5 if scale is None else scale
+  G = H // Hkv
+  res = {n: torch.zeros(s, dtype=torch.float64, device=DEV) for n, s in
+         (('out', (B, Tq, H, dv)), ('dq', q.shape), ('dk', k.shape), ('dv', v.shape), ('dlam', (H,)), ('dw', (dv,)))}
+  err = {n: torch.zeros_like(t) for n, t in res.items()}
+  W = torch.ones(dv, dtype=torch.float64, device=DEV) if w is None else w.double()
+  for b in range(B):
+    for h in range(H):
+      g = h // G
+      seen = keep[b].any(0)  # (values of keys that nobody sees may be anything)
+      K = torch.where(seen[:, None, None], k[b, :, g].double(), 0.0)
+      V = torch.where(seen[:, None], v[b, :, g].double(), 0.0)
+      L = float(lam[h if lam.numel() > 1 else 0])
+      P, eP, o, eo = [], [], [], []
+      for i in (0, 1):
+        Q = q[b, :, h, i].double()
+        s = (Q @ K[:, i].T * scale).masked_fill(~keep[b], -math.inf)
+        p = torch.nan_to_num(torch.softmax(s, 1), nan=0.0)
+        mags = (Q.abs() @ K[:, i].abs().T * scale).masked_fill(~keep[b], 0.0).amax(1, keepdim=True)
+        P.append(p)
+        eP.append(2 * (d + 40) * E32 * mags + (Tk + 64) * E32)  # relative: both scores and maximum, the exponential, the sum
+        o.append(p @ V)
+        eo.append((eP[i] + ut + (Tk + 16) * E32) * (p @ V.abs()))
+      O, eO = o[0] - L * o[1], eo[0] + abs(L) * eo[1] + 4 * E32 * (o[0].abs() + abs(L * o[1]))
+      r = 1.0 / torch.sqrt(O.pow(2).mean(1, keepdim=True) + eps) if norm else torch.ones_like(O[:, :1])
+      dr = lambda e: (r ** 3 * (O.abs() * e).mean(1, keepdim=True) + dv * E32 * r) if norm else 0.0 * r
+      res['out'][b, :, h] = c * O * r * W
+      err['out'][b, :, h] = abs(c) * W.abs() * (eO * r + O.abs() * dr(eO)) + (u + 8 * E32) * (c * O * r * W).abs()
+      if dout is None:
+        continue
+      t = c * W * dout[b, :, h].double()
+      eoS = [e + ut * x.abs() for e, x in zip(eo, o)]  # as stored
+      eOS = eoS[0] + abs(L) * eoS[1] + 4 * E32 * (o[0].abs() + abs(L * o[1]))
+      der, D = dr(eOS), dout[b, :, h].double().abs() * abs(c)
+      if norm:
+        m, ma = (t * O).mean(1, keepdim=True), (t * O).abs().mean(1, keepdim=True)
+        dO = r * t - O * r ** 3 * m
+        edO = der * t.abs() + r ** 3 * ma * eOS + 3 * r ** 2 * der * O.abs() * ma + O.abs() * r ** 3 * (t.abs() * eOS).mean(1, keepdim=True) + (dv + 32) * E32 * (r * t.abs() + O.abs() * r ** 3 * ma)
+      else:
+        dO, edO = t, 8 * E32 * t.abs()
+      res['dw'] += (c * dout[b, :, h].double() * O * r).sum(0)
+      err['dw'] += (D * (eOS * r + O.abs() * der)).sum(0) + (B * Tq * H + 16) * E32 * (D * O.abs() * r).sum(0)
+      res['dlam'][h] -= (dO * o[1]).sum()
+      err['dlam'][h] += (edO * o[1].abs() + dO.abs() * eoS[1]).sum() + (B * Tq + 300) * E32 * (dO * o[1]).abs().sum()
+      edO = edO + ut * dO.abs()
+      dP, edP = dO @ V.T, edO @ V.abs().T + (dv + 8) * E32 * (dO.abs() @ V.abs().T)
+      for i, f in ((0, 1.0), (1, -L)):
+        delta = (dO * o[i]).sum(1, keepdim=True)
+        ed = (edO * o[i].abs() + dO.abs() * eoS[i]).sum(1, keepdim=True) + (dv + 8) * E32 * (dO * o[i]).abs().sum(1, keepdim=True)
+        dS = f * P[i] * (dP - delta)
+        eS = abs(f) * P[i] * (edP + ed) + (eP[i] + ut + 8 * E32) * dS.abs()
+        res['dq'][b, :, h, i] = scale * (dS @ K[:, i])
+        err['dq'][b, :, h, i] = scale * ((eS + (Tk + 8) * E32 * dS.abs()) @ K[:, i].abs())
+        Qi = q[b, :, h, i].double()
+        res['dk'][b, :, g, i] += scale * (dS.T @ Qi)
+        err['dk'][b, :, g, i] += scale * ((eS + (G * Tq + 8) * E32 * dS.abs()).T @ Qi.abs())
+      Pd = P[0] - L * P[1]
+      ePd = eP[0] * P[0] + abs(L) * eP[1] * P[1] + (ut + 4 * E32) * Pd.abs()
+      res['dv'][b, :, g] += Pd.T @ dO
+      err['dv'][b, :, g] += ePd.T @ dO.abs() + Pd.abs().T @ (edO + (G * Tq + 8) * E32 * dO.abs())
+  if lam.numel() == 1:
+    res['dlam'], err['dlam'] = res['dlam'].sum().view(1), err['dlam'].sum().view(1)
+  for n in ('dq', 'dk', 'dv'):
+    err[n] += u * res[n].abs()
+  if w is not None:
+    err['dw'] += U[w.dtype] * res['dw'].abs()
+  return {n: (res[n], err[n]) for n in res}
+
+
+def attn_inputs(B, Tq, Tk, H, Hkv, d, dv, dtype, seed=0, lam_n=None):
+  q, k = randn(B, Tq, H, 2, d, dtype=dtype, seed=seed + 1, std=1.5), randn(B, Tk, Hkv, 2, d, dtype=dtype, seed=seed + 2)
+  v, dout = randn(B, Tk, Hkv, dv, dtype=dtype, seed=seed + 3), randn(B, Tq, H, dv, dtype=dtype, seed=seed + 4)
+  lam = randn(H if lam_n is None else lam_n, seed=seed + 5, std=0.2, mean=0.5)
+  return q, k, v, dout, lam
+
+
+def attn_compare(ops, q, k, v, dout, lam, w=None, train=True, keep=None, outs=None, norm=True, c=0.65, **opt):
+  B, Tq, Tk = q.shape[0], q.shape[1], k.shape[1]
+  vis = attn_visible(B, Tq, Tk, **{n: opt[n] for n in ('causal', 'kv_len', 'key_mask', 'q_start') if n in opt})
+  want = attn_oracle(q, k, v, lam, vis, dout=dout if train else None, scale=opt.get('scale'), norm=norm, w=w, c=c)
+  out, ctx = ops.diff_attn_fwd(q, k, v, lam, norm=norm, norm_weight=w, out_scale=c, save=train, **opt)
+  within('out', out, *want['out'])
+  empty = ~vis.any(2)
+  assert not out[empty].any()
+  if not train:
+    assert ctx is None
+    return out
+  plain, _ = ops.diff_attn_fwd(q, k, v, lam, norm=norm, norm_weight=w, out_scale=c, **opt)
+  assert torch.equal(plain, out)
+  got = dict(zip(('dq', 'dk', 'dv', 'dlam', 'dw'), ops.diff_attn_bwd(dout, q, k, v, lam, ctx, **(outs or {}))))
+  for n, g in got.items():
+    if g is None:
+      assert n == 'dw' and w is None
+      continue
+    within(n, g, *want[n])
+    if n in ('dq', 'dk', 'dv') and Tk >= 8:
+      # five roundings at most lie on the way to an element (P, O_i, dO, dS, the result), each U relative: far below what a wrong term would make
+      a, b = g.double(), want[n][0]
+      assert float((a - b).norm()) <= 6 * max(U[q.dtype], 2.0 ** -16) * float(b.norm()) + 1e-6, (n, float((a - b).norm() / b.norm()))
+  unseen = ~vis.any(1)
+  assert not got['dk'][unseen].any() and not got['dv'][unseen].any() and not got['dq'][empty].any()
+  again = ops.diff_attn_bwd(dout, q, k, v, lam, ctx)
+  assert all(x is None or torch.equal(x, y) for x, y in zip(got.values(), again)), 'not reproducible'
+  return out
+
+
+SHAPES = [(1, 1, 1, 1, 1, 1, 1), (2, 3, 5, 2, 1, 9, 18), (1, 64, 64, 4, 2, 16, 32), (2, 65, 130, 2, 2, 27, 54), (3, 129, 200, 4, 1, 64, 128), (1, 320, 320, 4, 4, 72, 144),
+          (1, 100, 77, 2, 1, 128, 256), (1, 33, 300, 3, 3, 80, 100), (8, 20, 70, 2, 2, 32, 64)]
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('mask', ['none', 'causal', 'len', 'keys', 'all'])
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+def test_diff_attention_forward_and_gradients(ops, shape, mask, dtype):
+  B, Tq, Tk, H, Hkv, d, dv = shape
+  q, k, v, dout, lam = attn_inputs(*shape, dtype)
+  g = torch.Generator().manual_seed(sum(shape))
+  lens = torch.randint(0, Tk + 1, (B,), generator=g, dtype=torch.int32)
+  keys = torch.rand(B, Tk, generator=g) < 0.7
+  keys[B - 1] = B > 1 and mask == 'all'  # (one sequence without any key)
+  opt = {}
+  if mask in ('causal', 'all'):
+    opt['causal'] = True
+  if mask in ('len', 'all'):
+    opt['kv_len'] = lens.to(DEV)
+  if mask in ('keys', 'all'):
+    opt['key_mask'] = keys.to(DEV)
+  if mask == 'all':
+    opt['q_start'] = torch.randint(-Tq, Tk, (B,), generator=g, dtype=torch.int32).to(DEV)
+  attn_compare(ops, q, k, v, dout, lam, w=randn(dv, dtype=dtype, seed=9, std=0.1, mean=1.0), **opt)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_diff_attention_options(ops, dtype):
+  """Without the norm, without weights, fp32 weights beside bf16 heads, one lambda for all heads, negative and zero lambda, another scale, an int q_start."""
+  q, k, v, dout, lam = attn_inputs(2, 40, 50, 4, 2, 24, 56, dtype, seed=20)
+  attn_compare(ops, q, k, v, dout, lam, norm=False)
+  attn_compare(ops, q, k, v, dout, lam)
+  attn_compare(ops, q, k, v, dout, lam, w=randn(56, seed=21, mean=1.0, std=0.1))
+  attn_compare(ops, q, k, v, dout, lam[:1].clone(), scale=0.3)
+  attn_compare(ops, q, k, v, dout, -lam, causal=True, q_start=-7)
+  attn_compare(ops, q, k, v, dout, torch.zeros_like(lam), causal=True, q_start=1000)
+  attn_compare(ops, q, k, v, dout, lam, key_mask=(torch.arange(50, device=DEV) % 3 != 1).to(torch.uint8).repeat(2, 1))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('d,off', [(32, 0), (32, 1), (20, 0)])
+def test_diff_attention_strides(ops, dtype, d, off):
+  """Slices of one fused projection (aligned or not), caches in [B, H, T] order, gradients written into the fused gradient; its other columns stay."""
+  B, T, H, Hkv, dv = 2, 70, 4, 2, 2 * d
+  width = 2 * H * d + 2 * Hkv * d + Hkv * dv + 3
+  fused = randn(B, T, width + off, dtype=dtype, seed=30)[..., off:]
+  cut = lambda x: (x[..., :2 * H * d].unflatten(-1, (H, 2, d)), x[..., 2 * H * d:2 * (H + Hkv) * d].unflatten(-1, (Hkv, 2, d)), x[..., 2 * (H + Hkv) * d:-3].unflatten(-1, (Hkv, dv)))
+  q, k, v = cut(fused)
+  dfused = torch.full((B, T, width + off), 7.0, dtype=dtype, device=DEV)[..., off:]
+  dq, dk, dv_ = cut(dfused)
+  _, _, _, dout, lam = attn_inputs(B, T, T, H, Hkv, d, dv, dtype, seed=31)
+  attn_compare(ops, q, k, v, dout.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3), lam, outs=dict(dq=dq, dk=dk, dv=dv_), causal=True)
+  assert (dfused[..., -3:] == 7.0).all()
+  # [B, H, 2, T, d] storage
+  q2, k2, v2 = q.permute(0, 2, 3, 1, 4).contiguous().permute(0, 3, 1, 2, 4), k.permute(0, 2, 3, 1, 4).contiguous().permute(0, 3, 1, 2, 4), v.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+  buf = torch.full((B, H, T, dv + 5), 7.0, dtype=dtype, device=DEV)
+  out, _ = ops.diff_attn_fwd(q2, k2, v2, lam, out=buf[..., :dv].permute(0, 2, 1, 3))
+  assert (buf[..., dv:] == 7.0).all()
+  ref, _ = ops.diff_attn_fwd(q.contiguous(), k.contiguous(), v.contiguous(), lam)
+  within('order', out, ref.double(), 2 * U[dtype] * ref.abs() + 1e-5)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('d', [32, 27])
+def test_diff_attention_left_out_keys_may_hold_anything(ops, dtype, d):
+  q, k, v, dout, lam = attn_inputs(3, 35, 150, 2, 2, d, 2 * d, dtype, seed=40)
+  lens = torch.tensor([150, 61, 0], dtype=torch.int32, device=DEV)
+  mask = torch.ones(3, 150, dtype=torch.bool, device=DEV)
+  mask[0, 3:40] = False
+  mask[1, ::2] = False
+  opt = dict(kv_len=lens, key_mask=mask)
+  clean = ops.diff_attn_fwd(q, k, v, lam, save=True, **opt)
+  cg = ops.diff_attn_bwd(dout, q, k, v, lam, clean[1])
+  gone = ~(mask & (torch.arange(150, device=DEV) < lens[:, None]))
+  for bad in (math.nan, math.inf, torch.finfo(dtype).min):
+    k2, v2 = k.clone(), v.clone()
+    k2[gone], v2[gone] = bad, bad
+    out, ctx = ops.diff_attn_fwd(q, k2, v2, lam, save=True, **opt)
+    assert torch.equal(out, clean[0])
+    assert all(x is None or torch.equal(x, y) for x, y in zip(cg, ops.diff_attn_bwd(dout, q, k2, v2, lam, ctx)))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_diff_attention_large_scores(ops, dtype):
+  """Scores of several hundred, rising and falling along the keys: the running maximum moves often, nothing overflows."""
+  q, k, v, dout, lam = attn_inputs(1, 64, 400, 2, 1, 64, 128, dtype, seed=50)
+  ramp = torch.linspace(-6, 6, 400, device=DEV).view(1, 400, 1, 1, 1)
+  for kk in ((k.float() * ramp).to(dtype), (k.float() * ramp.flip(1)).to(dtype)):
+    attn_compare(ops, q, kk, v, dout, lam, w=randn(128, dtype=dtype, seed=51, mean=1.0, std=0.1))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('Tq', [1, 2, 5, 17])
+@pytest.mark.parametrize('heads', [(4, 4, 72, 144), (8, 2, 64, 128), (16, 1, 32, 64), (2, 1, 128, 256), (3, 3, 9, 18)], ids=str)
+def test_diff_attention_new_tokens_against_a_cache(ops, heads, Tq, dtype):
+  H, Hkv, d, dv = heads
+  for Tk, lens in ((40, [17, 33, 40]), (3000, [2999, 18, 1500]), (6000, [5000])):
+    B = len(lens)
+    q, k, v, dout, lam = attn_inputs(B, Tq, Tk, H, Hkv, d, dv, dtype, seed=60)
+    kv_len = torch.tensor([max(n, Tq) for n in lens], dtype=torch.int32, device=DEV)
+    stale = torch.arange(Tk, device=DEV) >= kv_len[:, None]
+    k[stale], v[stale] = math.nan, math.nan
+    cache = dict(k=k.permute(0, 2, 3, 1, 4).contiguous().permute(0, 3, 1, 2, 4), v=v.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3))
+    for kk, vv in ((k, v), (cache['k'], cache['v'])):
+      attn_compare(ops, q, kk, vv, dout, lam, train=False, causal=True, kv_len=kv_len, q_start=kv_len - Tq, w=randn(dv, seed=61, mean=1.0, std=0.1))
+
+
+def test_diff_attention_cache_of_length_zero_and_masks_with_one_token(ops):
+  q, k, v, dout, lam = attn_inputs(4, 1, 2000, 4, 2, 64, 128, BF16, seed=70)
+  lens = torch.tensor([0, 1, 2000, 1024], dtype=torch.int32, device=DEV)
+  keys = torch.ones(4, 2000, dtype=torch.bool, device=DEV)
+  keys[2, 100:1900] = False
+  keys[3] = False
+  out = attn_compare(ops, q, k, v, dout, lam, train=False, kv_len=lens, key_mask=keys)
+  assert not out[0].any() and not out[3].any() and out[1].any()
+
+
+def test_diff_attention_cache_behind_32_bit_offsets(ops):
+  """A cache whose second sequence starts behind 2^31 elements, and whose tokens lie far apart."""
+  B, Tk, Hkv, d, dv = 2, 300, 1, 64, 128
+  ld = (1 << 31) // 300 + 64 - ((1 << 31) // 300) % 64
+  store = torch.empty(2 * Tk * ld + 4096, dtype=BF16, device=DEV)
+  k = store.as_strided((B, Tk, Hkv, 2, d), (Tk * ld, ld, 2 * d, d, 1))
+  v = store.as_strided((B, Tk, Hkv, dv), (Tk * ld, ld, dv, 1), 512)
+  q, k0, v0, dout, lam = attn_inputs(B, 3, Tk, 2, Hkv, d, dv, BF16, seed=80)
+  k.copy_(k0)
+  v.copy_(v0)
+  attn_compare(ops, q, k, v, dout, lam, train=False)
+  attn_compare(ops, q, k, v, dout, lam)
+
+
+def test_diff_attention_gradient_against_differences(ops):
+  """Directional derivatives of the 64-bit forward by central differences, lambda through its learned vectors."""
+  B, T, H, Hkv, d, dv = 1, 12, 2, 1, 8, 16
+  q, k, v, dout, _ = attn_inputs(B, T, T, H, Hkv, d, dv, F32, seed=90)
+  vec = [randn(H, d, seed=95 + i, std=0.3) for i in range(4)]
+  w = randn(dv, seed=99, mean=1.0, std=0.1)
+  keep = attn_visible(B, T, T, causal=True)
+  lam = ops.diff_lambda(*vec, 0.4)
+  out, ctx = ops.diff_attn_fwd(q, k, v, lam, causal=True, norm_weight=w, out_scale=0.6, save=True)
+  dq, dk, dvv, dlam, dw = ops.diff_attn_bwd(dout, q, k, v, lam, ctx)
+  grads = dict(zip(('q', 'k', 'v', 'w', 0, 1, 2, 3), [dq, dk, dvv, dw] + list(ops.diff_lambda_bwd(dlam, *vec))))
+
+  def loss(x):
+    e = lambda i: torch.exp((x[i] * x[i + 1]).sum(1))
+    L = e(0) - e(2) + 0.4
+    r = 0.0
+    for h in range(H):
+      p = [torch.softmax((x['q'][0, :, h, i] @ x['k'][0, :, 0, i].T * d ** -0.5).masked_fill(~keep[0], -math.inf), 1) for i in (0, 1)]
+      o = (p[0] - L[h] * p[1]) @ x['v'][0, :, 0]
+      o = 0.6 * x['w'] * o / torch.sqrt(o.pow(2).mean(1, keepdim=True) + 1e-5)
+      r = r + (o * dout[0, :, h].double()).sum()
+    return r
+
+  base = {'q': q.double(), 'k': k.double(), 'v': v.double(), 'w': w.double(), **{i: t.double() for i, t in enumerate(vec)}}
+  for n, g in grads.items():
+    direction = randn(*g.shape, seed=77).double()
+    e = 1e-6
+    num = float((loss({**base, n: base[n] + e * direction}) - loss({**base, n: base[n] - e * direction})) / (2 * e))
+    # truncation e^2, rounding 1e-16 / e in the difference; fp32 kernels: well under 1e-5 of the gradient's own size (sums of <= 200 terms)
+    assert abs(num - float((g.double() * direction).sum())) <= 2e-5 * float((g.double().abs() * direction.abs()).sum()) + 1e-7, n
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('shape', [(1, 1), (4, 9), (16, 128), (12,)], ids=str)
+def test_diff_lambda_and_gradient(ops, shape, dtype):
+  vec = [randn(*shape, dtype=dtype, seed=i, std=0.2) for i in range(4)]
+  d = shape[-1]
+  lam = ops.diff_lambda(*vec, 0.35)
+  a = [t.double().view(-1, d) for t in vec]
+  e = [torch.exp((a[0] * a[1]).sum(1)), torch.exp((a[2] * a[3]).sum(1))]
+  tol = (d + 16) * E32 * (e[0] * (1 + (a[0] * a[1]).abs().sum(1)) + e[1] * (1 + (a[2] * a[3]).abs().sum(1)) + 0.35)
+  within('lam', lam, e[0] - e[1] + 0.35, tol)
+  dl = randn(lam.numel(), seed=9)
+  want = [dl.double()[:, None] * s * x for s, x in ((e[0][:, None], a[1]), (e[0][:, None], a[0]), (-e[1][:, None], a[3]), (-e[1][:, None], a[2]))]
+  for g, x in zip(ops.diff_lambda_bwd(dl, *vec), want):
+    assert g.dtype == dtype and g.shape == vec[0].shape
+    within('vector', g.view(-1, d), x, (U[dtype] + (2 * d + 32) * E32) * x.abs())
+
+
+def test_diff_attention_empty_calls(ops):
+  lam = torch.full((2,), 0.5, device=DEV)
+  for B, Tq, Tk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+    q, k, v, dout, _ = attn_inputs(B, Tq, Tk, 2, 1, 16, 32, BF16)
+    out, ctx = ops.diff_attn_fwd(q, k, v, lam, save=True)
+    assert out.shape == (B, Tq, 2, 32) and not out.any()
+    for g in ops.diff_attn_bwd(dout, q, k, v, lam, ctx)[:4]:
+      assert not g.any()
+
+
+def test_diff_attention_refusals(ops):
+  q, k, v, dout, lam = attn_inputs(2, 6, 7, 4, 2, 16, 32, BF16)
+  i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+  bad = [dict(q=q.half(), k=k.half(), v=v.half()), dict(k=k.float()), dict(q=q.cpu()), dict(q=q[:1]), dict(q=q[:, :, :3]), dict(k=k[:, :6]), dict(v=v[:, :, :1]),
+         dict(q=q[..., :8]), dict(lam=lam[:2].clone()), dict(lam=lam.double()), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
+         dict(norm_eps=0.0), dict(norm=False, norm_weight=torch.ones(32, device=DEV)), dict(norm_weight=torch.ones(31, device=DEV)),
+         dict(norm_weight=torch.ones(32, device=DEV).half()), dict(kv_len=i32(1)), dict(kv_len=i32(1, 2).long()), dict(kv_len=i32(1, 2).cpu()), dict(q_start=i32(1, 2, 3)),
+         dict(q_start=1 << 30), dict(key_mask=torch.ones(2, 6, device=DEV, dtype=torch.bool)), dict(key_mask=torch.ones(2, 7, device=DEV)),
+         dict(key_mask=torch.ones(7, 2, device=DEV, dtype=torch.bool).t()), dict(out=torch.empty(2, 6, 4, 32, device=DEV)), dict(out=torch.empty(1, 6, 4, 32, device=DEV, dtype=BF16).expand(2, 6, 4, 32)),
+         dict(q=q.transpose(3, 4).contiguous().transpose(3, 4))]
+  for kw in bad:
+    kw = {'q': q, 'k': k, 'v': v, 'lam': lam, **kw}
+    with pytest.raises((ValueError, TypeError)):
+      ops.diff_attn_fwd(kw.pop('q'), kw.pop('k'), kw.pop('v'), kw.pop('lam'), **kw)
+  wide = attn_inputs(1, 2, 2, 1, 1, 129, 64, BF16)
+  with pytest.raises(ValueError):
+    ops.diff_attn_fwd(*wide[:3], wide[4])
+  wide = attn_inputs(1, 2, 2, 1, 1, 64, 257, BF16)
+  with pytest.raises(ValueError):
+    ops.diff_attn_fwd(*wide[:3], wide[4])
+  _, ctx = ops.diff_attn_fwd(q, k, v, lam, save=True)
+  for kw in (dict(dout=dout.float()), dict(dout=dout[:1]), dict(q=q[:1], k=k[:1], v=v[:1], dout=dout[:1]), dict(dk=torch.empty_like(v)), dict(dq=q[:, :1].expand_as(q))):
+    kw = {'dout': dout, 'q': q, 'k': k, 'v': v, **kw}
+    with pytest.raises((ValueError, TypeError)):
+      ops.diff_attn_bwd(kw.pop('dout'), kw.pop('q'), kw.pop('k'), kw.pop('v'), lam, ctx, **kw)
+  for vec in ([lam, lam, lam, lam.double()], [lam.double()] * 4, [lam, lam, lam, lam[:1]], [lam.cpu()] * 4):
+    with pytest.raises((ValueError, TypeError)):
+      ops.diff_lambda(*vec, 0.5)
+
+
+@pytest.mark.parametrize('Tq,Tk', [(200, 200), (1, 5000)])
+def test_diff_attention_captured_on_two_streams(ops, Tq, Tk):
+  """Forward and backward captured twice, replayed side by side on two streams between eager calls: every replay equals the eager result."""
+  q, k, v, dout, lam = attn_inputs(2, Tq, Tk, 4, 2, 64, 128, BF16, seed=100)
+
+  def step():
+    out, ctx = ops.diff_attn_fwd(q, k, v, lam, causal=True, save=True)
+    serve, _ = ops.diff_attn_fwd(q, k, v, lam, causal=True)
+    return [out, serve] + [t for t in ops.diff_attn_bwd(dout, q, k, v, lam, ctx) if t is not None]
+
+  step()
+  torch.cuda.synchronize()
+  graphs = []
+  for _ in range(2):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+      graphs.append((g, step()))
+  side = torch.cuda.Stream()
+  for n in range(4):
+    q.copy_(randn(*q.shape, dtype=BF16, seed=110 + n))
+    v.copy_(randn(*v.shape, dtype=BF16, seed=120 + n))
+    want = step()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+      graphs[0][0].replay()
+    graphs[1][0].replay()
+    torch.cuda.synchronize()
+    for _, outs in graphs:
+      assert all(torch.equal(a, b) for a, b in zip(outs, want))
+  with torch.cuda.stream(side):  # inputs made on one stream, used on another after an event
+    e = torch.cuda.Event()
+  e.record()
+  side.wait_event(e)
+  with torch.cuda.stream(side):
+    got = step()
+  torch.cuda.synchronize()
+  assert all(torch.equal(a, b) for a, b in zip(got, want))
