@@ -61,30 +61,35 @@ template <typename T, int CB> struct Img {
     else return (r >> 2) & 3;
   }
   __device__ static __forceinline__ int off(int r, int c) { return (r * NC + (c ^ swizzle(r))) * 16; }
-  // operand of 32 rows x 16 channels (channels 16 ks ..): lane l has row l % 32, channels 16 ks + 8 (l / 32) ..
-  __device__ static __forceinline__ void rows(const unsigned char* img, int row, int ks, int half, Frag8<T>& f) {
+  // Reads take a lane's byte offset for the first rows and channels (rows_at / cols_at, plus the image's place and 16-row steps, both multiples of a row)
+  // and reach the other channels by an XOR with a constant: one register for a whole image.
+  // Operand of 32 rows x 16 channels (16 ks ..): lane l has row l % 32, channels 16 ks + 8 (l / 32) ..
+  __device__ static __forceinline__ int rows_at(int lane) { return off(lane & 31, (sizeof(T) == 2 ? 1 : 2) * (lane >> 5)); }
+  __device__ static __forceinline__ void rows(const unsigned char* lds, int at, int ks, Frag8<T>& f) {
     if constexpr (sizeof(T) == 2) {
-      f.v = *reinterpret_cast<const uint4*>(img + off(row, 2 * ks + half));
+      f.v = *reinterpret_cast<const uint4*>(lds + (at ^ ks << 5));
     } else {
-      const float4 a = *reinterpret_cast<const float4*>(img + off(row, 4 * ks + 2 * half)), b = *reinterpret_cast<const float4*>(img + off(row, 4 * ks + 2 * half + 1));
+      const float4 a = *reinterpret_cast<const float4*>(lds + (at ^ ks << 6)), b = *reinterpret_cast<const float4*>(lds + (at ^ (ks << 6 | 16)));
       f.v[0] = a.x; f.v[1] = a.y; f.v[2] = a.z; f.v[3] = a.w; f.v[4] = b.x; f.v[5] = b.y; f.v[6] = b.z; f.v[7] = b.w;
     }
   }
-  // operand of 32 channels (32 cb ..) x 16 rows (row0 ..), contraction over rows in the C fragments' labelling
-  __device__ static __forceinline__ void cols(const unsigned char* img, int row0, int cb, int lane, Frag8<T>& f) {
-    const int half = lane >> 5;
-    if constexpr (sizeof(T) == 2) {
-      const int i = lane & 15, r = row0 + 4 * half + (i >> 2), c = cb * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
-      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(img + off(r, c) + sub));
-      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(img + off(r + 8, c) + sub));
+  // operand of 32 channels (32 cb ..) x 16 rows, contraction over rows in the C fragments' labelling
+  __device__ static __forceinline__ int cols_at(int lane) {
+    const int half = lane >> 5, i = lane & 15;
+    if constexpr (sizeof(T) == 2) return off(4 * half + (i >> 2), ((lane >> 4) & 1) * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
+    else return off(4 * half, (lane & 31) >> 2) + (lane & 3) * 4;
+  }
+  __device__ static __forceinline__ void cols(const unsigned char* lds, int at, int cb, Frag8<T>& f) {
+    if constexpr (sizeof(T) == 2) {  // rows + 8: the swizzle's bit 1 turns over
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(lds + (at ^ cb << 6)));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t __attribute__((address_space(3)))*)(lds + (at ^ (cb << 6 | 32)) + 8 * ROW_BYTES));
       const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
       f.v = make_uint4(a.x, a.y, b.x, b.y);
     } else {
-      const int m = cb * 32 + (lane & 31);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int r = row0 + 8 * (e >> 2) + 4 * half + (e & 3);
-        f.v[e] = *reinterpret_cast<const float*>(img + off(r, m >> 2) + (m & 3) * 4);
+      for (int e = 0; e < 8; ++e) {  // (the swizzle of 4 half + k is that of 4 half XOR that of k: the bits are disjoint)
+        const int k = 8 * (e >> 2) + (e & 3);
+        f.v[e] = *reinterpret_cast<const float*>(lds + (at ^ (cb << 7 ^ swizzle(k) << 4)) + k * ROW_BYTES);
       }
     }
   }
@@ -104,11 +109,12 @@ template <typename T, int CB> struct Img {
         if (u * NT + wave * 64 < SLOTS) {
           const int r = r0 + u * (NT / NC), c = (tid % NC) ^ swizzle(r);
           bool ok = c * VEC < n;
-          if (!all) ok = ok && ((valid >> r) & 1ull);
+          if (!all) ok = ok && (((valid >> (u * (NT / NC))) >> r0) & 1ull);
           __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t*)(img + (u * NT + wave * 64) * 16), 16, ok ? rowb + c * 16 : (int)0x80000000, u * (NT / NC) * ldb, 0, 0);
         }
       }
     } else {
+#pragma unroll 1
       for (int i = tid; i < ROWS * 32 * CB; i += NT) {
         const int r = i / (32 * CB), c = i % (32 * CB);
         T v = ElemTraits<T>::from_f(0.f);
@@ -162,11 +168,15 @@ __device__ __forceinline__ float norm_weight(const tfpp_diff_attn_params& p, int
   return !p.norm_w ? 1.f : (p.norm_w_bf16 ? bf2f(((const bf16_t*)p.norm_w)[c]) : ((const float*)p.norm_w)[c]);
 }
 
-// workgroup -> (tile, batch x head).  Workgroups go round the 8 XCDs in turn: all tiles of one key / value head stay on one XCD (its K and V
-// are read from that XCD's L2) where the heads divide evenly.
-__device__ __forceinline__ void place(int heads, int tiles, int& bh, int& tile) {
+// workgroup -> (tile, batch x head).  Workgroups go round the 8 XCDs in turn: where the heads divide evenly, all tiles of a head stay on one XCD (its
+// K and V are read from that XCD's L2).  Equal tiles: head after head, so that few heads share an L2 at a time; causal: tile after tile over all
+// heads, the caller turning the order so that the longest start first and the short ones fill the end.
+__device__ __forceinline__ void place(int heads, int tiles, bool by_tile, int& bh, int& tile) {
   const int id = blockIdx.x;
-  if (heads % 8 == 0) {
+  if (by_tile) {
+    bh = id % heads;
+    tile = id / heads;
+  } else if (heads % 8 == 0) {
     bh = (id % 8) + 8 * ((id / 8) / tiles);
     tile = (id / 8) % tiles;
   } else {
@@ -201,57 +211,171 @@ __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 
 template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// forward.  Workgroup = (batch, head, 128 queries), wave = 32 queries, lane l and l + 32 = one query.  S_i^T = K_i Q_i^T (keys x queries), running
-// maximum and sum per query, O_i^T += V^T P_i^T: both maps share every V operand.  O_1 and O_2 are kept apart to the end because their sums are
-// not known before; one pass, 4 d + 4 dv flop a pair.  Wide heads (SPLIT): O_1 and O_2 of 32 queries do not fit one wave's registers, so two waves
-// share the queries, one map each, and meet in LDS at the end.
+// forward.  A wave has 32 queries, lane l and l + 32 = one query.  S_i^T = K_i Q_i^T (keys x queries), running maximum and sum per query,
+// O_i^T += V^T P_i^T: both maps share every V operand.  O_1 and O_2 are kept apart to the end because their sums are not known before; one pass,
+// 4 d + 4 dv flop a pair.  Wide heads (split): O_1 and O_2 of 32 queries do not fit one wave's registers, so two waves share the queries, one map
+// each, and meet in LDS at the end.
 template <typename T, int NB> constexpr bool fwd_split() { return NB >= (sizeof(T) == 2 ? 8 : 5); }
+
+enum { Q_HELD, Q_GLOBAL, Q_LDS };  // where a wave's queries are: registers, or read again for every tile
+template <typename T, int NB, bool VECTOR, int Q, int MAPS> struct Fwd {
+  static constexpr int CD = (NB + 1) / 2;
+  typedef Img<T, CD> ImgK;
+  typedef Img<T, NB> ImgV;
+  int map0;        // the wave's (first) map
+  const T* qrow;   // the lane's query, map 0 (Q_GLOBAL)
+  int q_at, k_at, v_at;  // offsets in LDS: the queries of the wave's first map (Q_LDS), the lane's place in K and V images
+  long qmap;       // from map to map
+  Frag8<T> q[MAPS][Q == Q_HELD ? NB : 1];
+  f32x16_t o[MAPS][NB];
+  float m[MAPS], l[MAPS];  // m: both halves of a query agree; l: this half's keys
+
+  __device__ __forceinline__ void init(int map, const T* row, long to_map, int d, int lane) {
+    const int half = lane >> 5;
+    map0 = map; qrow = row; qmap = to_map;
+    q_at = 0; k_at = ImgK::rows_at(lane); v_at = ImgV::cols_at(lane);
+    if constexpr (Q == Q_HELD)
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i)
+#pragma unroll
+        for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(qrow + (long)(map0 + i) * qmap, ks * 16 + half * 8, d, true, q[i][ks]);
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) {
+      m[i] = NO_MAX; l[i] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][n][r] = 0.f;
+    }
+  }
+  // 32 keys: rows at kimg, vimg bytes into lds (kimg: the wave's first map, the other kbytes behind); vis: bit of a key, the lane's half already shifted out
+  __device__ __forceinline__ void tile(const unsigned char* lds, int kimg, int kbytes, int vimg, bool masked, unsigned vis, float c, int d, int half) {
+    const int kat = k_at + kimg, vat = v_at + vimg;
+    f32x16_t sc[MAPS];
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[i][r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i)
+#pragma unroll
+      for (int ks = 0; ks < NB; ++ks) {
+        Frag8<T> a;
+        ImgK::rows(lds + i * kbytes, kat, ks, a);
+        if constexpr (Q == Q_LDS) ImgK::rows(lds + i * 32 * ImgK::ROW_BYTES, q_at, ks, q[i][0]);
+        if constexpr (Q == Q_GLOBAL) load_frag<T, VECTOR>(qrow + (long)(map0 + i) * qmap, ks * 16 + half * 8, d, true, q[i][0]);
+        mma(a, q[i][Q == Q_HELD ? ks : 0], sc[i]);
+        if (sizeof(T) == 4 || ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    if (masked) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool keep = (vis >> (8 * (r >> 2) + (r & 3))) & 1u;
+#pragma unroll
+        for (int i = 0; i < MAPS; ++i) sc[i][r] = keep ? sc[i][r] : -INFINITY;
+      }
+    }
+    float mx[MAPS];
+    bool grew = false;
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) {
+      mx[i] = sc[i][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx[i] = fmaxf(mx[i], sc[i][r]);
+      mx[i] *= c;
+      grew = grew || mx[i] > m[i] + MAX_SLACK;
+    }
+    if (__any(grew)) {
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i) {
+        const float to = fmaxf(m[i], fmaxf(mx[i], other_half(mx[i])));
+        const float f = exp2f(m[i] - to);
+        m[i] = to;
+        l[i] *= f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][n][r] *= f;
+      }
+    }
+    Frag8<T> pf[MAPS][2];
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        sc[i][r] = __builtin_amdgcn_exp2f(fmaf(sc[i][r], c, -m[i]));
+        l[i] += sc[i][r];
+      }
+      to_frag(sc[i], 0, pf[i][0]);
+      to_frag(sc[i], 1, pf[i][1]);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (operands loaded far ahead of their products would not fit the registers)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        Frag8<T> v;
+        ImgV::cols(lds + 16 * t * ImgV::ROW_BYTES, vat, n, v);
+#pragma unroll
+        for (int i = 0; i < MAPS; ++i) mma(v, pf[i][t], o[i][n]);
+        if (sizeof(T) == 4 || n % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+};
+
+// 1 / sum of a query's exponentials: zero without a visible key, NaN stays NaN
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }
+// log2 of the sum; +inf for a query without keys: exp2(score - inf) = 0 in the backward passes
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? INFINITY : m + log2f(l); }
+
+// 32 channels (block n) of a query's result: f = out_scale / rms
+template <typename T> __device__ __forceinline__ void store_result(const tfpp_diff_attn_params& p, T* out, int n, int half, float f, const f32x16_t& o) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    __builtin_amdgcn_sched_barrier(0);  // (the weights of all channels at once would not fit the registers)
+    const int ch = n * 32 + 8 * g + 4 * half;
+    if (ch >= p.dv) continue;
+    float w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = p.norm && ch + e < p.dv ? f * norm_weight(p, ch + e) : f;
+    store4<T>(out, ch, p.dv, p.out_vec, o[4 * g] * w[0], o[4 * g + 1] * w[1], o[4 * g + 2] * w[2], o[4 * g + 3] * w[3]);
+  }
+}
+template <typename T> __device__ __forceinline__ void store_block(T* row, int n, int half, int dvs, const f32x16_t& o) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) store4<T>(row, n * 32 + 8 * g + 4 * half, dvs, true, o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
+}
+
+// many queries: workgroup = (batch, head, 128 queries), the waves' queries differ and the images are shared by the workgroup, one tile ahead
 template <typename T, int NB> constexpr int fwd_threads() { return fwd_split<T, NB>() && sizeof(T) == 2 ? 512 : 256; }
 template <typename T, int NB> constexpr int fwd_queries() { return fwd_threads<T, NB>() / (fwd_split<T, NB>() ? 4 : 2); }
 template <typename T, int NB> constexpr int fwd_lds() { return 2 * key_tile<T>() * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES); }
 
 template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_threads<T, NB>()), (fwd_threads<T, NB>() == 512 || NB <= (sizeof(T) == 2 ? 4 : 2) ? 2 : 1)) void diff_attn_fwd_kernel(tfpp_diff_attn_params p) {
-  constexpr int KT = key_tile<T>(), CD = (NB + 1) / 2, NT = fwd_threads<T, NB>(), MAPS = fwd_split<T, NB>() ? 1 : 2, QB = fwd_queries<T, NB>();
-  typedef Img<T, CD> ImgK;
-  typedef Img<T, NB> ImgV;
+  typedef Fwd<T, NB, VECTOR, (sizeof(T) == 2 ? VECTOR || NB < 8 : NB < 5) ? Q_HELD : Q_GLOBAL, fwd_split<T, NB>() ? 1 : 2> F;  // (wide fp32 heads do not fit the registers)
+  typedef typename F::ImgK ImgK;
+  typedef typename F::ImgV ImgV;
+  constexpr int KT = key_tile<T>(), NT = fwd_threads<T, NB>(), MAPS = fwd_split<T, NB>() ? 1 : 2, QB = fwd_queries<T, NB>();
   constexpr int K_BYTES = KT * ImgK::ROW_BYTES, V_BYTES = KT * ImgV::ROW_BYTES, BUF = 2 * K_BYTES + V_BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int tiles = (p.Tq + QB - 1) / QB;
   int bh, tile;
-  place(p.B * p.H, tiles, bh, tile);
+  place(p.B * p.H, tiles, p.causal, bh, tile);
   if (p.causal) tile = tiles - 1 - tile;  // the longest rows first
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
   const Seq sq = sequence(p, b);
-  const int map0 = MAPS == 1 ? wave & 1 : 0;  // this wave's (first) map
   const int w0 = tile * QB + (MAPS == 1 ? wave >> 1 : wave) * 32, qi = w0 + (lane & 31), qc = qi < p.Tq ? qi : p.Tq - 1;
   const T* kb = (const T*)p.k + (long)b * p.k_s[0] + (long)hk * p.k_s[2];
   const T* vb = (const T*)p.v + (long)b * p.v_s[0] + (long)hk * p.v_s[2];
-  constexpr bool HOLD = sizeof(T) == 2 ? VECTOR || NB < 8 : NB < 5;  // wide fp32 heads do not fit the registers: Q is read again for every tile
-  const T* qrow = (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2];
-  Frag8<T> q[MAPS][HOLD ? NB : 1];
-  if constexpr (HOLD)
-#pragma unroll
-    for (int i = 0; i < MAPS; ++i)
-#pragma unroll
-      for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(qrow + (long)(map0 + i) * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][ks]);
+  F f;
+  f.init(MAPS == 1 ? wave & 1 : 0, (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2], p.q_s[3], p.d, lane);
   const int last = tile * QB + QB < p.Tq ? tile * QB + QB : p.Tq;  // causal: the workgroup's last query bounds its keys
   int end = sq.len;
   if (p.causal) end = sq.start + last < end ? sq.start + last : end;
   const int steps = end > 0 ? (end + KT - 1) / KT : 0;
   const float c = p.scale * LOG2E;
-
-  f32x16_t o[MAPS][NB];
-#pragma unroll
-  for (int i = 0; i < MAPS; ++i)
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[i][n][r] = 0.f;
-  float m[MAPS], l[MAPS];  // m: both halves of a query agree; l: this half's keys
-
-#pragma unroll
-  for (int i = 0; i < MAPS; ++i) m[i] = NO_MAX, l[i] = 0.f;
 
   auto fill = [&](int step, unsigned long long bits) {
     unsigned char* buf = smem + (step & 1) * BUF;
@@ -278,75 +402,11 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_thr
     if (seen <= 0 || cur == 0) continue;
     const bool masked = (cur & low_bits(KT)) != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
     const unsigned long long mine = p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur;
-    const unsigned char* buf = smem + (s & 1) * BUF;
+    const int buf = (s & 1) * BUF;
 #pragma unroll 1
-    for (int kb32 = 0; kb32 < KT / 32; ++kb32) {
-      f32x16_t sc[MAPS];
-#pragma unroll
-      for (int i = 0; i < MAPS; ++i) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[i][r] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < NB; ++ks) {
-          Frag8<T> a;
-          ImgK::rows(buf + (map0 + i) * K_BYTES, kb32 * 32 + (lane & 31), ks, half, a);
-          if constexpr (!HOLD) load_frag<T, VECTOR>(qrow + (long)(map0 + i) * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][0]);
-          mma(a, q[i][HOLD ? ks : 0], sc[i]);
-        }
-      }
-      if (masked) {
-        const unsigned vis = (unsigned)(mine >> (kb32 * 32)) >> (4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool keep = (vis >> (8 * (r >> 2) + (r & 3))) & 1u;
-#pragma unroll
-          for (int i = 0; i < MAPS; ++i) sc[i][r] = keep ? sc[i][r] : -INFINITY;
-        }
-      }
-      float mx[MAPS];
-      bool grew = false;
-#pragma unroll
-      for (int i = 0; i < MAPS; ++i) {
-        mx[i] = sc[i][0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx[i] = fmaxf(mx[i], sc[i][r]);
-        mx[i] *= c;
-        grew = grew || mx[i] > m[i] + MAX_SLACK;
-      }
-      if (__any(grew)) {
-#pragma unroll
-        for (int i = 0; i < MAPS; ++i) {
-          const float to = fmaxf(m[i], fmaxf(mx[i], other_half(mx[i])));
-          const float f = exp2f(m[i] - to);
-          m[i] = to;
-          l[i] *= f;
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[i][n][r] *= f;
-        }
-      }
-      Frag8<T> pf[MAPS][2];
-#pragma unroll
-      for (int i = 0; i < MAPS; ++i) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          sc[i][r] = __builtin_amdgcn_exp2f(fmaf(sc[i][r], c, -m[i]));
-          l[i] += sc[i][r];
-        }
-        to_frag(sc[i], 0, pf[i][0]);
-        to_frag(sc[i], 1, pf[i][1]);
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          Frag8<T> v;
-          ImgV::cols(buf + 2 * K_BYTES, kb32 * 32 + 16 * t, n, lane, v);
-#pragma unroll
-          for (int i = 0; i < MAPS; ++i) mma(v, pf[i][t], o[i][n]);
-        }
-    }
+    for (int u = 0; u < KT / 32; ++u)
+      f.tile(smem, buf + f.map0 * K_BYTES + u * 32 * ImgK::ROW_BYTES, K_BYTES, buf + 2 * K_BYTES + u * 32 * ImgV::ROW_BYTES, masked, (unsigned)(mine >> (u * 32)) >> (4 * half), c, p.d,
+             half);
   }
 
   const float lam = p.lam[p.n_lam > 1 ? h : 0];
@@ -355,69 +415,322 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_thr
   const int dvs = (p.dv + 7) & ~7;
 #pragma unroll
   for (int i = 0; i < MAPS; ++i) {
-    l[i] += other_half(l[i]);
-    const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);  // no visible key: zeros; NaN stays
+    f.l[i] += other_half(f.l[i]);
+    const float inv = inverse_sum(f.l[i]);
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[i][n][r] *= inv;
-    // log2 of the sum; +inf for a query without keys: exp2(score - inf) = 0 in the backward passes
-    if (p.lse && live && half == 0) p.lse[(long)(map0 + i) * p.B * p.H * p.Tq + row] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
-    if (p.o1 && live) {
-      T* to = (T*)(map0 + i ? p.o2 : p.o1) + row * dvs;
+      for (int r = 0; r < 16; ++r) f.o[i][n][r] *= inv;
+    if (p.lse && live && half == 0) p.lse[(long)(f.map0 + i) * p.B * p.H * p.Tq + row] = log_sum(f.m[i], f.l[i]);
+    if (p.o1 && live)
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          store4<T>(to, n * 32 + 8 * g + 4 * half, dvs, true, o[i][n][4 * g], o[i][n][4 * g + 1], o[i][n][4 * g + 2], o[i][n][4 * g + 3]);
-    }
+      for (int n = 0; n < NB; ++n) store_block<T>((T*)(f.map0 + i ? p.o2 : p.o1) + row * dvs, n, half, dvs, f.o[i][n]);
   }
   if constexpr (MAPS == 1) {  // O_2 of the odd waves to the even ones, in the registers' own order
-    static_assert(fwd_lds<T, NB>() >= 4 * NB * 16 * 64 * 4, "the exchange fits the images' LDS");
+    static_assert(fwd_lds<T, NB>() >= NT / 128 * NB * 16 * 64 * 4, "the exchange fits the images' LDS");
     float* x = reinterpret_cast<float*>(smem) + (wave >> 1) * (NB * 16 * 64) + lane;
     __syncthreads();  // every wave is past its last image
-    if (map0)
+    if (f.map0)
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[(n * 16 + r) * 64] = o[0][n][r];
+        for (int r = 0; r < 16; ++r) x[(n * 16 + r) * 64] = f.o[0][n][r];
     __syncthreads();
-    if (map0) return;
+    if (f.map0) return;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[0][n][r] -= lam * x[(n * 16 + r) * 64];
+      for (int r = 0; r < 16; ++r) f.o[0][n][r] -= lam * x[(n * 16 + r) * 64];
   } else {
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[0][n][r] -= lam * o[MAPS - 1][n][r];
+      for (int r = 0; r < 16; ++r) f.o[0][n][r] -= lam * f.o[MAPS - 1][n][r];
   }
   float ss = 0.f;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) ss += o[0][n][r] * o[0][n][r];
-  float f = p.out_scale;
+    for (int r = 0; r < 16; ++r) ss += f.o[0][n][r] * f.o[0][n][r];
+  float g = p.out_scale;
   if (p.norm) {
     ss += other_half(ss);
-    f *= 1.f / sqrtf(ss / (float)p.dv + p.eps);
+    g *= 1.f / sqrtf(ss / (float)p.dv + p.eps);
   }
-  if (live) {
-    T* out = (T*)p.out + (long)b * p.o_s[0] + (long)qi * p.o_s[1] + (long)h * p.o_s[2];
-    const bool vec = p.out_vec;
+  if (!live) return;
+  T* out = (T*)p.out + (long)b * p.o_s[0] + (long)qi * p.o_s[1] + (long)h * p.o_s[2];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) store_result<T>(p, out, n, half, g, f.o[0][n]);
+}
+
+// few queries (single tokens against a cache, short sequences): workgroup = (batch, key / value head, 32 rows, split of the keys), a row being a
+// (query head of the group, query) pair, so that one read of the cache serves all heads that share it.  The WAVES take different keys, 32 at a time, from
+// images of their own (no barrier in the loop), and add up in LDS.  With more than one split the sums go to `partial` and
+// diff_attn_fwd_join_kernel finishes the rows: otherwise a cache would be read by as many CUs as there are heads.
+template <typename T, int NB> struct Few {
+  static constexpr int MAPS = NB >= 5 ? 1 : 2;
+  static constexpr int KEY_WAVES = MAPS == 2 ? 4 : (sizeof(T) == 2 ? 2 : 1), WAVES = KEY_WAVES * (3 - MAPS), THREADS = WAVES * 64;
+  static constexpr int K_BYTES = 32 * Img<T, (NB + 1) / 2>::ROW_BYTES, V_BYTES = 32 * Img<T, NB>::ROW_BYTES, IMAGES = MAPS * K_BYTES + V_BYTES;
+  static constexpr int STAGES = 2 * WAVES * IMAGES <= 128 * 1024 ? 2 : 1;
+  static constexpr int BLOCK = 16 * 64;  // floats of a 32 x 32 fragment block
+  static constexpr int EXCHANGE = WAVES * NB * BLOCK * 4;  // one map of every wave
+  static constexpr int SUMS = WAVES * 2 * 32 * 2 * 4;      // (m, l) of every wave and map; later the rows' sums of squares
+  static constexpr int QUERIES = 2 * K_BYTES;              // the 32 rows' queries, both maps
+  static constexpr int LDS = (STAGES * WAVES * IMAGES > EXCHANGE ? STAGES * WAVES * IMAGES : EXCHANGE) + QUERIES + SUMS;
+  static constexpr int ROW_FLOATS = 2 * (NB * 32 + 2);     // of one row in `partial`: both maps' sums, maxima, l
+};
+
+template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, NB>::THREADS), 1) void diff_attn_few_kernel(tfpp_diff_attn_params p) {
+  typedef Few<T, NB> W;
+  typedef Fwd<T, NB, VECTOR, Q_LDS, W::MAPS> F;
+  typedef typename F::ImgK ImgK;
+  typedef typename F::ImgV ImgV;
+  constexpr int MAPS = W::MAPS, WAVES = W::WAVES, KW = W::KEY_WAVES;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
+  const int group = p.H / p.Hkv, rows = group * p.Tq, tiles = (rows + 31) / 32, splits = p.splits;
+  int bh = blockIdx.x / (tiles * splits);
+  const int rest = blockIdx.x % (tiles * splits), tile = rest / splits, split = rest % splits;
+  const int b = bh / p.Hkv, hk = bh % p.Hkv;
+  const Seq sq = sequence(p, b);
+  const int r = tile * 32 + col, rc = r < rows ? r : rows - 1, h = hk * group + rc / p.Tq, qi = rc % p.Tq;
+  const bool live = r < rows;
+  const T* kb = (const T*)p.k + (long)b * p.k_s[0] + (long)hk * p.k_s[2];
+  const T* vb = (const T*)p.v + (long)b * p.v_s[0] + (long)hk * p.v_s[2];
+  F f;
+  f.init(MAPS == 1 ? wave & 1 : 0, nullptr, 0, p.d, lane);
+  unsigned char* qimg = smem + (W::LDS - W::SUMS - W::QUERIES);
+  f.q_at = W::LDS - W::SUMS - W::QUERIES + f.map0 * W::K_BYTES + ImgK::rows_at(lane);
+  // the rows' queries into LDS, 16 bytes (or elements, unaligned) at a time; their rows lie in several heads, so not by `fill`
+  for (int i = tid; i < 2 * 32 * ImgK::USED; i += W::THREADS) {
+    const int map = i / (32 * ImgK::USED), qr = i / ImgK::USED % 32, ch = i % ImgK::USED, n = tile * 32 + qr < rows ? tile * 32 + qr : rows - 1;
+    const T* src = (const T*)p.q + (long)b * p.q_s[0] + (long)(n % p.Tq) * p.q_s[1] + (long)(hk * group + n / p.Tq) * p.q_s[2] + (long)map * p.q_s[3] + ch * ImgK::VEC;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if constexpr (VECTOR) {
+      if (ch * ImgK::VEC < p.d) u = *reinterpret_cast<const uint4*>(src);
+    } else {
+      float t[ImgK::VEC];
+#pragma unroll
+      for (int e = 0; e < ImgK::VEC; ++e) t[e] = ch * ImgK::VEC + e < p.d ? ElemTraits<T>::to_f(src[e]) : 0.f;
+      u = pack16<T>(t);
+    }
+    *reinterpret_cast<uint4*>(qimg + map * W::K_BYTES + ImgK::off(qr, ch)) = u;
+  }
+  __syncthreads();
+  // keys of this split: whole blocks of 32, an equal share of what the tile's rows see
+  int end = sq.len;
+  if (p.causal) {
+    const int r1 = tile * 32 + 31 < rows ? tile * 32 + 31 : rows - 1, last = tile * 32 / p.Tq == r1 / p.Tq ? r1 % p.Tq : p.Tq - 1;
+    end = sq.start + last + 1 < end ? sq.start + last + 1 : end;
+  }
+  const int blocks = end > 0 ? (end + 31) / 32 : 0, per = (blocks + splits - 1) / splits;
+  const int first = split * per, stop = first + per < blocks ? first + per : blocks;
+  const float c = p.scale * LOG2E;
+  const int lim = p.causal ? sq.start + qi + 1 : end;  // keys this row sees
+
+  auto fill = [&](int block, int stage, unsigned bits) {
+    unsigned char* buf = smem + (stage * WAVES + wave) * W::IMAGES;
+    const long j0 = (long)block * 32;
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) ImgK::template fill<32, VECTOR, 64>(buf + i * W::K_BYTES, kb + j0 * p.k_s[1] + (f.map0 + i) * p.k_s[3], p.k_s[1], p.d, bits, lane);
+    ImgV::template fill<32, VECTOR, 64>(buf + MAPS * W::K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, bits, lane);
+  };
+  const int kw = MAPS == 1 ? wave >> 1 : wave;
+  unsigned bits = 0;
+  int stage = 0;
+  if (first + kw < stop) {
+    bits = (unsigned)key_bits(p, b, (first + kw) * 32, sq.len, lane);
+    fill(first + kw, 0, bits);
+  }
+  for (int k = first + kw; k < stop; k += KW) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's images are complete
+    const unsigned cur = bits;
+    const int buf = (stage * WAVES + wave) * W::IMAGES;
+    if constexpr (W::STAGES == 2) {
+      stage ^= 1;
+      if (k + KW < stop) {
+        bits = (unsigned)key_bits(p, b, (k + KW) * 32, sq.len, lane);
+        fill(k + KW, stage, bits);
+      }
+    }
+    const unsigned mine = cur & (unsigned)low_bits(lim - k * 32);
+    if (__any(mine != 0)) f.tile(smem, buf, W::K_BYTES, buf + MAPS * W::K_BYTES, __any(mine != ~0u), mine >> (4 * half), c, p.d, half);
+    if constexpr (W::STAGES == 1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (every read of the image has returned before it is filled again)
+      if (k + KW < stop) {
+        bits = (unsigned)key_bits(p, b, (k + KW) * 32, sq.len, lane);
+        fill(k + KW, 0, bits);
+      }
+    }
+  }
+
+  // add the waves up: maxima and sums of all waves first, then each map's O, block by block; wave w finishes the channel blocks w, w + WAVES, ..
+  float* ml = reinterpret_cast<float*>(smem + (W::LDS - W::SUMS));  // [wave][map of the wave][m, l][32]
+  float* x = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int i = 0; i < MAPS; ++i) {
+    f.l[i] += other_half(f.l[i]);
+    if (half == 0) {
+      ml[((wave * 2 + i) * 2) * 32 + col] = f.m[i];
+      ml[((wave * 2 + i) * 2 + 1) * 32 + col] = f.l[i];
+    }
+  }
+  __syncthreads();
+  float M[2], L[2];
+#pragma unroll
+  for (int map = 0; map < 2; ++map) {
+    M[map] = NO_MAX;
+    L[map] = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) M[map] = fmaxf(M[map], ml[(((MAPS == 1 ? 2 * w + map : w) * 2 + (MAPS == 1 ? 0 : map)) * 2) * 32 + col]);
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      const float* q = ml + (((MAPS == 1 ? 2 * w + map : w) * 2 + (MAPS == 1 ? 0 : map)) * 2) * 32 + col;
+      L[map] += q[32] * exp2f(q[0] - M[map]);
+    }
+  }
+  constexpr int MINE = (NB + WAVES - 1) / WAVES;
+  f32x16_t o[2][MINE];
+#pragma unroll
+  for (int round = 0; round < MAPS; ++round) {
+    const float g = exp2f(f.m[round] - (MAPS == 1 ? (f.map0 ? M[1] : M[0]) : M[round]));
+    if (round) __syncthreads();
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        __builtin_amdgcn_sched_barrier(0);  // (the weights of all channels at once would not fit the registers)
-        const int ch = n * 32 + 8 * g + 4 * half;
-        if (ch >= p.dv) continue;
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = p.norm && ch + e < p.dv ? f * norm_weight(p, ch + e) : f;
-        store4<T>(out, ch, p.dv, vec, o[0][n][4 * g] * w[0], o[0][n][4 * g + 1] * w[1], o[0][n][4 * g + 2] * w[2], o[0][n][4 * g + 3] * w[3]);
+      for (int e = 0; e < 16; ++e) {
+        x[(wave * NB + n) * W::BLOCK + e * 64 + lane] = f.o[round][n][e] * g;
+        if (e == 15) __builtin_amdgcn_sched_barrier(0);
       }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+      const int n = wave + j * WAVES;
+#pragma unroll
+      for (int map = 0; map < 2; ++map) {
+        if (MAPS == 2 && map != round) continue;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[map][j][e] = 0.f;
+        if (n < NB)
+#pragma unroll
+          for (int w = 0; w < KW; ++w) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[map][j][e] += x[((MAPS == 1 ? 2 * w + map : w) * NB + n) * W::BLOCK + e * 64 + lane];
+            __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+    }
+  }
+  if (splits > 1) {
+    float* out = p.partial + ((((long)split * p.B + b) * p.Hkv + hk) * rows + rc) * W::ROW_FLOATS;
+    if (!live) return;
+#pragma unroll
+    for (int map = 0; map < 2; ++map) {
+#pragma unroll
+      for (int j = 0; j < MINE; ++j)
+        if (wave + j * WAVES < NB)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float2*>(out + map * NB * 32 + (wave + j * WAVES) * 32 + 8 * g + 4 * half) = make_float2(o[map][j][4 * g], o[map][j][4 * g + 1]),
+            *reinterpret_cast<float2*>(out + map * NB * 32 + (wave + j * WAVES) * 32 + 8 * g + 4 * half + 2) = make_float2(o[map][j][4 * g + 2], o[map][j][4 * g + 3]);
+      if (wave == 0 && half == 0) {
+        out[2 * NB * 32 + map * 2] = M[map];
+        out[2 * NB * 32 + map * 2 + 1] = L[map];
+      }
+    }
+    return;
+  }
+  const float lam = p.lam[p.n_lam > 1 ? h : 0];
+  const long row = ((long)b * p.H + h) * p.Tq + qi;
+  const int dvs = (p.dv + 7) & ~7;
+  float ss = 0.f;
+#pragma unroll
+  for (int map = 0; map < 2; ++map) {
+    const float inv = inverse_sum(L[map]);
+    if (p.lse && live && half == 0 && wave == 0) p.lse[(long)map * p.B * p.H * p.Tq + row] = log_sum(M[map], L[map]);
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[map][j][e] *= inv;
+      if (p.o1 && live && wave + j * WAVES < NB) store_block<T>((T*)(map ? p.o2 : p.o1) + row * dvs, wave + j * WAVES, half, dvs, o[map][j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < MINE; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      o[0][j][e] -= lam * o[1][j][e];
+      ss += o[0][j][e] * o[0][j][e];
+    }
+  float g = p.out_scale;
+  if (p.norm) {
+    ss += other_half(ss);
+    __syncthreads();  // (m and l have been read)
+    if (half == 0) ml[wave * 32 + col] = ss;
+    __syncthreads();
+    ss = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) ss += ml[w * 32 + col];
+    g *= 1.f / sqrtf(ss / (float)p.dv + p.eps);
+  }
+  if (!live) return;
+  T* out = (T*)p.out + (long)b * p.o_s[0] + (long)qi * p.o_s[1] + (long)h * p.o_s[2];
+#pragma unroll
+  for (int j = 0; j < MINE; ++j)
+    if (wave + j * WAVES < NB) store_result<T>(p, out, wave + j * WAVES, half, g, o[0][j]);
+}
+
+// the splits' sums of a row -> its result: one wave a row, channels lane, lane + 64, ..
+template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(tfpp_diff_attn_params p, int width) {
+  const int lane = threadIdx.x & 63, group = p.H / p.Hkv, rows = group * p.Tq, dvs = (p.dv + 7) & ~7;
+  const long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6), all = (long)p.B * p.Hkv * rows, pitch = 2 * (width + 2);
+  if (n >= all) return;
+  const int r = (int)(n % rows), hk = (int)(n / rows % p.Hkv), b = (int)(n / rows / p.Hkv), h = hk * group + r / p.Tq, qi = r % p.Tq;
+  const float* src = p.partial + n * pitch;
+  const long row = ((long)b * p.H + h) * p.Tq + qi;
+  float M[2] = {NO_MAX, NO_MAX}, L[2] = {0.f, 0.f}, o[2][4];
+  for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+    for (int map = 0; map < 2; ++map) M[map] = fmaxf(M[map], src[s * all * pitch + 2 * width + 2 * map]);
+#pragma unroll
+  for (int map = 0; map < 2; ++map)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[map][e] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float* q = src + s * all * pitch;
+#pragma unroll
+    for (int map = 0; map < 2; ++map) {
+      const float f = exp2f(q[2 * width + 2 * map] - M[map]);
+      L[map] += f * q[2 * width + 2 * map + 1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < p.dv) o[map][e] += f * q[map * width + lane + 64 * e];
+    }
+  }
+  const float lam = p.lam[p.n_lam > 1 ? h : 0];
+#pragma unroll
+  for (int map = 0; map < 2; ++map) {
+    const float inv = inverse_sum(L[map]);
+    if (p.lse && lane == 0) p.lse[(long)map * p.B * p.H * p.Tq + row] = log_sum(M[map], L[map]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[map][e] *= inv;
+      if (p.o1 && lane + 64 * e < dvs) ((T*)(map ? p.o2 : p.o1))[row * dvs + lane + 64 * e] = ElemTraits<T>::from_f(o[map][e]);
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    o[0][e] -= lam * o[1][e];
+    ss += o[0][e] * o[0][e];
+  }
+  float g = p.out_scale;
+  if (p.norm) g *= 1.f / sqrtf(wave_sum(ss) / (float)p.dv + p.eps);
+  T* out = (T*)p.out + (long)b * p.o_s[0] + (long)qi * p.o_s[1] + (long)h * p.o_s[2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int ch = lane + 64 * e;
+    if (ch < p.dv) out[ch] = ElemTraits<T>::from_f(o[0][e] * (p.norm ? g * norm_weight(p, ch) : g));
   }
 }
 
@@ -541,7 +854,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int tiles = (p.Tq + QB - 1) / QB;
   int bh, tile;
-  place(p.B * p.H, tiles, bh, tile);
+  place(p.B * p.H, tiles, p.causal, bh, tile);
   if (p.causal) tile = tiles - 1 - tile;
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv), dvs = (p.dv + 7) & ~7;
   const Seq sq = sequence(p, b);
@@ -573,6 +886,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
     for (int n = 0; n < CD; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[i][n][r] = 0.f;
+  const int k_rows = ImgK::rows_at(lane), v_rows = ImgV::rows_at(lane), k_cols = ImgK::cols_at(lane);
   auto fill = [&](int step, unsigned long long bits) {
     unsigned char* buf = smem + (step & 1) * BUF;
     const long j0 = (long)step * KT;
@@ -597,7 +911,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
     if ((p.causal && sq.start + w0 + 32 - j0 <= 0) || cur == 0) continue;
     const bool masked = cur != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
     const unsigned vis = (unsigned)(p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur) >> (4 * half);
-    const unsigned char* buf = smem + (s & 1) * BUF;
+    const int buf = (s & 1) * BUF, kr = k_rows + buf, vr = v_rows + buf + 2 * K_BYTES, kc = k_cols + buf;
     f32x16_t sc[2], dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sc[0][r] = sc[1][r] = dp[r] = 0.f;
@@ -606,14 +920,14 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
 #pragma unroll
       for (int ks = 0; ks < NB; ++ks) {
         Frag8<T> a;
-        ImgK::rows(buf + i * K_BYTES, lane & 31, ks, half, a);
+        ImgK::rows(smem + i * K_BYTES, kr, ks, a);
         if constexpr (!HOLD) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][0]);
         mma(a, q[i][HOLD ? ks : 0], sc[i]);
       }
 #pragma unroll
     for (int ks = 0; ks < 2 * NB; ++ks) {
       Frag8<T> a;
-      ImgV::rows(buf + 2 * K_BYTES, lane & 31, ks, half, a);
+      ImgV::rows(smem, vr, ks, a);
       if constexpr (!HOLD) load_frag<T, true>((const T*)p.d_o + row * dvs, ks * 16 + half * 8, dvs, true, dof[0]);
       mma(a, dof[HOLD ? ks : 0], dp);
     }
@@ -637,7 +951,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
 #pragma unroll
         for (int n = 0; n < CD; ++n) {
           Frag8<T> a;
-          ImgK::cols(buf + i * K_BYTES, 16 * t, n, lane, a);
+          ImgK::cols(smem + i * K_BYTES + 16 * t * ImgK::ROW_BYTES, kc, n, a);
           mma(a, ds, dq[i][n]);
         }
       }
@@ -662,18 +976,18 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
 //    separate workgroups; S and dP are computed again (3 / 2 of the flop).
 enum { PART_ALL, PART_DK, PART_DV };
 template <typename T, int NB> constexpr bool dkv_split() { return NB >= (sizeof(T) == 2 ? 5 : 4); }
-template <typename T, int NB> constexpr int dkv_lds() { return 2 * (32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + 4 * 32 * 4); }
+template <typename T, int NB> constexpr int dkv_lds() { return 2 * (32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + 1024); }
 
 template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds__(256, (PART == PART_ALL ? NB <= (sizeof(T) == 2 ? 2 : 1) : NB <= (sizeof(T) == 2 ? 5 : 4)) ? 2 : 1) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
   constexpr int QT = 32, NT = 256, MAPS = PART == PART_DK ? 1 : 2, CD = (NB + 1) / 2;
   typedef Img<T, CD> ImgQ;
   typedef Img<T, NB> ImgO;
-  constexpr int Q_BYTES = QT * ImgQ::ROW_BYTES, O_BYTES = QT * ImgO::ROW_BYTES, BUF = 2 * Q_BYTES + O_BYTES + 4 * QT * 4;
+  constexpr int Q_BYTES = QT * ImgQ::ROW_BYTES, O_BYTES = QT * ImgO::ROW_BYTES, BUF = 2 * Q_BYTES + O_BYTES + 1024;  // (4 x 32 row values; images start at whole rows, <= 1 KB)
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int tiles = (p.Tk + QB - 1) / QB, group = p.H / p.Hkv;
   int bh, tile;
-  place(p.B * p.Hkv, tiles, bh, tile);
+  place(p.B * p.Hkv, tiles, p.causal, bh, tile);
   const int b = bh / p.Hkv, hk = bh % p.Hkv, dvs = (p.dv + 7) & ~7;
   const Seq sq = sequence(p, b);
   const int w0 = tile * QB + wave * 32, kj = w0 + (lane & 31);
@@ -712,6 +1026,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
   const bool any = tile * QB < sq.len && q_lo < p.Tq;
   const int per = any ? (p.Tq - q_lo + QT - 1) / QT : 0, steps = per * group;
 
+  const int q_rows = ImgQ::rows_at(lane), o_rows = ImgO::rows_at(lane), q_cols = ImgQ::cols_at(lane), o_cols = ImgO::cols_at(lane);
   auto fill = [&](int step) {
     unsigned char* buf = smem + (step & 1) * BUF;
     const int h = hk * group + step / per, q0 = q_lo + step % per * QT;
@@ -737,8 +1052,8 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
     if (p.causal && sq.start + q0 + QT - 1 < w0) continue;  // no query of the tile sees a key of this wave
     const bool diag = p.causal && sq.start + q0 < w0 + 31;
     const float lam = p.lam[p.n_lam > 1 ? h : 0];
-    const unsigned char* buf = smem + (s & 1) * BUF;
-    const float* st = reinterpret_cast<const float*>(buf + 2 * Q_BYTES + O_BYTES);
+    const int buf = (s & 1) * BUF, qr = q_rows + buf, orow = o_rows + buf + 2 * Q_BYTES, qcol = q_cols + buf, ocol = o_cols + buf + 2 * Q_BYTES;
+    const float* st = reinterpret_cast<const float*>(smem + buf + 2 * Q_BYTES + O_BYTES);
     f32x16_t sc[MAPS], dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -751,7 +1066,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
       for (int ks = 0; ks < NB; ++ks) {
         Frag8<T> a;
-        ImgQ::rows(buf + (map0 + i) * Q_BYTES, lane & 31, ks, half, a);
+        ImgQ::rows(smem + (map0 + i) * Q_BYTES, qr, ks, a);
         if constexpr (!HOLD) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, seen, k[i][0]);
         mma(a, k[i][HOLD ? ks : 0], sc[i]);
       }
@@ -759,7 +1074,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
       for (int ks = 0; ks < 2 * NB; ++ks) {
         Frag8<T> a;
-        ImgO::rows(buf + 2 * Q_BYTES, lane & 31, ks, half, a);
+        ImgO::rows(smem, orow, ks, a);
         if constexpr (!HOLD) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, seen, v[0]);
         mma(a, v[HOLD ? ks : 0], dp);
       }
@@ -792,7 +1107,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           Frag8<T> a;
-          ImgO::cols(buf + 2 * Q_BYTES, 16 * t, n, lane, a);
+          ImgO::cols(smem + 16 * t * ImgO::ROW_BYTES, ocol, n, a);
           mma(a, f, dv[n]);
         }
       }
@@ -803,7 +1118,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
           for (int n = 0; n < CD; ++n) {
             Frag8<T> a;
-            ImgQ::cols(buf + (map0 + i) * Q_BYTES, 16 * t, n, lane, a);
+            ImgQ::cols(smem + (map0 + i) * Q_BYTES + 16 * t * ImgQ::ROW_BYTES, qcol, n, a);
             mma(a, f, dk[i][n]);
           }
         }
@@ -901,9 +1216,19 @@ template <typename K> int start(K* kernel, dim3 grid, int threads, int lds, unsi
   return 0;
 }
 
-enum { STEP_FWD, STEP_DQ, STEP_DKV };
+enum { STEP_FWD, STEP_FEW, STEP_DQ, STEP_DKV };
 template <typename T, int NB, bool VECTOR> int launch(const tfpp_diff_attn_params& p, int step, hipStream_t st) {
-  static unsigned long long done[4] = {0, 0, 0, 0};
+  static unsigned long long done[5] = {0, 0, 0, 0, 0};
+  if (step == STEP_FEW) {
+    const long n = (long)p.B * p.Hkv * (((long)(p.H / p.Hkv) * p.Tq + 31) / 32) * p.splits;
+    if (n > 0x7fffffffl) return TFPP_EINVAL;
+    const int rc = start(diff_attn_few_kernel<T, NB, VECTOR>, dim3((unsigned)n), Few<T, NB>::THREADS, Few<T, NB>::LDS, &done[4], p, st);
+    if (rc || p.splits == 1) return rc;
+    const long rows = (long)p.B * p.H * p.Tq;
+    hipLaunchKernelGGL(diff_attn_fwd_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, NB * 32);
+    TFPP_CHECK_LAUNCH();
+    return 0;
+  }
   const int qb = step == STEP_FWD ? fwd_queries<T, NB>() : QB;
   const long tiles = ((step == STEP_DKV ? p.Tk : p.Tq) + qb - 1) / qb, n = tiles * p.B * (step == STEP_DKV ? p.Hkv : p.H);
   if (n > 0x7fffffffl) return TFPP_EINVAL;
@@ -929,6 +1254,19 @@ template <typename T> int dispatch(const tfpp_diff_attn_params& p, int step, hip
   return DA_GO(8);
 #undef DA_GO
 }
+int padded_blocks(const tfpp_diff_attn_params& p) {  // NB of dispatch()
+  const int need = (p.d + 15) / 16 > (p.dv + 31) / 32 ? (p.d + 15) / 16 : (p.dv + 31) / 32;
+  return need <= 2 ? need : (need <= 4 ? 4 : (need <= 5 ? 5 : 8));
+}
+// Which forward kernel, and how many splits of the keys?  0: the one for many queries.
+int few_splits(const tfpp_diff_attn_params& p) {
+  const long wg = (long)p.B * p.H * ((p.Tq + QB - 1) / QB);
+  if (wg >= 512) return 0;
+  const long rows = (long)(p.H / p.Hkv) * p.Tq, base = (long)p.B * p.Hkv * ((rows + 31) / 32);
+  long n = (512 + base - 1) / base, most = (p.Tk + 511) / 512;  // two workgroups a CU; at least 512 keys (4 blocks a wave) in a split
+  if (n > most) n = most;
+  return n < 1 ? 1 : (int)n;
+}
 int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass for each head: 64 rows each at least, about 1024 in all
   const long rows = (long)p.B * p.Tq;
   long n = 1024 / p.H > 1 ? 1024 / p.H : 1;
@@ -941,7 +1279,17 @@ extern "C" int tfpp_diff_attn_fwd(const tfpp_diff_attn_params* pp, int dtype, vo
   if (!pp || !valid(*pp, dtype) || !pp->out || (pp->o1 != nullptr) != (pp->o2 != nullptr)) return TFPP_EINVAL;
   tfpp_diff_attn_params p = *pp;
   p.out_vec = quad(p.out, p.o_s, 3, dtype == TFPP_F32 ? 4 : 2);
-  return dtype == TFPP_F32 ? dispatch<float>(p, STEP_FWD, (hipStream_t)stream) : dispatch<bf16_t>(p, STEP_FWD, (hipStream_t)stream);
+  p.splits = few_splits(p);
+  if (p.splits > 1 && !p.partial) return TFPP_EINVAL;
+  const int step = p.splits ? STEP_FEW : STEP_FWD;
+  return dtype == TFPP_F32 ? dispatch<float>(p, step, (hipStream_t)stream) : dispatch<bf16_t>(p, step, (hipStream_t)stream);
+}
+
+extern "C" int tfpp_diff_attn_fwd_partial_floats(const tfpp_diff_attn_params* p, int64_t* out) {
+  if (!p || !out || p->B < 1 || p->H < 1 || p->Hkv < 1 || p->Tq < 1 || p->Tk < 1 || p->d < 1 || p->dv < 1) return TFPP_EINVAL;
+  const int splits = few_splits(*p);
+  *out = splits > 1 ? (int64_t)splits * p->B * p->H * p->Tq * 2 * (padded_blocks(*p) * 32 + 2) : 0;
+  return 0;
 }
 
 extern "C" int tfpp_diff_attn_bwd_partial_floats(const tfpp_diff_attn_params* p, int64_t* out) {

@@ -1654,6 +1654,11 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
     p.o_s[:] = os_
     if save:
       p.o1, p.o2, p.lse = ctx.o1.data_ptr(), ctx.o2.data_ptr(), ctx.lse.data_ptr()
+    n_part = ctypes.c_int64()
+    lib.tfpp_diff_attn_fwd_partial_floats(ctypes.byref(p), ctypes.addressof(n_part))
+    if n_part.value:  # scratch of this call alone
+      partial = torch.empty(n_part.value, device=dev, dtype=torch.float32)
+      p.partial = partial.data_ptr()
     if lib.profiler is not None:
       lib.profiler.tag(f'diff_attn_fwd<{"f32" if q.dtype == torch.float32 else "bf16"}>', float(B * H * Tq * Tk * (4 * d + 4 * dv)))
     lib.tfpp_diff_attn_fwd(ctypes.byref(p), dt(q), stream())

@@ -724,11 +724,12 @@ typedef struct {
   void *dnorm_w, *dq_out, *dk_out, *dv_out;
   int64_t ld_mask, q_s[4], k_s[4], v_s[3], o_s[3], do_s[3], dq_s[4], dk_s[4], dv_s[3];
   int B, H, Hkv, Tq, Tk, d, dv, n_lam, norm, norm_w_bf16, causal, q_start_all;
-  int out_vec, dq_vec, dk_vec, dv_vec; /* set by the library */
+  int out_vec, dq_vec, dk_vec, dv_vec, splits; /* set by the library */
   float scale, out_scale, eps;
 } tfpp_diff_attn_params;
 int tfpp_diff_attn_fwd(const tfpp_diff_attn_params* p, int dtype, void* stream);
 int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* p, int dtype, void* stream);
+int tfpp_diff_attn_fwd_partial_floats(const tfpp_diff_attn_params* p, int64_t* out); /* floats the forward pass needs in partial: 0 or more */
 int tfpp_diff_attn_bwd_partial_floats(const tfpp_diff_attn_params* p, int64_t* out);
 /* lam[i] = exp(lq1[i] . lk1[i]) - exp(lq2[i] . lk2[i]) + init over n vectors of d values each, and the gradients of the vectors (stored). */
 int tfpp_diff_lambda(const void* lq1, const void* lk1, const void* lq2, const void* lk2, float init, float* lam, int n, int d, int dtype, void* stream);
