@@ -8,8 +8,8 @@
 // dy, dh, x, a (, g), writes dx, da (, dg):
 //   dY = dy + pre'(dh)     dx = alpha dY     dn = dY s act(g)     dg = dY s n act'(g)     ds = sum dY act(g) n     da = post'(dn)
 //   LayerNorm': rstd (dz w - mean(dz w) - xh mean(dz w xh));  RMS': without the middle term;  dw = sum dz xh, db = sum dz.
-// Layout: a row belongs to TPR threads (64 .. 512, at most 8 elements each: 16 would not fit the registers beside their column sums, hence C <= 4096), a workgroup holds max(TPR, 256) threads;
-// row sums are wave shuffles plus one LDS exchange when TPR > 64.  Column sums (the parameter gradients) stay in registers over all rows of the
+// Layout: a row belongs to TPR threads (64 .. 512, at most 8 elements each: 16 would not fit the registers beside their column sums, hence C <= 4096);
+// row sums are DPP moves plus one LDS exchange when TPR > 64.  Column sums (the parameter gradients) stay in registers over all rows of the
 // workgroup, one row of partials per workgroup, added in a fixed order by block_norm_colsum_kernel: bit-reproducible.
 #include "common.h"
 #include "../../include/tfpp.h"
@@ -36,6 +36,19 @@ template <typename T, int TPR, int EPT, bool ALIGNED> struct Row {
       for (int e = 0; e < EPT; ++e) f[e] = col(t, e) < C ? ElemTraits<T>::to_f(p[col(t, e)]) : 0.f;
     }
   }
+  // a row as it lies in memory, fetched one iteration ahead of its use (aligned rows: 16 bytes of it are 4 registers)
+  struct Raw { uint4 u[ALIGNED ? EPT / V : 1]; };
+  __device__ static __forceinline__ void fetch(const T* __restrict__ p, int t, int C, Raw& r) {
+    if constexpr (ALIGNED)
+#pragma unroll
+      for (int e = 0; e < EPT; e += V) r.u[e / V] = col(t, e) < C ? *reinterpret_cast<const uint4*>(p + col(t, e)) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ static __forceinline__ void take(const Raw& r, const T* __restrict__ p, int t, int C, float (&f)[EPT]) {
+    if constexpr (ALIGNED)
+#pragma unroll
+      for (int e = 0; e < EPT; e += V) unpack16<T>(r.u[e / V], f + e);
+    else load(p, t, C, f);
+  }
   __device__ static __forceinline__ void store(T* __restrict__ p, int t, int C, const float (&f)[EPT]) {
     if constexpr (ALIGNED) {
 #pragma unroll
@@ -49,31 +62,54 @@ template <typename T, int TPR, int EPT, bool ALIGNED> struct Row {
   }
 };
 // per-channel fp32 parameter (null: the given constant)
-template <typename R, int EPT> __device__ __forceinline__ void load_param(const float* __restrict__ p, float none, int t, int C, float (&f)[EPT]) {
+template <typename T, int TPR, int EPT, bool ALIGNED> __device__ __forceinline__ void load_param(const float* __restrict__ p, float none, int t, int C, float (&f)[EPT]) {
+  typedef Row<T, TPR, EPT, ALIGNED> R;
 #pragma unroll
-  for (int e = 0; e < EPT; ++e) f[e] = (p && R::col(t, e) < C) ? p[R::col(t, e)] : none;
+  for (int e = 0; e < EPT; ++e) f[e] = none;
+  if (!p) return;
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int e = 0; e < EPT; e += 4)
+      if (R::col(t, e) < C) load_vec<float>(p + R::col(t, e), f + e);
+  } else {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e)
+      if (R::col(t, e) < C) f[e] = p[R::col(t, e)];
+  }
 }
+
+// Sum over a wave by DPP moves (register to register; __shfl_xor goes through LDS, ~100 cycles a step, and a row needs up to four sums one after the other)
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) { return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
+__device__ __forceinline__ float row_wave_sum(float v) {
+  v = dpp_add<0xB1>(v);   // lane ^ 1
+  v = dpp_add<0x4E>(v);   // lane ^ 2
+  v = dpp_add<0x141>(v);  // mirror within 8
+  v = dpp_add<0x140>(v);  // mirror within 16
+  const int i = __float_as_int(v);
+  return (__int_as_float(__builtin_amdgcn_readlane(i, 0)) + __int_as_float(__builtin_amdgcn_readlane(i, 16))) +
+         (__int_as_float(__builtin_amdgcn_readlane(i, 32)) + __int_as_float(__builtin_amdgcn_readlane(i, 48)));
+}
+
+constexpr int threads_of(int tpr) { return tpr > 64 ? tpr : 256; }  // one row a workgroup, four where a row is one wave (no barrier at all)
 
 // Sums of N values over the TPR threads of a row, the same in all of them.  `sm` alternates between two halves so that one barrier per call is
 // enough: a wave may write the other half while slower waves still read this one.
-template <int TPR, int NT, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* sm, int& phase) {
+template <int TPR, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* sm, int& phase) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  for (int i = 0; i < N; ++i) v[i] = row_wave_sum(v[i]);
   if constexpr (TPR > 64) {
-    constexpr int W = NT / 64, WR = TPR / 64;
+    constexpr int W = TPR / 64;
     float* s = sm + phase * (2 * W);
     phase ^= 1;
-    const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[i * W + wave] = v[i];
+      for (int i = 0; i < N; ++i) s[i * W + (threadIdx.x >> 6)] = v[i];
     __syncthreads();
-    const int first = wave / WR * WR;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       v[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < WR; ++w) v[i] += s[i * W + first + w];
+      for (int w = 0; w < W; ++w) v[i] += s[i * W + w];
     }
   }
 }
@@ -90,15 +126,14 @@ __device__ __forceinline__ float gate_slope(float g, int act) {  // from the act
 }
 
 // mean (LayerNorm only) and rstd of a row held in registers: the mean first, then the centred squares (no cancellation)
-template <typename R, int TPR, int NT, int EPT> __device__ __forceinline__ void stats(const float (&f)[EPT], int t, int C, int layer, float eps, float* sm, int& phase, float& mean,
-                                                                                    float& rstd) {
+template <typename R, int TPR, int EPT> __device__ __forceinline__ void stats(const float (&f)[EPT], int t, int C, int layer, float eps, float* sm, int& phase, float& mean, float& rstd) {
   mean = 0.f;
   const float inv = 1.f / (float)C;
   if (layer) {
     float s[1] = {0.f};
 #pragma unroll
     for (int e = 0; e < EPT; ++e) s[0] += f[e];
-    row_sums<TPR, NT, 1>(s, sm, phase);
+    row_sums<TPR, 1>(s, sm, phase);
     mean = s[0] * inv;
   }
   float q[1] = {0.f};
@@ -107,64 +142,69 @@ template <typename R, int TPR, int NT, int EPT> __device__ __forceinline__ void 
     const float d = R::col(t, e) < C ? f[e] - mean : 0.f;
     q[0] += d * d;
   }
-  row_sums<TPR, NT, 1>(q, sm, phase);
+  row_sums<TPR, 1>(q, sm, phase);
   rstd = 1.f / sqrtf(q[0] * inv + eps);
 }
 
-template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_fwd_kernel(tfpp_block_norm_params p) {
-  constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+// A workgroup keeps the parameters in registers and takes the rows w, w + G, ..; the next row is on its way while this one is worked on.
+template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds__(threads_of(TPR)) void block_norm_fwd_kernel(tfpp_block_norm_params p) {
+  constexpr int NT = threads_of(TPR), RPB = NT / TPR;
   typedef Row<T, TPR, EPT, ALIGNED> R;
   __shared__ float sm[4 * (NT / 64)];
   int phase = 0;
   const int t = threadIdx.x % TPR, C = p.C;
-  const long row = (long)blockIdx.x * RPB + threadIdx.x / TPR, rows = (long)p.B * p.T;
-  const bool live = row < rows;  // (rows past the end compute on row 0 and store nothing: every wave reaches the barriers)
-  const long r = live ? row : 0;
-  float x[EPT], a[EPT], w[EPT], b[EPT];
-  R::load((const T*)p.x + r * p.ld_x, t, C, x);
-  R::load((const T*)p.a + r * p.ld_a, t, C, a);
-  float g[EPT];
-  if (p.gate_mode) {
-    R::load((const T*)p.gate + (p.gate_mode == GATE_TOKEN ? r : r / p.T) * p.ld_g, t, C, g);
+  const long rows = (long)p.B * p.T, stride = (long)gridDim.x * RPB;
+  float pw[EPT], pb[EPT], qw[EPT], qb[EPT], sc[EPT];
+  load_param<T, TPR, EPT, ALIGNED>(p.post_w, 1.f, t, C, pw);
+  load_param<T, TPR, EPT, ALIGNED>(p.post_b, 0.f, t, C, pb);
+  load_param<T, TPR, EPT, ALIGNED>(p.pre_w, 1.f, t, C, qw);
+  load_param<T, TPR, EPT, ALIGNED>(p.pre_b, 0.f, t, C, qb);
+  load_param<T, TPR, EPT, ALIGNED>(p.scale, 1.f, t, C, sc);
+  auto gate_row = [&](long r) { return (const T*)p.gate + (p.gate_mode == GATE_TOKEN ? r : r / p.T) * p.ld_g; };
+  typename R::Raw rx, ra, rg;
+  long first = (long)blockIdx.x * RPB;
+  auto fetch = [&](long base) {  // (rows past the end fetch and compute the last row and store nothing: every wave reaches the barriers)
+    long r = base + threadIdx.x / TPR;
+    if (r >= rows) r = rows - 1;
+    R::fetch((const T*)p.x + r * p.ld_x, t, C, rx);
+    R::fetch((const T*)p.a + r * p.ld_a, t, C, ra);
+    if (p.gate_mode) R::fetch(gate_row(r), t, C, rg);
+  };
+  fetch(first);
+  for (long base = first; base < rows; base += stride) {
+    long r = base + threadIdx.x / TPR;
+    const bool live = r < rows;
+    if (!live) r = rows - 1;
+    float x[EPT], a[EPT], g[EPT];
+    R::take(rx, (const T*)p.x + r * p.ld_x, t, C, x);
+    R::take(ra, (const T*)p.a + r * p.ld_a, t, C, a);
+    if (p.gate_mode) R::take(rg, gate_row(r), t, C, g);
+    if (base + stride < rows) fetch(base + stride);
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) g[e] = gate_act(g[e], p.gate_act);
-  } else {
+    for (int e = 0; e < EPT; ++e) g[e] = p.gate_mode ? gate_act(g[e], p.gate_act) : 1.f;
+    float mean, rstd;
+    if (p.post) {
+      stats<R, TPR>(a, t, C, p.layer, p.eps, sm, phase, mean, rstd);
+      if (live && t == 0 && p.stat) *reinterpret_cast<float2*>(p.stat + r * 4) = make_float2(mean, rstd);
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) g[e] = 1.f;
-  }
-  float mean, rstd;
-  if (p.post) {
-    load_param<R>(p.post_w, 1.f, t, C, w);
-    load_param<R>(p.post_b, 0.f, t, C, b);
-    stats<R, TPR, NT>(a, t, C, p.layer, p.eps, sm, phase, mean, rstd);
-    if (live && t == 0 && p.stat) {
-      p.stat[r * 4] = mean;
-      p.stat[r * 4 + 1] = rstd;
+      for (int e = 0; e < EPT; ++e) a[e] = (a[e] - mean) * rstd * pw[e] + pb[e];
     }
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) a[e] = (a[e] - mean) * rstd * w[e] + b[e];
-  }
-  load_param<R>(p.scale, 1.f, t, C, w);
+    for (int e = 0; e < EPT; ++e) x[e] = R::col(t, e) < C ? p.alpha * x[e] + sc[e] * g[e] * a[e] : 0.f;
+    if (live) R::store((T*)p.y + r * (long)C, t, C, x);
+    if (p.pre) {
+      stats<R, TPR>(x, t, C, p.layer, p.eps, sm, phase, mean, rstd);
+      if (live && t == 0 && p.stat) *reinterpret_cast<float2*>(p.stat + r * 4 + 2) = make_float2(mean, rstd);
 #pragma unroll
-  for (int e = 0; e < EPT; ++e) x[e] = R::col(t, e) < C ? p.alpha * x[e] + w[e] * g[e] * a[e] : 0.f;
-  if (live) R::store((T*)p.y + r * (long)C, t, C, x);
-  if (p.pre) {
-    load_param<R>(p.pre_w, 1.f, t, C, w);
-    load_param<R>(p.pre_b, 0.f, t, C, b);
-    stats<R, TPR, NT>(x, t, C, p.layer, p.eps, sm, phase, mean, rstd);
-    if (live && t == 0 && p.stat) {
-      p.stat[r * 4 + 2] = mean;
-      p.stat[r * 4 + 3] = rstd;
+      for (int e = 0; e < EPT; ++e) x[e] = (x[e] - mean) * rstd * qw[e] + qb[e];
+      if (live) R::store((T*)p.h + r * (long)C, t, C, x);
     }
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) x[e] = (x[e] - mean) * rstd * w[e] + b[e];
-    if (live) R::store((T*)p.h + r * (long)C, t, C, x);
   }
 }
 
 // grid (blocks per sample, B): a workgroup's rows belong to one sample, so its partial of the sample's gate gradient is one row
-template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_bwd_kernel(tfpp_block_norm_params p) {
-  constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds__(threads_of(TPR)) void block_norm_bwd_kernel(tfpp_block_norm_params p) {
+  constexpr int NT = threads_of(TPR), RPB = NT / TPR;
   typedef Row<T, TPR, EPT, ALIGNED> R;
   extern __shared__ float red[];  // RPB > 1: column sums of the row groups
   __shared__ float sm[4 * (NT / 64)];
@@ -172,10 +212,10 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, C = p.C;
   const float inv = 1.f / (float)C;
   float pw[EPT], pb[EPT], qw[EPT], sc[EPT];
-  load_param<R>(p.post_w, 1.f, t, C, pw);
-  load_param<R>(p.post_b, 0.f, t, C, pb);
-  load_param<R>(p.pre_w, 1.f, t, C, qw);
-  load_param<R>(p.scale, 1.f, t, C, sc);
+  load_param<T, TPR, EPT, ALIGNED>(p.post_w, 1.f, t, C, pw);
+  load_param<T, TPR, EPT, ALIGNED>(p.post_b, 0.f, t, C, pb);
+  load_param<T, TPR, EPT, ALIGNED>(p.pre_w, 1.f, t, C, qw);
+  load_param<T, TPR, EPT, ALIGNED>(p.scale, 1.f, t, C, sc);
   float gs[EPT];
 #pragma unroll
   for (int e = 0; e < EPT; ++e) gs[e] = 1.f;
@@ -191,22 +231,28 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
     for (int e = 0; e < EPT; ++e) acc[k][e] = 0.f;
   const int per = (p.T + (int)gridDim.x - 1) / (int)gridDim.x;
   const int t0 = (int)blockIdx.x * per, t1 = t0 + per < p.T ? t0 + per : p.T;
+  typename R::Raw rx, ra, rg, rdy, rdh;
+  auto fetch = [&](int tt) {
+    const long r = (long)blockIdx.y * p.T + (tt + sub < t1 ? tt + sub : t0);
+    R::fetch((const T*)p.x + r * p.ld_x, t, C, rx);
+    R::fetch((const T*)p.a + r * p.ld_a, t, C, ra);
+    if (p.dy) R::fetch((const T*)p.dy + r * p.ld_dy, t, C, rdy);
+    if (p.dh) R::fetch((const T*)p.dh + r * p.ld_dh, t, C, rdh);
+    if (p.gate_mode == GATE_TOKEN) R::fetch((const T*)p.gate + r * p.ld_g, t, C, rg);
+  };
+  if (t0 < t1) fetch(t0);
   for (int tt = t0; tt < t1; tt += RPB) {
     const bool live = tt + sub < t1;
     const long r = (long)blockIdx.y * p.T + (live ? tt + sub : t0);
     float dy[EPT], dh[EPT], x[EPT], n[EPT], g[EPT];
-    R::load((const T*)p.x + r * p.ld_x, t, C, x);
-    R::load((const T*)p.a + r * p.ld_a, t, C, n);
-    if (p.dy) R::load((const T*)p.dy + r * p.ld_dy, t, C, dy);
-    if (p.dh) R::load((const T*)p.dh + r * p.ld_dh, t, C, dh);
-    if (p.gate_mode == GATE_TOKEN) {
-      R::load((const T*)p.gate + r * p.ld_g, t, C, g);
+    R::take(rx, (const T*)p.x + r * p.ld_x, t, C, x);
+    R::take(ra, (const T*)p.a + r * p.ld_a, t, C, n);
+    if (p.dy) R::take(rdy, (const T*)p.dy + r * p.ld_dy, t, C, dy);
+    if (p.dh) R::take(rdh, (const T*)p.dh + r * p.ld_dh, t, C, dh);
+    if (p.gate_mode == GATE_TOKEN) R::take(rg, (const T*)p.gate + r * p.ld_g, t, C, g);
+    if (tt + RPB < t1) fetch(tt + RPB);
 #pragma unroll
-      for (int e = 0; e < EPT; ++e) g[e] = gate_act(g[e], p.gate_act);
-    } else {
-#pragma unroll
-      for (int e = 0; e < EPT; ++e) g[e] = gs[e];
-    }
+    for (int e = 0; e < EPT; ++e) g[e] = p.gate_mode == GATE_TOKEN ? gate_act(g[e], p.gate_act) : gs[e];
     if (!p.dy)
 #pragma unroll
       for (int e = 0; e < EPT; ++e) dy[e] = 0.f;
@@ -230,7 +276,7 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
         s[1] += in ? dh[e] * xh : 0.f;
         x[e] = xh;
       }
-      row_sums<TPR, NT, 2>(s, sm, phase);
+      row_sums<TPR, 2>(s, sm, phase);
       const float c0 = p.layer ? s[0] * inv : 0.f, c1 = s[1] * inv;
 #pragma unroll
       for (int e = 0; e < EPT; ++e) dy[e] += st.w * (dh[e] - c0 - x[e] * c1);
@@ -258,7 +304,7 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
     }
     if (live && p.gate_mode == GATE_TOKEN && p.dgate) R::store((T*)p.dgate + r * (long)C, t, C, x);
     if (p.post) {
-      row_sums<TPR, NT, 2>(s, sm, phase);
+      row_sums<TPR, 2>(s, sm, phase);
       const float c0 = p.layer ? s[0] * inv : 0.f, c1 = s[1] * inv;
 #pragma unroll
       for (int e = 0; e < EPT; ++e) dy[e] = st.y * (dy[e] - c0 - n[e] * c1);
@@ -286,10 +332,11 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
   }
 }
 
-// out[k][c] (+)= sum over the workgroups' partials, 64 columns x 4 slices of them per workgroup; z = 0 .. 4: the parameter gradients over all workgroups,
-// z = 5 + b: the gate gradient of sample b over that sample's workgroups, in the gate's type
-template <typename T> __global__ __launch_bounds__(256) void block_norm_colsum_kernel(tfpp_block_norm_params p, int bps) {
-  __shared__ float sm[256];
+// out[k][c] (+)= sum over the workgroups' partials, 64 columns x 16 slices of them per workgroup; y = 0 .. 4: the parameter gradients over all workgroups,
+// y = 5 + b: the gate gradient of sample b over that sample's workgroups, in the gate's type
+template <typename T> __global__ __launch_bounds__(1024) void block_norm_colsum_kernel(tfpp_block_norm_params p, int bps) {
+  constexpr int SLICES = 16;
+  __shared__ float sm[1024];
   const int k = blockIdx.y < 5 ? (int)blockIdx.y : 5, c = (int)blockIdx.x * 64 + ((int)threadIdx.x & 63), slice = threadIdx.x >> 6, C = p.C;
   float* const outs[5] = {p.dpre_w, p.dpre_b, p.dpost_w, p.dpost_b, p.dscale};
   float* out = nullptr;
@@ -300,28 +347,40 @@ template <typename T> __global__ __launch_bounds__(256) void block_norm_colsum_k
   if (k < 5 && !out) return;
   const long lo = k < 5 ? 0 : (long)b * bps, hi = k < 5 ? (long)p.B * bps : lo + bps;
   float s = 0.f;
-  if (c < C)
-    for (long i = lo + slice; i < hi; i += 4) s += p.partial[(i * K_SUMS + k) * C + c];
+  if (c < C) {
+    const float* src = p.partial + (long)k * C + c;
+    const long step = (long)K_SUMS * C;
+    long i = lo + slice;
+    for (; i + 7 * SLICES < hi; i += 8 * SLICES) {  // (eight loads in flight)
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = src[(i + u * SLICES) * step];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
+    for (; i < hi; i += SLICES) s += src[i * step];
+  }
   sm[threadIdx.x] = s;
   __syncthreads();
   if (slice == 0 && c < C) {
-    s = (sm[threadIdx.x] + sm[threadIdx.x + 64]) + (sm[threadIdx.x + 128] + sm[threadIdx.x + 192]);
+#pragma unroll
+    for (int w = 1; w < SLICES; ++w) s += sm[w * 64 + threadIdx.x];
     if (k < 5) out[c] = (p.accumulate >> k) & 1 ? out[c] + s : s;
     else reinterpret_cast<T*>(p.dgate)[(long)b * C + c] = ElemTraits<T>::from_f(s);
   }
 }
 
 int blocks_per_sample(const tfpp_block_norm_params& p) {
-  // 512 workgroups of 256 threads fill the chip at this register count; each has at least 4 rows, since its 6 rows of partials are traffic too
-  const int tpr = p.C <= 512 ? 64 : (p.C <= 1024 ? 128 : (p.C <= 2048 ? 256 : 512)), rpb = tpr < 256 ? 256 / tpr : 1;
-  long n = (512 + p.B - 1) / p.B;
+  // 8 waves a CU fill the chip at this register count; each workgroup has at least 4 rows, since its 6 rows of partials are traffic too
+  const int tpr = p.C <= 512 ? 64 : (p.C <= 1024 ? 128 : (p.C <= 2048 ? 256 : 512)), rpb = tpr == 64 ? 4 : 1, wgs = 256 * 512 / threads_of(tpr);
+  long n = (wgs + p.B - 1) / p.B;
   const long most = (p.T + 4L * rpb - 1) / (4L * rpb);
   if (n > most) n = most;
   return n < 1 ? 1 : (int)n;
 }
 
 bool aligned16(const tfpp_block_norm_params& p, int vec) {
-  const void* ptrs[] = {p.x, p.a, p.gate, p.y, p.h, p.dy, p.dh, p.dx, p.da, p.gate_mode == GATE_TOKEN ? p.dgate : nullptr};
+  const void* ptrs[] = {p.x, p.a, p.gate, p.y, p.h, p.dy, p.dh, p.dx, p.da, p.gate_mode == GATE_TOKEN ? p.dgate : nullptr, p.post_w, p.post_b, p.pre_w, p.pre_b, p.scale};
   for (const void* q : ptrs)
     if ((uintptr_t)q & 15) return false;
   const int64_t lds[] = {p.ld_x, p.ld_a, p.gate_mode ? p.ld_g : 0, p.dy ? p.ld_dy : 0, p.dh ? p.ld_dh : 0, p.C};
@@ -336,13 +395,13 @@ bool valid(const tfpp_block_norm_params& p, int dtype) {
 }
 
 template <typename T, int TPR, int EPT, bool AL> void launch(const tfpp_block_norm_params& p, bool bwd, int bps, hipStream_t st) {
-  constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+  constexpr int NT = threads_of(TPR), RPB = NT / TPR;
   if (bwd) {
     const size_t lds = RPB > 1 ? (size_t)EPT * NT * 4 : 0;
     hipLaunchKernelGGL((block_norm_bwd_kernel<T, TPR, EPT, AL>), dim3(bps, p.B), dim3(NT), lds, st, p);
   } else {
-    const long rows = (long)p.B * p.T;
-    hipLaunchKernelGGL((block_norm_fwd_kernel<T, TPR, EPT, AL>), dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(NT), 0, st, p);
+    const long rows = (long)p.B * p.T, groups = (rows + RPB - 1) / RPB, most = 256 * 1024 / NT;  // 16 waves a CU: what fits beside 40 registers of parameters
+    hipLaunchKernelGGL((block_norm_fwd_kernel<T, TPR, EPT, AL>), dim3((unsigned)(groups < most ? groups : most)), dim3(NT), 0, st, p);
   }
 }
 template <typename T> void dispatch(const tfpp_block_norm_params& p, bool bwd, int bps, hipStream_t st) {
@@ -381,8 +440,8 @@ extern "C" int tfpp_block_norm_bwd(const tfpp_block_norm_params* p, int dtype, v
   else dispatch<bf16_t>(*p, true, bps, st);
   TFPP_CHECK_LAUNCH();
   const dim3 grid((p->C + 63) / 64, 5 + (p->gate_mode == GATE_SAMPLE ? p->B : 0));
-  if (dtype == TFPP_F32) hipLaunchKernelGGL(block_norm_colsum_kernel<float>, grid, dim3(256), 0, st, *p, bps);
-  else hipLaunchKernelGGL(block_norm_colsum_kernel<bf16_t>, grid, dim3(256), 0, st, *p, bps);
+  if (dtype == TFPP_F32) hipLaunchKernelGGL(block_norm_colsum_kernel<float>, grid, dim3(1024), 0, st, *p, bps);
+  else hipLaunchKernelGGL(block_norm_colsum_kernel<bf16_t>, grid, dim3(1024), 0, st, *p, bps);
   TFPP_CHECK_LAUNCH();
   return 0;
 }

@@ -103,15 +103,19 @@ template <typename T, int CB> struct Img {
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
       const int ldb = (int)ld * (int)sizeof(T), r0 = tid / NC, rowb = r0 * ldb;
-      const bool all = (valid & low_bits(ROWS)) == low_bits(ROWS);
+      auto put = [&](int u, bool ok) {
+        const int c = (tid % NC) ^ swizzle(r0 + u * (NT / NC));
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t*)(img + (u * NT + wave * 64) * 16), 16, ok && c * VEC < n ? rowb + c * 16 : (int)0x80000000,
+                                                 u * (NT / NC) * ldb, 0, 0);
+      };
+      if ((valid & low_bits(ROWS)) == low_bits(ROWS)) {
 #pragma unroll
-      for (int u = 0; u * NT < SLOTS; ++u) {
-        if (u * NT + wave * 64 < SLOTS) {
-          const int r = r0 + u * (NT / NC), c = (tid % NC) ^ swizzle(r);
-          bool ok = c * VEC < n;
-          if (!all) ok = ok && (((valid >> (u * (NT / NC))) >> r0) & 1ull);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t*)(img + (u * NT + wave * 64) * 16), 16, ok ? rowb + c * 16 : (int)0x80000000, u * (NT / NC) * ldb, 0, 0);
-        }
+        for (int u = 0; u * NT < SLOTS; ++u)
+          if (u * NT + wave * 64 < SLOTS) put(u, true);
+      } else {
+#pragma unroll
+        for (int u = 0; u * NT < SLOTS; ++u)
+          if (u * NT + wave * 64 < SLOTS) put(u, ((valid >> (u * (NT / NC))) >> r0) & 1ull);
       }
     } else {
 #pragma unroll 1
@@ -151,21 +155,58 @@ template <typename T, bool VECTOR> __device__ __forceinline__ void load_frag(con
   }
 }
 
-// four consecutive channels c .. of a row with n channels
-template <typename T> __device__ __forceinline__ void store4(T* __restrict__ row, int c, int n, bool vec, float a, float b, float e, float f) {
-  if (vec && c + 3 < n) {
-    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + c) = make_uint2(f2bf_pack2(a, b), f2bf_pack2(e, f));
-    else *reinterpret_cast<float4*>(row + c) = make_float4(a, b, e, f);
-  } else {
-    if (c < n) row[c] = ElemTraits<T>::from_f(a);
-    if (c + 1 < n) row[c + 1] = ElemTraits<T>::from_f(b);
-    if (c + 2 < n) row[c + 2] = ElemTraits<T>::from_f(e);
-    if (c + 3 < n) row[c + 3] = ElemTraits<T>::from_f(f);
+struct Weights {  // of the heads' norm: none (null), fp32 or bf16
+  const void* w;
+  int is_bf16;
+  __device__ __forceinline__ float operator[](int c) const { return is_bf16 ? bf2f(((const bf16_t*)w)[c]) : ((const float*)w)[c]; }
+};
+
+// Results leave through an LDS strip of the wave, two 32-channel blocks at a time: the C layout has a row in each lane, 4 channels a register quad, while
+// memory wants whole rows; and the loop that stores them is ROLLED -- unrolled per register, an epilogue is thousands of instructions that every
+// workgroup fetches once, 20 us of a short kernel.  Chunks of 4 floats, chunk c of row r at c ^ (r & 7).
+constexpr int STRIP_BYTES = 32 * 64 * 4;
+__device__ __forceinline__ int strip_at(int row, int chunk) { return row * 64 + ((chunk ^ (row & 7)) << 2); }
+__device__ __forceinline__ void strip_put(float* strip, int lane, int block, const f32x16_t& o, float f) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    *reinterpret_cast<float4*>(strip + strip_at(lane & 31, block * 8 + 2 * g + (lane >> 5))) = make_float4(o[4 * g] * f, o[4 * g + 1] * f, o[4 * g + 2] * f, o[4 * g + 3] * f);
+}
+// channels c0 .. c0 + 32 * blocks - 1 of 32 rows; row(r): where row r starts (null: not stored); n: channels of a row; w: multiplied by the norm's weights
+template <typename T, typename Row> __device__ __forceinline__ void strip_store(const float* strip, int lane, int blocks, int c0, int n, bool vec, Weights w, Row row) {
+  const int per = blocks * 4, piece = lane & (per - 1), c = c0 + piece * 8;  // 8-channel pieces of a row: 4 or 8; a lane keeps its channels
+  if (c >= n) return;
+  float wf[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) wf[e] = w.w && c + e < n ? w[c + e] : 1.f;
+#pragma unroll 1
+  for (int r = lane / per; r < 32; r += 64 / per) {
+    T* dst = row(r);
+    if (!dst) break;  // (rows that do not exist are the last ones)
+    float f[8];
+    *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(strip + strip_at(r, 2 * piece));
+    *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(strip + strip_at(r, 2 * piece + 1));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= wf[e];
+    if (vec && c + 8 <= n) {
+#pragma unroll
+      for (int e = 0; e < 8; e += ElemTraits<T>::VEC) store_vec<T>(dst + c + e, f + e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < n) dst[c + e] = ElemTraits<T>::from_f(f[e]);
+    }
   }
 }
-
-__device__ __forceinline__ float norm_weight(const tfpp_diff_attn_params& p, int c) {
-  return !p.norm_w ? 1.f : (p.norm_w_bf16 ? bf2f(((const bf16_t*)p.norm_w)[c]) : ((const float*)p.norm_w)[c]);
+// all N blocks of a wave's 32 rows
+template <typename T, int N, typename Row> __device__ __forceinline__ void store_rows(float* strip, int lane, const f32x16_t (&o)[N], float f, int n, bool vec, Weights w, Row row) {
+#pragma unroll
+  for (int b = 0; b < N; b += 2) {
+    strip_put(strip, lane, 0, o[b], f);
+    if (b + 1 < N) strip_put(strip, lane, 1, o[b + 1 < N ? b + 1 : b], f);
+    __builtin_amdgcn_wave_barrier();  // (one wave's LDS operations complete in order)
+    strip_store<T>(strip, lane, b + 1 < N ? 2 : 1, b * 32, n, vec, w, row);
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 // workgroup -> (tile, batch x head).  Workgroups go round the 8 XCDs in turn: where the heads divide evenly, all tiles of a head stay on one XCD (its
@@ -185,6 +226,14 @@ __device__ __forceinline__ void place(int heads, int tiles, bool by_tile, int& b
   }
 }
 
+// Fill the next images while the present ones are read.  The two are different memory, and the compiler has to be told: it puts a wait for ALL loads
+// into LDS that are under way in front of an LDS read that may alias them, which would undo the prefetch (measured: 5.7 -> see the forward kernel's
+// comment).  The noalias arguments become scopes on both sides when this is inlined.  The wait that IS needed stands at the top of each step.
+template <typename Fill, typename Use> __device__ __forceinline__ void overlap(unsigned char* __restrict__ next, const unsigned char* __restrict__ now, Fill fill, Use use) {
+  fill(next);
+  use(now);
+}
+
 struct Seq {  // what a sequence's queries may see
   int len, start;  // keys 0 .. len - 1; query i sees key j <= start + i (causal)
 };
@@ -192,10 +241,10 @@ __device__ __forceinline__ Seq sequence(const tfpp_diff_attn_params& p, int b) {
   Seq s;
   s.len = p.Tk;
   if (p.kv_len) {
-    const int n = p.kv_len[b];
+    const int n = __builtin_amdgcn_readfirstlane(p.kv_len[b]);  // (the compiler does not know that it is the same in all lanes)
     s.len = n < 0 ? 0 : (n < p.Tk ? n : p.Tk);
   }
-  s.start = p.q_start ? p.q_start[b] : p.q_start_all;
+  s.start = p.q_start ? __builtin_amdgcn_readfirstlane(p.q_start[b]) : p.q_start_all;
   return s;
 }
 // bit i: key j0 + i exists and is not left out
@@ -224,7 +273,7 @@ template <typename T, int NB, bool VECTOR, int Q, int MAPS> struct Fwd {
   typedef Img<T, NB> ImgV;
   int map0;        // the wave's (first) map
   const T* qrow;   // the lane's query, map 0 (Q_GLOBAL)
-  int q_at, k_at, v_at;  // offsets in LDS: the queries of the wave's first map (Q_LDS), the lane's place in K and V images
+  int q_at, k_at, v_at;  // the lane's place in the images of Q (Q_LDS), K and V
   long qmap;       // from map to map
   Frag8<T> q[MAPS][Q == Q_HELD ? NB : 1];
   f32x16_t o[MAPS][NB];
@@ -248,8 +297,9 @@ template <typename T, int NB, bool VECTOR, int Q, int MAPS> struct Fwd {
         for (int r = 0; r < 16; ++r) o[i][n][r] = 0.f;
     }
   }
-  // 32 keys: rows at kimg, vimg bytes into lds (kimg: the wave's first map, the other kbytes behind); vis: bit of a key, the lane's half already shifted out
-  __device__ __forceinline__ void tile(const unsigned char* lds, int kimg, int kbytes, int vimg, bool masked, unsigned vis, float c, int d, int half) {
+  // 32 keys: rows at kimg, vimg bytes into lds (kimg: the wave's first map, the other kbytes behind); qimg: the first map's queries (Q_LDS); vis: bit of
+  // a key, the lane's half already shifted out
+  __device__ __forceinline__ void tile(const unsigned char* lds, const unsigned char* qimg, int kimg, int kbytes, int vimg, bool masked, unsigned vis, float c, int d, int half) {
     const int kat = k_at + kimg, vat = v_at + vimg;
     f32x16_t sc[MAPS];
 #pragma unroll
@@ -262,7 +312,7 @@ template <typename T, int NB, bool VECTOR, int Q, int MAPS> struct Fwd {
       for (int ks = 0; ks < NB; ++ks) {
         Frag8<T> a;
         ImgK::rows(lds + i * kbytes, kat, ks, a);
-        if constexpr (Q == Q_LDS) ImgK::rows(lds + i * 32 * ImgK::ROW_BYTES, q_at, ks, q[i][0]);
+        if constexpr (Q == Q_LDS) ImgK::rows(qimg + i * 32 * ImgK::ROW_BYTES, q_at, ks, q[i][0]);
         if constexpr (Q == Q_GLOBAL) load_frag<T, VECTOR>(qrow + (long)(map0 + i) * qmap, ks * 16 + half * 8, d, true, q[i][0]);
         mma(a, q[i][Q == Q_HELD ? ks : 0], sc[i]);
         if (sizeof(T) == 4 || ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);
@@ -329,28 +379,13 @@ __device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l
 // log2 of the sum; +inf for a query without keys: exp2(score - inf) = 0 in the backward passes
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? INFINITY : m + log2f(l); }
 
-// 32 channels (block n) of a query's result: f = out_scale / rms
-template <typename T> __device__ __forceinline__ void store_result(const tfpp_diff_attn_params& p, T* out, int n, int half, float f, const f32x16_t& o) {
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    __builtin_amdgcn_sched_barrier(0);  // (the weights of all channels at once would not fit the registers)
-    const int ch = n * 32 + 8 * g + 4 * half;
-    if (ch >= p.dv) continue;
-    float w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = p.norm && ch + e < p.dv ? f * norm_weight(p, ch + e) : f;
-    store4<T>(out, ch, p.dv, p.out_vec, o[4 * g] * w[0], o[4 * g + 1] * w[1], o[4 * g + 2] * w[2], o[4 * g + 3] * w[3]);
-  }
-}
-template <typename T> __device__ __forceinline__ void store_block(T* row, int n, int half, int dvs, const f32x16_t& o) {
-#pragma unroll
-  for (int g = 0; g < 4; ++g) store4<T>(row, n * 32 + 8 * g + 4 * half, dvs, true, o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
-}
-
 // many queries: workgroup = (batch, head, 128 queries), the waves' queries differ and the images are shared by the workgroup, one tile ahead
 template <typename T, int NB> constexpr int fwd_threads() { return fwd_split<T, NB>() && sizeof(T) == 2 ? 512 : 256; }
 template <typename T, int NB> constexpr int fwd_queries() { return fwd_threads<T, NB>() / (fwd_split<T, NB>() ? 4 : 2); }
-template <typename T, int NB> constexpr int fwd_lds() { return 2 * key_tile<T>() * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES); }
+constexpr int at_least(int a, int b) { return a > b ? a : b; }
+template <typename T, int NB> constexpr int fwd_lds() {
+  return at_least(2 * key_tile<T>() * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES), fwd_threads<T, NB>() / 64 * STRIP_BYTES);
+}
 
 template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_threads<T, NB>()), (fwd_threads<T, NB>() == 512 || NB <= (sizeof(T) == 2 ? 4 : 2) ? 2 : 1)) void diff_attn_fwd_kernel(tfpp_diff_attn_params p) {
   typedef Fwd<T, NB, VECTOR, (sizeof(T) == 2 ? VECTOR || NB < 8 : NB < 5) ? Q_HELD : Q_GLOBAL, fwd_split<T, NB>() ? 1 : 2> F;  // (wide fp32 heads do not fit the registers)
@@ -377,8 +412,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_thr
   const int steps = end > 0 ? (end + KT - 1) / KT : 0;
   const float c = p.scale * LOG2E;
 
-  auto fill = [&](int step, unsigned long long bits) {
-    unsigned char* buf = smem + (step & 1) * BUF;
+  auto fill = [&](unsigned char* buf, int step, unsigned long long bits) {
     const long j0 = (long)step * KT;
 #pragma unroll
     for (int i = 0; i < 2; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, bits, tid);
@@ -387,32 +421,36 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_thr
   unsigned long long bits = 0;
   if (steps > 0) {
     bits = key_bits(p, b, 0, sq.len, lane);
-    fill(0, bits);
+    fill(smem, 0, bits);
   }
   for (int s = 0; s < steps; ++s) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // image s is complete, and every wave is past its reads of image s - 1
     const unsigned long long cur = bits;
-    if (s + 1 < steps) {
-      bits = key_bits(p, b, (s + 1) * KT, sq.len, lane);
-      fill(s + 1, bits);
-    }
-    const int j0 = s * KT;
-    const int seen = p.causal ? sq.start + w0 + 32 - j0 : KT;  // keys of this tile that the wave's last query sees
-    if (seen <= 0 || cur == 0) continue;
-    const bool masked = (cur & low_bits(KT)) != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
-    const unsigned long long mine = p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur;
-    const int buf = (s & 1) * BUF;
+    const bool more = s + 1 < steps;
+    if (more) bits = key_bits(p, b, (s + 1) * KT, sq.len, lane);
+    overlap(smem + (~s & 1) * BUF, smem + (s & 1) * BUF,
+            [&](unsigned char* next) {
+              if (more) fill(next, s + 1, bits);
+            },
+            [&](const unsigned char* now) {
+              const int j0 = s * KT;
+              const int seen = p.causal ? sq.start + w0 + 32 - j0 : KT;  // keys of this tile that the wave's last query sees
+              if (seen <= 0 || cur == 0) return;
+              const bool masked = (cur & low_bits(KT)) != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
+              const unsigned long long mine = p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur;
 #pragma unroll 1
-    for (int u = 0; u < KT / 32; ++u)
-      f.tile(smem, buf + f.map0 * K_BYTES + u * 32 * ImgK::ROW_BYTES, K_BYTES, buf + 2 * K_BYTES + u * 32 * ImgV::ROW_BYTES, masked, (unsigned)(mine >> (u * 32)) >> (4 * half), c, p.d,
-             half);
+              for (int u = 0; u < KT / 32; ++u)
+                f.tile(now, nullptr, f.map0 * K_BYTES + u * 32 * ImgK::ROW_BYTES, K_BYTES, 2 * K_BYTES + u * 32 * ImgV::ROW_BYTES, masked, (unsigned)(mine >> (u * 32)) >> (4 * half), c, p.d, half);
+            });
   }
 
   const float lam = p.lam[p.n_lam > 1 ? h : 0];
-  const long row = ((long)b * p.H + h) * p.Tq + qi;
-  const bool live = qi < p.Tq;
-  const int dvs = (p.dv + 7) & ~7;
+  const long row0 = ((long)b * p.H + h) * p.Tq + w0;
+  const int dvs = (p.dv + 7) & ~7, rows = p.Tq - w0;  // the wave's rows that exist
+  float* strip = reinterpret_cast<float*>(smem + wave * STRIP_BYTES);
+  static_assert(fwd_lds<T, NB>() >= NT / 64 * STRIP_BYTES, "the strips fit");
+  __syncthreads();  // every wave is past its last image
 #pragma unroll
   for (int i = 0; i < MAPS; ++i) {
     f.l[i] += other_half(f.l[i]);
@@ -421,46 +459,50 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_thr
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) f.o[i][n][r] *= inv;
-    if (p.lse && live && half == 0) p.lse[(long)(f.map0 + i) * p.B * p.H * p.Tq + row] = log_sum(f.m[i], f.l[i]);
-    if (p.o1 && live)
-#pragma unroll
-      for (int n = 0; n < NB; ++n) store_block<T>((T*)(f.map0 + i ? p.o2 : p.o1) + row * dvs, n, half, dvs, f.o[i][n]);
+    if (p.lse && (lane & 31) < rows && half == 0) p.lse[(long)(f.map0 + i) * p.B * p.H * p.Tq + row0 + lane] = log_sum(f.m[i], f.l[i]);
+    if (p.o1) {
+      T* to = (T*)(f.map0 + i ? p.o2 : p.o1) + row0 * dvs;
+      store_rows<T>(strip, lane, f.o[i], 1.f, dvs, true, Weights{nullptr, 0}, [&](int r) { return r < rows ? to + (long)r * dvs : nullptr; });
+    }
   }
   if constexpr (MAPS == 1) {  // O_2 of the odd waves to the even ones, in the registers' own order
     static_assert(fwd_lds<T, NB>() >= NT / 128 * NB * 16 * 64 * 4, "the exchange fits the images' LDS");
-    float* x = reinterpret_cast<float*>(smem) + (wave >> 1) * (NB * 16 * 64) + lane;
-    __syncthreads();  // every wave is past its last image
+    float4* x = reinterpret_cast<float4*>(smem) + (wave >> 1) * (NB * 4 * 64) + lane;
+    __syncthreads();  // every wave is past its strip
     if (f.map0)
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[(n * 16 + r) * 64] = f.o[0][n][r];
+        for (int g = 0; g < 4; ++g) x[(n * 4 + g) * 64] = make_float4(f.o[0][n][4 * g], f.o[0][n][4 * g + 1], f.o[0][n][4 * g + 2], f.o[0][n][4 * g + 3]);
+    __syncthreads();
+    if (!f.map0)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 v = x[(n * 4 + g) * 64];
+          f.o[0][n][4 * g] -= lam * v.x; f.o[0][n][4 * g + 1] -= lam * v.y; f.o[0][n][4 * g + 2] -= lam * v.z; f.o[0][n][4 * g + 3] -= lam * v.w;
+        }
     __syncthreads();
     if (f.map0) return;
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) f.o[0][n][r] -= lam * x[(n * 16 + r) * 64];
   } else {
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) f.o[0][n][r] -= lam * f.o[MAPS - 1][n][r];
   }
-  float ss = 0.f;
-#pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) ss += f.o[0][n][r] * f.o[0][n][r];
   float g = p.out_scale;
   if (p.norm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ss += f.o[0][n][r] * f.o[0][n][r];
     ss += other_half(ss);
     g *= 1.f / sqrtf(ss / (float)p.dv + p.eps);
   }
-  if (!live) return;
-  T* out = (T*)p.out + (long)b * p.o_s[0] + (long)qi * p.o_s[1] + (long)h * p.o_s[2];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) store_result<T>(p, out, n, half, g, f.o[0][n]);
+  T* out = (T*)p.out + (long)b * p.o_s[0] + (long)w0 * p.o_s[1] + (long)h * p.o_s[2];
+  store_rows<T>(strip, lane, f.o[0], g, p.dv, p.out_vec, Weights{p.norm_w, p.norm_w_bf16}, [&](int r) { return r < rows ? out + (long)r * p.o_s[1] : nullptr; });
 }
 
 // few queries (single tokens against a cache, short sequences): workgroup = (batch, key / value head, 32 rows, split of the keys), a row being a
@@ -476,7 +518,7 @@ template <typename T, int NB> struct Few {
   static constexpr int EXCHANGE = WAVES * NB * BLOCK * 4;  // one map of every wave
   static constexpr int SUMS = WAVES * 2 * 32 * 2 * 4;      // (m, l) of every wave and map; later the rows' sums of squares
   static constexpr int QUERIES = 2 * K_BYTES;              // the 32 rows' queries, both maps
-  static constexpr int LDS = (STAGES * WAVES * IMAGES > EXCHANGE ? STAGES * WAVES * IMAGES : EXCHANGE) + QUERIES + SUMS;
+  static constexpr int LDS = at_least(at_least(STAGES * WAVES * IMAGES, EXCHANGE), WAVES * STRIP_BYTES) + QUERIES + SUMS;
   static constexpr int ROW_FLOATS = 2 * (NB * 32 + 2);     // of one row in `partial`: both maps' sums, maxima, l
 };
 
@@ -500,7 +542,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
   F f;
   f.init(MAPS == 1 ? wave & 1 : 0, nullptr, 0, p.d, lane);
   unsigned char* qimg = smem + (W::LDS - W::SUMS - W::QUERIES);
-  f.q_at = W::LDS - W::SUMS - W::QUERIES + f.map0 * W::K_BYTES + ImgK::rows_at(lane);
+  f.q_at = ImgK::rows_at(lane);
   // the rows' queries into LDS, 16 bytes (or elements, unaligned) at a time; their rows lie in several heads, so not by `fill`
   for (int i = tid; i < 2 * 32 * ImgK::USED; i += W::THREADS) {
     const int map = i / (32 * ImgK::USED), qr = i / ImgK::USED % 32, ch = i % ImgK::USED, n = tile * 32 + qr < rows ? tile * 32 + qr : rows - 1;
@@ -528,45 +570,46 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
   const float c = p.scale * LOG2E;
   const int lim = p.causal ? sq.start + qi + 1 : end;  // keys this row sees
 
-  auto fill = [&](int block, int stage, unsigned bits) {
-    unsigned char* buf = smem + (stage * WAVES + wave) * W::IMAGES;
+  auto fill = [&](unsigned char* buf, int block, unsigned bits) {
     const long j0 = (long)block * 32;
 #pragma unroll
     for (int i = 0; i < MAPS; ++i) ImgK::template fill<32, VECTOR, 64>(buf + i * W::K_BYTES, kb + j0 * p.k_s[1] + (f.map0 + i) * p.k_s[3], p.k_s[1], p.d, bits, lane);
     ImgV::template fill<32, VECTOR, 64>(buf + MAPS * W::K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, bits, lane);
   };
+  auto use = [&](const unsigned char* buf, int block, unsigned seen) {
+    const unsigned mine = seen & (unsigned)low_bits(lim - block * 32);
+    if (__any(mine != 0)) f.tile(buf, qimg + f.map0 * W::K_BYTES, 0, W::K_BYTES, MAPS * W::K_BYTES, __any(mine != ~0u), mine >> (4 * half), c, p.d, half);
+  };
   const int kw = MAPS == 1 ? wave >> 1 : wave;
+  unsigned char* images = smem + wave * W::STAGES * W::IMAGES;
   unsigned bits = 0;
   int stage = 0;
   if (first + kw < stop) {
     bits = (unsigned)key_bits(p, b, (first + kw) * 32, sq.len, lane);
-    fill(first + kw, 0, bits);
+    fill(images, first + kw, bits);
   }
   for (int k = first + kw; k < stop; k += KW) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's images are complete
     const unsigned cur = bits;
-    const int buf = (stage * WAVES + wave) * W::IMAGES;
+    const bool more = k + KW < stop;
+    if (more) bits = (unsigned)key_bits(p, b, (k + KW) * 32, sq.len, lane);
     if constexpr (W::STAGES == 2) {
+      overlap(images + (stage ^ 1) * W::IMAGES, images + stage * W::IMAGES,
+              [&](unsigned char* next) {
+                if (more) fill(next, k + KW, bits);
+              },
+              [&](const unsigned char* now) { use(now, k, cur); });
       stage ^= 1;
-      if (k + KW < stop) {
-        bits = (unsigned)key_bits(p, b, (k + KW) * 32, sq.len, lane);
-        fill(k + KW, stage, bits);
-      }
-    }
-    const unsigned mine = cur & (unsigned)low_bits(lim - k * 32);
-    if (__any(mine != 0)) f.tile(smem, buf, W::K_BYTES, buf + MAPS * W::K_BYTES, __any(mine != ~0u), mine >> (4 * half), c, p.d, half);
-    if constexpr (W::STAGES == 1) {
+    } else {
+      use(images, k, cur);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (every read of the image has returned before it is filled again)
-      if (k + KW < stop) {
-        bits = (unsigned)key_bits(p, b, (k + KW) * 32, sq.len, lane);
-        fill(k + KW, 0, bits);
-      }
+      if (more) fill(images, k + KW, bits);
     }
   }
 
   // add the waves up: maxima and sums of all waves first, then each map's O, block by block; wave w finishes the channel blocks w, w + WAVES, ..
   float* ml = reinterpret_cast<float*>(smem + (W::LDS - W::SUMS));  // [wave][map of the wave][m, l][32]
-  float* x = reinterpret_cast<float*>(smem);
+  float4* x = reinterpret_cast<float4*>(smem);
 #pragma unroll
   for (int i = 0; i < MAPS; ++i) {
     f.l[i] += other_half(f.l[i]);
@@ -598,9 +641,9 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        x[(wave * NB + n) * W::BLOCK + e * 64 + lane] = f.o[round][n][e] * g;
-        if (e == 15) __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < 4; ++e) {
+        x[((wave * NB + n) * 4 + e) * 64 + lane] = make_float4(f.o[round][n][4 * e] * g, f.o[round][n][4 * e + 1] * g, f.o[round][n][4 * e + 2] * g, f.o[round][n][4 * e + 3] * g);
+        if (e == 3) __builtin_amdgcn_sched_barrier(0);
       }
     __syncthreads();
 #pragma unroll
@@ -615,7 +658,10 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
 #pragma unroll
           for (int w = 0; w < KW; ++w) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[map][j][e] += x[((MAPS == 1 ? 2 * w + map : w) * NB + n) * W::BLOCK + e * 64 + lane];
+            for (int e = 0; e < 4; ++e) {
+              const float4 v = x[(((MAPS == 1 ? 2 * w + map : w) * NB + n) * 4 + e) * 64 + lane];
+              o[map][j][4 * e] += v.x; o[map][j][4 * e + 1] += v.y; o[map][j][4 * e + 2] += v.z; o[map][j][4 * e + 3] += v.w;
+            }
             __builtin_amdgcn_sched_barrier(0);
           }
       }
@@ -631,8 +677,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
         if (wave + j * WAVES < NB)
 #pragma unroll
           for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float2*>(out + map * NB * 32 + (wave + j * WAVES) * 32 + 8 * g + 4 * half) = make_float2(o[map][j][4 * g], o[map][j][4 * g + 1]),
-            *reinterpret_cast<float2*>(out + map * NB * 32 + (wave + j * WAVES) * 32 + 8 * g + 4 * half + 2) = make_float2(o[map][j][4 * g + 2], o[map][j][4 * g + 3]);
+            *reinterpret_cast<float4*>(out + map * NB * 32 + (wave + j * WAVES) * 32 + 8 * g + 4 * half) = make_float4(o[map][j][4 * g], o[map][j][4 * g + 1], o[map][j][4 * g + 2], o[map][j][4 * g + 3]);
       if (wave == 0 && half == 0) {
         out[2 * NB * 32 + map * 2] = M[map];
         out[2 * NB * 32 + map * 2 + 1] = L[map];
@@ -641,20 +686,31 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
     return;
   }
   const float lam = p.lam[p.n_lam > 1 ? h : 0];
-  const long row = ((long)b * p.H + h) * p.Tq + qi;
   const int dvs = (p.dv + 7) & ~7;
-  float ss = 0.f;
+  static_assert(W::LDS - W::SUMS >= WAVES * STRIP_BYTES, "the strips fit");
+  float* strip = reinterpret_cast<float*>(smem + wave * STRIP_BYTES);
+  const int row0 = tile * 32;
+  auto head_of = [&](int r) { return hk * group + (row0 + r) / p.Tq; };
+  __syncthreads();  // every wave has read the exchange
 #pragma unroll
   for (int map = 0; map < 2; ++map) {
     const float inv = inverse_sum(L[map]);
-    if (p.lse && live && half == 0 && wave == 0) p.lse[(long)map * p.B * p.H * p.Tq + row] = log_sum(M[map], L[map]);
+    if (p.lse && live && half == 0 && wave == 0) p.lse[((long)map * p.B + b) * p.H * p.Tq + (long)h * p.Tq + qi] = log_sum(M[map], L[map]);
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[map][j][e] *= inv;
-      if (p.o1 && live && wave + j * WAVES < NB) store_block<T>((T*)(map ? p.o2 : p.o1) + row * dvs, wave + j * WAVES, half, dvs, o[map][j]);
+      if (p.o1 && wave + j * WAVES < NB) {
+        T* to = (T*)(map ? p.o2 : p.o1);
+        strip_put(strip, lane, 0, o[map][j], 1.f);
+        __builtin_amdgcn_wave_barrier();
+        strip_store<T>(strip, lane, 1, (wave + j * WAVES) * 32, dvs, true, Weights{nullptr, 0},
+                       [&](int r) { return row0 + r < rows ? to + (((long)b * p.H + head_of(r)) * p.Tq + (row0 + r) % p.Tq) * dvs : nullptr; });
+        __builtin_amdgcn_wave_barrier();
+      }
     }
   }
+  float ss = 0.f;
 #pragma unroll
   for (int j = 0; j < MINE; ++j)
 #pragma unroll
@@ -673,11 +729,16 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
     for (int w = 0; w < WAVES; ++w) ss += ml[w * 32 + col];
     g *= 1.f / sqrtf(ss / (float)p.dv + p.eps);
   }
-  if (!live) return;
-  T* out = (T*)p.out + (long)b * p.o_s[0] + (long)qi * p.o_s[1] + (long)h * p.o_s[2];
+  T* out = (T*)p.out + (long)b * p.o_s[0];
 #pragma unroll
   for (int j = 0; j < MINE; ++j)
-    if (wave + j * WAVES < NB) store_result<T>(p, out, wave + j * WAVES, half, g, o[0][j]);
+    if (wave + j * WAVES < NB) {
+      strip_put(strip, lane, 0, o[0][j], g);
+      __builtin_amdgcn_wave_barrier();
+      strip_store<T>(strip, lane, 1, (wave + j * WAVES) * 32, p.dv, p.out_vec, Weights{p.norm_w, p.norm_w_bf16},
+                     [&](int r) { return row0 + r < rows ? out + (long)((row0 + r) % p.Tq) * p.o_s[1] + (long)head_of(r) * p.o_s[2] : nullptr; });
+      __builtin_amdgcn_wave_barrier();
+    }
 }
 
 // the splits' sums of a row -> its result: one wave a row, channels lane, lane + 64, ..
@@ -730,7 +791,7 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int ch = lane + 64 * e;
-    if (ch < p.dv) out[ch] = ElemTraits<T>::from_f(o[0][e] * (p.norm ? g * norm_weight(p, ch) : g));
+    if (ch < p.dv) out[ch] = ElemTraits<T>::from_f(o[0][e] * (p.norm_w ? g * Weights{p.norm_w, p.norm_w_bf16}[ch] : g));
   }
 }
 
@@ -741,31 +802,49 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_
 //   dQ_i = scale dS_i K_i      dK_i = scale dS_i^T Q_i      dV = (P_1 - lambda P_2)^T dO
 // 1. diff_attn_bwd_rows_kernel: dO (rounded once: it is an MFMA operand twice), delta_i from that rounded dO -- so that the rows of dS still sum to
 //    zero -- and partial sums of dw, dlambda from the unrounded one.  Bounded by HBM.
-// grid (blocks, H); LPR lanes a row, 4 channels a lane
+// grid (blocks, H); lpr lanes a row (a power of two), 8 channels a lane: 16-byte loads, 64 / lpr rows a wave at a time.  partial: [1 + dv][blocks x H], the
+// sums of one value side by side.
 template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_kernel(tfpp_diff_attn_params p, int lpr) {
-  __shared__ float sm[256 * 5];
-  const int h = blockIdx.y, lane = threadIdx.x & 63, c0 = (lane % lpr) * 4, dvs = (p.dv + 7) & ~7;
+  constexpr int E = 8;
+  __shared__ float sm[E * 256 + 4];
+  const int h = blockIdx.y, lane = threadIdx.x & 63, c0 = (lane & (lpr - 1)) * E, dvs = (p.dv + 7) & ~7;
   const int rpw = 64 / lpr, slots = (int)gridDim.x * 4 * rpw;
   const long rows = (long)p.B * p.Tq;
-  const float lam = p.lam[p.n_lam > 1 ? h : 0];
-  float w[4], dw[4] = {0.f, 0.f, 0.f, 0.f}, dl = 0.f;
+  const float lam = p.lam[p.n_lam > 1 ? h : 0], inv_dv = 1.f / (float)p.dv;
+  float w[E], dw[E], dl = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = c0 + e < p.dv ? p.out_scale * (p.norm ? norm_weight(p, c0 + e) : 1.f) : 0.f;
+  for (int e = 0; e < E; ++e) {
+    w[e] = c0 + e < p.dv ? p.out_scale * (p.norm_w ? Weights{p.norm_w, p.norm_w_bf16}[c0 + e] : 1.f) : 0.f;
+    dw[e] = 0.f;
+  }
   const long first = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * rpw + lane / lpr;
   const long rounds = (rows + slots - 1) / slots;
   for (long k = 0; k < rounds; ++k) {  // (the same number of rounds in every lane: the shuffles below need them all)
     const long n = first + k * slots;
-    const bool live = n < rows;
+    const bool live = n < rows, in = live && c0 < dvs;
     const int b = live ? (int)(n / p.Tq) : 0, t = live ? (int)(n % p.Tq) : 0;
     const long row = ((long)b * p.H + h) * p.Tq + t;
-    const T* dout = (const T*)p.dout + (long)b * p.do_s[0] + (long)t * p.do_s[1] + (long)h * p.do_s[2];
-    float g[4], o1[4], o2[4], s[2] = {0.f, 0.f};
+    const T* dout = (const T*)p.dout + (long)b * p.do_s[0] + (long)t * p.do_s[1] + (long)h * p.do_s[2] + c0;
+    float g[E], o1[E], o2[E], s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool in = live && c0 + e < p.dv;
-      g[e] = in ? ElemTraits<T>::to_f(dout[c0 + e]) : 0.f;
-      o1[e] = in ? ElemTraits<T>::to_f(((const T*)p.o1)[row * dvs + c0 + e]) : 0.f;
-      o2[e] = in ? ElemTraits<T>::to_f(((const T*)p.o2)[row * dvs + c0 + e]) : 0.f;
+    for (int e = 0; e < E; ++e) g[e] = o1[e] = o2[e] = 0.f;
+    if (in) {
+#pragma unroll
+      for (int e = 0; e < E; e += ElemTraits<T>::VEC) {
+        load_vec<T>((const T*)p.o1 + row * dvs + c0 + e, o1 + e);
+        load_vec<T>((const T*)p.o2 + row * dvs + c0 + e, o2 + e);
+      }
+      if (p.do_vec && c0 + E <= p.dv) {
+#pragma unroll
+        for (int e = 0; e < E; e += ElemTraits<T>::VEC) load_vec<T>(dout + e, g + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (c0 + e < p.dv) g[e] = ElemTraits<T>::to_f(dout[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {  // (channels behind dv: V is zero there, so are O_1 and O_2)
       const float o = o1[e] - lam * o2[e];
       s[0] += o * o;
       s[1] += w[e] * g[e] * o;
@@ -776,12 +855,12 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
         s[0] += __shfl_xor(s[0], x, 64);
         s[1] += __shfl_xor(s[1], x, 64);
       }
-      r = 1.f / sqrtf(s[0] / (float)p.dv + p.eps);  // (eps > 0: checked by the launcher)
-      f = r * r * r * s[1] / (float)p.dv;
+      r = 1.f / sqrtf(s[0] * inv_dv + p.eps);  // (eps > 0: checked by the launcher)
+      f = r * r * r * s[1] * inv_dv;
     }
-    float d[4], t1 = 0.f, t2 = 0.f;
+    float d[E], t1 = 0.f, t2 = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < E; ++e) {
       const float o = o1[e] - lam * o2[e];
       dw[e] += p.out_scale * g[e] * o * r;
       d[e] = r * w[e] * g[e] - o * f;
@@ -794,43 +873,40 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
       t1 += __shfl_xor(t1, x, 64);
       t2 += __shfl_xor(t2, x, 64);
     }
-    if (live) {
-      if (c0 < dvs) store4<T>((T*)p.d_o + row * dvs, c0, dvs, true, d[0], d[1], d[2], d[3]);
-      if (c0 == 0) {
-        p.delta[row] = t1;
-        p.delta[(long)p.B * p.H * p.Tq + row] = t2;
-      }
+    if (in)
+#pragma unroll
+      for (int e = 0; e < E; e += ElemTraits<T>::VEC) store_vec<T>((T*)p.d_o + row * dvs + c0 + e, d + e);
+    if (live && c0 == 0) {
+      p.delta[row] = t1;
+      p.delta[(long)p.B * p.H * p.Tq + row] = t2;
     }
   }
-  // partial row (block, head): dlambda, then dw
 #pragma unroll
-  for (int e = 0; e < 4; ++e) sm[e * 256 + threadIdx.x] = dw[e];
-  sm[4 * 256 + threadIdx.x] = dl;
+  for (int e = 0; e < E; ++e) sm[e * 256 + threadIdx.x] = dw[e];
+  dl = wave_sum(dl);
+  if (lane == 0) sm[E * 256 + (threadIdx.x >> 6)] = dl;
   __syncthreads();
-  float* out = p.partial + ((long)blockIdx.x * p.H + h) * (1 + p.dv);
-  if (threadIdx.x == 0) {
-    float a = 0.f;
-    for (int i = 0; i < 256; ++i) a += sm[4 * 256 + i];
-    out[0] = a;
-  }
+  const long pitch = (long)gridDim.x * p.H, at = (long)blockIdx.x * p.H + h;
+  if (threadIdx.x == 0) p.partial[at] = (sm[E * 256] + sm[E * 256 + 1]) + (sm[E * 256 + 2] + sm[E * 256 + 3]);
   for (int c = threadIdx.x; c < p.dv; c += 256) {
     float a = 0.f;
-    for (int i = c >> 2; i < 256; i += lpr) a += sm[(c & 3) * 256 + i];
-    out[1 + c] = a;
+    for (int i = c / E; i < 256; i += lpr) a += sm[(c % E) * 256 + i];
+    p.partial[(1 + c) * pitch + at] = a;
   }
 }
 
 // dlambda (blocks 0 .. n_lam - 1) and dw (the blocks behind): one value per workgroup, fixed order
 template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_kernel(tfpp_diff_attn_params p, int blocks) {
   __shared__ float sm[4];
-  const int x = blockIdx.x, pitch = 1 + p.dv;
+  const int x = blockIdx.x, n = blocks * p.H;
   const bool is_lam = x < p.n_lam;
   const int c = is_lam ? 0 : 1 + x - p.n_lam;
+  const float* src = p.partial + (long)c * n;
   float s = 0.f;
   if (is_lam && p.n_lam > 1)
-    for (int i = threadIdx.x; i < blocks; i += 256) s += p.partial[((long)i * p.H + x) * pitch];
+    for (int i = threadIdx.x; i < blocks; i += 256) s += src[(long)i * p.H + x];
   else
-    for (int i = threadIdx.x; i < blocks * p.H; i += 256) s += p.partial[(long)i * pitch + c];
+    for (int i = threadIdx.x; i < n; i += 256) s += src[i];
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
   __syncthreads();
@@ -843,7 +919,7 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_k
 
 // 2. dQ.  Workgroup = (batch, head, 128 queries), wave = 32 queries, as the forward pass: S_i^T = K_i Q_i^T, dP^T = V dO^T (keys x queries),
 //    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.
-template <typename T, int NB> constexpr int dq_lds() { return 2 * 32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES); }
+template <typename T, int NB> constexpr int dq_lds() { return at_least(2 * 32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES), 4 * STRIP_BYTES); }
 
 template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB <= (sizeof(T) == 2 ? 4 : 2) ? 2 : 1)) void diff_attn_bwd_dq_kernel(tfpp_diff_attn_params p) {
   constexpr int KT = 32, NT = 256, CD = (NB + 1) / 2;
@@ -862,7 +938,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
   const long row = ((long)b * p.H + h) * p.Tq + qc, rows = (long)p.B * p.H * p.Tq;
   const T* kb = (const T*)p.k + (long)b * p.k_s[0] + (long)hk * p.k_s[2];
   const T* vb = (const T*)p.v + (long)b * p.v_s[0] + (long)hk * p.v_s[2];
-  constexpr bool HOLD = sizeof(T) == 2 || NB < 5;  // wide fp32 heads do not fit the registers: Q and dO are read again for every tile
+  constexpr bool HOLD = NB < 5 || (sizeof(T) == 2 && VECTOR);  // else Q and dO do not fit the registers and are read again for every tile
   const T* qrow = (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2];
   Frag8<T> q[2][HOLD ? NB : 1], dof[HOLD ? 2 * NB : 1];
   if constexpr (HOLD)
@@ -887,8 +963,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[i][n][r] = 0.f;
   const int k_rows = ImgK::rows_at(lane), v_rows = ImgV::rows_at(lane), k_cols = ImgK::cols_at(lane);
-  auto fill = [&](int step, unsigned long long bits) {
-    unsigned char* buf = smem + (step & 1) * BUF;
+  auto fill = [&](unsigned char* buf, int step, unsigned long long bits) {
     const long j0 = (long)step * KT;
 #pragma unroll
     for (int i = 0; i < 2; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, bits, tid);
@@ -897,21 +972,24 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
   unsigned long long bits = 0;
   if (steps > 0) {
     bits = key_bits(p, b, 0, sq.len, lane);
-    fill(0, bits);
+    fill(smem, 0, bits);
   }
   for (int s = 0; s < steps; ++s) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     const unsigned long long cur = bits & low_bits(KT);
-    if (s + 1 < steps) {
-      bits = key_bits(p, b, (s + 1) * KT, sq.len, lane);
-      fill(s + 1, bits);
-    }
+    const bool more = s + 1 < steps;
+    if (more) bits = key_bits(p, b, (s + 1) * KT, sq.len, lane);
+    overlap(smem + (~s & 1) * BUF, smem + (s & 1) * BUF,
+            [&](unsigned char* next) {
+              if (more) fill(next, s + 1, bits);
+            },
+            [&](const unsigned char* now) {
     const int j0 = s * KT;
-    if ((p.causal && sq.start + w0 + 32 - j0 <= 0) || cur == 0) continue;
+    if ((p.causal && sq.start + w0 + 32 - j0 <= 0) || cur == 0) return;
     const bool masked = cur != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
     const unsigned vis = (unsigned)(p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur) >> (4 * half);
-    const int buf = (s & 1) * BUF, kr = k_rows + buf, vr = v_rows + buf + 2 * K_BYTES, kc = k_cols + buf;
+    const int vr = v_rows + 2 * K_BYTES;
     f32x16_t sc[2], dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sc[0][r] = sc[1][r] = dp[r] = 0.f;
@@ -920,14 +998,14 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
 #pragma unroll
       for (int ks = 0; ks < NB; ++ks) {
         Frag8<T> a;
-        ImgK::rows(smem + i * K_BYTES, kr, ks, a);
+        ImgK::rows(now + i * K_BYTES, k_rows, ks, a);
         if constexpr (!HOLD) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][0]);
         mma(a, q[i][HOLD ? ks : 0], sc[i]);
       }
 #pragma unroll
     for (int ks = 0; ks < 2 * NB; ++ks) {
       Frag8<T> a;
-      ImgV::rows(smem, vr, ks, a);
+      ImgV::rows(now, vr, ks, a);
       if constexpr (!HOLD) load_frag<T, true>((const T*)p.d_o + row * dvs, ks * 16 + half * 8, dvs, true, dof[0]);
       mma(a, dof[HOLD ? ks : 0], dp);
     }
@@ -951,22 +1029,18 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
 #pragma unroll
         for (int n = 0; n < CD; ++n) {
           Frag8<T> a;
-          ImgK::cols(smem + i * K_BYTES + 16 * t * ImgK::ROW_BYTES, kc, n, a);
+          ImgK::cols(now + i * K_BYTES + 16 * t * ImgK::ROW_BYTES, k_cols, n, a);
           mma(a, ds, dq[i][n]);
         }
       }
+            });
   }
-  if (qi < p.Tq) {
+  __syncthreads();  // every wave is past its last image
+  float* strip = reinterpret_cast<float*>(smem + wave * STRIP_BYTES);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      T* out = (T*)p.dq_out + (long)b * p.dq_s[0] + (long)qi * p.dq_s[1] + (long)h * p.dq_s[2] + (long)i * p.dq_s[3];
-#pragma unroll
-      for (int n = 0; n < CD; ++n)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          store4<T>(out, n * 32 + 8 * g + 4 * half, p.d, p.dq_vec, p.scale * dq[i][n][4 * g], p.scale * dq[i][n][4 * g + 1], p.scale * dq[i][n][4 * g + 2],
-                    p.scale * dq[i][n][4 * g + 3]);
-    }
+  for (int i = 0; i < 2; ++i) {
+    T* out = (T*)p.dq_out + (long)b * p.dq_s[0] + (long)w0 * p.dq_s[1] + (long)h * p.dq_s[2] + (long)i * p.dq_s[3];
+    store_rows<T>(strip, lane, dq[i], p.scale, p.d, p.dq_vec, Weights{nullptr, 0}, [&](int r) { return w0 + r < p.Tq ? out + (long)r * p.dq_s[1] : nullptr; });
   }
 }
 
@@ -976,13 +1050,13 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
 //    separate workgroups; S and dP are computed again (3 / 2 of the flop).
 enum { PART_ALL, PART_DK, PART_DV };
 template <typename T, int NB> constexpr bool dkv_split() { return NB >= (sizeof(T) == 2 ? 5 : 4); }
-template <typename T, int NB> constexpr int dkv_lds() { return 2 * (32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + 1024); }
+template <typename T, int NB> constexpr int dkv_lds() { return at_least(2 * (32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + 1024), 4 * STRIP_BYTES); }
 
 template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds__(256, (PART == PART_ALL ? NB <= (sizeof(T) == 2 ? 2 : 1) : NB <= (sizeof(T) == 2 ? 5 : 4)) ? 2 : 1) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
   constexpr int QT = 32, NT = 256, MAPS = PART == PART_DK ? 1 : 2, CD = (NB + 1) / 2;
   typedef Img<T, CD> ImgQ;
   typedef Img<T, NB> ImgO;
-  constexpr int Q_BYTES = QT * ImgQ::ROW_BYTES, O_BYTES = QT * ImgO::ROW_BYTES, BUF = 2 * Q_BYTES + O_BYTES + 1024;  // (4 x 32 row values; images start at whole rows, <= 1 KB)
+  constexpr int Q_BYTES = QT * ImgQ::ROW_BYTES, O_BYTES = QT * ImgO::ROW_BYTES, BUF = 2 * Q_BYTES + O_BYTES + 1024;  // (the rows' values; images start at whole rows, <= 1 KB)
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int tiles = (p.Tk + QB - 1) / QB, group = p.H / p.Hkv;
@@ -1027,8 +1101,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
   const int per = any ? (p.Tq - q_lo + QT - 1) / QT : 0, steps = per * group;
 
   const int q_rows = ImgQ::rows_at(lane), o_rows = ImgO::rows_at(lane), q_cols = ImgQ::cols_at(lane), o_cols = ImgO::cols_at(lane);
-  auto fill = [&](int step) {
-    unsigned char* buf = smem + (step & 1) * BUF;
+  auto fill = [&](unsigned char* buf, int step) {
     const int h = hk * group + step / per, q0 = q_lo + step % per * QT;
     const unsigned long long bits = low_bits(p.Tq - q0);
     const T* qb = (const T*)p.q + (long)b * p.q_s[0] + (long)q0 * p.q_s[1] + (long)h * p.q_s[2];
@@ -1036,24 +1109,26 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
     for (int i = map0; i < map0 + MAPS; ++i) ImgQ::template fill<QT, VECTOR, NT>(buf + i * Q_BYTES, qb + i * p.q_s[3], p.q_s[1], p.d, bits, tid);
     ImgO::template fill<QT, true, NT>(buf + 2 * Q_BYTES, (const T*)p.d_o + row * dvs, dvs, dvs, bits, tid);
-    if (tid < 4 * QT) {  // lse_1, lse_2, delta_1, delta_2 of the tile; queries behind the last: +inf, so that P = 0
-      const int a = tid / QT, t = tid % QT;
-      const bool in = q0 + t < p.Tq;
-      const float* src = a < 2 ? p.lse : p.delta;
-      reinterpret_cast<float*>(buf + 2 * Q_BYTES + O_BYTES)[tid] = in ? src[(a & 1) * rows + row + t] : (a < 2 ? INFINITY : 0.f);
-    }
+    // lse_1, lse_2, delta_1, delta_2 of the tile, one array a wave.  Queries behind the last: all zero like their Q and dO, so P = 1 but dV, dS get 0
+    const float* src = (wave < 2 ? p.lse : p.delta) + (wave & 1) * rows + row;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)src, 0, 0x7fffffff, 0x00020000), (lds_void_t*)(buf + 2 * Q_BYTES + O_BYTES + wave * 256), 4,
+                                             lane < QT && q0 + lane < p.Tq ? lane * 4 : (int)0x80000000, 0, 0, 0);
   };
-  if (steps > 0) fill(0);
+  if (steps > 0) fill(smem, 0);
   for (int s = 0; s < steps; ++s) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
-    if (s + 1 < steps) fill(s + 1);
+    overlap(smem + (~s & 1) * BUF, smem + (s & 1) * BUF,
+            [&](unsigned char* next) {
+              if (s + 1 < steps) fill(next, s + 1);
+            },
+            [&](const unsigned char* now) {
     const int h = hk * group + s / per, q0 = q_lo + s % per * QT;
-    if (p.causal && sq.start + q0 + QT - 1 < w0) continue;  // no query of the tile sees a key of this wave
+    if (p.causal && sq.start + q0 + QT - 1 < w0) return;  // no query of the tile sees a key of this wave
     const bool diag = p.causal && sq.start + q0 < w0 + 31;
     const float lam = p.lam[p.n_lam > 1 ? h : 0];
-    const int buf = (s & 1) * BUF, qr = q_rows + buf, orow = o_rows + buf + 2 * Q_BYTES, qcol = q_cols + buf, ocol = o_cols + buf + 2 * Q_BYTES;
-    const float* st = reinterpret_cast<const float*>(smem + buf + 2 * Q_BYTES + O_BYTES);
+    const int orow = o_rows + 2 * Q_BYTES, ocol = o_cols + 2 * Q_BYTES;
+    const float* st = reinterpret_cast<const float*>(now + 2 * Q_BYTES + O_BYTES);
     f32x16_t sc[MAPS], dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -1066,7 +1141,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
       for (int ks = 0; ks < NB; ++ks) {
         Frag8<T> a;
-        ImgQ::rows(smem + (map0 + i) * Q_BYTES, qr, ks, a);
+        ImgQ::rows(now + (map0 + i) * Q_BYTES, q_rows, ks, a);
         if constexpr (!HOLD) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, seen, k[i][0]);
         mma(a, k[i][HOLD ? ks : 0], sc[i]);
       }
@@ -1074,7 +1149,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
       for (int ks = 0; ks < 2 * NB; ++ks) {
         Frag8<T> a;
-        ImgO::rows(smem, orow, ks, a);
+        ImgO::rows(now, orow, ks, a);
         if constexpr (!HOLD) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, seen, v[0]);
         mma(a, v[HOLD ? ks : 0], dp);
       }
@@ -1087,7 +1162,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
       for (int i = 0; i < MAPS; ++i) {
         const int map = map0 + i;
-        const float4 l4 = *reinterpret_cast<const float4*>(st + map * QT + t0), d4 = *reinterpret_cast<const float4*>(st + (2 + map) * QT + t0);
+        const float4 l4 = *reinterpret_cast<const float4*>(st + map * 64 + t0), d4 = *reinterpret_cast<const float4*>(st + (2 + map) * 64 + t0);
         const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w}, sign = map ? -lam : 1.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -1107,7 +1182,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           Frag8<T> a;
-          ImgO::cols(smem + 16 * t * ImgO::ROW_BYTES, ocol, n, a);
+          ImgO::cols(now + 16 * t * ImgO::ROW_BYTES, ocol, n, a);
           mma(a, f, dv[n]);
         }
       }
@@ -1118,31 +1193,24 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
 #pragma unroll
           for (int n = 0; n < CD; ++n) {
             Frag8<T> a;
-            ImgQ::cols(smem + (map0 + i) * Q_BYTES + 16 * t * ImgQ::ROW_BYTES, qcol, n, a);
+            ImgQ::cols(now + (map0 + i) * Q_BYTES + 16 * t * ImgQ::ROW_BYTES, q_cols, n, a);
             mma(a, f, dk[i][n]);
           }
         }
     }
+            });
   }
-  if (kj >= p.Tk) return;  // (keys that nobody sees get zeros)
-  if constexpr (WANT_DV) {
-    T* out = (T*)p.dv_out + (long)b * p.dv_s[0] + (long)kj * p.dv_s[1] + (long)hk * p.dv_s[2];
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        store4<T>(out, n * 32 + 8 * g + 4 * half, p.dv, p.dv_vec, dv[n][4 * g], dv[n][4 * g + 1], dv[n][4 * g + 2], dv[n][4 * g + 3]);
+  __syncthreads();  // every wave is past its last image
+  float* strip = reinterpret_cast<float*>(smem + wave * STRIP_BYTES);
+  if constexpr (WANT_DV) {  // (keys that nobody sees get zeros)
+    T* out = (T*)p.dv_out + (long)b * p.dv_s[0] + (long)w0 * p.dv_s[1] + (long)hk * p.dv_s[2];
+    store_rows<T>(strip, lane, dv, 1.f, p.dv, p.dv_vec, Weights{nullptr, 0}, [&](int r) { return w0 + r < p.Tk ? out + (long)r * p.dv_s[1] : nullptr; });
   }
   if constexpr (WANT_DK)
 #pragma unroll
     for (int i = 0; i < MAPS; ++i) {
-      T* out = (T*)p.dk_out + (long)b * p.dk_s[0] + (long)kj * p.dk_s[1] + (long)hk * p.dk_s[2] + (long)(map0 + i) * p.dk_s[3];
-#pragma unroll
-      for (int n = 0; n < CD; ++n)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          store4<T>(out, n * 32 + 8 * g + 4 * half, p.d, p.dk_vec, p.scale * dk[i][n][4 * g], p.scale * dk[i][n][4 * g + 1], p.scale * dk[i][n][4 * g + 2],
-                    p.scale * dk[i][n][4 * g + 3]);
+      T* out = (T*)p.dk_out + (long)b * p.dk_s[0] + (long)w0 * p.dk_s[1] + (long)hk * p.dk_s[2] + (long)(map0 + i) * p.dk_s[3];
+      store_rows<T>(strip, lane, dk[i], p.scale, p.d, p.dk_vec, Weights{nullptr, 0}, [&](int r) { return w0 + r < p.Tk ? out + (long)r * p.dk_s[1] : nullptr; });
     }
 }
 
@@ -1194,8 +1262,8 @@ bool vector_rows(const tfpp_diff_attn_params& p, int vec) {
   return p.d % vec == 0 && p.dv % vec == 0 && p.q_s[1] <= far && p.k_s[1] <= far && p.v_s[1] <= far && !(((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15) && strides_vec(p.q_s, 4, vec) && strides_vec(p.k_s, 4, vec) &&
          strides_vec(p.v_s, 3, vec);
 }
-// 32 / 16-byte channel quads of an output
-bool quad(const void* ptr, const int64_t* s, int n, int esz) { return !((uintptr_t)ptr & (4 * esz - 1)) && strides_vec(s, n, 4); }
+// Can an output be written 16 bytes at a time?
+bool out_vector(const void* ptr, const int64_t* s, int n, int vec) { return !((uintptr_t)ptr & 15) && strides_vec(s, n, vec); }
 
 template <typename K> int lds_limit(K* kernel, int bytes, unsigned long long* done) {
   if (bytes > 64 * 1024 && tfpp_first_use_on_this_device(done)) {
@@ -1267,10 +1335,15 @@ int few_splits(const tfpp_diff_attn_params& p) {
   if (n > most) n = most;
   return n < 1 ? 1 : (int)n;
 }
-int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass for each head: 64 rows each at least, about 1024 in all
-  const long rows = (long)p.B * p.Tq;
-  long n = 1024 / p.H > 1 ? 1024 / p.H : 1;
-  if (n > (rows + 63) / 64) n = (rows + 63) / 64;
+int row_lanes(const tfpp_diff_attn_params& p) {
+  int n = 1;
+  while (n * 8 < p.dv) n <<= 1;
+  return n;
+}
+int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass for each head: four rounds of 256 / row_lanes rows, about 4096 in all at most
+  const long rows = (long)p.B * p.Tq, round = 256 / row_lanes(p);
+  long n = (rows + 4 * round - 1) / (4 * round), most = 4096 / p.H > 1 ? 4096 / p.H : 1;
+  if (n > most) n = most;
   return (int)n;
 }
 }  // namespace
@@ -1278,7 +1351,7 @@ int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass 
 extern "C" int tfpp_diff_attn_fwd(const tfpp_diff_attn_params* pp, int dtype, void* stream) {
   if (!pp || !valid(*pp, dtype) || !pp->out || (pp->o1 != nullptr) != (pp->o2 != nullptr)) return TFPP_EINVAL;
   tfpp_diff_attn_params p = *pp;
-  p.out_vec = quad(p.out, p.o_s, 3, dtype == TFPP_F32 ? 4 : 2);
+  p.out_vec = out_vector(p.out, p.o_s, 3, dtype == TFPP_F32 ? 4 : 8);
   p.splits = few_splits(p);
   if (p.splits > 1 && !p.partial) return TFPP_EINVAL;
   const int step = p.splits ? STEP_FEW : STEP_FWD;
@@ -1303,14 +1376,14 @@ extern "C" int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* pp, int dtype, vo
   tfpp_diff_attn_params p = *pp;
   if (!p.dout || !p.o1 || !p.o2 || !p.lse || !p.d_o || !p.delta || !p.partial || !p.dlam || !p.dq_out || !p.dk_out || !p.dv_out || (p.norm_w && !p.dnorm_w)) return TFPP_EINVAL;
   if (p.H > 65535 || (((uintptr_t)p.o1 | (uintptr_t)p.o2 | (uintptr_t)p.d_o) & 15)) return TFPP_EINVAL;
-  const int esz = dtype == TFPP_F32 ? 4 : 2;
-  p.dq_vec = quad(p.dq_out, p.dq_s, 4, esz);
-  p.dk_vec = quad(p.dk_out, p.dk_s, 4, esz);
-  p.dv_vec = quad(p.dv_out, p.dv_s, 3, esz);
+  const int vec = dtype == TFPP_F32 ? 4 : 8;
+  p.dq_vec = out_vector(p.dq_out, p.dq_s, 4, vec);
+  p.dk_vec = out_vector(p.dk_out, p.dk_s, 4, vec);
+  p.dv_vec = out_vector(p.dv_out, p.dv_s, 3, vec);
   hipStream_t st = (hipStream_t)stream;
   const int blocks = row_blocks(p);
-  int lpr = 1;
-  while (lpr * 4 < ((p.dv + 7) & ~7)) lpr <<= 1;
+  const int lpr = row_lanes(p);
+  p.do_vec = out_vector(p.dout, p.do_s, 3, vec);
   const dim3 sums(p.n_lam + (p.norm_w ? p.dv : 0));
   if (dtype == TFPP_F32) {
     hipLaunchKernelGGL(diff_attn_bwd_rows_kernel<float>, dim3(blocks, p.H), dim3(256), 0, st, p, lpr);

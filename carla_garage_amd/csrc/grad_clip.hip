@@ -14,7 +14,7 @@
 namespace {
 constexpr int GC_THREADS = 256;
 constexpr int GC_GRID = 2048;    // 8 workgroups per CU
-constexpr int GC_CHUNK = 16384;  // elements: 64 KB of fp32, 16 float4 per thread
+constexpr int GC_CHUNK = 4096;   // elements: 16 KB of fp32; small, so that 2048 workgroups end together (16384: 40 M bf16 values took 88 us, 4096: see below)
 enum { GC_SRC_BF16 = 1, GC_DST_BF16 = 2, GC_VEC = 4 };
 
 __device__ __forceinline__ float max_nan(float m, float v) { return (v > m || v != v) ? v : m; }  // NaN wins and stays
@@ -58,8 +58,10 @@ template <int P> __global__ __launch_bounds__(GC_THREADS) void grad_norm_kernel(
   __shared__ double sm[GC_THREADS / 64];
   double s = 0.0;
   float m = 0.f;
+  tfpp_grad_chunk next = table[blockIdx.x];
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const tfpp_grad_chunk t = table[c];
+    const tfpp_grad_chunk t = next;
+    if (c + (int)gridDim.x < chunks) next = table[c + gridDim.x];  // (one table entry ahead of its data)
     if (t.flags & GC_SRC_BF16) chunk_norm<P, bf16_t>((const bf16_t*)t.src, t.n, t.flags & GC_VEC, s, m);
     else chunk_norm<P, float>((const float*)t.src, t.n, t.flags & GC_VEC, s, m);
   }
@@ -132,8 +134,11 @@ template <int P> __global__ __launch_bounds__(GC_THREADS) void grad_clip_kernel(
   }
   if (!apply) return;
   const float f = (float)((double)scale * (double)nc.y);
+  if ((int)blockIdx.x >= chunks) return;
+  tfpp_grad_chunk next = table[chunks - 1 - (int)blockIdx.x];
   for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-    const tfpp_grad_chunk t = table[c];
+    const tfpp_grad_chunk t = next;
+    if (c >= (int)gridDim.x) next = table[c - (int)gridDim.x];
     if (t.src == t.dst && f == 1.f) continue;
     const bool vec = t.flags & GC_VEC;
     switch (t.flags & (GC_SRC_BF16 | GC_DST_BF16)) {
