@@ -203,7 +203,8 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
 }
 
 // grid (blocks per sample, B): a workgroup's rows belong to one sample, so its partial of the sample's gate gradient is one row
-template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds__(threads_of(TPR)) void block_norm_bwd_kernel(tfpp_block_norm_params p) {
+// BIAS, GSUM: which column sums exist at all (24 and 8 registers a thread: an occupancy step)
+template <typename T, int TPR, int EPT, bool ALIGNED, bool BIAS, bool GSUM> __global__ __launch_bounds__(threads_of(TPR)) void block_norm_bwd_kernel(tfpp_block_norm_params p) {
   constexpr int NT = threads_of(TPR), RPB = NT / TPR;
   typedef Row<T, TPR, EPT, ALIGNED> R;
   extern __shared__ float red[];  // RPB > 1: column sums of the row groups
@@ -213,7 +214,7 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
   const float inv = 1.f / (float)C;
   float pw[EPT], pb[EPT], qw[EPT], sc[EPT];
   load_param<T, TPR, EPT, ALIGNED>(p.post_w, 1.f, t, C, pw);
-  load_param<T, TPR, EPT, ALIGNED>(p.post_b, 0.f, t, C, pb);
+  load_param<T, TPR, EPT, ALIGNED>(BIAS ? p.post_b : nullptr, 0.f, t, C, pb);
   load_param<T, TPR, EPT, ALIGNED>(p.pre_w, 1.f, t, C, qw);
   load_param<T, TPR, EPT, ALIGNED>(p.scale, 1.f, t, C, sc);
   float gs[EPT];
@@ -268,7 +269,7 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
         const float xh = (p.alpha * x[e] + sc[e] * g[e] * nn - st.z) * st.w;
         if (live) {
           acc[0][e] += dh[e] * xh;
-          acc[1][e] += dh[e];
+          if constexpr (BIAS) acc[1][e] += dh[e];
         }
         const bool in = R::col(t, e) < C;
         dh[e] *= qw[e];
@@ -292,9 +293,9 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
       const float dg = d * sc[e] * nn * gate_slope(g[e], p.gate_act), dn = d * sc[e] * g[e];
       if (live) {
         acc[4][e] += d * g[e] * nn;
-        acc[5][e] += dg;
+        if constexpr (GSUM) acc[5][e] += dg;
         acc[2][e] += dn * n[e];
-        acc[3][e] += dn;
+        if constexpr (BIAS) acc[3][e] += dn;
       }
       x[e] = dg;
       const bool in = R::col(t, e) < C;
@@ -314,7 +315,7 @@ template <typename T, int TPR, int EPT, bool ALIGNED> __global__ __launch_bounds
   float* out = p.partial + ((long)blockIdx.y * gridDim.x + blockIdx.x) * K_SUMS * C;
 #pragma unroll
   for (int k = 0; k < K_SUMS; ++k) {
-    if (k == K_SUMS - 1 && p.gate_mode != GATE_SAMPLE) break;
+    if ((!GSUM && k == 5) || (!BIAS && (k == 1 || k == 3))) continue;
     if constexpr (RPB > 1) {
       __syncthreads();
 #pragma unroll
@@ -370,9 +371,11 @@ template <typename T> __global__ __launch_bounds__(1024) void block_norm_colsum_
   }
 }
 
+bool has_bias(const tfpp_block_norm_params& p) { return p.post_b || p.dpost_b || p.dpre_b; }
+
 int blocks_per_sample(const tfpp_block_norm_params& p) {
-  // 8 waves a CU fill the chip at this register count; each workgroup has at least 4 rows, since its 6 rows of partials are traffic too
-  const int tpr = p.C <= 512 ? 64 : (p.C <= 1024 ? 128 : (p.C <= 2048 ? 256 : 512)), rpb = tpr == 64 ? 4 : 1, wgs = 256 * 512 / threads_of(tpr);
+  // 8 waves a CU fill the chip at this register count (12 without the sums that few of them need); each workgroup has at least 4 rows, since its 6 rows of partials are traffic too
+  const int tpr = p.C <= 512 ? 64 : (p.C <= 1024 ? 128 : (p.C <= 2048 ? 256 : 512)), rpb = tpr == 64 ? 4 : 1, waves = has_bias(p) || p.gate_mode == GATE_SAMPLE ? 8 : 12, wgs = 256 * 64 * waves / threads_of(tpr);
   long n = (wgs + p.B - 1) / p.B;
   const long most = (p.T + 4L * rpb - 1) / (4L * rpb);
   if (n > most) n = most;
@@ -398,7 +401,12 @@ template <typename T, int TPR, int EPT, bool AL> void launch(const tfpp_block_no
   constexpr int NT = threads_of(TPR), RPB = NT / TPR;
   if (bwd) {
     const size_t lds = RPB > 1 ? (size_t)EPT * NT * 4 : 0;
-    hipLaunchKernelGGL((block_norm_bwd_kernel<T, TPR, EPT, AL>), dim3(bps, p.B), dim3(NT), lds, st, p);
+    const bool bias = !AL || has_bias(p), gsum = !AL || p.gate_mode == GATE_SAMPLE;
+    const dim3 grid(bps, p.B);
+    if (bias && gsum) hipLaunchKernelGGL((block_norm_bwd_kernel<T, TPR, EPT, AL, true, true>), grid, dim3(NT), lds, st, p);
+    else if (bias) hipLaunchKernelGGL((block_norm_bwd_kernel<T, TPR, EPT, AL, true, !AL>), grid, dim3(NT), lds, st, p);
+    else if (gsum) hipLaunchKernelGGL((block_norm_bwd_kernel<T, TPR, EPT, AL, !AL, true>), grid, dim3(NT), lds, st, p);
+    else hipLaunchKernelGGL((block_norm_bwd_kernel<T, TPR, EPT, AL, !AL, !AL>), grid, dim3(NT), lds, st, p);
   } else {
     const long rows = (long)p.B * p.T, groups = (rows + RPB - 1) / RPB, most = 256 * 1024 / NT;  // 16 waves a CU: what fits beside 40 registers of parameters
     hipLaunchKernelGGL((block_norm_fwd_kernel<T, TPR, EPT, AL>), dim3((unsigned)(groups < most ? groups : most)), dim3(NT), 0, st, p);

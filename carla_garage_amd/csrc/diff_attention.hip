@@ -51,6 +51,12 @@ __device__ __forceinline__ void to_frag(const f32x16_t& c, int t, Frag8<float>& 
 __device__ __forceinline__ unsigned long long low_bits(int n) { return n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1ull); }
 constexpr int pow2_at_least(int n) { return n <= 1 ? 1 : 2 * pow2_at_least((n + 1) / 2); }
 
+struct Rows {  // which rows of a tile exist
+  int count;                 // rows 0 .. count - 1 ..
+  bool holes;                // .. but only those whose bit is set
+  unsigned long long bits;
+};
+
 // LDS image of rows with 32 * CB channels (NC 16-byte chunks a row, a power of two)
 template <typename T, int CB> struct Img {
   static constexpr int VEC = ElemTraits<T>::VEC, USED = 32 * CB / VEC, NC = pow2_at_least(USED);
@@ -93,36 +99,37 @@ template <typename T, int CB> struct Img {
       }
     }
   }
-  // fill ROWS rows: row r comes from base + r * ld (n channels), zeros where its bit in `valid` is not set and behind channel n.  VECTOR: buffer loads
-  // into LDS, one 32-bit offset a lane (64 rows stay below 2 GB: checked by the launcher); a chunk that is left out gets an offset behind the
-  // descriptor's range, for which the hardware returns zeros without touching memory.
-  template <int ROWS, bool VECTOR, int NT> __device__ static __forceinline__ void fill(unsigned char* img, const T* __restrict__ base, long ld, int n, unsigned long long valid, int tid) {
+  // fill ROWS rows: row r comes from base + r * ld (n channels), zeros from row `have.count` on, where a row is left out, and behind channel n.  VECTOR:
+  // buffer loads into LDS, one 32-bit offset a lane (64 rows stay below 2 GB: checked by the launcher).  The descriptor ends with the last row that
+  // exists, a chunk that is left out gets an offset behind it, and the hardware returns zeros for both without touching memory.
+  template <int ROWS, bool VECTOR, int NT> __device__ static __forceinline__ void fill(unsigned char* img, const T* __restrict__ base, long ld, int n, Rows have, int tid) {
     constexpr int SLOTS = ROWS * NC;
+    const int count = have.count < 0 ? 0 : (have.count < ROWS ? have.count : ROWS);
     if constexpr (VECTOR) {
       static_assert(NT % NC == 0 && SLOTS % 64 == 0, "a thread keeps its position in the row");
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
       const int ldb = (int)ld * (int)sizeof(T), r0 = tid / NC, rowb = r0 * ldb;
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, count > 0 ? (count - 1) * ldb + n * (int)sizeof(T) : 0, 0x00020000);
       auto put = [&](int u, bool ok) {
         const int c = (tid % NC) ^ swizzle(r0 + u * (NT / NC));
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t*)(img + (u * NT + wave * 64) * 16), 16, ok && c * VEC < n ? rowb + c * 16 : (int)0x80000000,
-                                                 u * (NT / NC) * ldb, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t*)(img + (u * NT + wave * 64) * 16), 16,
+                                                 (ok && c * VEC < n ? rowb + c * 16 : (int)0x80000000) + u * (NT / NC) * ldb, 0, 0, 0);
       };
-      if ((valid & low_bits(ROWS)) == low_bits(ROWS)) {
+      if (!have.holes) {
 #pragma unroll
         for (int u = 0; u * NT < SLOTS; ++u)
           if (u * NT + wave * 64 < SLOTS) put(u, true);
       } else {
 #pragma unroll
         for (int u = 0; u * NT < SLOTS; ++u)
-          if (u * NT + wave * 64 < SLOTS) put(u, ((valid >> (u * (NT / NC))) >> r0) & 1ull);
+          if (u * NT + wave * 64 < SLOTS) put(u, ((have.bits >> (u * (NT / NC))) >> r0) & 1ull);
       }
     } else {
 #pragma unroll 1
       for (int i = tid; i < ROWS * 32 * CB; i += NT) {
         const int r = i / (32 * CB), c = i % (32 * CB);
         T v = ElemTraits<T>::from_f(0.f);
-        if (c < n && ((valid >> r) & 1ull)) v = base[(long)r * ld + c];
+        if (c < n && r < count && (!have.holes || ((have.bits >> r) & 1ull))) v = base[(long)r * ld + c];
         *reinterpret_cast<T*>(img + off(r, c / VEC) + (c % VEC) * sizeof(T)) = v;
       }
     }
@@ -249,10 +256,9 @@ __device__ __forceinline__ Seq sequence(const tfpp_diff_attn_params& p, int b) {
 }
 // bit i: key j0 + i exists and is not left out
 __device__ __forceinline__ unsigned long long key_bits(const tfpp_diff_attn_params& p, int b, int j0, int len, int lane) {
+  if (!p.key_mask) return low_bits(len - j0);
   const int j = j0 + lane;
-  bool ok = j < len;
-  if (p.key_mask && ok) ok = p.key_mask[(long)b * p.ld_mask + j] != 0;
-  return __ballot(ok);
+  return __ballot(j < len && p.key_mask[(long)b * p.ld_mask + (j < len ? j : 0)] != 0);
 }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
@@ -264,7 +270,7 @@ template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32
 // O_i^T += V^T P_i^T: both maps share every V operand.  O_1 and O_2 are kept apart to the end because their sums are not known before; one pass,
 // 4 d + 4 dv flop a pair.  Wide heads (split): O_1 and O_2 of 32 queries do not fit one wave's registers, so two waves share the queries, one map
 // each, and meet in LDS at the end.
-template <typename T, int NB> constexpr bool fwd_split() { return NB >= (sizeof(T) == 2 ? 8 : 5); }
+template <typename T, int NB> constexpr bool fwd_split() { return NB >= 5; }
 
 enum { Q_HELD, Q_GLOBAL, Q_LDS };  // where a wave's queries are: registers, or read again for every tile
 template <typename T, int NB, bool VECTOR, int Q, int MAPS> struct Fwd {
@@ -414,9 +420,10 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_thr
 
   auto fill = [&](unsigned char* buf, int step, unsigned long long bits) {
     const long j0 = (long)step * KT;
+    const Rows have = {sq.len - step * KT, p.key_mask != nullptr, bits};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, bits, tid);
-    ImgV::template fill<KT, VECTOR, NT>(buf + 2 * K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, bits, tid);
+    for (int i = 0; i < 2; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, have, tid);
+    ImgV::template fill<KT, VECTOR, NT>(buf + 2 * K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, have, tid);
   };
   unsigned long long bits = 0;
   if (steps > 0) {
@@ -522,7 +529,7 @@ template <typename T, int NB> struct Few {
   static constexpr int ROW_FLOATS = 2 * (NB * 32 + 2);     // of one row in `partial`: both maps' sums, maxima, l
 };
 
-template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, NB>::THREADS), 1) void diff_attn_few_kernel(tfpp_diff_attn_params p) {
+template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, NB>::THREADS), (sizeof(T) == 2 || NB <= 2 ? 2 : 1)) void diff_attn_few_kernel(tfpp_diff_attn_params p) {
   typedef Few<T, NB> W;
   typedef Fwd<T, NB, VECTOR, Q_LDS, W::MAPS> F;
   typedef typename F::ImgK ImgK;
@@ -572,13 +579,14 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
 
   auto fill = [&](unsigned char* buf, int block, unsigned bits) {
     const long j0 = (long)block * 32;
+    const Rows have = {sq.len - block * 32, p.key_mask != nullptr, bits};
 #pragma unroll
-    for (int i = 0; i < MAPS; ++i) ImgK::template fill<32, VECTOR, 64>(buf + i * W::K_BYTES, kb + j0 * p.k_s[1] + (f.map0 + i) * p.k_s[3], p.k_s[1], p.d, bits, lane);
-    ImgV::template fill<32, VECTOR, 64>(buf + MAPS * W::K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, bits, lane);
+    for (int i = 0; i < MAPS; ++i) ImgK::template fill<32, VECTOR, 64>(buf + i * W::K_BYTES, kb + j0 * p.k_s[1] + (f.map0 + i) * p.k_s[3], p.k_s[1], p.d, have, lane);
+    ImgV::template fill<32, VECTOR, 64>(buf + MAPS * W::K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, have, lane);
   };
   auto use = [&](const unsigned char* buf, int block, unsigned seen) {
     const unsigned mine = seen & (unsigned)low_bits(lim - block * 32);
-    if (__any(mine != 0)) f.tile(buf, qimg + f.map0 * W::K_BYTES, 0, W::K_BYTES, MAPS * W::K_BYTES, __any(mine != ~0u), mine >> (4 * half), c, p.d, half);
+    f.tile(buf, qimg + f.map0 * W::K_BYTES, 0, W::K_BYTES, MAPS * W::K_BYTES, __any(mine != ~0u), mine >> (4 * half), c, p.d, half);
   };
   const int kw = MAPS == 1 ? wave >> 1 : wave;
   unsigned char* images = smem + wave * W::STAGES * W::IMAGES;
@@ -741,58 +749,56 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
     }
 }
 
-// the splits' sums of a row -> its result: one wave a row, channels lane, lane + 64, ..
+// the splits' sums of a row -> its result: one wave a row, channels 4 lane ..; lane s holds split s's maxima and sums (splits <= 64)
 template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(tfpp_diff_attn_params p, int width) {
-  const int lane = threadIdx.x & 63, group = p.H / p.Hkv, rows = group * p.Tq, dvs = (p.dv + 7) & ~7;
-  const long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6), all = (long)p.B * p.Hkv * rows, pitch = 2 * (width + 2);
+  const int lane = threadIdx.x & 63, group = p.H / p.Hkv, rows = group * p.Tq, dvs = (p.dv + 7) & ~7, c = lane * 4;
+  const long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6), all = (long)p.B * p.Hkv * rows, pitch = 2 * width + 4;
   if (n >= all) return;
   const int r = (int)(n % rows), hk = (int)(n / rows % p.Hkv), b = (int)(n / rows / p.Hkv), h = hk * group + r / p.Tq, qi = r % p.Tq;
   const float* src = p.partial + n * pitch;
   const long row = ((long)b * p.H + h) * p.Tq + qi;
-  float M[2] = {NO_MAX, NO_MAX}, L[2] = {0.f, 0.f}, o[2][4];
-  for (int s = 0; s < p.splits; ++s)
-#pragma unroll
-    for (int map = 0; map < 2; ++map) M[map] = fmaxf(M[map], src[s * all * pitch + 2 * width + 2 * map]);
-#pragma unroll
-  for (int map = 0; map < 2; ++map)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[map][e] = 0.f;
+  float4 ml = make_float4(NO_MAX, 0.f, NO_MAX, 0.f);  // m_1, l_1, m_2, l_2
+  if (lane < p.splits) ml = *reinterpret_cast<const float4*>(src + lane * all * pitch + 2 * width);
+  const float M[2] = {wave_max(ml.x), wave_max(ml.z)};
+  const float f[2] = {exp2f(ml.x - M[0]), exp2f(ml.z - M[1])};
+  const float L[2] = {wave_sum(f[0] * ml.y), wave_sum(f[1] * ml.w)};
+  float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  __shared__ float fs[4][2][64];
+  float(*mine)[64] = fs[threadIdx.x >> 6];
+  mine[0][lane] = f[0];
+  mine[1][lane] = f[1];
+  __builtin_amdgcn_wave_barrier();
+  const float* q0 = src + (c < width ? c : 0);
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
-    const float* q = src + s * all * pitch;
+    const float* q = q0 + s * all * pitch;
 #pragma unroll
     for (int map = 0; map < 2; ++map) {
-      const float f = exp2f(q[2 * width + 2 * map] - M[map]);
-      L[map] += f * q[2 * width + 2 * map + 1];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < p.dv) o[map][e] += f * q[map * width + lane + 64 * e];
+      const float w = mine[map][s];
+      const float4 v = *reinterpret_cast<const float4*>(q + map * width);
+      o[map].x += w * v.x; o[map].y += w * v.y; o[map].z += w * v.z; o[map].w += w * v.w;
     }
   }
   const float lam = p.lam[p.n_lam > 1 ? h : 0];
+  float d[4];
 #pragma unroll
   for (int map = 0; map < 2; ++map) {
     const float inv = inverse_sum(L[map]);
     if (p.lse && lane == 0) p.lse[(long)map * p.B * p.H * p.Tq + row] = log_sum(M[map], L[map]);
+    const float f = c < width ? inv : 0.f;  // (the lanes behind the last channel have read channel 0)
+    const float v[4] = {o[map].x * f, o[map].y * f, o[map].z * f, o[map].w * f};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      o[map][e] *= inv;
-      if (p.o1 && lane + 64 * e < dvs) ((T*)(map ? p.o2 : p.o1))[row * dvs + lane + 64 * e] = ElemTraits<T>::from_f(o[map][e]);
+      if (p.o1 && c + e < dvs) ((T*)(map ? p.o2 : p.o1))[row * dvs + c + e] = ElemTraits<T>::from_f(v[e]);
+      d[e] = map ? d[e] - lam * v[e] : v[e];
     }
   }
-  float ss = 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    o[0][e] -= lam * o[1][e];
-    ss += o[0][e] * o[0][e];
-  }
   float g = p.out_scale;
-  if (p.norm) g *= 1.f / sqrtf(wave_sum(ss) / (float)p.dv + p.eps);
+  if (p.norm) g *= 1.f / sqrtf(wave_sum(d[0] * d[0] + d[1] * d[1] + d[2] * d[2] + d[3] * d[3]) / (float)p.dv + p.eps);
   T* out = (T*)p.out + (long)b * p.o_s[0] + (long)qi * p.o_s[1] + (long)h * p.o_s[2];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int ch = lane + 64 * e;
-    if (ch < p.dv) out[ch] = ElemTraits<T>::from_f(o[0][e] * (p.norm_w ? g * Weights{p.norm_w, p.norm_w_bf16}[ch] : g));
-  }
+  for (int e = 0; e < 4; ++e)
+    if (c + e < p.dv) out[c + e] = ElemTraits<T>::from_f(d[e] * (p.norm_w ? g * Weights{p.norm_w, p.norm_w_bf16}[c + e] : g));
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -938,7 +944,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
   const long row = ((long)b * p.H + h) * p.Tq + qc, rows = (long)p.B * p.H * p.Tq;
   const T* kb = (const T*)p.k + (long)b * p.k_s[0] + (long)hk * p.k_s[2];
   const T* vb = (const T*)p.v + (long)b * p.v_s[0] + (long)hk * p.v_s[2];
-  constexpr bool HOLD = NB < 5 || (sizeof(T) == 2 && VECTOR);  // else Q and dO do not fit the registers and are read again for every tile
+  constexpr bool HOLD = VECTOR ? sizeof(T) == 2 || NB < 5 : NB < 4;  // else Q and dO do not fit the registers and are read again for every tile
   const T* qrow = (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2];
   Frag8<T> q[2][HOLD ? NB : 1], dof[HOLD ? 2 * NB : 1];
   if constexpr (HOLD)
@@ -965,9 +971,10 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
   const int k_rows = ImgK::rows_at(lane), v_rows = ImgV::rows_at(lane), k_cols = ImgK::cols_at(lane);
   auto fill = [&](unsigned char* buf, int step, unsigned long long bits) {
     const long j0 = (long)step * KT;
+    const Rows have = {sq.len - step * KT, p.key_mask != nullptr, bits};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, bits, tid);
-    ImgV::template fill<KT, VECTOR, NT>(buf + 2 * K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, bits, tid);
+    for (int i = 0; i < 2; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, have, tid);
+    ImgV::template fill<KT, VECTOR, NT>(buf + 2 * K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, have, tid);
   };
   unsigned long long bits = 0;
   if (steps > 0) {
@@ -986,7 +993,8 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
             },
             [&](const unsigned char* now) {
     const int j0 = s * KT;
-    if ((p.causal && sq.start + w0 + 32 - j0 <= 0) || cur == 0) return;
+    // (no early way out for a tile that the wave's queries do not see: with accumulators in AGPRs a branch round their products costs a copy of all of
+    // them at every step; such a tile is masked to zeros)
     const bool masked = cur != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
     const unsigned vis = (unsigned)(p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur) >> (4 * half);
     const int vr = v_rows + 2 * K_BYTES;
@@ -1049,10 +1057,13 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
 //    Wide heads: the accumulators of all three do not fit one wave's registers, so dK_1, dK_2 (PART_DK, the map in the grid's y) and dV (PART_DV) are
 //    separate workgroups; S and dP are computed again (3 / 2 of the flop).
 enum { PART_ALL, PART_DK, PART_DV };
-template <typename T, int NB> constexpr bool dkv_split() { return NB >= (sizeof(T) == 2 ? 5 : 4); }
-template <typename T, int NB> constexpr int dkv_lds() { return at_least(2 * (32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + 1024), 4 * STRIP_BYTES); }
+template <typename T, int NB, bool VECTOR> constexpr bool dkv_split() { return NB >= (sizeof(T) == 2 && VECTOR ? 5 : 4); }
+// d = 33 .. 64, bf16: the 128 keys' V stays in LDS instead of 32 registers, which lets two waves share a SIMD (256 registers each, no AGPR copies)
+template <typename T, int NB> constexpr bool dkv_v_in_lds() { return sizeof(T) == 2 && NB == 4; }
+template <typename T, int NB> constexpr int dkv_images() { return 2 * (32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + 1024); }
+template <typename T, int NB> constexpr int dkv_lds() { return at_least(dkv_images<T, NB>() + (dkv_v_in_lds<T, NB>() ? QB * Img<T, NB>::ROW_BYTES : 0), 4 * STRIP_BYTES); }
 
-template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds__(256, (PART == PART_ALL ? NB <= (sizeof(T) == 2 ? 2 : 1) : NB <= (sizeof(T) == 2 ? 5 : 4)) ? 2 : 1) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
+template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds__(256, (PART == PART_ALL ? NB <= (sizeof(T) == 2 ? 4 : 1) : NB <= (sizeof(T) == 2 ? 5 : 4)) ? 2 : 1) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
   constexpr int QT = 32, NT = 256, MAPS = PART == PART_DK ? 1 : 2, CD = (NB + 1) / 2;
   typedef Img<T, CD> ImgQ;
   typedef Img<T, NB> ImgO;
@@ -1068,19 +1079,20 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
   bool seen = kj < sq.len;
   if (seen && p.key_mask) seen = p.key_mask[(long)b * p.ld_mask + kj] != 0;
   const int kc = kj < p.Tk ? kj : p.Tk - 1;
-  constexpr bool HOLD = sizeof(T) == 2 || NB < 4, WANT_DK = PART != PART_DV, WANT_DV = PART != PART_DK;
+  constexpr bool V_LDS = dkv_v_in_lds<T, NB>() && PART == PART_ALL, HOLD = sizeof(T) == 2 || NB < 4, WANT_DK = PART != PART_DV, WANT_DV = PART != PART_DK;
+  constexpr bool FENCE = V_LDS;  // (operands loaded far ahead of their products would not fit the registers)
   const int map0 = PART == PART_DK ? (int)blockIdx.y : 0;  // wide fp32 heads do not fit the registers: K and V are read again for every tile
   const T* krow = (const T*)p.k + (long)b * p.k_s[0] + (long)kc * p.k_s[1] + (long)hk * p.k_s[2];
   const T* vrow = (const T*)p.v + (long)b * p.v_s[0] + (long)kc * p.v_s[1] + (long)hk * p.v_s[2];
-  Frag8<T> k[MAPS][HOLD ? NB : 1], v[HOLD && WANT_DK ? 2 * NB : 1];
+  Frag8<T> k[MAPS][HOLD ? NB : 1], v[HOLD && WANT_DK && !V_LDS ? 2 * NB : 1];
   if constexpr (HOLD) {
 #pragma unroll
     for (int i = 0; i < MAPS; ++i)
 #pragma unroll
-      for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, seen, k[i][ks]);
-    if constexpr (WANT_DK)
+      for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, true, k[i][ks]);
+    if constexpr (WANT_DK && !V_LDS)
 #pragma unroll
-      for (int ks = 0; ks < 2 * NB; ++ks) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, seen, v[ks]);
+      for (int ks = 0; ks < 2 * NB; ++ks) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, true, v[ks]);
   }
   f32x16_t dk[WANT_DK ? MAPS : 1][CD], dv[WANT_DV ? NB : 1];
 #pragma unroll
@@ -1101,94 +1113,130 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
   const int per = any ? (p.Tq - q_lo + QT - 1) / QT : 0, steps = per * group;
 
   const int q_rows = ImgQ::rows_at(lane), o_rows = ImgO::rows_at(lane), q_cols = ImgQ::cols_at(lane), o_cols = ImgO::cols_at(lane);
-  auto fill = [&](unsigned char* buf, int step) {
-    const int h = hk * group + step / per, q0 = q_lo + step % per * QT;
-    const unsigned long long bits = low_bits(p.Tq - q0);
+  auto fill = [&](unsigned char* buf, int h, int q0) {
+    const Rows have = {p.Tq - q0, false, 0ull};
     const T* qb = (const T*)p.q + (long)b * p.q_s[0] + (long)q0 * p.q_s[1] + (long)h * p.q_s[2];
     const long row = ((long)b * p.H + h) * p.Tq + q0;
 #pragma unroll
-    for (int i = map0; i < map0 + MAPS; ++i) ImgQ::template fill<QT, VECTOR, NT>(buf + i * Q_BYTES, qb + i * p.q_s[3], p.q_s[1], p.d, bits, tid);
-    ImgO::template fill<QT, true, NT>(buf + 2 * Q_BYTES, (const T*)p.d_o + row * dvs, dvs, dvs, bits, tid);
+    for (int i = map0; i < map0 + MAPS; ++i) ImgQ::template fill<QT, VECTOR, NT>(buf + i * Q_BYTES, qb + i * p.q_s[3], p.q_s[1], p.d, have, tid);
+    ImgO::template fill<QT, true, NT>(buf + 2 * Q_BYTES, (const T*)p.d_o + row * dvs, dvs, dvs, have, tid);
     // lse_1, lse_2, delta_1, delta_2 of the tile, one array a wave.  Queries behind the last: all zero like their Q and dO, so P = 1 but dV, dS get 0
     const float* src = (wave < 2 ? p.lse : p.delta) + (wave & 1) * rows + row;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)src, 0, 0x7fffffff, 0x00020000), (lds_void_t*)(buf + 2 * Q_BYTES + O_BYTES + wave * 256), 4,
                                              lane < QT && q0 + lane < p.Tq ? lane * 4 : (int)0x80000000, 0, 0, 0);
   };
-  if (steps > 0) fill(smem, 0);
+  int v_at = 0;
+  if constexpr (V_LDS) {  // 32 keys a wave, filled as every other image; complete at the first step's wait
+    const int place = dkv_images<T, NB>() + wave * 32 * ImgO::ROW_BYTES;
+    ImgO::template fill<32, VECTOR, 64>(smem + place, (const T*)p.v + (long)b * p.v_s[0] + (long)w0 * p.v_s[1] + (long)hk * p.v_s[2], p.v_s[1], p.dv, Rows{sq.len - w0, p.key_mask != nullptr, __ballot(seen)}, lane);
+    v_at = place + ImgO::rows_at(lane);
+  }
+  // the query head and first query of a step, without divisions in the loop
+  int h = hk * group, q0 = q_lo, h_next = h, q_next = q_lo;
+  auto advance = [&] {
+    q_next += QT;
+    if (q_next >= p.Tq) {
+      q_next = q_lo;
+      ++h_next;
+    }
+  };
+  float lam = 0.f;
+  if (steps > 0) fill(smem, h, q0);
   for (int s = 0; s < steps; ++s) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
+    if (q0 == q_lo) lam = p.lam[p.n_lam > 1 ? h : 0];
     overlap(smem + (~s & 1) * BUF, smem + (s & 1) * BUF,
             [&](unsigned char* next) {
-              if (s + 1 < steps) fill(next, s + 1);
+              advance();
+              if (s + 1 < steps) fill(next, h_next, q_next);
             },
             [&](const unsigned char* now) {
-    const int h = hk * group + s / per, q0 = q_lo + s % per * QT;
-    if (p.causal && sq.start + q0 + QT - 1 < w0) return;  // no query of the tile sees a key of this wave
     const bool diag = p.causal && sq.start + q0 < w0 + 31;
-    const float lam = p.lam[p.n_lam > 1 ? h : 0];
     const int orow = o_rows + 2 * Q_BYTES, ocol = o_cols + 2 * Q_BYTES;
     const float* st = reinterpret_cast<const float*>(now + 2 * Q_BYTES + O_BYTES);
-    f32x16_t sc[MAPS], dp;
+    // S, P, then dV += dO^T (P_1 - lambda P_2) before dP: the fewest values live at a time
+    f32x16_t sc[MAPS];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      dp[r] = 0.f;
+    for (int i = 0; i < MAPS; ++i)
 #pragma unroll
-      for (int i = 0; i < MAPS; ++i) sc[i][r] = 0.f;
-    }
+      for (int r = 0; r < 16; ++r) sc[i][r] = 0.f;
 #pragma unroll
     for (int i = 0; i < MAPS; ++i)
 #pragma unroll
       for (int ks = 0; ks < NB; ++ks) {
         Frag8<T> a;
         ImgQ::rows(now + (map0 + i) * Q_BYTES, q_rows, ks, a);
-        if constexpr (!HOLD) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, seen, k[i][0]);
+        if constexpr (!HOLD) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, true, k[i][0]);
         mma(a, k[i][HOLD ? ks : 0], sc[i]);
+        if (FENCE && ks % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
-    if constexpr (WANT_DK)
-#pragma unroll
-      for (int ks = 0; ks < 2 * NB; ++ks) {
-        Frag8<T> a;
-        ImgO::rows(now, orow, ks, a);
-        if constexpr (!HOLD) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, seen, v[0]);
-        mma(a, v[HOLD ? ks : 0], dp);
-      }
-    f32x16_t pd;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int t0 = 8 * g + 4 * half;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pd[4 * g + e] = 0.f;
-#pragma unroll
       for (int i = 0; i < MAPS; ++i) {
-        const int map = map0 + i;
-        const float4 l4 = *reinterpret_cast<const float4*>(st + map * 64 + t0), d4 = *reinterpret_cast<const float4*>(st + (2 + map) * 64 + t0);
-        const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w}, sign = map ? -lam : 1.f;
+        const float4 l4 = *reinterpret_cast<const float4*>(st + (map0 + i) * 64 + t0);
+        const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e;
-          float pr = __builtin_amdgcn_exp2f(fmaf(sc[i][r], c, -ls[e]));
-          pr = seen && (!diag || kj <= sq.start + q0 + t0 + e) ? sign * pr : 0.f;
-          pd[r] += pr;
-          sc[i][r] = pr * (dp[r] - de[e]);
+          sc[i][4 * g + e] = __builtin_amdgcn_exp2f(fmaf(sc[i][4 * g + e], c, -ls[e]));
         }
       }
     }
+    if (diag) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      Frag8<T> f;
-      if constexpr (WANT_DV) {
+      for (int r = 0; r < 16; ++r) {
+        const bool keep = kj <= sq.start + q0 + 8 * (r >> 2) + 4 * half + (r & 3);
+#pragma unroll
+        for (int i = 0; i < MAPS; ++i) sc[i][r] = keep ? sc[i][r] : 0.f;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (WANT_DV) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x16_t pd;
+#pragma unroll
+        for (int r = 8 * t; r < 8 * t + 8; ++r) pd[r] = fmaf(-lam, sc[MAPS - 1][r], sc[0][r]);
+        Frag8<T> f;
         to_frag(pd, t, f);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           Frag8<T> a;
           ImgO::cols(now + 16 * t * ImgO::ROW_BYTES, ocol, n, a);
           mma(a, f, dv[n]);
+          if (FENCE && n % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if constexpr (WANT_DK)
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (WANT_DK) {
+      f32x16_t dp;
 #pragma unroll
-        for (int i = 0; i < MAPS; ++i) {
+      for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 2 * NB; ++ks) {
+        Frag8<T> a;
+        ImgO::rows(now, orow, ks, a);
+        if constexpr (V_LDS) ImgO::rows(smem, v_at, ks, v[0]);
+        else if constexpr (!HOLD) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, true, v[0]);
+        mma(a, v[HOLD && !V_LDS ? ks : 0], dp);
+        if (FENCE && ks % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i) {
+        const float sign = map0 + i ? -lam : 1.f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 d4 = *reinterpret_cast<const float4*>(st + (2 + map0 + i) * 64 + 8 * g + 4 * half);
+          const float de[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][4 * g + e] *= map0 + i ? sign * (dp[4 * g + e] - de[e]) : dp[4 * g + e] - de[e];
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Frag8<T> f;
           to_frag(sc[i], t, f);
 #pragma unroll
           for (int n = 0; n < CD; ++n) {
@@ -1196,13 +1244,31 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
             ImgQ::cols(now + (map0 + i) * Q_BYTES + 16 * t * ImgQ::ROW_BYTES, q_cols, n, a);
             mma(a, f, dk[i][n]);
           }
+          if (FENCE) __builtin_amdgcn_sched_barrier(0);
         }
+      }
     }
             });
+    h = h_next;
+    q0 = q_next;
   }
   __syncthreads();  // every wave is past its last image
   float* strip = reinterpret_cast<float*>(smem + wave * STRIP_BYTES);
-  if constexpr (WANT_DV) {  // (keys that nobody sees get zeros)
+  // A key that is left out has a column of its own in every product: whatever its K and V made of it is dropped here
+  if (!seen) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (WANT_DV)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) dv[n][r] = 0.f;
+      if constexpr (WANT_DK)
+#pragma unroll
+        for (int n = 0; n < CD; ++n)
+#pragma unroll
+          for (int i = 0; i < MAPS; ++i) dk[i][n][r] = 0.f;
+    }
+  }
+  if constexpr (WANT_DV) {
     T* out = (T*)p.dv_out + (long)b * p.dv_s[0] + (long)w0 * p.dv_s[1] + (long)hk * p.dv_s[2];
     store_rows<T>(strip, lane, dv, 1.f, p.dv, p.dv_vec, Weights{nullptr, 0}, [&](int r) { return w0 + r < p.Tk ? out + (long)r * p.dv_s[1] : nullptr; });
   }
@@ -1303,7 +1369,7 @@ template <typename T, int NB, bool VECTOR> int launch(const tfpp_diff_attn_param
   const dim3 grid((unsigned)n);
   if (step == STEP_FWD) return start(diff_attn_fwd_kernel<T, NB, VECTOR>, grid, fwd_threads<T, NB>(), fwd_lds<T, NB>(), &done[0], p, st);
   if (step == STEP_DQ) return start(diff_attn_bwd_dq_kernel<T, NB, VECTOR>, grid, 256, dq_lds<T, NB>(), &done[1], p, st);
-  if constexpr (dkv_split<T, NB>()) {
+  if constexpr (dkv_split<T, NB, VECTOR>()) {
     const int rc = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DK>, dim3((unsigned)n, 2), 256, dkv_lds<T, NB>(), &done[2], p, st);
     return rc ? rc : start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DV>, grid, 256, dkv_lds<T, NB>(), &done[3], p, st);
   } else {
@@ -1333,6 +1399,7 @@ int few_splits(const tfpp_diff_attn_params& p) {
   const long rows = (long)(p.H / p.Hkv) * p.Tq, base = (long)p.B * p.Hkv * ((rows + 31) / 32);
   long n = (512 + base - 1) / base, most = (p.Tk + 511) / 512;  // two workgroups a CU; at least 512 keys (4 blocks a wave) in a split
   if (n > most) n = most;
+  if (n > 64) n = 64;  // (the join holds one split a lane)
   return n < 1 ? 1 : (int)n;
 }
 int row_lanes(const tfpp_diff_attn_params& p) {

@@ -8,13 +8,15 @@
 //   2. grad_clip_kernel: EVERY workgroup adds the partials in index order (<= 16 KB out of L2, bit-identical in all of them and from run
 //      to run; no ticket, no atomics, no state between calls), then writes its chunks -- walked from the LAST chunk to the first, since
 //      the end of the gradient is what launch 1 left in the 256 MB memory-side cache.  In place with s coef == 1 nothing is touched.
+#include <type_traits>
+
 #include "common.h"
 #include "../../include/tfpp.h"
 
 namespace {
 constexpr int GC_THREADS = 256;
 constexpr int GC_GRID = 2048;    // 8 workgroups per CU
-constexpr int GC_CHUNK = 4096;   // elements: 16 KB of fp32; small, so that 2048 workgroups end together (16384: 40 M bf16 values took 88 us, 4096: see below)
+constexpr int GC_CHUNK = 16384;  // most elements of a chunk; the table's maker takes 16 or 32 KB of the source, so that 2048 workgroups end together
 enum { GC_SRC_BF16 = 1, GC_DST_BF16 = 2, GC_VEC = 4 };
 
 __device__ __forceinline__ float max_nan(float m, float v) { return (v > m || v != v) ? v : m; }  // NaN wins and stays
@@ -26,11 +28,12 @@ template <int P> __device__ __forceinline__ void accumulate(double& s, float& m,
 }
 
 template <int P, typename T> __device__ __forceinline__ void chunk_norm(const T* __restrict__ p, int n, bool vec, double& s, float& m) {
-  constexpr int V = ElemTraits<T>::VEC, U = 4;
+  constexpr int V = ElemTraits<T>::VEC, U = 4;  // (four 16-byte loads in flight)
   int done = 0;
   if (vec) {
     const int nv = n / V;
     int i = threadIdx.x;
+#pragma unroll 2
     for (; i + (U - 1) * GC_THREADS < nv; i += U * GC_THREADS) {
       uint4 r[U];
 #pragma unroll
@@ -111,15 +114,28 @@ template <typename S, typename D> __device__ __forceinline__ void chunk_scale(co
   int done = 0;
   if (vec) {
     const int nv = n / V;
-    for (int i = threadIdx.x; i < nv; i += GC_THREADS) {
-      float x[V];
+    int i = threadIdx.x;
+    auto step = [&](auto count) {
+      constexpr int U = decltype(count)::value;
+      uint4 r[U][V / ElemTraits<S>::VEC];
 #pragma unroll
-      for (int e = 0; e < V; e += ElemTraits<S>::VEC) load_vec<S>(src + (size_t)i * V + e, x + e);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[e] *= f;
+        for (int e = 0; e < V; e += ElemTraits<S>::VEC) r[u][e / ElemTraits<S>::VEC] = *reinterpret_cast<const uint4*>(src + (size_t)(i + u * GC_THREADS) * V + e);
 #pragma unroll
-      for (int e = 0; e < V; e += ElemTraits<D>::VEC) store_vec<D>(dst + (size_t)i * V + e, x + e);
-    }
+      for (int u = 0; u < U; ++u) {
+        float x[V];
+#pragma unroll
+        for (int e = 0; e < V; e += ElemTraits<S>::VEC) unpack16<S>(r[u][e / ElemTraits<S>::VEC], x + e);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] *= f;
+#pragma unroll
+        for (int e = 0; e < V; e += ElemTraits<D>::VEC) store_vec<D>(dst + (size_t)(i + u * GC_THREADS) * V + e, x + e);
+      }
+      i += U * GC_THREADS;
+    };
+    while (i + 3 * GC_THREADS < nv) step(std::integral_constant<int, 4>());
+    while (i < nv) step(std::integral_constant<int, 1>());
     done = nv * V;
   }
   for (int i = done + threadIdx.x; i < n; i += GC_THREADS) dst[i] = ElemTraits<D>::from_f(ElemTraits<S>::to_f(src[i]) * f);

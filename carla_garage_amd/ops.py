@@ -1300,12 +1300,14 @@ class GradClip:
     end, end_out = np.maximum.accumulate(np.concatenate([[0], hi]))[:-1], np.maximum.accumulate(np.concatenate([[0], np.where(written, hi, 0)]))[:-1]
     if (lo < np.where(written, end, end_out)).any():
       raise ValueError('the same memory is given twice: a clipped gradient may not overlap another one')
-    chunk = lib.raw('tfpp_grad_clip_chunk')()
+    # bytes of a chunk: 64 KB, or 16 KB where the launch's 2048 workgroups would have too few to end together
+    size = 65536 if int((n * ss).sum()) >= 1 << 28 else 16384
+    chunk = np.minimum(size // ss, lib.raw('tfpp_grad_clip_chunk')())
     per = (n + chunk - 1) // chunk
     which = np.repeat(np.arange(n.size), per)
-    off = (np.arange(which.size) - np.repeat(np.cumsum(per) - per, per)) * chunk
+    off = (np.arange(which.size) - np.repeat(np.cumsum(per) - per, per)) * chunk[which]
     table = np.empty(which.size, dtype=[('src', '<i8'), ('dst', '<i8'), ('n', '<i4'), ('flags', '<i4')])
-    table['src'], table['dst'], table['n'] = src[which] + off * ss[which], dst[which] + off * ds[which], np.minimum(n[which] - off, chunk)
+    table['src'], table['dst'], table['n'] = src[which] + off * ss[which], dst[which] + off * ds[which], np.minimum(n[which] - off, chunk[which])
     table['flags'] = ((ss == 2) * 1 + (ds == 2) * 2 + ((src | dst) % 16 == 0) * 4)[which]
     self.chunks = int(which.size)
     if self.chunks >= 1 << 31:
@@ -1487,15 +1489,16 @@ def block_norm_bwd(dy, dh, ctx, into=None):
         zero_(out['gate'])
     else:
       p = _block_norm_params(ctx)
-      n_part = ctypes.c_int64()
-      lib.tfpp_block_norm_bwd_partial_floats(ctypes.byref(p), ctypes.addressof(n_part))
-      partial = torch.empty(n_part.value, device=dev, dtype=torch.float32)
       p.dy, p.dh, p.ld_dy, p.ld_dh = ptr(dy), ptr(dh), lds[0], lds[1]
-      p.dx, p.da, p.dgate, p.partial = out['x'].data_ptr(), out['a'].data_ptr(), ptr(out['gate']), partial.data_ptr()
+      p.dx, p.da, p.dgate = out['x'].data_ptr(), out['a'].data_ptr(), ptr(out['gate'])
       for n in names:
         field, bit = _BLOCK_NORM_SUMS[n]
         setattr(p, field, out[n].data_ptr())
         p.accumulate |= bit if n in into else 0
+      n_part = ctypes.c_int64()
+      lib.tfpp_block_norm_bwd_partial_floats(ctypes.byref(p), ctypes.addressof(n_part))
+      partial = torch.empty(n_part.value, device=dev, dtype=torch.float32)
+      p.partial = partial.data_ptr()
       if lib.profiler is not None:
         lib.profiler.tag('block_norm_bwd', 0.0, float(rows * C * x.element_size() * (4 + (dy is not None) + (dh is not None) + 2 * (ctx.mode == 2))))
       lib.tfpp_block_norm_bwd(ctypes.byref(p), dt(x), stream())
@@ -1601,8 +1604,8 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
     h // (H // Hkv)); any strides with a contiguous last dimension (slices of a fused projection, [B, H, T, ...] caches seen through permute).
     lam: fp32 [H] or [1].  norm_weight: [dv], fp32 or bf16, or None.  scale > 0, default d ** -0.5.
   Which keys a query sees: kv_len (int32 [B] on the device) leaves out keys >= kv_len[b]; key_mask (bool or uint8 [B, Tk]) those where it is 0; causal
-  those with key > q_start + query, q_start an int, int32 [B] on the device, or None for Tk - Tq.  k and v of keys left out by kv_len or key_mask are
-  not read and may hold anything; the other values have to be finite.  A query that sees no key gives zeros.
+  those with key > q_start + query, q_start an int, int32 [B] on the device, or None for Tk - Tq.  k and v of keys left out by kv_len or key_mask may
+  hold anything; the other values have to be finite.  A query that sees no key gives zeros.
   New tokens against a cache: q [B, 1, ...], k and v the whole cache, kv_len the tokens it holds (the new ones among them); for several new tokens
   causal=True and q_start = kv_len - Tq.
   save=True keeps what diff_attn_bwd needs.  ``out``: written in place of a new tensor, any strides that do not overlap."""

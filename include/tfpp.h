@@ -682,7 +682,8 @@ int tfpp_grad_clip_partials(int chunks);     /* returns the count (not an error 
  * layer: LayerNorm, else RMS.  gate_mode 0 none, 1 one row per sample [B, C], 2 one per token; gate_act TFPP_ACT_NONE / SIGMOID / TANH.
  * stat: 4 floats a row (mean, rstd of post; mean, rstd of pre; 16-byte aligned), written by forward when given, read by backward.  Backward takes the
  * forward's x, a, gate and recomputes the rest; dy or dh may be null (not both; dh needs pre).  Parameter gradients (each nullable) are stored, or
- * added to their destination where a bit of accumulate is set: 1 dpre_w, 2 dpre_b, 4 dpost_w, 8 dpost_b, 16 dscale.  C <= 4096.  partial: tfpp_block_norm_bwd_partial_floats. */
+ * added to their destination where a bit of accumulate is set: 1 dpre_w, 2 dpre_b, 4 dpost_w, 8 dpost_b, 16 dscale.  C <= 4096.  partial: tfpp_block_norm_bwd_partial_floats of
+ * the same params. */
 typedef struct {
   const void *x, *a, *gate;
   const float *post_w, *post_b, *pre_w, *pre_b, *scale;
@@ -704,8 +705,8 @@ int tfpp_block_norm_bwd_partial_floats(const tfpp_block_norm_params* p, int64_t*
  * (norm = 0: out = out_scale * O).  Element (b, t, h, i, c) of q lies at b q_s[0] + t q_s[1] + h q_s[2] + i q_s[3] + c, and so on: strides in
  * elements, the last dimension contiguous.  H is a multiple of Hkv: query head h reads key / value head h / (H / Hkv).  d <= 128, dv <= 256.
  * lam: n_lam = H (or 1) fp32 values.  kv_len (nullable): valid keys of each sequence; key_mask (nullable, [B] rows of pitch ld_mask): 0 leaves a key
- * out; causal: key j is seen by query i when j <= q_start[b] + i (q_start null: q_start_all).  K and V of keys left out by kv_len or key_mask are
- * not read.  A query without keys: out = 0.
+ * out; causal: key j is seen by query i when j <= q_start[b] + i (q_start null: q_start_all).  K and V of keys left out by kv_len or key_mask may
+ * hold anything.  A query without keys: out = 0.
  * Forward for training also writes o1, o2 ([B, H, Tq, dv rounded up to 8], P_i V in `dtype`) and lse ([2, B, H, Tq], log2).  Backward reads them, dout
  * and the inputs, and writes d_o (layout of o1), delta (layout of lse), partial (tfpp_diff_attn_bwd_partial_floats): scratch; dlam [n_lam], dnorm_w
  * (type of norm_w), and the gradients dq_out, dk_out, dv_out with their own strides.  Fixed summation order throughout. */
