@@ -76,8 +76,8 @@ class DiffAttnParams(ctypes.Structure):
   _fields_ = [(n, vp) for n in ('q', 'k', 'v', 'lam', 'norm_w', 'out', 'o1', 'o2', 'lse', 'kv_len', 'q_start', 'key_mask', 'dout', 'd_o', 'delta', 'partial', 'dlam',
                                 'dnorm_w', 'dq_out', 'dk_out', 'dv_out')] + \
       [('ld_mask', i64), ('q_s', i64 * 4), ('k_s', i64 * 4), ('v_s', i64 * 3), ('o_s', i64 * 3), ('do_s', i64 * 3), ('dq_s', i64 * 4), ('dk_s', i64 * 4), ('dv_s', i64 * 3)] + \
-      [(n, i32) for n in ('B', 'H', 'Hkv', 'Tq', 'Tk', 'd', 'dv', 'n_lam', 'norm', 'norm_w_bf16', 'causal', 'q_start_all', 'out_vec', 'do_vec', 'dq_vec', 'dk_vec', 'dv_vec', 'splits')] + \
-      [('scale', f32), ('out_scale', f32), ('eps', f32)]
+      [(n, i32) for n in ('B', 'H', 'Hkv', 'Tq', 'Tk', 'd', 'dv', 'n_lam', 'norm', 'norm_w_bf16', 'causal', 'q_start_all', 'out_vec', 'do_vec', 'dq_vec', 'dk_vec', 'dv_vec', 'splits', 'dkv_splits')] + \
+      [('scale', f32), ('out_scale', f32), ('eps', f32), ('dkv', vp)]
 
 
 _CTYPE = {'int': i32, 'int32_t': i32, 'int64_t': i64, 'uint64_t': ctypes.c_uint64, 'uint32_t': ctypes.c_uint32, 'float': f32, 'double': ctypes.c_double}

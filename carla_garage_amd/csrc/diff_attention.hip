@@ -1058,10 +1058,11 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
 //    separate workgroups; S and dP are computed again (3 / 2 of the flop).
 enum { PART_ALL, PART_DK, PART_DV };
 template <typename T, int NB, bool VECTOR> constexpr bool dkv_split() { return NB >= (sizeof(T) == 2 && VECTOR ? 5 : 4); }
-// d = 33 .. 64, bf16: the 128 keys' V stays in LDS instead of 32 registers, which lets two waves share a SIMD (256 registers each, no AGPR copies)
+// d = 33 .. 64, bf16: the 128 keys' V and the last 16 channels of their K stay in LDS instead of 40 registers, which lets two waves share a SIMD (256
+// registers each, no AGPR copies, no scratch)
 template <typename T, int NB> constexpr bool dkv_v_in_lds() { return sizeof(T) == 2 && NB == 4; }
 template <typename T, int NB> constexpr int dkv_images() { return 2 * (32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + 1024); }
-template <typename T, int NB> constexpr int dkv_lds() { return at_least(dkv_images<T, NB>() + (dkv_v_in_lds<T, NB>() ? QB * Img<T, NB>::ROW_BYTES : 0), 4 * STRIP_BYTES); }
+template <typename T, int NB> constexpr int dkv_lds() { return at_least(dkv_images<T, NB>() + (dkv_v_in_lds<T, NB>() ? QB * Img<T, NB>::ROW_BYTES + 4 * 2 * 64 * 16 : 0), 4 * STRIP_BYTES); }
 
 template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds__(256, (PART == PART_ALL ? NB <= (sizeof(T) == 2 ? 4 : 1) : NB <= (sizeof(T) == 2 ? 5 : 4)) ? 2 : 1) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
   constexpr int QT = 32, NT = 256, MAPS = PART == PART_DK ? 1 : 2, CD = (NB + 1) / 2;
@@ -1073,6 +1074,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
   const int tiles = (p.Tk + QB - 1) / QB, group = p.H / p.Hkv;
   int bh, tile;
   place(p.B * p.Hkv, tiles, p.causal, bh, tile);
+  const int part = PART == PART_DK ? (int)blockIdx.y >> 1 : (int)blockIdx.y;  // of the queries
   const int b = bh / p.Hkv, hk = bh % p.Hkv, dvs = (p.dv + 7) & ~7;
   const Seq sq = sequence(p, b);
   const int w0 = tile * QB + wave * 32, kj = w0 + (lane & 31);
@@ -1081,15 +1083,16 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
   const int kc = kj < p.Tk ? kj : p.Tk - 1;
   constexpr bool V_LDS = dkv_v_in_lds<T, NB>() && PART == PART_ALL, HOLD = sizeof(T) == 2 || NB < 4, WANT_DK = PART != PART_DV, WANT_DV = PART != PART_DK;
   constexpr bool FENCE = V_LDS;  // (operands loaded far ahead of their products would not fit the registers)
-  const int map0 = PART == PART_DK ? (int)blockIdx.y : 0;  // wide fp32 heads do not fit the registers: K and V are read again for every tile
+  const int map0 = PART == PART_DK ? (int)blockIdx.y & 1 : 0;  // wide fp32 heads do not fit the registers: K and V are read again for every tile
   const T* krow = (const T*)p.k + (long)b * p.k_s[0] + (long)kc * p.k_s[1] + (long)hk * p.k_s[2];
   const T* vrow = (const T*)p.v + (long)b * p.v_s[0] + (long)kc * p.v_s[1] + (long)hk * p.v_s[2];
-  Frag8<T> k[MAPS][HOLD ? NB : 1], v[HOLD && WANT_DK && !V_LDS ? 2 * NB : 1];
+  constexpr int K_HELD = V_LDS ? NB - 1 : NB;
+  Frag8<T> k[MAPS][HOLD ? K_HELD : 1], v[HOLD && WANT_DK && !V_LDS ? 2 * NB : 1];
   if constexpr (HOLD) {
 #pragma unroll
     for (int i = 0; i < MAPS; ++i)
 #pragma unroll
-      for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, true, k[i][ks]);
+      for (int ks = 0; ks < K_HELD; ++ks) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, true, k[i][ks]);
     if constexpr (WANT_DK && !V_LDS)
 #pragma unroll
       for (int ks = 0; ks < 2 * NB; ++ks) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, true, v[ks]);
@@ -1110,46 +1113,67 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
   int q_lo = 0;
   if (p.causal && tile * QB > sq.start) q_lo = (tile * QB - sq.start) / QT * QT;
   const bool any = tile * QB < sq.len && q_lo < p.Tq;
-  const int per = any ? (p.Tq - q_lo + QT - 1) / QT : 0, steps = per * group;
+  const int per = any ? (p.Tq - q_lo + QT - 1) / QT : 0, all = per * group;
+  const int share = (all + p.dkv_splits - 1) / p.dkv_splits, first = part * share, steps = all - first < share ? all - first : share;  // (may be <= 0)
 
   const int q_rows = ImgQ::rows_at(lane), o_rows = ImgO::rows_at(lane), q_cols = ImgQ::cols_at(lane), o_cols = ImgO::cols_at(lane);
-  auto fill = [&](unsigned char* buf, int h, int q0) {
-    const Rows have = {p.Tq - q0, false, 0ull};
-    const T* qb = (const T*)p.q + (long)b * p.q_s[0] + (long)q0 * p.q_s[1] + (long)h * p.q_s[2];
-    const long row = ((long)b * p.H + h) * p.Tq + q0;
+  // the next step's query head and first query, and where its Q, dO and row values lie: carried along, without divisions or long products in the loop
+  int h_next = hk * group + (per ? first / per : 0), q_next = q_lo + (per ? first % per : 0) * QT;
+  const long row0 = ((long)b * p.H + h_next) * p.Tq + q_lo;
+  const T* q_head = (const T*)p.q + (long)b * p.q_s[0] + (long)q_lo * p.q_s[1] + (long)h_next * p.q_s[2];  // at the head's first step
+  const T* o_head = (const T*)p.d_o + row0 * dvs;
+  const float* s_head = (wave < 2 ? p.lse : p.delta) + (wave & 1) * rows + row0;  // lse_1, lse_2, delta_1, delta_2: one array a wave
+  const T *q_tile = q_head + (long)(q_next - q_lo) * p.q_s[1], *o_tile = o_head + (long)(q_next - q_lo) * dvs;
+  const float* s_tile = s_head + (q_next - q_lo);
+  const long q_ld = p.q_s[1];
+  auto fill = [&](unsigned char* buf) {
+    const Rows have = {p.Tq - q_next, false, 0ull};
+    int tid = (int)threadIdx.x;
+    if (FENCE) asm volatile("" : "+v"(tid));  // (the offsets made of it are worked out again each time: kept, they would not fit the registers)
 #pragma unroll
-    for (int i = map0; i < map0 + MAPS; ++i) ImgQ::template fill<QT, VECTOR, NT>(buf + i * Q_BYTES, qb + i * p.q_s[3], p.q_s[1], p.d, have, tid);
-    ImgO::template fill<QT, true, NT>(buf + 2 * Q_BYTES, (const T*)p.d_o + row * dvs, dvs, dvs, have, tid);
-    // lse_1, lse_2, delta_1, delta_2 of the tile, one array a wave.  Queries behind the last: all zero like their Q and dO, so P = 1 but dV, dS get 0
-    const float* src = (wave < 2 ? p.lse : p.delta) + (wave & 1) * rows + row;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)src, 0, 0x7fffffff, 0x00020000), (lds_void_t*)(buf + 2 * Q_BYTES + O_BYTES + wave * 256), 4,
-                                             lane < QT && q0 + lane < p.Tq ? lane * 4 : (int)0x80000000, 0, 0, 0);
+    for (int i = map0; i < map0 + MAPS; ++i) ImgQ::template fill<QT, VECTOR, NT>(buf + i * Q_BYTES, q_tile + i * p.q_s[3], q_ld, p.d, have, tid);
+    ImgO::template fill<QT, true, NT>(buf + 2 * Q_BYTES, o_tile, dvs, dvs, have, tid);
+    // queries behind the last: all zero like their Q and dO, so P = 1 but dV, dS get 0
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)s_tile, 0, have.count < QT ? have.count * 4 : QT * 4, 0x00020000),
+                                             (lds_void_t*)(buf + 2 * Q_BYTES + O_BYTES + wave * 256), 4, lane * 4, 0, 0, 0);
+  };
+  auto advance = [&] {
+    q_next += QT;
+    q_tile += QT * q_ld;
+    o_tile += QT * dvs;
+    s_tile += QT;
+    if (q_next >= p.Tq) {
+      q_next = q_lo;
+      ++h_next;
+      q_tile = q_head += p.q_s[2];
+      o_tile = o_head += (long)p.Tq * dvs;
+      s_tile = s_head += p.Tq;
+    }
   };
   int v_at = 0;
+  uint4* stash = reinterpret_cast<uint4*>(smem + dkv_images<T, NB>() + QB * ImgO::ROW_BYTES) + wave * 2 * 64 + lane;  // (V_LDS) a lane's own operands
   if constexpr (V_LDS) {  // 32 keys a wave, filled as every other image; complete at the first step's wait
     const int place = dkv_images<T, NB>() + wave * 32 * ImgO::ROW_BYTES;
     ImgO::template fill<32, VECTOR, 64>(smem + place, (const T*)p.v + (long)b * p.v_s[0] + (long)w0 * p.v_s[1] + (long)hk * p.v_s[2], p.v_s[1], p.dv, Rows{sq.len - w0, p.key_mask != nullptr, __ballot(seen)}, lane);
     v_at = place + ImgO::rows_at(lane);
-  }
-  // the query head and first query of a step, without divisions in the loop
-  int h = hk * group, q0 = q_lo, h_next = h, q_next = q_lo;
-  auto advance = [&] {
-    q_next += QT;
-    if (q_next >= p.Tq) {
-      q_next = q_lo;
-      ++h_next;
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) {
+      Frag8<T> last;
+      load_frag<T, VECTOR>(krow + (long)i * p.k_s[3], K_HELD * 16 + half * 8, p.d, true, last);
+      stash[i * 64] = last.v;
     }
-  };
+  }
+  int h = h_next, q0 = q_next;
   float lam = 0.f;
-  if (steps > 0) fill(smem, h, q0);
+  if (steps > 0) fill(smem);
   for (int s = 0; s < steps; ++s) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
-    if (q0 == q_lo) lam = p.lam[p.n_lam > 1 ? h : 0];
+    if (s == 0 || q0 == q_lo) lam = p.lam[p.n_lam > 1 ? h : 0];
     overlap(smem + (~s & 1) * BUF, smem + (s & 1) * BUF,
             [&](unsigned char* next) {
               advance();
-              if (s + 1 < steps) fill(next, h_next, q_next);
+              if (s + 1 < steps) fill(next);
             },
             [&](const unsigned char* now) {
     const bool diag = p.causal && sq.start + q0 < w0 + 31;
@@ -1168,11 +1192,18 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
         Frag8<T> a;
         ImgQ::rows(now + (map0 + i) * Q_BYTES, q_rows, ks, a);
         if constexpr (!HOLD) load_frag<T, VECTOR>(krow + (long)(map0 + i) * p.k_s[3], ks * 16 + half * 8, p.d, true, k[i][0]);
-        mma(a, k[i][HOLD ? ks : 0], sc[i]);
+        if constexpr (V_LDS) {
+          Frag8<T> last;
+          if (ks == K_HELD) last.v = stash[i * 64];
+          mma(a, ks == K_HELD ? last : k[i][ks < K_HELD ? ks : 0], sc[i]);
+        } else {
+          mma(a, k[i][HOLD ? ks : 0], sc[i]);
+        }
         if (FENCE && ks % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
+      if (FENCE) __builtin_amdgcn_sched_barrier(0);
       const int t0 = 8 * g + 4 * half;
 #pragma unroll
       for (int i = 0; i < MAPS; ++i) {
@@ -1222,13 +1253,14 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
         if constexpr (V_LDS) ImgO::rows(smem, v_at, ks, v[0]);
         else if constexpr (!HOLD) load_frag<T, VECTOR>(vrow, ks * 16 + half * 8, p.dv, true, v[0]);
         mma(a, v[HOLD && !V_LDS ? ks : 0], dp);
-        if (FENCE && ks % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        if (FENCE) __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int i = 0; i < MAPS; ++i) {
         const float sign = map0 + i ? -lam : 1.f;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
+          if (FENCE) __builtin_amdgcn_sched_barrier(0);
           const float4 d4 = *reinterpret_cast<const float4*>(st + (2 + map0 + i) * 64 + 8 * g + 4 * half);
           const float de[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
@@ -1268,6 +1300,16 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
           for (int i = 0; i < MAPS; ++i) dk[i][n][r] = 0.f;
     }
   }
+  if (p.dkv_splits > 1) {  // fp32 sums of this part: rows of both maps' dK and dV, added by diff_attn_bwd_join_kernel
+    constexpr int WIDTH = 2 * CD * 32 + NB * 32;
+    float* out = p.dkv + ((((long)part * p.B + b) * p.Hkv + hk) * p.Tk + w0) * WIDTH;
+    auto row = [&](int r) { return w0 + r < p.Tk ? out + (long)r * WIDTH : nullptr; };
+    if constexpr (WANT_DV) store_rows<float>(strip, lane, dv, 1.f, NB * 32, true, Weights{nullptr, 0}, [&](int r) { return row(r) ? row(r) + 2 * CD * 32 : nullptr; });
+    if constexpr (WANT_DK)
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i) store_rows<float>(strip, lane, dk[i], p.scale, CD * 32, true, Weights{nullptr, 0}, [&](int r) { return row(r) ? row(r) + (map0 + i) * CD * 32 : nullptr; });
+    return;
+  }
   if constexpr (WANT_DV) {
     T* out = (T*)p.dv_out + (long)b * p.dv_s[0] + (long)w0 * p.dv_s[1] + (long)hk * p.dv_s[2];
     store_rows<T>(strip, lane, dv, 1.f, p.dv, p.dv_vec, Weights{nullptr, 0}, [&](int r) { return w0 + r < p.Tk ? out + (long)r * p.dv_s[1] : nullptr; });
@@ -1278,6 +1320,33 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
       T* out = (T*)p.dk_out + (long)b * p.dk_s[0] + (long)w0 * p.dk_s[1] + (long)hk * p.dk_s[2] + (long)(map0 + i) * p.dk_s[3];
       store_rows<T>(strip, lane, dk[i], p.scale, p.d, p.dk_vec, Weights{nullptr, 0}, [&](int r) { return w0 + r < p.Tk ? out + (long)r * p.dk_s[1] : nullptr; });
     }
+}
+
+// dK, dV of one key: the parts' sums in order; one wave a (batch, key, head), 4 channels a lane
+template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_join_kernel(tfpp_diff_attn_params p, int kc, int vc) {
+  const long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6), all = (long)p.B * p.Hkv * p.Tk;
+  if (n >= all) return;
+  const int j = (int)(n % p.Tk), hk = (int)(n / p.Tk % p.Hkv), b = (int)(n / p.Tk / p.Hkv), width = 2 * kc + vc;
+  const float* src = p.dkv + n * width;
+  for (int c = ((int)threadIdx.x & 63) * 4; c < width; c += 256) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < p.dkv_splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(src + k * all * width + c);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    const int map = c < 2 * kc ? c / kc : 2, ch = map < 2 ? c % kc : c - 2 * kc, limit = map < 2 ? p.d : p.dv;
+    T* to = map < 2 ? (T*)p.dk_out + (long)b * p.dk_s[0] + (long)j * p.dk_s[1] + (long)hk * p.dk_s[2] + (long)map * p.dk_s[3] + ch
+                    : (T*)p.dv_out + (long)b * p.dv_s[0] + (long)j * p.dv_s[1] + (long)hk * p.dv_s[2] + ch;
+    if ((map < 2 ? p.dk_vec : p.dv_vec) && ch + 4 <= limit) {
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(to) = make_uint2(f2bf_pack2(s.x, s.y), f2bf_pack2(s.z, s.w));
+      else *reinterpret_cast<float4*>(to) = s;
+    } else {
+      const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (ch + e < limit) to[e] = ElemTraits<T>::from_f(v[e]);
+    }
+  }
 }
 
 // lambda[h] = exp(lq1 . lk1) - exp(lq2 . lk2) + init of the four learned vectors of a head (one wave a head), and its gradient
@@ -1370,11 +1439,19 @@ template <typename T, int NB, bool VECTOR> int launch(const tfpp_diff_attn_param
   if (step == STEP_FWD) return start(diff_attn_fwd_kernel<T, NB, VECTOR>, grid, fwd_threads<T, NB>(), fwd_lds<T, NB>(), &done[0], p, st);
   if (step == STEP_DQ) return start(diff_attn_bwd_dq_kernel<T, NB, VECTOR>, grid, 256, dq_lds<T, NB>(), &done[1], p, st);
   if constexpr (dkv_split<T, NB, VECTOR>()) {
-    const int rc = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DK>, dim3((unsigned)n, 2), 256, dkv_lds<T, NB>(), &done[2], p, st);
-    return rc ? rc : start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DV>, grid, 256, dkv_lds<T, NB>(), &done[3], p, st);
+    const int rc = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DK>, dim3((unsigned)n, 2 * p.dkv_splits), 256, dkv_lds<T, NB>(), &done[2], p, st);
+    if (rc) return rc;
+    const int rv = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DV>, dim3((unsigned)n, p.dkv_splits), 256, dkv_lds<T, NB>(), &done[3], p, st);
+    if (rv) return rv;
   } else {
-    return start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_ALL>, grid, 256, dkv_lds<T, NB>(), &done[2], p, st);
+    const int rc = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_ALL>, dim3((unsigned)n, p.dkv_splits), 256, dkv_lds<T, NB>(), &done[2], p, st);
+    if (rc) return rc;
   }
+  if (p.dkv_splits > 1) {
+    hipLaunchKernelGGL(diff_attn_bwd_join_kernel<T>, dim3((unsigned)(((long)p.B * p.Hkv * p.Tk + 3) / 4)), dim3(256), 0, st, p, (NB + 1) / 2 * 32, NB * 32);
+    TFPP_CHECK_LAUNCH();
+  }
+  return 0;
 }
 // channels are padded to 16 NB / 32 NB: the width classes of the fusion transformers' heads (d 9, 27, 72) and the powers of two
 template <typename T> int dispatch(const tfpp_diff_attn_params& p, int step, hipStream_t st) {
@@ -1383,24 +1460,32 @@ template <typename T> int dispatch(const tfpp_diff_attn_params& p, int step, hip
 #define DA_GO(NB) (v ? launch<T, NB, true>(p, step, st) : launch<T, NB, false>(p, step, st))
   if (need <= 1) return DA_GO(1);
   if (need <= 2) return DA_GO(2);
-  if (need <= 4) return DA_GO(4);
+  if (need <= 4 && v) return launch<T, 4, true>(p, step, st);  // (element by element the next width serves as well)
   if (need <= 5) return DA_GO(5);
   return DA_GO(8);
 #undef DA_GO
 }
-int padded_blocks(const tfpp_diff_attn_params& p) {  // NB of dispatch()
+int padded_blocks(const tfpp_diff_attn_params& p) {  // NB of dispatch(), or more: the scratch is sized by it
   const int need = (p.d + 15) / 16 > (p.dv + 31) / 32 ? (p.d + 15) / 16 : (p.dv + 31) / 32;
-  return need <= 2 ? need : (need <= 4 ? 4 : (need <= 5 ? 5 : 8));
+  return need <= 2 ? need : (need <= 5 ? 5 : 8);
 }
 // Which forward kernel, and how many splits of the keys?  0: the one for many queries.
 int few_splits(const tfpp_diff_attn_params& p) {
   const long wg = (long)p.B * p.H * ((p.Tq + QB - 1) / QB);
-  if (wg >= 512) return 0;
+  if (wg >= 512 || (p.Tq > 64 && wg > 64)) return 0;  // (12 x 4 heads x 320 queries: 27 us there, 44 us here)
   const long rows = (long)(p.H / p.Hkv) * p.Tq, base = (long)p.B * p.Hkv * ((rows + 31) / 32);
   long n = (512 + base - 1) / base, most = (p.Tk + 511) / 512;  // two workgroups a CU; at least 512 keys (4 blocks a wave) in a split
   if (n > most) n = most;
   if (n > 64) n = 64;  // (the join holds one split a lane)
   return n < 1 ? 1 : (int)n;
+}
+// Parts of the queries in the dK / dV pass: 1024 workgroups (two a CU and as many to follow) where there are few keys and heads, each with at least 32 tiles
+// of 32 queries -- the parts' fp32 sums are written and read once more.
+int dkv_parts(const tfpp_diff_attn_params& p) {
+  const long wg = (long)p.B * p.Hkv * ((p.Tk + QB - 1) / QB), steps = (long)(p.H / p.Hkv) * ((p.Tq + 31) / 32);
+  long n = (1024 + wg - 1) / wg;
+  if (n > steps / 32) n = steps / 32;
+  return n < 1 ? 1 : (n > 16 ? 16 : (int)n);
 }
 int row_lanes(const tfpp_diff_attn_params& p) {
   int n = 1;
@@ -1413,6 +1498,7 @@ int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass 
   if (n > most) n = most;
   return (int)n;
 }
+int64_t row_floats(const tfpp_diff_attn_params& p) { return ((int64_t)row_blocks(p) * p.H * (1 + p.dv) + 63) & ~63ll; }
 }  // namespace
 
 extern "C" int tfpp_diff_attn_fwd(const tfpp_diff_attn_params* pp, int dtype, void* stream) {
@@ -1433,8 +1519,9 @@ extern "C" int tfpp_diff_attn_fwd_partial_floats(const tfpp_diff_attn_params* p,
 }
 
 extern "C" int tfpp_diff_attn_bwd_partial_floats(const tfpp_diff_attn_params* p, int64_t* out) {
-  if (!p || !out || p->B < 1 || p->H < 1 || p->Tq < 1 || p->dv < 1) return TFPP_EINVAL;
-  *out = (int64_t)row_blocks(*p) * p->H * (1 + p->dv);
+  if (!p || !out || p->B < 1 || p->H < 1 || p->Hkv < 1 || p->Tq < 1 || p->Tk < 1 || p->d < 1 || p->dv < 1) return TFPP_EINVAL;
+  const int nb = padded_blocks(*p), parts = dkv_parts(*p);
+  *out = row_floats(*p) + (parts > 1 ? (int64_t)parts * p->B * p->Hkv * p->Tk * (2 * ((nb + 1) / 2) + nb) * 32 : 0);
   return 0;
 }
 
@@ -1449,6 +1536,8 @@ extern "C" int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* pp, int dtype, vo
   p.dv_vec = out_vector(p.dv_out, p.dv_s, 3, vec);
   hipStream_t st = (hipStream_t)stream;
   const int blocks = row_blocks(p);
+  p.dkv_splits = dkv_parts(p);
+  p.dkv = p.partial + row_floats(p);
   const int lpr = row_lanes(p);
   p.do_vec = out_vector(p.dout, p.do_s, 3, vec);
   const dim3 sums(p.n_lam + (p.norm_w ? p.dv : 0));

@@ -725,8 +725,9 @@ typedef struct {
   void *dnorm_w, *dq_out, *dk_out, *dv_out;
   int64_t ld_mask, q_s[4], k_s[4], v_s[3], o_s[3], do_s[3], dq_s[4], dk_s[4], dv_s[3];
   int B, H, Hkv, Tq, Tk, d, dv, n_lam, norm, norm_w_bf16, causal, q_start_all;
-  int out_vec, do_vec, dq_vec, dk_vec, dv_vec, splits; /* set by the library */
+  int out_vec, do_vec, dq_vec, dk_vec, dv_vec, splits, dkv_splits; /* set by the library */
   float scale, out_scale, eps;
+  float* dkv; /* set by the library */
 } tfpp_diff_attn_params;
 int tfpp_diff_attn_fwd(const tfpp_diff_attn_params* p, int dtype, void* stream);
 int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* p, int dtype, void* stream);
