@@ -2,6 +2,8 @@
 every function takes CUDA(HIP) tensors, passes raw device pointers + the current stream to ``libtfpp_hip.so``
 and returns/fills tensors allocated with ``torch.empty``.  No ATen compute kernels run here."""
 import ctypes
+import functools
+import struct
 
 import torch
 
@@ -1245,6 +1247,30 @@ def one_device(*tensors):
   return dev
 
 
+class _Current:
+
+  def __enter__(self):
+    pass
+
+  def __exit__(self, *exc):
+    pass
+
+
+_CURRENT = _Current()
+
+
+def device_guard(dev):
+  """``torch.cuda.device(dev)``, free where dev is the current device already (2 us a call otherwise: half of a single-token norm)."""
+  return _CURRENT if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _layout(fmt, mirror):
+  """struct.Struct of a parameter struct: one pack call in place of sixty ctypes attributes (30 us)."""
+  out = struct.Struct('@' + fmt)
+  assert out.size <= ctypes.sizeof(mirror) < out.size + 8, (mirror, out.size)  # (the mirror may end with padding)
+  return out
+
+
 def is_dense(t):
   """Do the elements of ``t`` fill one gap-free span of memory (in any order of its dimensions)?"""
   want = 1
@@ -1321,7 +1347,7 @@ class GradClip:
       raise ValueError(f'norm_type is 1, 2 or inf, got {norm_type}')
     if not float(max_norm) >= 0.0:
       raise ValueError(f'max_norm is not negative, got {max_norm}')
-    with torch.cuda.device(self.device):
+    with device_guard(self.device):
       # scratch of this call alone (captured graphs keep theirs in the graph's own pool): nothing is shared between streams or graphs
       buf = torch.empty(self._partials + 1, device=self.device, dtype=torch.float64)
       res = buf[self._partials:].view(torch.float32)
@@ -1380,19 +1406,26 @@ class BlockNormContext:
   __slots__ = ('x', 'a', 'gate', 'stat', 'opt', 'params', 'mode', 'lds', 'shape')
 
 
-_BLOCK_NORM_SUMS = {'pre_weight': ('dpre_w', 1), 'pre_bias': ('dpre_b', 2), 'post_weight': ('dpost_w', 4), 'post_bias': ('dpost_b', 8), 'scale': ('dscale', 16)}
+# tfpp_block_norm_params: x a gate | post_w post_b pre_w pre_b scale | y h stat | dy dh dx da dgate | dpost_w dpost_b dpre_w dpre_b dscale partial |
+# ld_x ld_a ld_g ld_dy ld_dh | B T C layer post pre gate_mode gate_act accumulate | alpha eps  (a null pointer is 0; padding to 8 bytes at the end)
+_BLOCK_NORM = _layout('22Q5q9i2f4x', BlockNormParams)
+_BLOCK_NORM_PARAMS = ('post_weight', 'post_bias', 'pre_weight', 'pre_bias', 'scale')
+_BLOCK_NORM_BITS = {'pre_weight': 1, 'pre_bias': 2, 'post_weight': 4, 'post_bias': 8, 'scale': 16}
 
 
-def _block_norm_params(ctx):
+def _addr(t):
+  return 0 if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=512)
+def _block_norm_partial(shape, mode, bias):
   p = BlockNormParams()
-  B, T, C = ctx.shape
-  p.x, p.a, p.gate = ctx.x.data_ptr(), ctx.a.data_ptr(), ptr(ctx.gate)
-  p.post_w, p.post_b, p.pre_w, p.pre_b, p.scale = (ptr(ctx.params[n]) for n in ('post_weight', 'post_bias', 'pre_weight', 'pre_bias', 'scale'))
-  p.ld_x, p.ld_a, p.ld_g = ctx.lds
-  p.B, p.T, p.C, p.gate_mode = B, T, C, ctx.mode
-  p.layer, p.post, p.pre, p.gate_act, p.alpha, p.eps = ctx.opt
-  p.stat = ptr(ctx.stat)
-  return p
+  p.B, p.T, p.C = shape
+  p.gate_mode = mode
+  p.dpost_b = p.dpre_b = 16 if bias else None  # (never dereferenced: which sums there are decides the number of workgroups)
+  n = ctypes.c_int64()
+  lib.tfpp_block_norm_bwd_partial_floats(ctypes.byref(p), ctypes.addressof(n))
+  return n.value
 
 
 def block_norm_fwd(x, a, *, kind='layer', post=True, pre=True, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, gate=None, gate_act=ACT_NONE,
@@ -1438,16 +1471,17 @@ def block_norm_fwd(x, a, *, kind='layer', post=True, pre=True, post_weight=None,
     raise ValueError(f'block_norm_fwd: too many rows ({rows}) or samples ({B})')
   ctx.x, ctx.a, ctx.gate, ctx.lds, ctx.shape = x, a, gate, (ld_x, ld_a, ld_g), (B, T, C)
   ctx.opt = (int(kind == 'layer'), int(post), int(pre), gate_act, float(alpha), float(eps))
-  with torch.cuda.device(dev):
+  with device_guard(dev):
     y = torch.empty(x.shape, device=dev, dtype=x.dtype)
     h = torch.empty(x.shape, device=dev, dtype=x.dtype) if pre else None
     ctx.stat = torch.empty((max(rows, 1), 4), device=dev, dtype=torch.float32) if save else None
     if rows:
-      p = _block_norm_params(ctx)
-      p.y, p.h = y.data_ptr(), ptr(h)
+      p = _BLOCK_NORM.pack(x.data_ptr(), a.data_ptr(), _addr(gate), _addr(post_weight), _addr(post_bias), _addr(pre_weight), _addr(pre_bias), _addr(scale),
+                           y.data_ptr(), _addr(h), _addr(ctx.stat), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, ld_x, ld_a, ld_g, 0, 0, B, T, C, ctx.opt[0], ctx.opt[1], ctx.opt[2], ctx.mode,
+                           gate_act, 0, ctx.opt[4], ctx.opt[5])
       if lib.profiler is not None:
         lib.profiler.tag('block_norm_fwd', 0.0, float(rows * C * x.element_size() * (3 + pre + (ctx.mode == 2))))
-      lib.tfpp_block_norm_fwd(ctypes.byref(p), dt(x), stream())
+      lib.tfpp_block_norm_fwd(p, dt(x), stream())
   return y, h, (ctx if save else None)
 
 
@@ -1474,7 +1508,7 @@ def block_norm_bwd(dy, dh, ctx, into=None):
       raise TypeError(f'{n} is {t.dtype}, expected {x.dtype}')
     lds.append(_row_view(t, x.shape, n) if t is not None else 0)
   rows = B * T
-  with torch.cuda.device(dev):
+  with device_guard(dev):
     out = {n: None for n in ('x', 'a', 'gate', 'scale', 'post_weight', 'post_bias', 'pre_weight', 'pre_bias')}
     out['x'], out['a'] = torch.empty(x.shape, device=dev, dtype=x.dtype), torch.empty(x.shape, device=dev, dtype=x.dtype)
     if ctx.gate is not None:
@@ -1488,20 +1522,15 @@ def block_norm_bwd(dy, dh, ctx, into=None):
       if out['gate'] is not None and out['gate'].numel():
         zero_(out['gate'])
     else:
-      p = _block_norm_params(ctx)
-      p.dy, p.dh, p.ld_dy, p.ld_dh = ptr(dy), ptr(dh), lds[0], lds[1]
-      p.dx, p.da, p.dgate = out['x'].data_ptr(), out['a'].data_ptr(), ptr(out['gate'])
-      for n in names:
-        field, bit = _BLOCK_NORM_SUMS[n]
-        setattr(p, field, out[n].data_ptr())
-        p.accumulate |= bit if n in into else 0
-      n_part = ctypes.c_int64()
-      lib.tfpp_block_norm_bwd_partial_floats(ctypes.byref(p), ctypes.addressof(n_part))
-      partial = torch.empty(n_part.value, device=dev, dtype=torch.float32)
-      p.partial = partial.data_ptr()
+      bias = ctx.params['post_bias'] is not None or ctx.params['pre_bias'] is not None
+      partial = torch.empty(_block_norm_partial(ctx.shape, ctx.mode, bias), device=dev, dtype=torch.float32)
+      accumulate = sum(_BLOCK_NORM_BITS[n] for n in into)
+      p = _BLOCK_NORM.pack(x.data_ptr(), ctx.a.data_ptr(), _addr(ctx.gate), *[_addr(ctx.params[n]) for n in _BLOCK_NORM_PARAMS], 0, 0, ctx.stat.data_ptr(), _addr(dy), _addr(dh),
+                           out['x'].data_ptr(), out['a'].data_ptr(), _addr(out['gate']), *[_addr(out[n]) for n in _BLOCK_NORM_PARAMS], partial.data_ptr(), *ctx.lds, *lds,
+                           B, T, C, ctx.opt[0], ctx.opt[1], ctx.opt[2], ctx.mode, ctx.opt[3], accumulate, ctx.opt[4], ctx.opt[5])
       if lib.profiler is not None:
         lib.profiler.tag('block_norm_bwd', 0.0, float(rows * C * x.element_size() * (4 + (dy is not None) + (dh is not None) + 2 * (ctx.mode == 2))))
-      lib.tfpp_block_norm_bwd(ctypes.byref(p), dt(x), stream())
+      lib.tfpp_block_norm_bwd(p, dt(x), stream())
   return out
 
 
@@ -1509,7 +1538,7 @@ def block_norm_bwd(dy, dh, ctx, into=None):
 def diff_lambda(lq1, lk1, lq2, lk2, init):
   """lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + init of learned vectors [n, d] (or [d]: one lambda for all heads), fp32 or bf16 -> fp32 [n]."""
   n, d = _lambda_vectors(lq1, lk1, lq2, lk2)
-  with torch.cuda.device(lq1.device):
+  with device_guard(lq1.device):
     lam = torch.empty(n, device=lq1.device, dtype=torch.float32)
     lib.tfpp_diff_lambda(ptr(lq1), ptr(lk1), ptr(lq2), ptr(lk2), float(init), ptr(lam), n, d, dt(lq1), stream())
   return lam
@@ -1521,7 +1550,7 @@ def diff_lambda_bwd(dlam, lq1, lk1, lq2, lk2):
   one_device(lq1, dlam)
   if dlam.dtype != torch.float32 or dlam.numel() != n or not dlam.is_contiguous():
     raise ValueError(f'dlam: {n} contiguous fp32 values, got {dlam.dtype} {tuple(dlam.shape)}')
-  with torch.cuda.device(lq1.device):
+  with device_guard(lq1.device):
     out = [torch.empty_like(t) for t in (lq1, lk1, lq2, lk2)]
     lib.tfpp_diff_lambda_bwd(ptr(dlam), ptr(lq1), ptr(lk1), ptr(lq2), ptr(lk2), *[ptr(t) for t in out], n, d, dt(lq1), stream())
   return out
@@ -1584,16 +1613,18 @@ def _diff_attn_check(q, k, v, lam):
   return dev, qs, ks, vs, (B, Tq, Tk, H, Hkv, d, dv)
 
 
-def _diff_attn_params(q, k, v, lam, qs, ks, vs, shape, norm_weight, key_mask, kv_len, q_start, opt):
+# tfpp_diff_attn_params: q k v lam norm_w out o1 o2 lse kv_len q_start key_mask dout d_o delta partial dlam dnorm_w dq dk dv | ld_mask q_s[4] k_s[4] v_s[3]
+# o_s[3] do_s[3] dq_s[4] dk_s[4] dv_s[3] | B H Hkv Tq Tk d dv n_lam norm norm_w_bf16 causal q_start_all, 7 set by the library | scale out_scale eps | dkv
+_DIFF_ATTN = _layout('21Q29q19i3fQ', DiffAttnParams)
+
+
+@functools.lru_cache(maxsize=512)
+def _diff_attn_partial(shape, backward):
   p = DiffAttnParams()
   p.B, p.Tq, p.Tk, p.H, p.Hkv, p.d, p.dv = shape
-  p.q, p.k, p.v, p.lam, p.n_lam = q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), lam.numel()
-  p.q_s[:], p.k_s[:], p.v_s[:] = qs, ks, vs
-  p.scale, p.causal, p.norm, p.eps, p.out_scale, p.q_start_all = opt
-  p.norm_w, p.norm_w_bf16 = ptr(norm_weight), int(norm_weight is not None and norm_weight.dtype == torch.bfloat16)
-  p.kv_len, p.q_start, p.key_mask = ptr(kv_len), ptr(q_start), ptr(key_mask)
-  p.ld_mask = key_mask.stride(0) if key_mask is not None else 0
-  return p
+  n = ctypes.c_int64()
+  (lib.tfpp_diff_attn_bwd_partial_floats if backward else lib.tfpp_diff_attn_fwd_partial_floats)(ctypes.byref(p), ctypes.addressof(n))
+  return n.value
 
 
 def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_len=None, key_mask=None, norm=True, norm_weight=None, norm_eps=1e-5, out_scale=1.0,
@@ -1631,7 +1662,7 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
   if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != (B, Tk) or (Tk > 1 and key_mask.stride(1) != 1) or
                                key_mask.device != dev):
     raise ValueError(f'key_mask: bool or uint8 {(B, Tk)} on {dev} with contiguous rows, got {key_mask.dtype} {tuple(key_mask.shape)}')
-  with torch.cuda.device(dev):
+  with device_guard(dev):
     if out is None:
       out = torch.empty((B, Tq, H, dv), device=dev, dtype=q.dtype)
     else:
@@ -1652,19 +1683,16 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
     if Tk == 0:
       out.zero_()
       return out, ctx
-    p = _diff_attn_params(q, k, v, lam, qs, ks, vs, shape, norm_weight, key_mask, kv_len, start_t, (scale, int(causal), int(norm), norm_eps, out_scale, start_all))
-    p.out = out.data_ptr()
-    p.o_s[:] = os_
-    if save:
-      p.o1, p.o2, p.lse = ctx.o1.data_ptr(), ctx.o2.data_ptr(), ctx.lse.data_ptr()
-    n_part = ctypes.c_int64()
-    lib.tfpp_diff_attn_fwd_partial_floats(ctypes.byref(p), ctypes.addressof(n_part))
-    if n_part.value:  # scratch of this call alone
-      partial = torch.empty(n_part.value, device=dev, dtype=torch.float32)
-      p.partial = partial.data_ptr()
+    n_part = _diff_attn_partial(shape, False)
+    partial = torch.empty(n_part, device=dev, dtype=torch.float32) if n_part else None  # scratch of this call alone
+    o1, o2, lse = (ctx.o1.data_ptr(), ctx.o2.data_ptr(), ctx.lse.data_ptr()) if save else (0, 0, 0)
+    p = _DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(norm_weight), out.data_ptr(), o1, o2, lse, _addr(kv_len), _addr(start_t), _addr(key_mask),
+                        0, 0, 0, _addr(partial), 0, 0, 0, 0, 0, key_mask.stride(0) if key_mask is not None else 0, *qs, *ks, *vs, *os_, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                        B, H, Hkv, Tq, Tk, d, dv, lam.numel(), norm, norm_weight is not None and norm_weight.dtype == torch.bfloat16, causal, start_all, 0, 0, 0, 0, 0, 0, 0,
+                        scale, out_scale, norm_eps, 0)
     if lib.profiler is not None:
       lib.profiler.tag(f'diff_attn_fwd<{"f32" if q.dtype == torch.float32 else "bf16"}>', float(B * H * Tq * Tk * (4 * d + 4 * dv)))
-    lib.tfpp_diff_attn_fwd(ctypes.byref(p), dt(q), stream())
+    lib.tfpp_diff_attn_fwd(p, dt(q), stream())
   return out, ctx
 
 
@@ -1679,7 +1707,7 @@ def diff_attn_bwd(dout, q, k, v, lam, ctx, dq=None, dk=None, dv=None):
   if tuple(dout.shape) != (B, Tq, H, dvn) or dout.dtype != q.dtype or dout.device != dev:
     raise ValueError(f'dout: {q.dtype} {(B, Tq, H, dvn)} on {dev}, got {dout.dtype} {tuple(dout.shape)}')
   dos = _last_contiguous(dout, 'dout', 4)
-  with torch.cuda.device(dev):
+  with device_guard(dev):
     outs = []
     for n, t, like in (('dq', dq, q), ('dk', dk, k), ('dv', dv, v)):
       if t is None:
@@ -1696,18 +1724,16 @@ def diff_attn_bwd(dout, q, k, v, lam, ctx, dq=None, dk=None, dv=None):
       for t in outs + [dlam] + ([dw] if dw is not None else []):
         t.zero_()
       return (*outs, dlam, dw)
-    p = _diff_attn_params(q, k, v, lam, qs, ks, vs, shape, w, ctx.key_mask, ctx.kv_len, ctx.q_start, ctx.opt)
-    n_part = ctypes.c_int64()
-    lib.tfpp_diff_attn_bwd_partial_floats(ctypes.byref(p), ctypes.addressof(n_part))
     # scratch of this call alone: captured graphs keep theirs in the graph's own pool
     d_o = torch.empty_like(ctx.o1)
     delta = torch.empty_like(ctx.lse)
-    partial = torch.empty(n_part.value, device=dev, dtype=torch.float32)
-    p.o1, p.o2, p.lse, p.dout = ctx.o1.data_ptr(), ctx.o2.data_ptr(), ctx.lse.data_ptr(), dout.data_ptr()
-    p.d_o, p.delta, p.partial, p.dlam, p.dnorm_w = d_o.data_ptr(), delta.data_ptr(), partial.data_ptr(), dlam.data_ptr(), ptr(dw)
-    p.dq_out, p.dk_out, p.dv_out = (t.data_ptr() for t in outs)
-    p.do_s[:], p.dq_s[:], p.dk_s[:], p.dv_s[:] = dos, *strides
+    partial = torch.empty(_diff_attn_partial(shape, True), device=dev, dtype=torch.float32)
+    scale, causal, norm, eps, out_scale, start_all = ctx.opt
+    p = _DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(w), 0, ctx.o1.data_ptr(), ctx.o2.data_ptr(), ctx.lse.data_ptr(), _addr(ctx.kv_len),
+                        _addr(ctx.q_start), _addr(ctx.key_mask), dout.data_ptr(), d_o.data_ptr(), delta.data_ptr(), partial.data_ptr(), dlam.data_ptr(), _addr(dw),
+                        *[t.data_ptr() for t in outs], ctx.key_mask.stride(0) if ctx.key_mask is not None else 0, *qs, *ks, *vs, 0, 0, 0, *dos, *strides[0], *strides[1], *strides[2],
+                        B, H, Hkv, Tq, Tk, d, dvn, lam.numel(), norm, w is not None and w.dtype == torch.bfloat16, causal, start_all, 0, 0, 0, 0, 0, 0, 0, scale, out_scale, eps, 0)
     if lib.profiler is not None:
       lib.profiler.tag(f'diff_attn_bwd<{"f32" if q.dtype == torch.float32 else "bf16"}>', float(B * H * Tq * Tk * (16 * d + 6 * dvn)))
-    lib.tfpp_diff_attn_bwd(ctypes.byref(p), dt(q), stream())
+    lib.tfpp_diff_attn_bwd(p, dt(q), stream())
   return (*outs, dlam, dw)
