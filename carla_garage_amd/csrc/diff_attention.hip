@@ -38,7 +38,7 @@ __device__ __forceinline__ void mma(const Frag8<float>& a, const Frag8<float>& b
 #pragma unroll
   for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
 }
-// C registers 8 t .. 8 t + 7 as an operand.  bf16: one rounding (2^-9 relative) of each probability / score gradient, as its partner operand has
+// C registers 8 t .. 8 t + 7 as an operand.  bf16: one rounding (2^-8 relative at most) of each probability / score gradient, as its partner operand has
 __device__ __forceinline__ void to_frag(const f32x16_t& c, int t, Frag8<bf16_t>& f) {
   f.v = make_uint4(f2bf_pack2(c[8 * t], c[8 * t + 1]), f2bf_pack2(c[8 * t + 2], c[8 * t + 3]), f2bf_pack2(c[8 * t + 4], c[8 * t + 5]),
                    f2bf_pack2(c[8 * t + 6], c[8 * t + 7]));
@@ -251,7 +251,8 @@ __device__ __forceinline__ Seq sequence(const tfpp_diff_attn_params& p, int b) {
     const int n = __builtin_amdgcn_readfirstlane(p.kv_len[b]);  // (the compiler does not know that it is the same in all lanes)
     s.len = n < 0 ? 0 : (n < p.Tk ? n : p.Tk);
   }
-  s.start = p.q_start ? __builtin_amdgcn_readfirstlane(p.q_start[b]) : p.q_start_all;
+  const int start = p.q_start ? __builtin_amdgcn_readfirstlane(p.q_start[b]) : p.q_start_all;
+  s.start = start < -p.Tq ? -p.Tq : (start < p.Tk ? start : p.Tk);  // (beyond: nothing is seen, everything is; sums with positions stay in 32 bits)
   return s;
 }
 // bit i: key j0 + i exists and is not left out
@@ -1389,7 +1390,7 @@ bool strides_vec(const int64_t* s, int n, int vec) {
 bool valid(const tfpp_diff_attn_params& p, int dtype) {
   return (dtype == TFPP_F32 || dtype == TFPP_BF16) && p.q && p.k && p.v && p.lam && p.B >= 1 && p.H >= 1 && p.Hkv >= 1 && p.H % p.Hkv == 0 && p.Tq >= 1 && p.Tk >= 1 &&
          p.d >= 1 && p.d <= 128 && p.dv >= 1 && p.dv <= 256 && (p.n_lam == 1 || p.n_lam == p.H) && p.scale > 0.f && std::isfinite(p.scale) && (!p.norm || p.eps > 0.f) &&
-         p.Tq < (1 << 30) && p.Tk < (1 << 30) && (long)p.B * p.H < (1l << 24);
+         p.Tq < (1 << 29) && p.Tk < (1 << 29) && (long)p.B * p.H < (1l << 24);
 }
 // Can q, k, v be read 16 bytes at a time?
 bool vector_rows(const tfpp_diff_attn_params& p, int vec) {

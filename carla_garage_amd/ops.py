@@ -34,7 +34,7 @@ def pad_to(n, m):
 
 
 def stream():
-  return torch.cuda.current_stream().cuda_stream
+  return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())  # the handle alone: no Stream object is built (3 us a launch)
 
 
 def ptr(t):
@@ -1501,6 +1501,9 @@ def block_norm_bwd(dy, dh, ctx, into=None):
     if n not in names:
       raise ValueError(f'block_norm_bwd: the forward pass had no {n}')
     _channel_param(t, C, dev, n)
+  at = sorted(t.data_ptr() for t in into.values())
+  if any(b - a < 4 * C for a, b in zip(at, at[1:])):
+    raise ValueError('block_norm_bwd: two gradients of `into` overlap in memory')
   one_device(x, dy, dh)
   lds = []
   for n, t in (('dy', dy), ('dh', dh)):
@@ -1568,7 +1571,7 @@ def _lambda_vectors(*ts):
 
 class DiffAttnContext:
   """What diff_attn_bwd needs of its forward pass: P_1 V, P_2 V, the rows' log-sums and the options."""
-  __slots__ = ('o1', 'o2', 'lse', 'norm_weight', 'opt', 'kv_len', 'q_start', 'key_mask', 'shape')
+  __slots__ = ('saved', 'addr', 'norm_weight', 'opt', 'kv_len', 'q_start', 'key_mask', 'shape')
 
 
 def _last_contiguous(t, name, dims):
@@ -1586,6 +1589,30 @@ def _disjoint(t, name):
     if st < want:
       raise ValueError(f'{name}: elements overlap in memory (strides {t.stride()})')
     want = st * n
+
+
+def _apart(out, name, others):
+  """``out`` (given by the caller) shares no element with any of ``others`` [(name, tensor)].  Views of one buffer pass where their spans are apart, or
+  where both lie in periods of it (rows of a fused projection, the batches of a cache) at places that do not meet; what cannot be told apart is refused."""
+  span = lambda t, st, lim: sum((n - 1) * s for n, s in zip(t.shape, st) if s < lim) * t.element_size() + t.element_size()
+  for other, t in others:
+    if t is None or t is out or not t.numel() or not out.numel():
+      if t is out and t.numel():
+        raise ValueError(f'{name} and {other} are the same tensor')
+      continue
+    a, b, sa, sb = out.data_ptr(), t.data_ptr(), out.stride(), t.stride()
+    big = 1 << 62
+    if a + span(out, sa, big) <= b or b + span(t, sb, big) <= a:
+      continue
+    size = out.element_size()
+    for per in {s for s, n in zip(sa, out.shape) if n > 1 and s > 0} & {s for s, n in zip(sb, t.shape) if n > 1 and s > 0} if t.element_size() == size else ():
+      # every larger stride a multiple of the period, the smaller ones inside it: each tensor lies in [start, start + inner span) of every period
+      if all(s < per or s % per == 0 for x in (out, t) for s, n in zip(x.stride(), x.shape) if n > 1):
+        la, lb, p = span(out, sa, per), span(t, sb, per), per * size
+        if (b - a) % p >= la and (a - b) % p >= lb:
+          break
+    else:
+      raise ValueError(f'{name} overlaps {other} in memory')
 
 
 def _int_rows(t, n, dev, name):
@@ -1606,7 +1633,7 @@ def _diff_attn_check(q, k, v, lam):
     raise ValueError(f'differential attention: d 1 to 128 and dv 1 to 256, got d = {d}, dv = {dv}')
   if H < 1 or Hkv < 1 or H % Hkv:
     raise ValueError(f'{H} query heads over {Hkv} key / value heads')
-  if max(Tq, Tk) >= 1 << 30 or B * H >= 1 << 24:
+  if max(Tq, Tk) >= 1 << 29 or B * H >= 1 << 24:
     raise ValueError('differential attention: too many tokens or heads')
   if lam.dtype != torch.float32 or lam.numel() not in (1, H) or not lam.is_contiguous():
     raise ValueError(f'lam: 1 or {H} contiguous fp32 values, got {lam.dtype} {tuple(lam.shape)}')
@@ -1627,6 +1654,11 @@ def _diff_attn_partial(shape, backward):
   return n.value
 
 
+def _diff_attn_rows(rows, dv, size):
+  """Bytes of one result [B, H, Tq, dv rounded up to 8] in q's type and of the two fp32 statistics of its rows, each a multiple of 256."""
+  return pad_to(rows * pad_to(dv, 8) * size, 256), pad_to(rows * 8, 256)
+
+
 def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_len=None, key_mask=None, norm=True, norm_weight=None, norm_eps=1e-5, out_scale=1.0,
                   save=False, out=None):
   """Differential attention: P_i = softmax(scale q_i k_i^T) for the two halves of every head, O = (P_1 - lam P_2) v, each head's result normalised:
@@ -1636,7 +1668,7 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
     lam: fp32 [H] or [1].  norm_weight: [dv], fp32 or bf16, or None.  scale > 0, default d ** -0.5.
   Which keys a query sees: kv_len (int32 [B] on the device) leaves out keys >= kv_len[b]; key_mask (bool or uint8 [B, Tk]) those where it is 0; causal
   those with key > q_start + query, q_start an int, int32 [B] on the device, or None for Tk - Tq.  k and v of keys left out by kv_len or key_mask may
-  hold anything; the other values have to be finite.  A query that sees no key gives zeros.
+  hold anything; the other values have to be finite, the scaled scores below 1e30.  A query that sees no key gives zeros.
   New tokens against a cache: q [B, 1, ...], k and v the whole cache, kv_len the tokens it holds (the new ones among them); for several new tokens
   causal=True and q_start = kv_len - Tq.
   save=True keeps what diff_attn_bwd needs.  ``out``: written in place of a new tensor, any strides that do not overlap."""
@@ -1669,14 +1701,16 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
       if tuple(out.shape) != (B, Tq, H, dv) or out.dtype != q.dtype or out.device != dev:
         raise ValueError(f'out: {q.dtype} {(B, Tq, H, dv)} on {dev}, got {out.dtype} {tuple(out.shape)}')
       _disjoint(out, 'out')
+      _apart(out, 'out', (('q', q), ('k', k), ('v', v)))
     os_ = _last_contiguous(out, 'out', 4)
     ctx = None
     if save:
       ctx = DiffAttnContext()
-      dvs = pad_to(dv, 8)
-      ctx.o1, ctx.o2 = (torch.empty((B, H, Tq, dvs), device=dev, dtype=q.dtype) for _ in range(2))
-      ctx.lse = torch.empty((2, B, H, Tq), device=dev, dtype=torch.float32)
-      ctx.norm_weight, ctx.opt, ctx.shape = norm_weight, (scale, int(causal), int(norm), float(norm_eps), float(out_scale), start_all), shape
+      n_o, n_row = _diff_attn_rows(B * H * Tq, dv, q.element_size())
+      ctx.saved = torch.empty(2 * n_o + n_row, device=dev, dtype=torch.uint8)  # o1 | o2 (in q's type) | lse: one allocation
+      at = ctx.saved.data_ptr()
+      ctx.addr = (at, at + n_o, at + 2 * n_o)
+      ctx.norm_weight, ctx.opt, ctx.shape = norm_weight, (scale, int(causal), int(norm), float(norm_eps), float(out_scale), start_all, q.dtype), shape
       ctx.kv_len, ctx.q_start, ctx.key_mask = kv_len, start_t, key_mask
     if B == 0 or Tq == 0:
       return out, ctx
@@ -1685,7 +1719,7 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
       return out, ctx
     n_part = _diff_attn_partial(shape, False)
     partial = torch.empty(n_part, device=dev, dtype=torch.float32) if n_part else None  # scratch of this call alone
-    o1, o2, lse = (ctx.o1.data_ptr(), ctx.o2.data_ptr(), ctx.lse.data_ptr()) if save else (0, 0, 0)
+    o1, o2, lse = ctx.addr if save else (0, 0, 0)
     p = _DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(norm_weight), out.data_ptr(), o1, o2, lse, _addr(kv_len), _addr(start_t), _addr(key_mask),
                         0, 0, 0, _addr(partial), 0, 0, 0, 0, 0, key_mask.stride(0) if key_mask is not None else 0, *qs, *ks, *vs, *os_, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
                         B, H, Hkv, Tq, Tk, d, dv, lam.numel(), norm, norm_weight is not None and norm_weight.dtype == torch.bfloat16, causal, start_all, 0, 0, 0, 0, 0, 0, 0,
@@ -1701,8 +1735,8 @@ def diff_attn_bwd(dout, q, k, v, lam, ctx, dq=None, dk=None, dv=None):
   dq / dk / dv: tensors (views of a fused gradient, any strides that do not overlap) to be written in place of new ones.  dlam has lam's shape (summed over
   the heads when lam is one value), dnorm_weight the weight's type, None without one.  Nothing is added atomically: bit-reproducible."""
   dev, qs, ks, vs, shape = _diff_attn_check(q, k, v, lam)
-  if ctx.shape != shape or ctx.o1.dtype != q.dtype:
-    raise ValueError(f'the context belongs to another forward pass: {ctx.shape} {ctx.o1.dtype}, now {shape} {q.dtype}')
+  if ctx.shape != shape or ctx.opt[-1] != q.dtype or ctx.saved.device != dev:
+    raise ValueError(f'the context belongs to another forward pass: {ctx.shape} {ctx.opt[-1]} on {ctx.saved.device}, now {shape} {q.dtype} on {dev}')
   B, Tq, Tk, H, Hkv, d, dvn = shape
   if tuple(dout.shape) != (B, Tq, H, dvn) or dout.dtype != q.dtype or dout.device != dev:
     raise ValueError(f'dout: {q.dtype} {(B, Tq, H, dvn)} on {dev}, got {dout.dtype} {tuple(dout.shape)}')
@@ -1716,6 +1750,7 @@ def diff_attn_bwd(dout, q, k, v, lam, ctx, dq=None, dk=None, dv=None):
         if t.shape != like.shape or t.dtype != q.dtype or t.device != dev:
           raise ValueError(f'{n}: {q.dtype} {tuple(like.shape)} on {dev}, got {t.dtype} {tuple(t.shape)}')
         _disjoint(t, n)
+        _apart(t, n, (('dout', dout), ('q', q), ('k', k), ('v', v), *zip(('dq', 'dk'), outs)))
       outs.append(t)
     strides = [_last_contiguous(t, n, dims) for n, t, dims in zip(('dq', 'dk', 'dv'), outs, (5, 5, 4))]
     w = ctx.norm_weight
@@ -1725,12 +1760,14 @@ def diff_attn_bwd(dout, q, k, v, lam, ctx, dq=None, dk=None, dv=None):
         t.zero_()
       return (*outs, dlam, dw)
     # scratch of this call alone: captured graphs keep theirs in the graph's own pool
-    d_o = torch.empty_like(ctx.o1)
-    delta = torch.empty_like(ctx.lse)
-    partial = torch.empty(_diff_attn_partial(shape, True), device=dev, dtype=torch.float32)
-    scale, causal, norm, eps, out_scale, start_all = ctx.opt
-    p = _DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(w), 0, ctx.o1.data_ptr(), ctx.o2.data_ptr(), ctx.lse.data_ptr(), _addr(ctx.kv_len),
-                        _addr(ctx.q_start), _addr(ctx.key_mask), dout.data_ptr(), d_o.data_ptr(), delta.data_ptr(), partial.data_ptr(), dlam.data_ptr(), _addr(dw),
+    n_o, n_row = _diff_attn_rows(B * H * Tq, dvn, q.element_size())
+    scratch = torch.empty(n_o + n_row + 4 * _diff_attn_partial(shape, True), device=dev, dtype=torch.uint8)
+    d_o = scratch.data_ptr()
+    delta = d_o + n_o
+    partial = delta + n_row
+    scale, causal, norm, eps, out_scale, start_all, _ = ctx.opt
+    p = _DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(w), 0, *ctx.addr, _addr(ctx.kv_len),
+                        _addr(ctx.q_start), _addr(ctx.key_mask), dout.data_ptr(), d_o, delta, partial, dlam.data_ptr(), _addr(dw),
                         *[t.data_ptr() for t in outs], ctx.key_mask.stride(0) if ctx.key_mask is not None else 0, *qs, *ks, *vs, 0, 0, 0, *dos, *strides[0], *strides[1], *strides[2],
                         B, H, Hkv, Tq, Tk, d, dvn, lam.numel(), norm, w is not None and w.dtype == torch.bfloat16, causal, start_all, 0, 0, 0, 0, 0, 0, 0, scale, out_scale, eps, 0)
     if lib.profiler is not None:

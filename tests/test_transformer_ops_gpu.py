@@ -807,3 +807,225 @@ def test_diff_attention_captured_on_two_streams(ops, Tq, Tk):
     got = step()
   torch.cuda.synchronize()
   assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('shape', [(1, 1100, 96, 2, 1, 32, 64), (1, 540, 70, 4, 1, 72, 144), (1, 2080, 33, 1, 1, 128, 256)], ids=str)
+def test_diff_attention_gradients_with_the_queries_split(ops, shape, dtype):
+  """Few keys and many tiles of queries: dK and dV are summed in parts and joined."""
+  B, Tq, Tk, H, Hkv, d, dv = shape
+  assert (H // Hkv) * ((Tq + 31) // 32) >= 64
+  q, k, v, dout, lam = attn_inputs(*shape, dtype, seed=170)
+  keys = torch.arange(Tk, device=DEV)[None] % 5 != 2
+  attn_compare(ops, q, k, v, dout, lam, w=randn(dv, seed=171, mean=1.0, std=0.2), key_mask=keys)
+  attn_compare(ops, q, k, v, dout, lam, causal=True, q_start=-Tq // 2)
+
+
+def test_diff_attention_query_starts_at_the_ends_of_their_range(ops):
+  q, k, v, dout, lam = attn_inputs(4, 40, 70, 2, 1, 32, 64, BF16, seed=180)
+  top = 2 ** 31 - 1
+  starts = torch.tensor([-top - 1, top, -(1 << 30), 1 << 30], dtype=torch.int32, device=DEV)
+  lens = torch.tensor([top, 70, -top - 1, 10], dtype=torch.int32, device=DEV)
+  out, ctx = ops.diff_attn_fwd(q, k, v, lam, causal=True, q_start=starts, kv_len=lens, save=True)
+  grads = ops.diff_attn_bwd(dout, q, k, v, lam, ctx)
+  want, wctx = ops.diff_attn_fwd(q[[1, 3]], k[[1, 3]], v[[1, 3]], lam, kv_len=torch.tensor([70, 10], dtype=torch.int32, device=DEV), save=True)
+  wgrads = ops.diff_attn_bwd(dout[[1, 3]], q[[1, 3]], k[[1, 3]], v[[1, 3]], lam, wctx)
+  assert not out[[0, 2]].any() and torch.equal(out[[1, 3]], want)
+  for g, w in zip(grads[:3], wgrads):
+    assert not g[[0, 2]].any() and torch.equal(g[[1, 3]], w)
+
+
+def test_diff_attention_outputs_may_not_overlap(ops):
+  B, T, H, d = 2, 9, 2, 16
+  fused = randn(B, T, H, 8 * d, dtype=BF16, seed=190)
+  q, k, v = fused[..., :2 * d].unflatten(3, (2, d)), fused[..., 2 * d:4 * d].unflatten(3, (2, d)), fused[..., 4 * d:6 * d]
+  lam = torch.full((1,), 0.5, device=DEV)
+  want, ctx = ops.diff_attn_fwd(q, k, v, lam, save=True)
+  got, _ = ops.diff_attn_fwd(q, k, v, lam, out=fused[..., 6 * d:])  # the free quarter of the same rows
+  assert torch.equal(got, want)
+  for bad in (fused[..., 4 * d:6 * d], fused[..., 3 * d:5 * d], fused[..., 5 * d:7 * d]):
+    with pytest.raises(ValueError):
+      ops.diff_attn_fwd(q, k, v, lam, out=bad)
+  g = torch.empty_like(fused)
+  dq, dk, dv = g[..., :2 * d].unflatten(3, (2, d)), g[..., 2 * d:4 * d].unflatten(3, (2, d)), g[..., 4 * d:6 * d]
+  dout = randn(B, T, H, 2 * d, dtype=BF16, seed=191)
+  res, plain = ops.diff_attn_bwd(dout, q, k, v, lam, ctx, dq=dq, dk=dk, dv=dv), ops.diff_attn_bwd(dout, q, k, v, lam, ctx)
+  assert all(torch.equal(a, b) for a, b in zip(res[:4], plain))
+  for bad in (dict(dq=dq, dk=dq), dict(dq=q), dict(dv=v), dict(dk=dk, dv=g[..., 3 * d:5 * d]), dict(dv=dout)):
+    with pytest.raises(ValueError):
+      ops.diff_attn_bwd(dout, q, k, v, lam, ctx, **bad)
+  one = torch.zeros(3 * 32, device=DEV)
+  x = randn(2, 32)
+  _, _, nctx = ops.block_norm_fwd(x, x, post_weight=one[:32].clone(), pre_weight=one[:32].clone())
+  with pytest.raises(ValueError):
+    ops.block_norm_bwd(x, x, nctx, into=dict(post_weight=one[:32], pre_weight=one[16:48]))
+
+
+# ------------------------------------------------------------------------------------------------ the operators together
+def block_params(C, H, Hkv, d, dv, dtype, seed):
+  p = {'w_in': randn(C, H * 2 * d + Hkv * (2 * d + dv), dtype=dtype, seed=seed, std=C ** -0.5), 'w_out': randn(H * dv, C, dtype=dtype, seed=seed + 1, std=(H * dv) ** -0.5)}
+  for i, n in enumerate(('lq1', 'lk1', 'lq2', 'lk2')):
+    p[n] = randn(H, d, seed=seed + 2 + i, std=0.1)
+  for i, n in enumerate(('pre1', 'pre2', 'post2', 'scale2', 'head')):
+    p[n] = randn(dv if n == 'head' else C, seed=seed + 8 + i, std=0.1, mean=1.0)
+  return p
+
+
+def block_plain(p, x, r, gate, heads, key_mask):
+  """r joins the stream, its norm is the attention's input, the result is normalised, gated per sample and joins the stream; 64 bits."""
+  H, Hkv, d, dv = heads
+  B, T, C = x.shape
+  norm = lambda z, w, eps=1e-5: z / torch.sqrt(z.pow(2).mean(-1, keepdim=True) + eps) * w
+  y = x + r
+  z = norm(y, p['pre1']) @ p['w_in']
+  q, k, v = z[..., :H * 2 * d].view(B, T, H, 2, d), z[..., H * 2 * d:-Hkv * dv].view(B, T, Hkv, 2, d), z[..., -Hkv * dv:].view(B, T, Hkv, dv)
+  lam = torch.exp((p['lq1'] * p['lk1']).sum(1)) - torch.exp((p['lq2'] * p['lk2']).sum(1)) + 0.3
+  k, v = k.repeat_interleave(H // Hkv, 2), v.repeat_interleave(H // Hkv, 2)
+  keep = attn_visible(B, T, T, causal=True, key_mask=key_mask)[:, None]
+  P = []
+  for i in (0, 1):
+    s = (q[:, :, :, i].transpose(1, 2) @ k[:, :, :, i].transpose(1, 2).transpose(2, 3)) * d ** -0.5
+    e = torch.exp((s - s.masked_fill(~keep, -1e30).amax(-1, keepdim=True).detach()).masked_fill(~keep, -1e4))  # (hidden: zero, and no gradient)
+    P.append(e / e.sum(-1, keepdim=True).clamp_min(1e-30))
+  o = (P[0] - lam[None, :, None, None] * P[1]) @ v.transpose(1, 2)
+  a = (0.7 * norm(o, p['head'])).transpose(1, 2).reshape(B, T, H * dv) @ p['w_out']
+  y2 = y + p['scale2'] * torch.sigmoid(gate)[:, None] * norm(a, p['post2'])
+  return y2, norm(y2, p['pre2'])
+
+
+def block_own(ops, p, x, r, gate, heads, key_mask, dy, dh, clip, grads):
+  H, Hkv, d, dv = heads
+  B, T, C = x.shape
+  y, h, c1 = ops.block_norm_fwd(x, r, kind='rms', post=False, pre_weight=p['pre1'])
+  z = h.view(B * T, C) @ p['w_in']
+  view = lambda t: (t[:, :H * 2 * d].view(B, T, H, 2, d), t[:, H * 2 * d:-Hkv * dv].view(B, T, Hkv, 2, d), t[:, -Hkv * dv:].view(B, T, Hkv, dv))
+  vec = [p[n] for n in ('lq1', 'lk1', 'lq2', 'lk2')]
+  lam = ops.diff_lambda(*vec, 0.3)
+  o, ca = ops.diff_attn_fwd(*view(z), lam, causal=True, key_mask=key_mask, norm_weight=p['head'], out_scale=0.7, save=True)
+  o = o.view(B * T, H * dv)
+  a = (o @ p['w_out']).view(B, T, C)
+  y2, h2, c2 = ops.block_norm_fwd(y, a, kind='rms', post_weight=p['post2'], pre_weight=p['pre2'], scale=p['scale2'], gate=gate, gate_act=ops.ACT_SIGMOID)
+
+  for n in ('post2', 'pre2', 'scale2', 'pre1'):
+    ops.zero_(grads[n])
+  g2 = ops.block_norm_bwd(dy, dh, c2, into=dict(post_weight=grads['post2'], pre_weight=grads['pre2'], scale=grads['scale2']))
+  da = g2['a'].view(B * T, C)
+  torch.mm(o.t(), da, out=grads['w_out'])
+  do = torch.mm(da, p['w_out'].t().contiguous()).view(B, T, H, dv)
+  dz = torch.empty_like(z)
+  dq, dk, dvv = view(dz)
+  _, _, _, dlam, dhead = ops.diff_attn_bwd(do, *view(z), lam, ca, dq=dq, dk=dk, dv=dvv)
+  grads['head'].copy_(dhead)
+  for n, t in zip(('lq1', 'lk1', 'lq2', 'lk2'), ops.diff_lambda_bwd(dlam, *vec)):
+    grads[n].copy_(t)
+  torch.mm(h.view(B * T, C).t(), dz, out=grads['w_in'])
+  g1 = ops.block_norm_bwd(g2['x'], torch.mm(dz, p['w_in'].t().contiguous()).view(B, T, C), c1, into=dict(pre_weight=grads['pre1']))
+  norm = clip.clip_(0.5)
+  return dict(y=y2, h=h2, x=g1['x'], r=g1['a'], gate=g2['gate'], norm=norm, **grads)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_transformer_block_step_eager_and_captured(ops, dtype):
+  """Norms, attention, gradients and their clipping as one training step, against autograd of the plain block in 64 bits, then captured: replays equal
+  the eager step.  Tolerance, relative in the 2-norm: at most 12 roundings in the storage type lie on a path through the block and its backward (bf16:
+  12 * 2^-8), sums of at most 192 terms in fp32 at each of these 12 stages (12 * 192 * 2^-24 = 1.4e-4), times 8 for what the norms' and softmaxes'
+  derivatives amplify at rows of unit variance; roundings are independent, so bf16 is held to sqrt(12) * 8 * 2^-8 = 0.108 and fp32 to 1.1e-3."""
+  tol = 1.1e-3 if dtype == F32 else 0.108
+  B, T, C, heads = 2, 70, 96, (4, 2, 24, 48)
+  p = block_params(C, *heads, dtype, 200)
+  x, r, gate = randn(B, T, C, dtype=dtype, seed=220), randn(B, T, C, dtype=dtype, seed=221), randn(B, C, dtype=dtype, seed=222)
+  dy, dh = randn(B, T, C, dtype=dtype, seed=223), randn(B, T, C, dtype=dtype, seed=224)
+  mask = torch.ones(B, T, dtype=torch.bool, device=DEV)
+  mask[1, 50:] = False
+  mask[1, 0] = False  # the first query of this sequence sees no key
+  grads = {n: torch.zeros_like(t) for n, t in p.items()}
+  clip = ops.GradClip(list(grads.values()))
+  step = lambda: block_own(ops, p, x, r, gate, heads, mask, dy, dh, clip, grads)
+
+  def check(got):
+    leaves = {n: t.double().requires_grad_() for n, t in (*p.items(), ('x', x), ('r', r), ('gate', gate))}
+    y, h = block_plain({n: leaves[n] for n in p}, leaves['x'], leaves['r'], leaves['gate'], heads, mask)
+    want = dict(zip(leaves, torch.autograd.grad([y, h], list(leaves.values()), [dy.double(), dh.double()])), y=y.detach(), h=h.detach())
+    norm = torch.sqrt(sum(want[n].pow(2).sum() for n in p))
+    assert abs(float(got['norm']) - float(norm)) <= tol * float(norm)
+    coef = min(1.0, 0.5 / float(norm))
+    for n, w in want.items():
+      w = w * (coef if n in p else 1.0)
+      err, size = float((got[n].double() - w).norm()), float(w.norm())
+      assert err <= (2 * tol if n in p else tol) * size, (n, err / size)  # (clipped ones: the norm's error comes on top)
+
+  keep = lambda res: {n: t.clone() for n, t in res.items()}
+  check(keep(step()))
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    outs = step()
+  for i in range(3):
+    x.copy_(randn(B, T, C, dtype=dtype, seed=230 + i))
+    want = keep(step())
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    for n, t in want.items():
+      assert torch.equal(outs[n], t), n
+  check(want)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_answers_token_by_token_equal_the_whole_sequence(ops, dtype):
+  """A sequence written into a cache token by token, each through the norm and the attention over what the cache holds, equals the causal pass over the
+  whole sequence.  Both sides are within the bound of the 64-bit formula, so they are within twice that of each other."""
+  B, T, C, (H, Hkv, d, dv) = 2, 45, 64, (4, 2, 32, 64)
+  q, k, v, _, lam = attn_inputs(B, T, T, H, Hkv, d, dv, dtype, seed=240)
+  x, a, w = randn(B, T, C, dtype=dtype, seed=250), randn(B, T, C, dtype=dtype, seed=251), randn(C, seed=252)
+  whole, _ = ops.diff_attn_fwd(q, k, v, lam, causal=True, out_scale=0.65)
+  _, err = attn_oracle(q, k, v, lam, attn_visible(B, T, T, causal=True), c=0.65)['out']
+  y, h, _ = ops.block_norm_fwd(x, a, kind='rms', pre_weight=w, save=False)
+  kc, vc = torch.full((B, 64, Hkv, 2, d), math.nan, device=DEV, dtype=dtype), torch.full((B, 64, Hkv, dv), math.nan, device=DEV, dtype=dtype)
+  lens = torch.zeros(B, dtype=torch.int32, device=DEV)
+  for t in range(T):
+    kc[:, t], vc[:, t] = k[:, t], v[:, t]
+    lens += 1
+    out, _ = ops.diff_attn_fwd(q[:, t:t + 1], kc, vc, lam, kv_len=lens, out_scale=0.65)
+    within(f'token {t}', out[:, 0], whole[:, t].double(), 2 * err[:, t])
+    yt, ht, _ = ops.block_norm_fwd(x[:, t], a[:, t], kind='rms', pre_weight=w, save=False)
+    assert torch.equal(yt, y[:, t]) and torch.equal(ht, h[:, t])
+
+
+def test_trainer_clips_the_averaged_gradients(ops):
+  """Trainer(max_grad_norm): the reported norm is that of the arena, the moments are those of the clipped gradient -- eager and replayed -- and a bound
+  above the norm changes no bit of the update."""
+  from carla_garage_amd.config import GlobalConfig
+  from carla_garage_amd.graph import GraphedTrainStep
+  from carla_garage_amd.model import LidarCenterNet
+  from carla_garage_amd.trainer import Trainer
+  from oracle import tfpp_port as P
+  m = LidarCenterNet(GlobalConfig(tfpp_dtype='bf16'))
+  m.load_state_dict(P.make_state_dict(), strict=True)
+  m.cuda().train()
+  batch = {k: v.cuda() for k, v in P.make_labels(2).items()}
+  for k, v in zip(('rgb', 'lidar_bev', 'target_point', 'ego_vel', 'command'), P.make_inputs(2)):
+    batch[k] = v.cuda()
+  tr = Trainer(m, lr=1e-5, max_grad_norm=0.25)
+
+  def check(run, bound):
+    tr.max_grad_norm = bound
+    tr.apply_observed_layout()  # (the next eager step would move the arenas)
+    m0, v0 = tr.exp_avg.clone(), tr.exp_avg_sq.clone()
+    run()
+    g = tr.eng.flat_grad.double()
+    norm = g.norm()
+    within('norm', tr.grad_norm, norm, 2 * U[F32] * norm)
+    assert float(norm) > 0.25
+    c = min(1.0, bound / (float(norm) + 1e-6))
+    # three roundings of the coefficient, one of its product with g, three (five for the square) of the moment's update
+    for got, old, b, x, k in ((tr.exp_avg, m0, 0.9, c * g, 8), (tr.exp_avg_sq, v0, 0.999, (c * g) ** 2, 14)):
+      b32 = float(torch.tensor(b, dtype=F32))
+      new, mag = b32 * old.double() + (1 - b32) * x, b32 * old.double().abs() + (1 - b32) * x.abs()
+      within('moment', got, new, k * U[F32] * mag + 1e-37 + 2e-8 * x.abs())  # (1 - beta is rounded in fp32: 2^-24 absolute, squared gradients below 2^-126 vanish)
+
+  check(lambda: tr.train_step(batch), 0.25)
+  check(lambda: tr.train_step(batch), 0.25)
+  step = GraphedTrainStep(tr, batch, warmup=1)
+  for bound in (0.25, 0.01, 1e9):
+    check(step, bound)
