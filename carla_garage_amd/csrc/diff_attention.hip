@@ -388,17 +388,17 @@ __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? I
 
 // many queries: workgroup = (batch, head, 128 queries), the waves' queries differ and the images are shared by the workgroup, one tile ahead
 template <typename T, int NB> constexpr int fwd_threads() { return fwd_split<T, NB>() && sizeof(T) == 2 ? 512 : 256; }
-template <typename T, int NB> constexpr int fwd_queries() { return fwd_threads<T, NB>() / (fwd_split<T, NB>() ? 4 : 2); }
+template <typename T, int NB> constexpr int fwd_queries(int threads) { return threads / (fwd_split<T, NB>() ? 4 : 2); }
 constexpr int at_least(int a, int b) { return a > b ? a : b; }
 template <typename T, int NB> constexpr int fwd_lds() {
   return at_least(2 * key_tile<T>() * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES), fwd_threads<T, NB>() / 64 * STRIP_BYTES);
 }
 
-template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((fwd_threads<T, NB>()), (fwd_threads<T, NB>() == 512 || NB <= (sizeof(T) == 2 ? 4 : 2) ? 2 : 1)) void diff_attn_fwd_kernel(tfpp_diff_attn_params p) {
+template <typename T, int NB, bool VECTOR, int NT> __global__ __launch_bounds__(NT, (fwd_threads<T, NB>() == 512 || NB <= (sizeof(T) == 2 ? 4 : 2) ? 2 : 1)) void diff_attn_fwd_kernel(tfpp_diff_attn_params p) {
   typedef Fwd<T, NB, VECTOR, (sizeof(T) == 2 ? VECTOR || NB < 8 : NB < 5) ? Q_HELD : Q_GLOBAL, fwd_split<T, NB>() ? 1 : 2> F;  // (wide fp32 heads do not fit the registers)
   typedef typename F::ImgK ImgK;
   typedef typename F::ImgV ImgV;
-  constexpr int KT = key_tile<T>(), NT = fwd_threads<T, NB>(), MAPS = fwd_split<T, NB>() ? 1 : 2, QB = fwd_queries<T, NB>();
+  constexpr int KT = key_tile<T>(), MAPS = fwd_split<T, NB>() ? 1 : 2, QB = fwd_queries<T, NB>(NT);
   constexpr int K_BYTES = KT * ImgK::ROW_BYTES, V_BYTES = KT * ImgV::ROW_BYTES, BUF = 2 * K_BYTES + V_BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
@@ -811,6 +811,15 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_
 //    zero -- and partial sums of dw, dlambda from the unrounded one.  Bounded by HBM.
 // grid (blocks, H); lpr lanes a row (a power of two), 8 channels a lane: 16-byte loads, 64 / lpr rows a wave at a time.  partial: [1 + dv][blocks x H], the
 // sums of one value side by side.
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) { return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
+__device__ __forceinline__ float row_sum(float v, int lpr) {  // of lpr neighbouring lanes, in each of them; moves within 16 lanes cost no LDS round trip
+  if (lpr > 1) v = dpp_add<0xB1>(v);   // lane ^ 1
+  if (lpr > 2) v = dpp_add<0x4E>(v);   // lane ^ 2
+  if (lpr > 4) v = dpp_add<0x141>(v);  // mirror within 8
+  if (lpr > 8) v = dpp_add<0x140>(v);  // mirror within 16
+  if (lpr > 16) v += __shfl_xor(v, 16, 64);
+  return v;
+}
 template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_kernel(tfpp_diff_attn_params p, int lpr) {
   constexpr int E = 8;
   __shared__ float sm[E * 256 + 4];
@@ -858,10 +867,8 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
     }
     float r = 1.f, f = 0.f;
     if (p.norm) {
-      for (int x = 1; x < lpr; x <<= 1) {
-        s[0] += __shfl_xor(s[0], x, 64);
-        s[1] += __shfl_xor(s[1], x, 64);
-      }
+      s[0] = row_sum(s[0], lpr);
+      s[1] = row_sum(s[1], lpr);
       r = 1.f / sqrtf(s[0] * inv_dv + p.eps);  // (eps > 0: checked by the launcher)
       f = r * r * r * s[1] * inv_dv;
     }
@@ -876,10 +883,8 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
       t1 += dr * o1[e];
       t2 += dr * o2[e];
     }
-    for (int x = 1; x < lpr; x <<= 1) {
-      t1 += __shfl_xor(t1, x, 64);
-      t2 += __shfl_xor(t2, x, 64);
-    }
+    t1 = row_sum(t1, lpr);
+    t2 = row_sum(t2, lpr);
     if (in)
 #pragma unroll
       for (int e = 0; e < E; e += ElemTraits<T>::VEC) store_vec<T>((T*)p.d_o + row * dvs + c0 + e, d + e);
@@ -926,13 +931,15 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_k
 
 // 2. dQ.  Workgroup = (batch, head, 128 queries), wave = 32 queries, as the forward pass: S_i^T = K_i Q_i^T, dP^T = V dO^T (keys x queries),
 //    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.
-template <typename T, int NB> constexpr int dq_lds() { return at_least(2 * 32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES), 4 * STRIP_BYTES); }
+//    Wide heads: a workgroup has one map (the grid's y), dP is computed by both: 21 / 16 of the flop, and two waves fit a SIMD in place of one.
+template <typename T, int NB> constexpr int dq_maps() { return NB >= (sizeof(T) == 2 ? 5 : 4) ? 1 : 2; }
+template <typename T, int NB> constexpr int dq_lds() { return at_least(2 * 32 * (dq_maps<T, NB>() * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES), 4 * STRIP_BYTES); }
 
-template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB <= (sizeof(T) == 2 ? 4 : 2) ? 2 : 1)) void diff_attn_bwd_dq_kernel(tfpp_diff_attn_params p) {
-  constexpr int KT = 32, NT = 256, CD = (NB + 1) / 2;
+template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) void diff_attn_bwd_dq_kernel(tfpp_diff_attn_params p) {
+  constexpr int KT = 32, NT = 256, CD = (NB + 1) / 2, MAPS = dq_maps<T, NB>();
   typedef Img<T, CD> ImgK;
   typedef Img<T, NB> ImgV;
-  constexpr int K_BYTES = KT * ImgK::ROW_BYTES, V_BYTES = KT * ImgV::ROW_BYTES, BUF = 2 * K_BYTES + V_BYTES;
+  constexpr int K_BYTES = KT * ImgK::ROW_BYTES, V_BYTES = KT * ImgV::ROW_BYTES, BUF = MAPS * K_BYTES + V_BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int tiles = (p.Tq + QB - 1) / QB;
@@ -943,28 +950,29 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
   const Seq sq = sequence(p, b);
   const int w0 = tile * QB + wave * 32, qi = w0 + (lane & 31), qc = qi < p.Tq ? qi : p.Tq - 1;
   const long row = ((long)b * p.H + h) * p.Tq + qc, rows = (long)p.B * p.H * p.Tq;
-  const T* kb = (const T*)p.k + (long)b * p.k_s[0] + (long)hk * p.k_s[2];
+  const int map0 = MAPS == 1 ? (int)blockIdx.y : 0;
+  const T* kb = (const T*)p.k + (long)b * p.k_s[0] + (long)hk * p.k_s[2] + map0 * p.k_s[3];
   const T* vb = (const T*)p.v + (long)b * p.v_s[0] + (long)hk * p.v_s[2];
   constexpr bool HOLD = VECTOR ? sizeof(T) == 2 || NB < 5 : NB < 4;  // else Q and dO do not fit the registers and are read again for every tile
-  const T* qrow = (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2];
-  Frag8<T> q[2][HOLD ? NB : 1], dof[HOLD ? 2 * NB : 1];
+  const T* qrow = (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2] + map0 * p.q_s[3];
+  Frag8<T> q[MAPS][HOLD ? NB : 1], dof[HOLD ? 2 * NB : 1];
   if constexpr (HOLD)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MAPS; ++i)
 #pragma unroll
       for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][ks]);
   if constexpr (HOLD)
 #pragma unroll
     for (int ks = 0; ks < 2 * NB; ++ks) load_frag<T, true>((const T*)p.d_o + row * dvs, ks * 16 + half * 8, dvs, true, dof[ks]);
-  const float lse[2] = {p.lse[row], p.lse[rows + row]}, delta[2] = {p.delta[row], p.delta[rows + row]};
-  const float lam = p.lam[p.n_lam > 1 ? h : 0], c = p.scale * LOG2E;
+  const float lse[2] = {p.lse[map0 * rows + row], p.lse[rows + row]}, delta[2] = {p.delta[map0 * rows + row], p.delta[rows + row]};  // (one map: the first of each)
+  const float lam = p.lam[p.n_lam > 1 ? h : 0], sign = map0 ? -lam : 1.f, c = p.scale * LOG2E;
   const int last = tile * QB + QB < p.Tq ? tile * QB + QB : p.Tq;
   int end = sq.len;
   if (p.causal) end = sq.start + last < end ? sq.start + last : end;
   const int steps = end > 0 ? (end + KT - 1) / KT : 0;
-  f32x16_t dq[2][CD];
+  f32x16_t dq[MAPS][CD];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < MAPS; ++i)
 #pragma unroll
     for (int n = 0; n < CD; ++n)
 #pragma unroll
@@ -974,8 +982,8 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
     const long j0 = (long)step * KT;
     const Rows have = {sq.len - step * KT, p.key_mask != nullptr, bits};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, have, tid);
-    ImgV::template fill<KT, VECTOR, NT>(buf + 2 * K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, have, tid);
+    for (int i = 0; i < MAPS; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, have, tid);
+    ImgV::template fill<KT, VECTOR, NT>(buf + MAPS * K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, have, tid);
   };
   unsigned long long bits = 0;
   if (steps > 0) {
@@ -998,12 +1006,16 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
     // them at every step; such a tile is masked to zeros)
     const bool masked = cur != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
     const unsigned vis = (unsigned)(p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur) >> (4 * half);
-    const int vr = v_rows + 2 * K_BYTES;
-    f32x16_t sc[2], dp;
+    const int vr = v_rows + MAPS * K_BYTES;
+    f32x16_t sc[MAPS], dp;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sc[0][r] = sc[1][r] = dp[r] = 0.f;
+    for (int r = 0; r < 16; ++r) {
+      dp[r] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < MAPS; ++i) sc[i][r] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i)
 #pragma unroll
       for (int ks = 0; ks < NB; ++ks) {
         Frag8<T> a;
@@ -1020,17 +1032,16 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      float p0 = __builtin_amdgcn_exp2f(fmaf(sc[0][r], c, -lse[0])), p1 = __builtin_amdgcn_exp2f(fmaf(sc[1][r], c, -lse[1]));
-      if (masked) {
-        const bool keep = (vis >> (8 * (r >> 2) + (r & 3))) & 1u;
-        p0 = keep ? p0 : 0.f;
-        p1 = keep ? p1 : 0.f;
+      const bool keep = !masked || ((vis >> (8 * (r >> 2) + (r & 3))) & 1u);
+#pragma unroll
+      for (int i = 0; i < MAPS; ++i) {
+        float pr = __builtin_amdgcn_exp2f(fmaf(sc[i][r], c, -lse[i]));
+        if (masked) pr = keep ? pr : 0.f;
+        sc[i][r] = pr * (dp[r] - delta[i]) * (MAPS == 1 ? sign : (i ? -lam : 1.f));
       }
-      sc[0][r] = p0 * (dp[r] - delta[0]);
-      sc[1][r] = p1 * (dp[r] - delta[1]) * -lam;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MAPS; ++i)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         Frag8<T> ds;
@@ -1047,8 +1058,8 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (NB
   __syncthreads();  // every wave is past its last image
   float* strip = reinterpret_cast<float*>(smem + wave * STRIP_BYTES);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    T* out = (T*)p.dq_out + (long)b * p.dq_s[0] + (long)w0 * p.dq_s[1] + (long)h * p.dq_s[2] + (long)i * p.dq_s[3];
+  for (int i = 0; i < MAPS; ++i) {
+    T* out = (T*)p.dq_out + (long)b * p.dq_s[0] + (long)w0 * p.dq_s[1] + (long)h * p.dq_s[2] + (long)(map0 + i) * p.dq_s[3];
     store_rows<T>(strip, lane, dq[i], p.scale, p.d, p.dq_vec, Weights{nullptr, 0}, [&](int r) { return w0 + r < p.Tq ? out + (long)r * p.dq_s[1] : nullptr; });
   }
 }
@@ -1065,7 +1076,7 @@ template <typename T, int NB> constexpr bool dkv_v_in_lds() { return sizeof(T) =
 template <typename T, int NB> constexpr int dkv_images() { return 2 * (32 * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + 1024); }
 template <typename T, int NB> constexpr int dkv_lds() { return at_least(dkv_images<T, NB>() + (dkv_v_in_lds<T, NB>() ? QB * Img<T, NB>::ROW_BYTES + 4 * 2 * 64 * 16 : 0), 4 * STRIP_BYTES); }
 
-template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds__(256, (PART == PART_ALL ? NB <= (sizeof(T) == 2 ? 4 : 1) : NB <= (sizeof(T) == 2 ? 5 : 4)) ? 2 : 1) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
+template <typename T, int NB, bool VECTOR, int PART> __device__ __forceinline__ void bwd_dkv(const tfpp_diff_attn_params& p, int y) {
   constexpr int QT = 32, NT = 256, MAPS = PART == PART_DK ? 1 : 2, CD = (NB + 1) / 2;
   typedef Img<T, CD> ImgQ;
   typedef Img<T, NB> ImgO;
@@ -1075,7 +1086,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
   const int tiles = (p.Tk + QB - 1) / QB, group = p.H / p.Hkv;
   int bh, tile;
   place(p.B * p.Hkv, tiles, p.causal, bh, tile);
-  const int part = PART == PART_DK ? (int)blockIdx.y >> 1 : (int)blockIdx.y;  // of the queries
+  const int part = PART == PART_DK ? y >> 1 : y;  // of the queries
   const int b = bh / p.Hkv, hk = bh % p.Hkv, dvs = (p.dv + 7) & ~7;
   const Seq sq = sequence(p, b);
   const int w0 = tile * QB + wave * 32, kj = w0 + (lane & 31);
@@ -1084,7 +1095,7 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
   const int kc = kj < p.Tk ? kj : p.Tk - 1;
   constexpr bool V_LDS = dkv_v_in_lds<T, NB>() && PART == PART_ALL, HOLD = sizeof(T) == 2 || NB < 4, WANT_DK = PART != PART_DV, WANT_DV = PART != PART_DK;
   constexpr bool FENCE = V_LDS;  // (operands loaded far ahead of their products would not fit the registers)
-  const int map0 = PART == PART_DK ? (int)blockIdx.y & 1 : 0;  // wide fp32 heads do not fit the registers: K and V are read again for every tile
+  const int map0 = PART == PART_DK ? y & 1 : 0;  // wide fp32 heads do not fit the registers: K and V are read again for every tile
   const T* krow = (const T*)p.k + (long)b * p.k_s[0] + (long)kc * p.k_s[1] + (long)hk * p.k_s[2];
   const T* vrow = (const T*)p.v + (long)b * p.v_s[0] + (long)kc * p.v_s[1] + (long)hk * p.v_s[2];
   constexpr int K_HELD = V_LDS ? NB - 1 : NB;
@@ -1323,6 +1334,16 @@ template <typename T, int NB, bool VECTOR, int PART> __global__ __launch_bounds_
     }
 }
 
+template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (dkv_split<T, NB, VECTOR>() ? NB <= (sizeof(T) == 2 ? 5 : 4) : NB <= (sizeof(T) == 2 ? 4 : 1)) ? 2 : 1) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
+  if constexpr (dkv_split<T, NB, VECTOR>()) {
+    const int y = blockIdx.y, n = 2 * p.dkv_splits;  // both maps' dK, the longer ones, start first
+    if (y < n) bwd_dkv<T, NB, VECTOR, PART_DK>(p, y);
+    else bwd_dkv<T, NB, VECTOR, PART_DV>(p, y - n);
+  } else {
+    bwd_dkv<T, NB, VECTOR, PART_ALL>(p, blockIdx.y);
+  }
+}
+
 // dK, dV of one key: the parts' sums in order; one wave a (batch, key, head), 4 channels a lane
 template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_join_kernel(tfpp_diff_attn_params p, int kc, int vc) {
   const long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6), all = (long)p.B * p.Hkv * p.Tk;
@@ -1433,21 +1454,20 @@ template <typename T, int NB, bool VECTOR> int launch(const tfpp_diff_attn_param
     TFPP_CHECK_LAUNCH();
     return 0;
   }
-  const int qb = step == STEP_FWD ? fwd_queries<T, NB>() : QB;
-  const long tiles = ((step == STEP_DKV ? p.Tk : p.Tq) + qb - 1) / qb, n = tiles * p.B * (step == STEP_DKV ? p.Hkv : p.H);
-  if (n > 0x7fffffffl) return TFPP_EINVAL;
-  const dim3 grid((unsigned)n);
-  if (step == STEP_FWD) return start(diff_attn_fwd_kernel<T, NB, VECTOR>, grid, fwd_threads<T, NB>(), fwd_lds<T, NB>(), &done[0], p, st);
-  if (step == STEP_DQ) return start(diff_attn_bwd_dq_kernel<T, NB, VECTOR>, grid, 256, dq_lds<T, NB>(), &done[1], p, st);
-  if constexpr (dkv_split<T, NB, VECTOR>()) {
-    const int rc = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DK>, dim3((unsigned)n, 2 * p.dkv_splits), 256, dkv_lds<T, NB>(), &done[2], p, st);
-    if (rc) return rc;
-    const int rv = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_DV>, dim3((unsigned)n, p.dkv_splits), 256, dkv_lds<T, NB>(), &done[3], p, st);
-    if (rv) return rv;
-  } else {
-    const int rc = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR, PART_ALL>, dim3((unsigned)n, p.dkv_splits), 256, dkv_lds<T, NB>(), &done[2], p, st);
-    if (rc) return rc;
+  if (step == STEP_FWD) {
+    // half the queries a workgroup where whole ones would leave CUs without any
+    constexpr int FULL = fwd_threads<T, NB>(), MOST = fwd_queries<T, NB>(FULL);
+    auto groups = [&](int queries) { return (long)p.B * p.H * ((p.Tq + queries - 1) / queries); };
+    if (groups(MOST) > 0x7fffffffl) return TFPP_EINVAL;
+    if constexpr (VECTOR)
+      if (groups(MOST) < 256) return start(diff_attn_fwd_kernel<T, NB, true, FULL / 2>, dim3((unsigned)groups(MOST / 2)), FULL / 2, fwd_lds<T, NB>(), &done[3], p, st);
+    return start(diff_attn_fwd_kernel<T, NB, VECTOR, FULL>, dim3((unsigned)groups(MOST)), FULL, fwd_lds<T, NB>(), &done[0], p, st);
   }
+  const long n = (long)(((step == STEP_DQ ? p.Tq : p.Tk) + QB - 1) / QB) * p.B * (step == STEP_DQ ? p.H : p.Hkv);
+  if (n > 0x7fffffffl) return TFPP_EINVAL;
+  if (step == STEP_DQ) return start(diff_attn_bwd_dq_kernel<T, NB, VECTOR>, dim3((unsigned)n, 3 - dq_maps<T, NB>()), 256, dq_lds<T, NB>(), &done[1], p, st);
+  const int rc = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR>, dim3((unsigned)n, (dkv_split<T, NB, VECTOR>() ? 3 : 1) * p.dkv_splits), 256, dkv_lds<T, NB>(), &done[2], p, st);
+  if (rc) return rc;
   if (p.dkv_splits > 1) {
     hipLaunchKernelGGL(diff_attn_bwd_join_kernel<T>, dim3((unsigned)(((long)p.B * p.Hkv * p.Tk + 3) / 4)), dim3(256), 0, st, p, (NB + 1) / 2 * 32, NB * 32);
     TFPP_CHECK_LAUNCH();
@@ -1493,9 +1513,9 @@ int row_lanes(const tfpp_diff_attn_params& p) {
   while (n * 8 < p.dv) n <<= 1;
   return n;
 }
-int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass for each head: four rounds of 256 / row_lanes rows, about 4096 in all at most
+int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass for each head: two rounds of 256 / row_lanes rows, about 4096 in all at most
   const long rows = (long)p.B * p.Tq, round = 256 / row_lanes(p);
-  long n = (rows + 4 * round - 1) / (4 * round), most = 4096 / p.H > 1 ? 4096 / p.H : 1;
+  long n = (rows + 2 * round - 1) / (2 * round), most = 4096 / p.H > 1 ? 4096 / p.H : 1;
   if (n > most) n = most;
   return (int)n;
 }
