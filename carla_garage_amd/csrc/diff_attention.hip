@@ -271,7 +271,7 @@ template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32
 // O_i^T += V^T P_i^T: both maps share every V operand.  O_1 and O_2 are kept apart to the end because their sums are not known before; one pass,
 // 4 d + 4 dv flop a pair.  Wide heads (split): O_1 and O_2 of 32 queries do not fit one wave's registers, so two waves share the queries, one map
 // each, and meet in LDS at the end.
-template <typename T, int NB> constexpr bool fwd_split() { return NB >= 5; }
+template <typename T, int NB> constexpr bool fwd_split() { return NB >= (sizeof(T) == 2 ? 5 : 4); }
 
 enum { Q_HELD, Q_GLOBAL, Q_LDS };  // where a wave's queries are: registers, or read again for every tile
 template <typename T, int NB, bool VECTOR, int Q, int MAPS> struct Fwd {
@@ -394,7 +394,7 @@ template <typename T, int NB> constexpr int fwd_lds() {
   return at_least(2 * key_tile<T>() * (2 * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES), fwd_threads<T, NB>() / 64 * STRIP_BYTES);
 }
 
-template <typename T, int NB, bool VECTOR, int NT> __global__ __launch_bounds__(NT, (fwd_threads<T, NB>() == 512 || NB <= (sizeof(T) == 2 ? 4 : 2) ? 2 : 1)) void diff_attn_fwd_kernel(tfpp_diff_attn_params p) {
+template <typename T, int NB, bool VECTOR, int NT> __global__ __launch_bounds__(NT, 2) void diff_attn_fwd_kernel(tfpp_diff_attn_params p) {
   typedef Fwd<T, NB, VECTOR, (sizeof(T) == 2 ? VECTOR || NB < 8 : NB < 5) ? Q_HELD : Q_GLOBAL, fwd_split<T, NB>() ? 1 : 2> F;  // (wide fp32 heads do not fit the registers)
   typedef typename F::ImgK ImgK;
   typedef typename F::ImgV ImgV;
@@ -530,7 +530,7 @@ template <typename T, int NB> struct Few {
   static constexpr int ROW_FLOATS = 2 * (NB * 32 + 2);     // of one row in `partial`: both maps' sums, maxima, l
 };
 
-template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, NB>::THREADS), (sizeof(T) == 2 || NB <= 2 ? 2 : 1)) void diff_attn_few_kernel(tfpp_diff_attn_params p) {
+template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, NB>::THREADS), (sizeof(T) == 2 || NB <= 2 || NB == 5 ? 2 : 1)) void diff_attn_few_kernel(tfpp_diff_attn_params p) {
   typedef Few<T, NB> W;
   typedef Fwd<T, NB, VECTOR, Q_LDS, W::MAPS> F;
   typedef typename F::ImgK ImgK;
@@ -1334,7 +1334,7 @@ template <typename T, int NB, bool VECTOR, int PART> __device__ __forceinline__ 
     }
 }
 
-template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (dkv_split<T, NB, VECTOR>() ? NB <= (sizeof(T) == 2 ? 5 : 4) : NB <= (sizeof(T) == 2 ? 4 : 1)) ? 2 : 1) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
+template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (sizeof(T) == 4 || NB <= 5 ? 2 : 1)) void diff_attn_bwd_dkv_kernel(tfpp_diff_attn_params p) {
   if constexpr (dkv_split<T, NB, VECTOR>()) {
     const int y = blockIdx.y, n = 2 * p.dkv_splits;  // both maps' dK, the longer ones, start first
     if (y < n) bwd_dkv<T, NB, VECTOR, PART_DK>(p, y);
