@@ -234,8 +234,8 @@ __device__ __forceinline__ void place(int heads, int tiles, bool by_tile, int& b
 }
 
 // Fill the next images while the present ones are read.  The two are different memory, and the compiler has to be told: it puts a wait for ALL loads
-// into LDS that are under way in front of an LDS read that may alias them, which would undo the prefetch (measured: 5.7 -> see the forward kernel's
-// comment).  The noalias arguments become scopes on both sides when this is inlined.  The wait that IS needed stands at the top of each step.
+// into LDS that are under way in front of an LDS read that may alias them, which would undo the prefetch.
+// The noalias arguments become scopes on both sides when this is inlined.  The wait that IS needed stands at the top of each step.
 template <typename Fill, typename Use> __device__ __forceinline__ void overlap(unsigned char* __restrict__ next, const unsigned char* __restrict__ now, Fill fill, Use use) {
   fill(next);
   use(now);
@@ -269,7 +269,10 @@ template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32
 // ---------------------------------------------------------------------------------------------------------------------------------
 // forward.  A wave has 32 queries, lane l and l + 32 = one query.  S_i^T = K_i Q_i^T (keys x queries), running maximum and sum per query,
 // O_i^T += V^T P_i^T: both maps share every V operand.  O_1 and O_2 are kept apart to the end because their sums are not known before; one pass,
-// 4 d + 4 dv flop a pair.  Wide heads (split): O_1 and O_2 of 32 queries do not fit one wave's registers, so two waves share the queries, one map
+// 4 d + 4 dv flop a pair.  Long sequences are bounded by the matrix unit and what stands between its products (the exponentials, the LDS reads of
+// operands), short ones by the latency of that chain in a single wave.  8100 causal tokens, 8 heads of 128 / 256: 410 us, 655 TFLOP/s (a product of
+// 8192^3 by the library: 1189); 2 x 4096 causal, 16 heads of 64 / 128: 255 us; 12 x 320, 4 heads of 72 / 144: 25 us, 10 of them launch, first loads
+// and epilogue.  Wide heads (split): O_1 and O_2 of 32 queries do not fit one wave's registers, so two waves share the queries, one map
 // each, and meet in LDS at the end.
 template <typename T, int NB> constexpr bool fwd_split() { return NB >= (sizeof(T) == 2 ? 5 : 4); }
 
@@ -516,7 +519,9 @@ template <typename T, int NB, bool VECTOR, int NT> __global__ __launch_bounds__(
 // few queries (single tokens against a cache, short sequences): workgroup = (batch, key / value head, 32 rows, split of the keys), a row being a
 // (query head of the group, query) pair, so that one read of the cache serves all heads that share it.  The WAVES take different keys, 32 at a time, from
 // images of their own (no barrier in the loop), and add up in LDS.  With more than one split the sums go to `partial` and
-// diff_attn_fwd_join_kernel finishes the rows: otherwise a cache would be read by as many CUs as there are heads.
+// diff_attn_fwd_join_kernel finishes the rows: otherwise a cache would be read by as many CUs as there are heads.  Bounded by HBM where the cache is
+// long: 16 sequences of 4096 to 16384 tokens, 4 heads of 64 / 128 shared by 16: 318 MB in 68 us (4.7 TB/s; a copy reaches 5.1) and 5 us for the join;
+// by latency where it is short: 320 tokens, 17 us.
 template <typename T, int NB> struct Few {
   static constexpr int MAPS = NB >= 5 ? 1 : 2;
   static constexpr int KEY_WAVES = MAPS == 2 ? 4 : (sizeof(T) == 2 ? 2 : 1), WAVES = KEY_WAVES * (3 - MAPS), THREADS = WAVES * 64;
@@ -808,7 +813,7 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_
 //   dP = dO V^T      delta_i = dO . O_i      dS_1 = P_1 (dP - delta_1)      dS_2 = -lambda P_2 (dP - delta_2)
 //   dQ_i = scale dS_i K_i      dK_i = scale dS_i^T Q_i      dV = (P_1 - lambda P_2)^T dO
 // 1. diff_attn_bwd_rows_kernel: dO (rounded once: it is an MFMA operand twice), delta_i from that rounded dO -- so that the rows of dS still sum to
-//    zero -- and partial sums of dw, dlambda from the unrounded one.  Bounded by HBM.
+//    zero -- and partial sums of dw, dlambda from the unrounded one.  Bounded by HBM: 131072 rows of 128, 134 MB in 36 us (3.7 TB/s).
 // grid (blocks, H); lpr lanes a row (a power of two), 8 channels a lane: 16-byte loads, 64 / lpr rows a wave at a time.  partial: [1 + dv][blocks x H], the
 // sums of one value side by side.
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) { return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
@@ -930,8 +935,10 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_k
 }
 
 // 2. dQ.  Workgroup = (batch, head, 128 queries), wave = 32 queries, as the forward pass: S_i^T = K_i Q_i^T, dP^T = V dO^T (keys x queries),
-//    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.
-//    Wide heads: a workgroup has one map (the grid's y), dP is computed by both: 21 / 16 of the flop, and two waves fit a SIMD in place of one.
+//    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.  2 x 4096 causal, 16 heads of 64 / 128: 270 us; 12 x 320, 4 heads
+//    of 72 / 144: 24 us.
+//    Wide heads: a workgroup has one map (the grid's y), dP is computed by both: 21 / 16 of the flop, and two waves fit a SIMD in place of one
+//    (12 x 320 queries over 1280 keys: 68 us, 82 us with both maps in a wave).
 template <typename T, int NB> constexpr int dq_maps() { return NB >= (sizeof(T) == 2 ? 5 : 4) ? 1 : 2; }
 template <typename T, int NB> constexpr int dq_lds() { return at_least(2 * 32 * (dq_maps<T, NB>() * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES), 4 * STRIP_BYTES); }
 
@@ -1067,7 +1074,8 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
 // 3. dK, dV.  Workgroup = (batch, key / value head, 128 keys), wave = 32 keys, lane l and l + 32 = one key: S_i = Q_i K_i^T and dP = dO V^T
 //    (queries x keys), dV^T += dO^T (P_1 - lambda P_2), dK_i^T += Q_i^T dS_i, over all queries of all heads that share the key / value head.
 //    Wide heads: the accumulators of all three do not fit one wave's registers, so dK_1, dK_2 (PART_DK, the map in the grid's y) and dV (PART_DV) are
-//    separate workgroups; S and dP are computed again (3 / 2 of the flop).
+//    separate workgroups of one launch; S and dP are computed again (3 / 2 of the flop).  Bounded by the matrix unit and the registers: 2 x 4096 causal, 4
+//    heads of 64 / 128 shared by 16: 460 us and 23 us for the join; 12 x 320, 4 heads of 72 / 144: 26 us (39 us as two launches).
 enum { PART_ALL, PART_DK, PART_DV };
 template <typename T, int NB, bool VECTOR> constexpr bool dkv_split() { return NB >= (sizeof(T) == 2 && VECTOR ? 5 : 4); }
 // d = 33 .. 64, bf16: the 128 keys' V and the last 16 channels of their K stay in LDS instead of 40 registers, which lets two waves share a SIMD (256
@@ -1455,7 +1463,7 @@ template <typename T, int NB, bool VECTOR> int launch(const tfpp_diff_attn_param
     return 0;
   }
   if (step == STEP_FWD) {
-    // half the queries a workgroup where whole ones would leave CUs without any
+    // half the queries a workgroup where whole ones would leave CUs without any (144 or 240 workgroups: 27 or 25 us)
     constexpr int FULL = fwd_threads<T, NB>(), MOST = fwd_queries<T, NB>(FULL);
     auto groups = [&](int queries) { return (long)p.B * p.H * ((p.Tq + queries - 1) / queries); };
     if (groups(MOST) > 0x7fffffffl) return TFPP_EINVAL;
