@@ -402,7 +402,7 @@ bool aligned16(const tfpp_block_norm_params& p, int vec) {
 }
 
 bool valid(const tfpp_block_norm_params& p, int dtype) {
-  return (dtype == TFPP_F32 || dtype == TFPP_BF16) && p.C >= 1 && p.C <= 4096 && p.B >= 1 && p.T >= 1 && p.x && p.a && p.gate_mode >= 0 && p.gate_mode <= 2 &&
+  return (dtype == TFPP_F32 || dtype == TFPP_BF16) && p.C >= 1 && p.C <= 4096 && p.B >= 1 && p.T >= 1 && (long)p.B * p.T < (1l << 30) && p.x && p.a && p.gate_mode >= 0 && p.gate_mode <= 2 &&
          (!p.gate_mode || p.gate) && (p.gate_act == ACT_NONE || p.gate_act == ACT_SIGMOID || p.gate_act == ACT_TANH);
 }
 
@@ -434,7 +434,6 @@ template <typename T> void dispatch(const tfpp_block_norm_params& p, bool bwd, i
 
 extern "C" int tfpp_block_norm_fwd(const tfpp_block_norm_params* p, int dtype, void* stream) {
   if (!p || !valid(*p, dtype) || !p->y || (p->pre && !p->h)) return TFPP_EINVAL;
-  if ((long)p->B * p->T > 0x7fffffffL) return TFPP_EINVAL;  // one workgroup holds at least one row: the grid's x limit
   if (dtype == TFPP_F32) dispatch<float>(*p, false, 0, (hipStream_t)stream);
   else dispatch<bf16_t>(*p, false, 0, (hipStream_t)stream);
   TFPP_CHECK_LAUNCH();

@@ -827,7 +827,7 @@ __device__ __forceinline__ float row_sum(float v, int lpr) {  // of lpr neighbou
 }
 template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_kernel(tfpp_diff_attn_params p, int lpr) {
   constexpr int E = 8;
-  __shared__ float sm[E * 256 + 4];
+  __shared__ float sm[4 * 256 + 4];  // of each wave: the columns' sums; dlambda
   const int h = blockIdx.y, lane = threadIdx.x & 63, c0 = (lane & (lpr - 1)) * E, dvs = (p.dv + 7) & ~7;
   const int rpw = 64 / lpr, slots = (int)gridDim.x * 4 * rpw;
   const long rows = (long)p.B * p.Tq;
@@ -898,18 +898,19 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
       p.delta[(long)p.B * p.H * p.Tq + row] = t2;
     }
   }
+  for (int x = lpr; x < 64; x <<= 1)  // the wave's rows
 #pragma unroll
-  for (int e = 0; e < E; ++e) sm[e * 256 + threadIdx.x] = dw[e];
+    for (int e = 0; e < E; ++e) dw[e] += __shfl_xor(dw[e], x, 64);
+  if (lane < lpr)
+#pragma unroll
+    for (int e = 0; e < E; ++e) sm[((int)threadIdx.x >> 6) * 256 + c0 + e] = dw[e];
   dl = wave_sum(dl);
-  if (lane == 0) sm[E * 256 + (threadIdx.x >> 6)] = dl;
+  if (lane == 0) sm[4 * 256 + (threadIdx.x >> 6)] = dl;
   __syncthreads();
   const long pitch = (long)gridDim.x * p.H, at = (long)blockIdx.x * p.H + h;
-  if (threadIdx.x == 0) p.partial[at] = (sm[E * 256] + sm[E * 256 + 1]) + (sm[E * 256 + 2] + sm[E * 256 + 3]);
-  for (int c = threadIdx.x; c < p.dv; c += 256) {
-    float a = 0.f;
-    for (int i = c / E; i < 256; i += lpr) a += sm[(c % E) * 256 + i];
-    p.partial[(1 + c) * pitch + at] = a;
-  }
+  if (threadIdx.x == 0) p.partial[at] = (sm[1024] + sm[1025]) + (sm[1026] + sm[1027]);
+  const int c = threadIdx.x;
+  if (c < p.dv) p.partial[(1 + c) * pitch + at] = (sm[c] + sm[256 + c]) + (sm[512 + c] + sm[768 + c]);
 }
 
 // dlambda (blocks 0 .. n_lam - 1) and dw (the blocks behind): one value per workgroup, fixed order

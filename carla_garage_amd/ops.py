@@ -1467,7 +1467,7 @@ def block_norm_fwd(x, a, *, kind='layer', post=True, pre=True, post_weight=None,
         ctx.mode, B, T = 2, 1, rows
     else:
       raise ValueError(f'gate has shape {tuple(gate.shape)}, expected {tuple(x.shape)} or {(x.shape[0], C)}')
-  if rows > 0x7fffffff or (ctx.mode == 1 and B > 65530):
+  if rows >= 1 << 30 or (ctx.mode == 1 and B > 65530):
     raise ValueError(f'block_norm_fwd: too many rows ({rows}) or samples ({B})')
   ctx.x, ctx.a, ctx.gate, ctx.lds, ctx.shape = x, a, gate, (ld_x, ld_a, ld_g), (B, T, C)
   ctx.opt = (int(kind == 'layer'), int(post), int(pre), gate_act, float(alpha), float(eps))
