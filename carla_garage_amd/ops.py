@@ -1671,7 +1671,8 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
   hold anything; the other values have to be finite, the scaled scores below 1e30.  A query that sees no key gives zeros.
   New tokens against a cache: q [B, 1, ...], k and v the whole cache, kv_len the tokens it holds (the new ones among them); for several new tokens
   causal=True and q_start = kv_len - Tq.
-  save=True keeps what diff_attn_bwd needs.  ``out``: written in place of a new tensor, any strides that do not overlap."""
+  save=True keeps what diff_attn_bwd needs.  ``out``: written in place of a new tensor, any strides that do not overlap, no memory shared
+  with q, k or v (slices of one buffer that do not meet are fine)."""
   dev, qs, ks, vs, shape = _diff_attn_check(q, k, v, lam)
   B, Tq, Tk, H, Hkv, d, dv = shape
   if norm_weight is not None and (norm_weight.dtype not in (torch.float32, torch.bfloat16) or norm_weight.numel() != dv or not norm_weight.is_contiguous() or
@@ -1732,7 +1733,7 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
 
 def diff_attn_bwd(dout, q, k, v, lam, ctx, dq=None, dk=None, dv=None):
   """(dq, dk, dv, dlam, dnorm_weight) of diff_attn_fwd(q, k, v, lam, ..., save=True); kv_len, q_start and key_mask may not change in between.
-  dq / dk / dv: tensors (views of a fused gradient, any strides that do not overlap) to be written in place of new ones.  dlam has lam's shape (summed over
+  dq / dk / dv: tensors (views of a fused gradient, any strides; no memory shared with another argument) to be written in place of new ones.  dlam has lam's shape (summed over
   the heads when lam is one value), dnorm_weight the weight's type, None without one.  Nothing is added atomically: bit-reproducible."""
   dev, qs, ks, vs, shape = _diff_attn_check(q, k, v, lam)
   if ctx.shape != shape or ctx.opt[-1] != q.dtype or ctx.saved.device != dev:
