@@ -914,7 +914,7 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
 }
 
 // dlambda (blocks 0 .. n_lam - 1) and dw (the blocks behind): one value per workgroup, fixed order
-template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_kernel(tfpp_diff_attn_params p, int blocks) {
+template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_kernel(tfpp_diff_attn_params p, int blocks, const float* rest, int rest_rows) {
   __shared__ float sm[4];
   const int x = blockIdx.x, n = blocks * p.H;
   const bool is_lam = x < p.n_lam;
@@ -925,6 +925,10 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_k
     for (int i = threadIdx.x; i < blocks; i += 256) s += src[(long)i * p.H + x];
   else
     for (int i = threadIdx.x; i < n; i += 256) s += src[i];
+  if (is_lam && p.n_lam > 1)
+    for (int i = threadIdx.x; i < rest_rows; i += 256) s -= rest[(long)i * p.H + x];
+  else if (is_lam)
+    for (long i = threadIdx.x; i < (long)rest_rows * p.H; i += 256) s -= rest[i];
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
   __syncthreads();
@@ -938,10 +942,14 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_k
 // 2. dQ.  Workgroup = (batch, head, 128 queries), wave = 32 queries, as the forward pass: S_i^T = K_i Q_i^T, dP^T = V dO^T (keys x queries),
 //    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.  2 x 4096 causal, 16 heads of 64 / 128: 270 us; 12 x 320, 4 heads
 //    of 72 / 144: 24 us.
+//    The row pass's dlambda has the rounding of O_2 (its own and that of the probabilities it was made of) in it, up to a percent where the heads are few
+//    and the sum is small.  sum_j P_2 (dP - delta_2) is what that rounding made of delta_2: with P_2 and dP at hand in 32 bits it is added here.
 //    Wide heads: a workgroup has one map (the grid's y), dP is computed by both: 21 / 16 of the flop, and two waves fit a SIMD in place of one
 //    (12 x 320 queries over 1280 keys: 68 us, 82 us with both maps in a wave).
 template <typename T, int NB> constexpr int dq_maps() { return NB >= (sizeof(T) == 2 ? 5 : 4) ? 1 : 2; }
-template <typename T, int NB> constexpr int dq_lds() { return at_least(2 * 32 * (dq_maps<T, NB>() * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES), 4 * STRIP_BYTES); }
+// bf16 heads of 81 .. 128: the last 16 channels of a wave's queries stay in LDS, which spares the registers that would go to scratch
+template <typename T, int NB> constexpr bool dq_stash() { return sizeof(T) == 2 && NB == 8; }
+template <typename T, int NB> constexpr int dq_lds() { return at_least(2 * 32 * (dq_maps<T, NB>() * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + (dq_stash<T, NB>() ? 256 * 16 : 0), 4 * STRIP_BYTES); }
 
 template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) void diff_attn_bwd_dq_kernel(tfpp_diff_attn_params p) {
   constexpr int KT = 32, NT = 256, CD = (NB + 1) / 2, MAPS = dq_maps<T, NB>();
@@ -963,17 +971,26 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
   const T* vb = (const T*)p.v + (long)b * p.v_s[0] + (long)hk * p.v_s[2];
   constexpr bool HOLD = VECTOR ? sizeof(T) == 2 || NB < 5 : NB < 4;  // else Q and dO do not fit the registers and are read again for every tile
   const T* qrow = (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2] + map0 * p.q_s[3];
-  Frag8<T> q[MAPS][HOLD ? NB : 1], dof[HOLD ? 2 * NB : 1];
+  constexpr bool STASH = dq_stash<T, NB>() && HOLD;
+  constexpr int HELD = STASH ? NB - 1 : NB;
+  uint4* stash = reinterpret_cast<uint4*>(smem + 2 * BUF) + tid;  // (a lane's own operand)
+  Frag8<T> q[MAPS][HOLD ? HELD : 1], dof[HOLD ? 2 * NB : 1];
   if constexpr (HOLD)
 #pragma unroll
     for (int i = 0; i < MAPS; ++i)
 #pragma unroll
-      for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][ks]);
+      for (int ks = 0; ks < HELD; ++ks) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][ks]);
+  if constexpr (STASH) {
+    Frag8<T> last;
+    load_frag<T, VECTOR>(qrow, HELD * 16 + half * 8, p.d, true, last);
+    *stash = last.v;
+  }
   if constexpr (HOLD)
 #pragma unroll
     for (int ks = 0; ks < 2 * NB; ++ks) load_frag<T, true>((const T*)p.d_o + row * dvs, ks * 16 + half * 8, dvs, true, dof[ks]);
-  const float lse[2] = {p.lse[map0 * rows + row], p.lse[rows + row]}, delta[2] = {p.delta[map0 * rows + row], p.delta[rows + row]};  // (one map: the first of each)
-  const float lam = p.lam[p.n_lam > 1 ? h : 0], sign = map0 ? -lam : 1.f, c = p.scale * LOG2E;
+  const bool exists = qi < p.Tq;  // (the lanes behind the last query: P = 0)
+  const float lse[2] = {exists ? p.lse[map0 * rows + row] : INFINITY, exists ? p.lse[rows + row] : INFINITY}, delta[2] = {p.delta[map0 * rows + row], p.delta[rows + row]};  // (one map: the first of each)
+  const float lam = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(p.lam[p.n_lam > 1 ? h : 0]))), sign = map0 ? -lam : 1.f, c = p.scale * LOG2E;
   const int last = tile * QB + QB < p.Tq ? tile * QB + QB : p.Tq;
   int end = sq.len;
   if (p.causal) end = sq.start + last < end ? sq.start + last : end;
@@ -985,6 +1002,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
     for (int n = 0; n < CD; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[i][n][r] = 0.f;
+  float rest = 0.f;  // of the last map: sum of P_2 (dP - delta_2)
   const int k_rows = ImgK::rows_at(lane), v_rows = ImgV::rows_at(lane), k_cols = ImgK::cols_at(lane);
   auto fill = [&](unsigned char* buf, int step, unsigned long long bits) {
     const long j0 = (long)step * KT;
@@ -1029,7 +1047,13 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
         Frag8<T> a;
         ImgK::rows(now + i * K_BYTES, k_rows, ks, a);
         if constexpr (!HOLD) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][0]);
-        mma(a, q[i][HOLD ? ks : 0], sc[i]);
+        if constexpr (STASH) {
+          Frag8<T> last;
+          if (ks == HELD) last.v = *stash;
+          mma(a, ks == HELD ? last : q[i][ks < HELD ? ks : 0], sc[i]);
+        } else {
+          mma(a, q[i][HOLD ? ks : 0], sc[i]);
+        }
       }
 #pragma unroll
     for (int ks = 0; ks < 2 * NB; ++ks) {
@@ -1045,7 +1069,9 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
       for (int i = 0; i < MAPS; ++i) {
         float pr = __builtin_amdgcn_exp2f(fmaf(sc[i][r], c, -lse[i]));
         if (masked) pr = keep ? pr : 0.f;
-        sc[i][r] = pr * (dp[r] - delta[i]) * (MAPS == 1 ? sign : (i ? -lam : 1.f));
+        const float ds = pr * (dp[r] - delta[i]);
+        if (i == MAPS - 1) rest += ds;
+        sc[i][r] = ds * (MAPS == 1 ? sign : (i ? -lam : 1.f));
       }
     }
 #pragma unroll
@@ -1063,7 +1089,11 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
       }
             });
   }
+  __shared__ float sums[4];
+  rest = wave_sum(rest);
+  if (lane == 0) sums[wave] = rest;
   __syncthreads();  // every wave is past its last image
+  if ((MAPS == 2 || map0) && tid == 0) p.partial[((long)tile * p.B + b) * p.H + h] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   float* strip = reinterpret_cast<float*>(smem + wave * STRIP_BYTES);
 #pragma unroll
   for (int i = 0; i < MAPS; ++i) {
@@ -1528,6 +1558,8 @@ int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass 
   if (n > most) n = most;
   return (int)n;
 }
+int rest_rows(const tfpp_diff_attn_params& p) { return (int)((p.Tq + QB - 1) / QB) * p.B; }
+int64_t rest_floats(const tfpp_diff_attn_params& p) { return ((int64_t)rest_rows(p) * p.H + 63) & ~63ll; }  // dQ's part of dlambda, in front of the row pass's sums
 int64_t row_floats(const tfpp_diff_attn_params& p) { return ((int64_t)row_blocks(p) * p.H * (1 + p.dv) + 63) & ~63ll; }
 }  // namespace
 
@@ -1551,7 +1583,7 @@ extern "C" int tfpp_diff_attn_fwd_partial_floats(const tfpp_diff_attn_params* p,
 extern "C" int tfpp_diff_attn_bwd_partial_floats(const tfpp_diff_attn_params* p, int64_t* out) {
   if (!p || !out || p->B < 1 || p->H < 1 || p->Hkv < 1 || p->Tq < 1 || p->Tk < 1 || p->d < 1 || p->dv < 1) return TFPP_EINVAL;
   const int nb = padded_blocks(*p), parts = dkv_parts(*p);
-  *out = row_floats(*p) + (parts > 1 ? (int64_t)parts * p->B * p->Hkv * p->Tk * (2 * ((nb + 1) / 2) + nb) * 32 : 0);
+  *out = rest_floats(*p) + row_floats(*p) + (parts > 1 ? (int64_t)parts * p->B * p->Hkv * p->Tk * (2 * ((nb + 1) / 2) + nb) * 32 : 0);
   return 0;
 }
 
@@ -1567,23 +1599,21 @@ extern "C" int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* pp, int dtype, vo
   hipStream_t st = (hipStream_t)stream;
   const int blocks = row_blocks(p);
   p.dkv_splits = dkv_parts(p);
-  p.dkv = p.partial + row_floats(p);
+  p.dkv = p.partial + rest_floats(p) + row_floats(p);
   const int lpr = row_lanes(p);
   p.do_vec = out_vector(p.dout, p.do_s, 3, vec);
   const dim3 sums(p.n_lam + (p.norm_w ? p.dv : 0));
-  if (dtype == TFPP_F32) {
-    hipLaunchKernelGGL(diff_attn_bwd_rows_kernel<float>, dim3(blocks, p.H), dim3(256), 0, st, p, lpr);
-    hipLaunchKernelGGL(diff_attn_bwd_sum_kernel<float>, sums, dim3(256), 0, st, p, blocks);
-  } else {
-    hipLaunchKernelGGL(diff_attn_bwd_rows_kernel<bf16_t>, dim3(blocks, p.H), dim3(256), 0, st, p, lpr);
-    hipLaunchKernelGGL(diff_attn_bwd_sum_kernel<bf16_t>, sums, dim3(256), 0, st, p, blocks);
-  }
+  tfpp_diff_attn_params pr = p;
+  pr.partial += rest_floats(p);
+  if (dtype == TFPP_F32) hipLaunchKernelGGL(diff_attn_bwd_rows_kernel<float>, dim3(blocks, p.H), dim3(256), 0, st, pr, lpr);
+  else hipLaunchKernelGGL(diff_attn_bwd_rows_kernel<bf16_t>, dim3(blocks, p.H), dim3(256), 0, st, pr, lpr);
   TFPP_CHECK_LAUNCH();
-  for (int step : {STEP_DQ, STEP_DKV}) {
-    const int rc = dtype == TFPP_F32 ? dispatch<float>(p, step, st) : dispatch<bf16_t>(p, step, st);
-    if (rc) return rc;
-  }
-  return 0;
+  int rc = dtype == TFPP_F32 ? dispatch<float>(p, STEP_DQ, st) : dispatch<bf16_t>(p, STEP_DQ, st);
+  if (rc) return rc;
+  if (dtype == TFPP_F32) hipLaunchKernelGGL(diff_attn_bwd_sum_kernel<float>, sums, dim3(256), 0, st, pr, blocks, p.partial, rest_rows(p));
+  else hipLaunchKernelGGL(diff_attn_bwd_sum_kernel<bf16_t>, sums, dim3(256), 0, st, pr, blocks, p.partial, rest_rows(p));
+  TFPP_CHECK_LAUNCH();
+  return dtype == TFPP_F32 ? dispatch<float>(p, STEP_DKV, st) : dispatch<bf16_t>(p, STEP_DKV, st);
 }
 
 extern "C" int tfpp_diff_lambda(const void* lq1, const void* lk1, const void* lq2, const void* lk2, float init, float* lam, int n, int d, int dtype, void* stream) {

@@ -1029,3 +1029,34 @@ def test_trainer_clips_the_averaged_gradients(ops):
   step = GraphedTrainStep(tr, batch, warmup=1)
   for bound in (0.25, 0.01, 1e9):
     check(step, bound)
+
+
+@pytest.mark.parametrize('seed', range(6))
+@pytest.mark.parametrize('heads', [(1, 1, 9, 18), (1, 1, 72, 144), (2, 1, 64, 128)], ids=str)
+def test_diff_attention_lambda_gradient_of_few_heads(ops, heads, seed):
+  """dlambda of one or two heads is one number, often small beside the terms it is the sum of: the roundings of P and of the saved O_2 to bf16 may not be
+  in it directly.  They remain in O, which dO(O) is made of.  With f(O) = sum of dO(O) . O_2 and g its derivative by O (O_2 held), independent roundings of
+  at most 2^-8 relative, standard deviation 2^-8 / sqrt(3) at most, of O_1 and O_2 as stored and of each P give dlambda the deviation 2^-8 / sqrt(3) times
+  the root of sum g^2 (O_1^2 + lam^2 O_2^2 + (P_1^2 + lam^2 P_2^2) V^2): four of these are allowed, and fp32 sums (1e-4 of the terms' root)."""
+  H, Hkv, d, dv = heads
+  B, T = 2, 333
+  q, k, v, dout, lam = attn_inputs(B, T, T, H, Hkv, d, dv, BF16, seed=300 + 10 * seed)
+  _, ctx = ops.diff_attn_fwd(q, k, v, lam, causal=True, save=True)
+  got = ops.diff_attn_bwd(dout, q, k, v, lam, ctx)[3]
+  keep = attn_visible(B, T, T, causal=True)
+  want = attn_oracle(q, k, v, lam, keep, dout=dout)['dlam'][0]
+  for h in range(H):
+    L, terms, dev = float(lam[h]), 0.0, 0.0
+    for b in range(B):
+      V, P = v[b, :, h // (H // Hkv)].double(), []
+      for i in (0, 1):
+        P.append(torch.softmax((q[b, :, h, i].double() @ k[b, :, h // (H // Hkv), i].double().T * d ** -0.5).masked_fill(~keep[b], -math.inf), 1))
+      o = [p @ V for p in P]
+      O, u = (o[0] - L * o[1]).requires_grad_(), dout[b, :, h].double()
+      r = 1.0 / torch.sqrt(O.pow(2).mean(1, keepdim=True) + 1e-5)
+      each = (r * u - O * r ** 3 * (u * O).mean(1, keepdim=True)) * o[1]
+      g, = torch.autograd.grad(each.sum(), O)
+      dev += float((g.pow(2) * (o[0].pow(2) + L ** 2 * o[1].pow(2) + (P[0].pow(2) + L ** 2 * P[1].pow(2)) @ V.pow(2))).sum())
+      terms += float(each.detach().pow(2).sum())
+    tol = 4 * 2.0 ** -8 / math.sqrt(3) * math.sqrt(dev) + 1e-4 * math.sqrt(terms)
+    assert abs(float(got[h] - want[h])) <= tol, (float(got[h]), float(want[h]), tol, math.sqrt(terms))
