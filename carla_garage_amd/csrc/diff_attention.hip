@@ -38,7 +38,9 @@ __device__ __forceinline__ void mma(const Frag8<float>& a, const Frag8<float>& b
 #pragma unroll
   for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
 }
-// C registers 8 t .. 8 t + 7 as an operand.  bf16: one rounding (2^-8 relative at most) of each probability / score gradient, as its partner operand has
+// C registers 8 t .. 8 t + 7 as an operand.  bf16: one rounding (2^-8 relative at most) of each probability / score gradient, as its partner operand has:
+// the matrix unit takes both in one type, and a second product for what the rounding takes off would double the work with V.  It leaves outputs 2.4e-3
+// off in the 2-norm where the rounding of the result alone leaves 1.7e-3, gradients 3.5e-3.
 __device__ __forceinline__ void to_frag(const f32x16_t& c, int t, Frag8<bf16_t>& f) {
   f.v = make_uint4(f2bf_pack2(c[8 * t], c[8 * t + 1]), f2bf_pack2(c[8 * t + 2], c[8 * t + 3]), f2bf_pack2(c[8 * t + 4], c[8 * t + 5]),
                    f2bf_pack2(c[8 * t + 6], c[8 * t + 7]));
@@ -471,15 +473,14 @@ template <typename T, int NB, bool VECTOR, int NT> __global__ __launch_bounds__(
 #pragma unroll
       for (int r = 0; r < 16; ++r) f.o[i][n][r] *= inv;
     if (p.lse && (lane & 31) < rows && half == 0) p.lse[(long)(f.map0 + i) * p.B * p.H * p.Tq + row0 + lane] = log_sum(f.m[i], f.l[i]);
-    if (p.o1) {
-      T* to = (T*)(f.map0 + i ? p.o2 : p.o1) + row0 * dvs;
-      store_rows<T>(strip, lane, f.o[i], 1.f, dvs, true, Weights{nullptr, 0}, [&](int r) { return r < rows ? to + (long)r * dvs : nullptr; });
-    }
   }
+  auto save = [&](void* to, const f32x16_t(&o)[NB]) {
+    T* at = (T*)to + row0 * dvs;
+    store_rows<T>(strip, lane, o, 1.f, dvs, true, Weights{nullptr, 0}, [&](int r) { return r < rows ? at + (long)r * dvs : nullptr; });
+  };
   if constexpr (MAPS == 1) {  // O_2 of the odd waves to the even ones, in the registers' own order
     static_assert(fwd_lds<T, NB>() >= NT / 128 * NB * 16 * 64 * 4, "the exchange fits the images' LDS");
     float4* x = reinterpret_cast<float4*>(smem) + (wave >> 1) * (NB * 4 * 64) + lane;
-    __syncthreads();  // every wave is past its strip
     if (f.map0)
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -495,13 +496,18 @@ template <typename T, int NB, bool VECTOR, int NT> __global__ __launch_bounds__(
           f.o[0][n][4 * g] -= lam * v.x; f.o[0][n][4 * g + 1] -= lam * v.y; f.o[0][n][4 * g + 2] -= lam * v.z; f.o[0][n][4 * g + 3] -= lam * v.w;
         }
     __syncthreads();
-    if (f.map0) return;
+    if (f.map0) {
+      if (p.o2) save(p.o2, f.o[0]);
+      return;
+    }
   } else {
+    if (p.o2) save(p.o2, f.o[MAPS - 1]);
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) f.o[0][n][r] -= lam * f.o[MAPS - 1][n][r];
   }
+  if (p.o1) save(p.o1, f.o[0]);  // (O and not P_1 V: rounded behind the subtraction, so that what both maps have in common is not in the rounding)
   float g = p.out_scale;
   if (p.norm) {
     float ss = 0.f;
@@ -714,14 +720,6 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
     for (int j = 0; j < MINE; ++j) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[map][j][e] *= inv;
-      if (p.o1 && wave + j * WAVES < NB) {
-        T* to = (T*)(map ? p.o2 : p.o1);
-        strip_put(strip, lane, 0, o[map][j], 1.f);
-        __builtin_amdgcn_wave_barrier();
-        strip_store<T>(strip, lane, 1, (wave + j * WAVES) * 32, dvs, true, Weights{nullptr, 0},
-                       [&](int r) { return row0 + r < rows ? to + (((long)b * p.H + head_of(r)) * p.Tq + (row0 + r) % p.Tq) * dvs : nullptr; });
-        __builtin_amdgcn_wave_barrier();
-      }
     }
   }
   float ss = 0.f;
@@ -732,6 +730,19 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__((Few<T, 
       o[0][j][e] -= lam * o[1][j][e];
       ss += o[0][j][e] * o[0][j][e];
     }
+  if (p.o1)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)  // O and O_2
+#pragma unroll
+      for (int j = 0; j < MINE; ++j)
+        if (wave + j * WAVES < NB) {
+          T* to = (T*)(i ? p.o2 : p.o1);
+          strip_put(strip, lane, 0, o[i][j], 1.f);
+          __builtin_amdgcn_wave_barrier();
+          strip_store<T>(strip, lane, 1, (wave + j * WAVES) * 32, dvs, true, Weights{nullptr, 0},
+                         [&](int r) { return row0 + r < rows ? to + (((long)b * p.H + head_of(r)) * p.Tq + (row0 + r) % p.Tq) * dvs : nullptr; });
+          __builtin_amdgcn_wave_barrier();
+        }
   float g = p.out_scale;
   if (p.norm) {
     ss += other_half(ss);
@@ -795,8 +806,11 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_
     const float v[4] = {o[map].x * f, o[map].y * f, o[map].z * f, o[map].w * f};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (p.o1 && c + e < dvs) ((T*)(map ? p.o2 : p.o1))[row * dvs + c + e] = ElemTraits<T>::from_f(v[e]);
       d[e] = map ? d[e] - lam * v[e] : v[e];
+      if (p.o1 && map && c + e < dvs) {
+        ((T*)p.o1)[row * dvs + c + e] = ElemTraits<T>::from_f(d[e]);
+        ((T*)p.o2)[row * dvs + c + e] = ElemTraits<T>::from_f(v[e]);
+      }
     }
   }
   float g = p.out_scale;
@@ -812,8 +826,11 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_
 //   r = 1 / sqrt(mean(O^2) + eps)      dO = r u - O r^3 mean(u O)  (without the norm: dO = u)     dw = sum out_scale dout O r     dlambda = - sum dO . O_2
 //   dP = dO V^T      delta_i = dO . O_i      dS_1 = P_1 (dP - delta_1)      dS_2 = -lambda P_2 (dP - delta_2)
 //   dQ_i = scale dS_i K_i      dK_i = scale dS_i^T Q_i      dV = (P_1 - lambda P_2)^T dO
-// 1. diff_attn_bwd_rows_kernel: dO (rounded once: it is an MFMA operand twice), delta_i from that rounded dO -- so that the rows of dS still sum to
-//    zero -- and partial sums of dw, dlambda from the unrounded one.  Bounded by HBM: 131072 rows of 128, 134 MB in 36 us (3.7 TB/s).
+// 1. diff_attn_bwd_rows_kernel: dO (rounded once: it is an MFMA operand twice), delta_i from that rounded dO, as dP is, with O_1 = O + lambda O_2 of the
+//    saved O and O_2 (whose rounding, 2^-8 relative at most, stays in delta_i), and partial sums of dw, dlambda from the unrounded dO.
+//    The forward pass saves O, not O_1: r, dO and dw are made of it, and a difference of two saved maps would hold their roundings, |O_1| / |O| times as
+//    large (64 / 128, V of mean 1, lambda 0.95: dw 1.8e-2 off, 3.4e-3 with O saved).
+//    Bounded by HBM: 131072 rows of 128, 134 MB in 36 us (3.7 TB/s).
 // grid (blocks, H); lpr lanes a row (a power of two), 8 channels a lane: 16-byte loads, 64 / lpr rows a wave at a time.  partial: [1 + dv][blocks x H], the
 // sums of one value side by side.
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) { return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
@@ -846,13 +863,13 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
     const int b = live ? (int)(n / p.Tq) : 0, t = live ? (int)(n % p.Tq) : 0;
     const long row = ((long)b * p.H + h) * p.Tq + t;
     const T* dout = (const T*)p.dout + (long)b * p.do_s[0] + (long)t * p.do_s[1] + (long)h * p.do_s[2] + c0;
-    float g[E], o1[E], o2[E], s[2] = {0.f, 0.f};
+    float g[E], o[E], o2[E], s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < E; ++e) g[e] = o1[e] = o2[e] = 0.f;
+    for (int e = 0; e < E; ++e) g[e] = o[e] = o2[e] = 0.f;
     if (in) {
 #pragma unroll
       for (int e = 0; e < E; e += ElemTraits<T>::VEC) {
-        load_vec<T>((const T*)p.o1 + row * dvs + c0 + e, o1 + e);
+        load_vec<T>((const T*)p.o1 + row * dvs + c0 + e, o + e);
         load_vec<T>((const T*)p.o2 + row * dvs + c0 + e, o2 + e);
       }
       if (p.do_vec && c0 + E <= p.dv) {
@@ -865,10 +882,9 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
       }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) {  // (channels behind dv: V is zero there, so are O_1 and O_2)
-      const float o = o1[e] - lam * o2[e];
-      s[0] += o * o;
-      s[1] += w[e] * g[e] * o;
+    for (int e = 0; e < E; ++e) {  // (channels behind dv: V is zero there, so are O and O_2)
+      s[0] += o[e] * o[e];
+      s[1] += w[e] * g[e] * o[e];
     }
     float r = 1.f, f = 0.f;
     if (p.norm) {
@@ -880,12 +896,11 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
     float d[E], t1 = 0.f, t2 = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float o = o1[e] - lam * o2[e];
-      dw[e] += p.out_scale * g[e] * o * r;
-      d[e] = r * w[e] * g[e] - o * f;
+      dw[e] += p.out_scale * g[e] * o[e] * r;
+      d[e] = r * w[e] * g[e] - o[e] * f;
       dl -= d[e] * o2[e];
       const float dr = ElemTraits<T>::to_f(ElemTraits<T>::from_f(d[e]));
-      t1 += dr * o1[e];
+      t1 += dr * (o[e] + lam * o2[e]);
       t2 += dr * o2[e];
     }
     t1 = row_sum(t1, lpr);

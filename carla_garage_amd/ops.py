@@ -1570,7 +1570,7 @@ def _lambda_vectors(*ts):
 
 
 class DiffAttnContext:
-  """What diff_attn_bwd needs of its forward pass: P_1 V, P_2 V, the rows' log-sums and the options."""
+  """What diff_attn_bwd needs of its forward pass: O = (P_1 - lam P_2) V, P_2 V, the rows' log-sums and the options."""
   __slots__ = ('saved', 'addr', 'norm_weight', 'opt', 'kv_len', 'q_start', 'key_mask', 'shape')
 
 
@@ -1708,7 +1708,7 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
     if save:
       ctx = DiffAttnContext()
       n_o, n_row = _diff_attn_rows(B * H * Tq, dv, q.element_size())
-      ctx.saved = torch.empty(2 * n_o + n_row, device=dev, dtype=torch.uint8)  # o1 | o2 (in q's type) | lse: one allocation
+      ctx.saved = torch.empty(2 * n_o + n_row, device=dev, dtype=torch.uint8)  # O | P_2 V (in q's type) | lse: one allocation
       at = ctx.saved.data_ptr()
       ctx.addr = (at, at + n_o, at + 2 * n_o)
       ctx.norm_weight, ctx.opt, ctx.shape = norm_weight, (scale, int(causal), int(norm), float(norm_eps), float(out_scale), start_all, q.dtype), shape
