@@ -17,7 +17,7 @@ LIB_PATH = os.path.join(PKG_DIR, 'libtfpp_hip.so')
 SOURCES = ['gemm_kernels.hip', 'gemm_glds.hip', 'gemm_wgrad_glds.hip', 'attention_kernels.hip', 'conv3x3_halo.hip', 'wgrad3x3_halo.hip', 'pointwise_kernels.hip', 'norm_kernels.hip', 'bn_rows_kernels.hip', 'misc_kernels.hip', 'lidar_kernels.hip', 'swin_kernels.hip', 'bev_kernels.hip', 'head_kernels.hip', 'augment_kernels.hip', 'grad_clip.hip', 'block_norm.hip', 'diff_attention.hip']
 
 F32, BF16 = 0, 1
-ABI_VERSION = 9  # include/tfpp.h TFPP_ABI_VERSION
+ABI_VERSION = 10  # include/tfpp.h TFPP_ABI_VERSION
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_GELU, ACT_TANH = 0, 1, 2, 3, 4
 EINVAL = -1000
 
@@ -73,7 +73,7 @@ class BlockNormParams(ctypes.Structure):
 
 
 class DiffAttnParams(ctypes.Structure):
-  _fields_ = [(n, vp) for n in ('q', 'k', 'v', 'lam', 'norm_w', 'out', 'o1', 'o2', 'lse', 'kv_len', 'q_start', 'key_mask', 'dout', 'd_o', 'delta', 'partial', 'dlam',
+  _fields_ = [(n, vp) for n in ('q', 'k', 'v', 'lam', 'norm_w', 'out', 'o1', 'o2', 'lse', 'kv_len', 'q_start', 'key_mask', 'dout', 'd_o', 'slope', 'delta', 'partial', 'dlam',
                                 'dnorm_w', 'dq_out', 'dk_out', 'dv_out')] + \
       [('ld_mask', i64), ('q_s', i64 * 4), ('k_s', i64 * 4), ('v_s', i64 * 3), ('o_s', i64 * 3), ('do_s', i64 * 3), ('dq_s', i64 * 4), ('dk_s', i64 * 4), ('dv_s', i64 * 3)] + \
       [(n, i32) for n in ('B', 'H', 'Hkv', 'Tq', 'Tk', 'd', 'dv', 'n_lam', 'norm', 'norm_w_bf16', 'causal', 'q_start_all', 'out_vec', 'do_vec', 'dq_vec', 'dk_vec', 'dv_vec', 'splits', 'dkv_splits')] + \

@@ -829,8 +829,8 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_
 // 1. diff_attn_bwd_rows_kernel: dO (rounded once: it is an MFMA operand twice), delta_i from that rounded dO, as dP is, with O_1 = O + lambda O_2 of the
 //    saved O and O_2 (whose rounding, 2^-8 relative at most, stays in delta_i), and partial sums of dw, dlambda from the unrounded dO.
 //    The forward pass saves O, not O_1: r, dO and dw are made of it, and a difference of two saved maps would hold their roundings, |O_1| / |O| times as
-//    large (64 / 128, V of mean 1, lambda 0.95: dw 1.8e-2 off, 3.4e-3 with O saved).
-//    Bounded by HBM: 131072 rows of 128, 134 MB in 36 us (3.7 TB/s).
+//    large (64 / 128, V of mean 1, lambda 0.95: dw 1.8e-2 off, 3.4e-3 with O saved).  For bf16 also g, see dQ.
+//    Bounded by HBM: 131072 rows of 128, 168 MB in 45 us (3.8 TB/s).
 // grid (blocks, H); lpr lanes a row (a power of two), 8 channels a lane: 16-byte loads, 64 / lpr rows a wave at a time.  partial: [1 + dv][blocks x H], the
 // sums of one value side by side.
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) { return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
@@ -849,6 +849,7 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
   const int rpw = 64 / lpr, slots = (int)gridDim.x * 4 * rpw;
   const long rows = (long)p.B * p.Tq;
   const float lam = p.lam[p.n_lam > 1 ? h : 0], inv_dv = 1.f / (float)p.dv;
+  constexpr bool SLOPE = sizeof(T) == 2;
   float w[E], dw[E], dl = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -863,7 +864,7 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
     const int b = live ? (int)(n / p.Tq) : 0, t = live ? (int)(n % p.Tq) : 0;
     const long row = ((long)b * p.H + h) * p.Tq + t;
     const T* dout = (const T*)p.dout + (long)b * p.do_s[0] + (long)t * p.do_s[1] + (long)h * p.do_s[2] + c0;
-    float g[E], o[E], o2[E], s[2] = {0.f, 0.f};
+    float g[E], o[E], o2[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) g[e] = o[e] = o2[e] = 0.f;
     if (in) {
@@ -881,33 +882,52 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_rows_
           if (c0 + e < p.dv) g[e] = ElemTraits<T>::to_f(dout[e]);
       }
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {  // (channels behind dv: V is zero there, so are O and O_2)
-      s[0] += o[e] * o[e];
-      s[1] += w[e] * g[e] * o[e];
-    }
-    float r = 1.f, f = 0.f;
-    if (p.norm) {
-      s[0] = row_sum(s[0], lpr);
-      s[1] = row_sum(s[1], lpr);
-      r = 1.f / sqrtf(s[0] * inv_dv + p.eps);  // (eps > 0: checked by the launcher)
-      f = r * r * r * s[1] * inv_dv;
-    }
-    float d[E], t1 = 0.f, t2 = 0.f;
+    float ss = 0.f, uo = 0.f, oo2 = 0.f, uo2 = 0.f, r = 1.f, a = 0.f, f = 0.f;  // (channels behind dv: V is zero there, so are O and O_2)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      dw[e] += p.out_scale * g[e] * o[e] * r;
-      d[e] = r * w[e] * g[e] - o[e] * f;
+      const float u = w[e] * g[e];
+      ss += o[e] * o[e];
+      uo += u * o[e];
+      if constexpr (SLOPE) {
+        oo2 += o[e] * o2[e];
+        uo2 += u * o2[e];
+      }
+    }
+    if (p.norm) {
+      ss = row_sum(ss, lpr);
+      uo = row_sum(uo, lpr);
+      if constexpr (SLOPE) {
+        oo2 = row_sum(oo2, lpr);
+        uo2 = row_sum(uo2, lpr);
+      }
+      r = 1.f / sqrtf(ss * inv_dv + p.eps);  // (eps > 0: checked by the launcher)
+      a = r * inv_dv * uo;                   // mean(u O^), O^ = r O; every product below has O^, which is at most sqrt(dv) in size whatever r is
+      f = r * inv_dv;
+    }
+    const float b2 = r * oo2, c2 = uo2 - 3.f * a * b2;  // O^ . O_2
+    float d[E], sg[E], t1 = 0.f, t2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float u = w[e] * g[e], on = r * o[e];
+      dw[e] += p.out_scale * g[e] * on;
+      d[e] = r * (u - on * a);
       dl -= d[e] * o2[e];
       const float dr = ElemTraits<T>::to_f(ElemTraits<T>::from_f(d[e]));
       t1 += dr * (o[e] + lam * o2[e]);
       t2 += dr * o2[e];
+      if constexpr (SLOPE) {
+        sg[e] = -r * (f * (c2 * on + b2 * u) + a * o2[e] * r);
+        dl += ElemTraits<T>::to_f(ElemTraits<T>::from_f(sg[e])) * o[e];
+      }
     }
     t1 = row_sum(t1, lpr);
     t2 = row_sum(t2, lpr);
     if (in)
 #pragma unroll
-      for (int e = 0; e < E; e += ElemTraits<T>::VEC) store_vec<T>((T*)p.d_o + row * dvs + c0 + e, d + e);
+      for (int e = 0; e < E; e += ElemTraits<T>::VEC) {
+        store_vec<T>((T*)p.d_o + row * dvs + c0 + e, d + e);
+        if constexpr (SLOPE) store_vec<T>((T*)p.slope + row * dvs + c0 + e, sg + e);
+      }
     if (live && c0 == 0) {
       p.delta[row] = t1;
       p.delta[(long)p.B * p.H * p.Tq + row] = t2;
@@ -955,18 +975,26 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_k
 }
 
 // 2. dQ.  Workgroup = (batch, head, 128 queries), wave = 32 queries, as the forward pass: S_i^T = K_i Q_i^T, dP^T = V dO^T (keys x queries),
-//    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.  2 x 4096 causal, 16 heads of 64 / 128: 270 us; 12 x 320, 4 heads
-//    of 72 / 144: 24 us.
-//    The row pass's dlambda has the rounding of O_2 (its own and that of the probabilities it was made of) in it, up to a percent where the heads are few
-//    and the sum is small.  sum_j P_2 (dP - delta_2) is what that rounding made of delta_2: with P_2 and dP at hand in 32 bits it is added here.
-//    Wide heads: a workgroup has one map (the grid's y), dP is computed by both: 21 / 16 of the flop, and two waves fit a SIMD in place of one
-//    (12 x 320 queries over 1280 keys: 68 us, 82 us with both maps in a wave).
+//    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.  2 x 4096 causal, 16 heads of 64 / 128: 354 us; 12 x 320, 4 heads
+//    of 72 / 144: 30 us.
+//    bf16: dlambda = - sum f, f = dO(O) . O_2, is a sum that cancels, and the row pass has it from the saved O and O_2, which are rounded and made of
+//    rounded probabilities: percents of it where the heads are few.  Here P is at hand in 32 bits, and both are put right to first order:
+//      O_2 beside dO:  sum_j P_2 (dP - delta_2) = dO . (O_2 - saved O_2)
+//      O inside dO:    sum_j (P_1 - lambda P_2) g . V_j - g . saved O = g . (O - saved O),  g = df/dO = - r^2 / dv ((u . O_2 - 3 a b) O^ + b u + dv a O_2)
+//                      with O^ = r O, a = mean(u O^), b = O^ . O_2  (the row pass subtracts g . saved O)
+//    The product with g shares the V operand of dP: 2 dv of 8 d + 4 dv flop a pair.  What is left is of second order, 1e-5 of the terms' root
+//    (before: 2e-3 to 3e-2).  2 x 4096 causal: 273 -> 354 us; 12 x 320: 25 -> 30 us.
+//    Wide heads: a workgroup has one map (the grid's y), dP is computed by both, and two waves fit a SIMD in place of one
+//    (12 x 320 queries over 1280 keys, without g: 68 us, 82 us with both maps in a wave).  bf16 heads of 81 .. 128 hold q, dO, g and dQ in the registers of
+//    one wave a SIMD (8 heads of 128 / 256 over 2 x 2048: backward 456 us; with both maps in a wave 481).
 template <typename T, int NB> constexpr int dq_maps() { return NB >= (sizeof(T) == 2 ? 5 : 4) ? 1 : 2; }
-// bf16 heads of 81 .. 128: the last 16 channels of a wave's queries stay in LDS, which spares the registers that would go to scratch
-template <typename T, int NB> constexpr bool dq_stash() { return sizeof(T) == 2 && NB == 8; }
-template <typename T, int NB> constexpr int dq_lds() { return at_least(2 * 32 * (dq_maps<T, NB>() * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES) + (dq_stash<T, NB>() ? 256 * 16 : 0), 4 * STRIP_BYTES); }
+template <typename T, int NB, bool VECTOR> constexpr int dq_waves() { return sizeof(T) == 2 && NB == 8 && VECTOR ? 1 : 2; }  // of a SIMD
+// bf16 heads of 33 .. 64: the last fragments of a wave's g stay in LDS, which spares the registers that would go to scratch
+template <typename T, int NB, bool VECTOR> constexpr int dq_stash() { return sizeof(T) == 2 && NB == 4 && VECTOR ? 4 : 0; }
+template <typename T, int NB, bool VECTOR> constexpr int dq_images() { return 2 * 32 * (dq_maps<T, NB>() * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES); }
+template <typename T, int NB, bool VECTOR> constexpr int dq_lds() { return at_least(dq_images<T, NB, VECTOR>() + dq_stash<T, NB, VECTOR>() * 256 * 16, 4 * STRIP_BYTES); }
 
-template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) void diff_attn_bwd_dq_kernel(tfpp_diff_attn_params p) {
+template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (dq_waves<T, NB, VECTOR>())) void diff_attn_bwd_dq_kernel(tfpp_diff_attn_params p) {
   constexpr int KT = 32, NT = 256, CD = (NB + 1) / 2, MAPS = dq_maps<T, NB>();
   typedef Img<T, CD> ImgK;
   typedef Img<T, NB> ImgV;
@@ -986,23 +1014,26 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
   const T* vb = (const T*)p.v + (long)b * p.v_s[0] + (long)hk * p.v_s[2];
   constexpr bool HOLD = VECTOR ? sizeof(T) == 2 || NB < 5 : NB < 4;  // else Q and dO do not fit the registers and are read again for every tile
   const T* qrow = (const T*)p.q + (long)b * p.q_s[0] + (long)qc * p.q_s[1] + (long)h * p.q_s[2] + map0 * p.q_s[3];
-  constexpr bool STASH = dq_stash<T, NB>() && HOLD;
-  constexpr int HELD = STASH ? NB - 1 : NB;
-  uint4* stash = reinterpret_cast<uint4*>(smem + 2 * BUF) + tid;  // (a lane's own operand)
-  Frag8<T> q[MAPS][HOLD ? HELD : 1], dof[HOLD ? 2 * NB : 1];
-  if constexpr (HOLD)
+  constexpr bool SLOPE = sizeof(T) == 2;
+  constexpr int STASH = dq_stash<T, NB, VECTOR>(), HELD = 2 * NB - STASH;
+  static_assert(!STASH || (HOLD && SLOPE), "what is put away are held fragments of g");
+  Frag8<T> q[MAPS][HOLD ? NB : 1], dof[HOLD ? 2 * NB : 1], slope[HOLD && SLOPE ? HELD : 1];
+  if constexpr (HOLD) {
 #pragma unroll
     for (int i = 0; i < MAPS; ++i)
 #pragma unroll
-      for (int ks = 0; ks < HELD; ++ks) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][ks]);
-  if constexpr (STASH) {
-    Frag8<T> last;
-    load_frag<T, VECTOR>(qrow, HELD * 16 + half * 8, p.d, true, last);
-    *stash = last.v;
-  }
-  if constexpr (HOLD)
+      for (int ks = 0; ks < NB; ++ks) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][ks]);
 #pragma unroll
-    for (int ks = 0; ks < 2 * NB; ++ks) load_frag<T, true>((const T*)p.d_o + row * dvs, ks * 16 + half * 8, dvs, true, dof[ks]);
+    for (int ks = 0; ks < 2 * NB; ++ks) {
+      load_frag<T, true>((const T*)p.d_o + row * dvs, ks * 16 + half * 8, dvs, true, dof[ks]);
+      if constexpr (SLOPE) {
+        Frag8<T> g;
+        load_frag<T, true>((const T*)p.slope + row * dvs, ks * 16 + half * 8, dvs, true, g);
+        if (ks < HELD) slope[ks < HELD ? ks : 0] = g;
+        else if constexpr (STASH) *reinterpret_cast<uint4*>(smem + 2 * BUF + ((ks - HELD) * NT + tid) * 16) = g.v;  // (read by the lane that wrote it)
+      }
+    }
+  }
   const bool exists = qi < p.Tq;  // (the lanes behind the last query: P = 0)
   const float lse[2] = {exists ? p.lse[map0 * rows + row] : INFINITY, exists ? p.lse[rows + row] : INFINITY}, delta[2] = {p.delta[map0 * rows + row], p.delta[rows + row]};  // (one map: the first of each)
   const float lam = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(p.lam[p.n_lam > 1 ? h : 0]))), sign = map0 ? -lam : 1.f, c = p.scale * LOG2E;
@@ -1017,11 +1048,13 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
     for (int n = 0; n < CD; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[i][n][r] = 0.f;
-  float rest = 0.f;  // of the last map: sum of P_2 (dP - delta_2)
+  float rest = 0.f, rise = 0.f;  // sums of the last map's P_2 (dP - delta_2), of (P_1 - lambda P_2) g . V (one map a workgroup: of its P g . V)
   const int k_rows = ImgK::rows_at(lane), v_rows = ImgV::rows_at(lane), k_cols = ImgK::cols_at(lane);
   auto fill = [&](unsigned char* buf, int step, unsigned long long bits) {
     const long j0 = (long)step * KT;
     const Rows have = {sq.len - step * KT, p.key_mask != nullptr, bits};
+    int tid = (int)threadIdx.x;
+    if (STASH) asm volatile("" : "+v"(tid));  // (the offsets made of it are worked out again each time: kept, they would not fit the registers)
 #pragma unroll
     for (int i = 0; i < MAPS; ++i) ImgK::template fill<KT, VECTOR, NT>(buf + i * K_BYTES, kb + j0 * p.k_s[1] + i * p.k_s[3], p.k_s[1], p.d, have, tid);
     ImgV::template fill<KT, VECTOR, NT>(buf + MAPS * K_BYTES, vb + j0 * p.v_s[1], p.v_s[1], p.dv, have, tid);
@@ -1048,10 +1081,10 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
     const bool masked = cur != low_bits(KT) || (p.causal && sq.start + w0 + 1 - j0 < KT);
     const unsigned vis = (unsigned)(p.causal ? cur & low_bits(sq.start + qi + 1 - j0) : cur) >> (4 * half);
     const int vr = v_rows + MAPS * K_BYTES;
-    f32x16_t sc[MAPS], dp;
+    f32x16_t sc[MAPS], dp, gv;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      dp[r] = 0.f;
+      dp[r] = gv[r] = 0.f;
 #pragma unroll
       for (int i = 0; i < MAPS; ++i) sc[i][r] = 0.f;
     }
@@ -1062,13 +1095,8 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
         Frag8<T> a;
         ImgK::rows(now + i * K_BYTES, k_rows, ks, a);
         if constexpr (!HOLD) load_frag<T, VECTOR>(qrow + (long)i * p.q_s[3], ks * 16 + half * 8, p.d, true, q[i][0]);
-        if constexpr (STASH) {
-          Frag8<T> last;
-          if (ks == HELD) last.v = *stash;
-          mma(a, ks == HELD ? last : q[i][ks < HELD ? ks : 0], sc[i]);
-        } else {
-          mma(a, q[i][HOLD ? ks : 0], sc[i]);
-        }
+        mma(a, q[i][HOLD ? ks : 0], sc[i]);
+        if (STASH && ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (operands loaded far ahead of their products would not fit the registers)
       }
 #pragma unroll
     for (int ks = 0; ks < 2 * NB; ++ks) {
@@ -1076,6 +1104,17 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
       ImgV::rows(now, vr, ks, a);
       if constexpr (!HOLD) load_frag<T, true>((const T*)p.d_o + row * dvs, ks * 16 + half * 8, dvs, true, dof[0]);
       mma(a, dof[HOLD ? ks : 0], dp);
+      if constexpr (SLOPE) {
+        if constexpr (!HOLD) load_frag<T, true>((const T*)p.slope + row * dvs, ks * 16 + half * 8, dvs, true, slope[0]);
+        if (HOLD && ks >= HELD) {
+          Frag8<T> g;
+          if constexpr (STASH) g.v = *reinterpret_cast<const uint4*>(now + (2 - (s & 1)) * BUF + ((ks - HELD) * NT + tid) * 16);  // (an address made of `now`: see overlap)
+          mma(a, g, gv);
+        } else {
+          mma(a, slope[HOLD ? (ks < HELD ? ks : 0) : 0], gv);
+        }
+      }
+      if (STASH && ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -1086,6 +1125,7 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
         if (masked) pr = keep ? pr : 0.f;
         const float ds = pr * (dp[r] - delta[i]);
         if (i == MAPS - 1) rest += ds;
+        if constexpr (SLOPE) rise += (i ? -lam * pr : pr) * gv[r];
         sc[i][r] = ds * (MAPS == 1 ? sign : (i ? -lam : 1.f));
       }
     }
@@ -1105,10 +1145,11 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, 2) 
             });
   }
   __shared__ float sums[4];
-  rest = wave_sum(rest);
+  rest = wave_sum(MAPS == 2 ? rest + rise : (map0 ? rest - lam * rise : rise));
   if (lane == 0) sums[wave] = rest;
   __syncthreads();  // every wave is past its last image
-  if ((MAPS == 2 || map0) && tid == 0) p.partial[((long)tile * p.B + b) * p.H + h] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  if (tid == 0) p.partial[(((long)map0 * tiles + tile) * p.B + b) * p.H + h] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  if (MAPS == 2 && tid == 0) p.partial[(((long)tiles + tile) * p.B + b) * p.H + h] = 0.f;  // (the place of the second map's workgroup)
   float* strip = reinterpret_cast<float*>(smem + wave * STRIP_BYTES);
 #pragma unroll
   for (int i = 0; i < MAPS; ++i) {
@@ -1519,7 +1560,7 @@ template <typename T, int NB, bool VECTOR> int launch(const tfpp_diff_attn_param
   }
   const long n = (long)(((step == STEP_DQ ? p.Tq : p.Tk) + QB - 1) / QB) * p.B * (step == STEP_DQ ? p.H : p.Hkv);
   if (n > 0x7fffffffl) return TFPP_EINVAL;
-  if (step == STEP_DQ) return start(diff_attn_bwd_dq_kernel<T, NB, VECTOR>, dim3((unsigned)n, 3 - dq_maps<T, NB>()), 256, dq_lds<T, NB>(), &done[1], p, st);
+  if (step == STEP_DQ) return start(diff_attn_bwd_dq_kernel<T, NB, VECTOR>, dim3((unsigned)n, 3 - dq_maps<T, NB>()), 256, dq_lds<T, NB, VECTOR>(), &done[1], p, st);
   const int rc = start(diff_attn_bwd_dkv_kernel<T, NB, VECTOR>, dim3((unsigned)n, (dkv_split<T, NB, VECTOR>() ? 3 : 1) * p.dkv_splits), 256, dkv_lds<T, NB>(), &done[2], p, st);
   if (rc) return rc;
   if (p.dkv_splits > 1) {
@@ -1573,7 +1614,7 @@ int row_blocks(const tfpp_diff_attn_params& p) {  // workgroups of the row pass 
   if (n > most) n = most;
   return (int)n;
 }
-int rest_rows(const tfpp_diff_attn_params& p) { return (int)((p.Tq + QB - 1) / QB) * p.B; }
+int rest_rows(const tfpp_diff_attn_params& p) { return 2 * (int)((p.Tq + QB - 1) / QB) * p.B; }  // (both maps, also where one workgroup has both)
 int64_t rest_floats(const tfpp_diff_attn_params& p) { return ((int64_t)rest_rows(p) * p.H + 63) & ~63ll; }  // dQ's part of dlambda, in front of the row pass's sums
 int64_t row_floats(const tfpp_diff_attn_params& p) { return ((int64_t)row_blocks(p) * p.H * (1 + p.dv) + 63) & ~63ll; }
 }  // namespace
@@ -1605,8 +1646,8 @@ extern "C" int tfpp_diff_attn_bwd_partial_floats(const tfpp_diff_attn_params* p,
 extern "C" int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* pp, int dtype, void* stream) {
   if (!pp || !valid(*pp, dtype)) return TFPP_EINVAL;
   tfpp_diff_attn_params p = *pp;
-  if (!p.dout || !p.o1 || !p.o2 || !p.lse || !p.d_o || !p.delta || !p.partial || !p.dlam || !p.dq_out || !p.dk_out || !p.dv_out || (p.norm_w && !p.dnorm_w)) return TFPP_EINVAL;
-  if (p.H > 65535 || (((uintptr_t)p.o1 | (uintptr_t)p.o2 | (uintptr_t)p.d_o) & 15)) return TFPP_EINVAL;
+  if (!p.dout || !p.o1 || !p.o2 || !p.lse || !p.d_o || (dtype == TFPP_BF16 && !p.slope) || !p.delta || !p.partial || !p.dlam || !p.dq_out || !p.dk_out || !p.dv_out || (p.norm_w && !p.dnorm_w)) return TFPP_EINVAL;
+  if (p.H > 65535 || (((uintptr_t)p.o1 | (uintptr_t)p.o2 | (uintptr_t)p.d_o | (dtype == TFPP_BF16 ? (uintptr_t)p.slope : 0)) & 15)) return TFPP_EINVAL;
   const int vec = dtype == TFPP_F32 ? 4 : 8;
   p.dq_vec = out_vector(p.dq_out, p.dq_s, 4, vec);
   p.dk_vec = out_vector(p.dk_out, p.dk_s, 4, vec);

@@ -1640,9 +1640,9 @@ def _diff_attn_check(q, k, v, lam):
   return dev, qs, ks, vs, (B, Tq, Tk, H, Hkv, d, dv)
 
 
-# tfpp_diff_attn_params: q k v lam norm_w out o1 o2 lse kv_len q_start key_mask dout d_o delta partial dlam dnorm_w dq dk dv | ld_mask q_s[4] k_s[4] v_s[3]
+# tfpp_diff_attn_params: q k v lam norm_w out o1 o2 lse kv_len q_start key_mask dout d_o slope delta partial dlam dnorm_w dq dk dv | ld_mask q_s[4] k_s[4] v_s[3]
 # o_s[3] do_s[3] dq_s[4] dk_s[4] dv_s[3] | B H Hkv Tq Tk d dv n_lam norm norm_w_bf16 causal q_start_all, 7 set by the library | scale out_scale eps | dkv
-_DIFF_ATTN = _layout('21Q29q19i3fQ', DiffAttnParams)
+_DIFF_ATTN = _layout('22Q29q19i3fQ', DiffAttnParams)
 
 
 @functools.lru_cache(maxsize=512)
@@ -1722,7 +1722,7 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
     partial = torch.empty(n_part, device=dev, dtype=torch.float32) if n_part else None  # scratch of this call alone
     o1, o2, lse = ctx.addr if save else (0, 0, 0)
     p = _DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(norm_weight), out.data_ptr(), o1, o2, lse, _addr(kv_len), _addr(start_t), _addr(key_mask),
-                        0, 0, 0, _addr(partial), 0, 0, 0, 0, 0, key_mask.stride(0) if key_mask is not None else 0, *qs, *ks, *vs, *os_, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                        0, 0, 0, 0, _addr(partial), 0, 0, 0, 0, 0, key_mask.stride(0) if key_mask is not None else 0, *qs, *ks, *vs, *os_, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
                         B, H, Hkv, Tq, Tk, d, dv, lam.numel(), norm, norm_weight is not None and norm_weight.dtype == torch.bfloat16, causal, start_all, 0, 0, 0, 0, 0, 0, 0,
                         scale, out_scale, norm_eps, 0)
     if lib.profiler is not None:
@@ -1762,13 +1762,15 @@ def diff_attn_bwd(dout, q, k, v, lam, ctx, dq=None, dk=None, dv=None):
       return (*outs, dlam, dw)
     # scratch of this call alone: captured graphs keep theirs in the graph's own pool
     n_o, n_row = _diff_attn_rows(B * H * Tq, dvn, q.element_size())
-    scratch = torch.empty(n_o + n_row + 4 * _diff_attn_partial(shape, True), device=dev, dtype=torch.uint8)
+    n_slope = n_o if q.dtype == torch.bfloat16 else 0
+    scratch = torch.empty(n_o + n_slope + n_row + 4 * _diff_attn_partial(shape, True), device=dev, dtype=torch.uint8)
     d_o = scratch.data_ptr()
-    delta = d_o + n_o
+    slope = d_o + n_o
+    delta = slope + n_slope
     partial = delta + n_row
     scale, causal, norm, eps, out_scale, start_all, _ = ctx.opt
     p = _DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(w), 0, *ctx.addr, _addr(ctx.kv_len),
-                        _addr(ctx.q_start), _addr(ctx.key_mask), dout.data_ptr(), d_o, delta, partial, dlam.data_ptr(), _addr(dw),
+                        _addr(ctx.q_start), _addr(ctx.key_mask), dout.data_ptr(), d_o, slope, delta, partial, dlam.data_ptr(), _addr(dw),
                         *[t.data_ptr() for t in outs], ctx.key_mask.stride(0) if ctx.key_mask is not None else 0, *qs, *ks, *vs, 0, 0, 0, *dos, *strides[0], *strides[1], *strides[2],
                         B, H, Hkv, Tq, Tk, d, dvn, lam.numel(), norm, w is not None and w.dtype == torch.bfloat16, causal, start_all, 0, 0, 0, 0, 0, 0, 0, scale, out_scale, eps, 0)
     if lib.profiler is not None:

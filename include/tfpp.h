@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define TFPP_ABI_VERSION 9
+#define TFPP_ABI_VERSION 10
 #define TFPP_EINVAL (-1000)
 #define TFPP_F32 0
 #define TFPP_BF16 1
@@ -707,9 +707,9 @@ int tfpp_block_norm_bwd_partial_floats(const tfpp_block_norm_params* p, int64_t*
  * lam: n_lam = H (or 1) fp32 values.  kv_len (nullable): valid keys of each sequence; key_mask (nullable, [B] rows of pitch ld_mask): 0 leaves a key
  * out; causal: key j is seen by query i when j <= q_start[b] + i (q_start null: q_start_all).  K and V of keys left out by kv_len or key_mask may
  * hold anything.  A query without keys: out = 0.  Forward: partial is scratch of tfpp_diff_attn_fwd_partial_floats (null where that is 0).
- * Forward for training also writes o1, o2 ([B, H, Tq, dv rounded up to 8], O and P_2 V in `dtype`) and lse ([2, B, H, Tq], log2).  Backward reads them, dout
- * and the inputs, and writes d_o (layout of o1), delta (layout of lse), partial (tfpp_diff_attn_bwd_partial_floats): scratch; dlam [n_lam], dnorm_w
- * (type of norm_w), and the gradients dq_out, dk_out, dv_out with their own strides.  Fixed summation order throughout. */
+ * Forward for training also writes o1, o2 ([B, H, Tq, dv rounded up to 8]: O and P_2 V in `dtype`, 16-byte aligned) and lse ([2, B, H, Tq], log2).
+ * Backward reads them, dout and the inputs, and writes d_o, slope (bf16 only; both in the layout of o1), delta (layout of lse), partial
+ * (tfpp_diff_attn_bwd_partial_floats): scratch; dlam [n_lam], dnorm_w (type of norm_w), and the gradients dq_out, dk_out, dv_out with their own strides.  Fixed summation order throughout. */
 typedef struct {
   const void *q, *k, *v;
   const float* lam;
@@ -720,7 +720,7 @@ typedef struct {
   const int32_t *kv_len, *q_start;
   const uint8_t* key_mask;
   const void* dout;
-  void *d_o;
+  void *d_o, *slope;
   float *delta, *partial, *dlam;
   void *dnorm_w, *dq_out, *dk_out, *dv_out;
   int64_t ld_mask, q_s[4], k_s[4], v_s[3], o_s[3], do_s[3], dq_s[4], dk_s[4], dv_s[3];

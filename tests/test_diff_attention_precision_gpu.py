@@ -55,3 +55,23 @@ def test_diff_attention_gradients_of_maps_with_a_common_part(ops, shape, lam):
   got = dict(zip(('dq', 'dk', 'dv', 'dlam', 'dw'), ops.diff_attn_bwd(dout, q, k, v, lam, ctx)))
   off = {n: float((got[n].double() - want[n]).norm() / want[n].norm()) for n in ('dq', 'dk', 'dv', 'dw')}
   assert off['dw'] <= 6e-3 and off['dv'] <= 6.5e-3 and off['dq'] <= 9e-3 and off['dk'] <= 9e-3, off
+
+
+@pytest.mark.parametrize('B,T,causal,ragged', [(1, 230, False, False), (2, 333, True, False), (12, 16, True, True), (3, 200, False, True)])
+@pytest.mark.parametrize('d', [9, 16, 27, 32, 64, 72, 128])
+def test_diff_attention_lambda_gradient_is_free_of_first_order_roundings(ops, d, B, T, causal, ragged):
+  """dlambda is a sum over all rows that cancels: the roundings of P and of the saved results may reach it in second order only, both where they stand
+  beside dO and through O, which dO is made of.  A row's O is off by at most 2^-8 / sqrt(3) * sqrt(2 + 1) = 3.9e-3 relative (P of both maps, the saved value), a
+  deviation; the second derivative of a row's term is at most a few times the term over |O|^2, so that the row is off by some 1e-4 of itself, and the rows'
+  signs are independent: 2.5e-4 of the root of the terms' squares is allowed, which also is 2.5e-3 of dlambda wherever it is more than a tenth of that root.
+  fp32 sums are 1e-6 of it."""
+  for H, one in ((1, False), (2, False), (2, True)):
+    for seed in range(20):
+      q, k, v, dout, _ = attn_inputs(B, T, T, H, 1, d, 2 * d, BF16, seed=1000 + 10 * seed)
+      lam = ops.diff_lambda(*[randn(1 if one else H, d, seed=2000 + 4 * seed + i, std=0.1) for i in range(4)], 0.3555)
+      lens = torch.randint(1, T + 1, (B,), generator=torch.Generator().manual_seed(seed), dtype=torch.int32).to(DEV) if ragged else None
+      _, ctx = ops.diff_attn_fwd(q, k, v, lam, causal=causal, kv_len=lens, out_scale=0.65, save=True)
+      got = ops.diff_attn_bwd(dout, q, k, v, lam, ctx)[3].double()
+      want = formula(q, k, v, 0.65 * dout.double(), lam, attn_visible(B, T, T, causal=causal, kv_len=lens))
+      value, root = (want['dlam'].sum().view(1), want['root'].norm().view(1)) if one else (want['dlam'], want['root'])
+      assert ((got - value).abs() <= 2.5e-4 * root).all(), (H, one, seed, ((got - value).abs() / root).tolist(), (value.abs() / root).tolist())
