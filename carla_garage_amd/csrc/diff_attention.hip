@@ -2,7 +2,9 @@
 //   P_i = softmax(scale Q_i K_i^T) (i = 1, 2)      O = (P_1 - lambda P_2) V      out = out_scale * w * O / sqrt(mean(O^2) + eps)
 // Q [B, Tq, H, 2, d], K [B, Tk, Hkv, 2, d], V [B, Tk, Hkv, dv] with any strides but a contiguous last dimension; H / Hkv query heads share a key /
 // value head; d <= 128, dv <= 256.  Keys are left out by kv_len (per sequence), key_mask (per key) and causality (key <= q_start + query); a query
-// that sees no key gives zeros and takes no part in any gradient.  Left-out keys are never read: what lies there (NaN included) has no effect.
+// that sees no key gives zeros and takes no part in any gradient.  What lies at keys that no query of the sequence sees (NaN included) has no effect: they are
+// zeros in the images, and their own columns in dK / dV, which may have read them, are dropped.  A key that causality hides from some queries only is read
+// beside them, with a probability of zero: it has to be finite.
 //
 // All products are 32 x 32 x 16 MFMA tiles (bf16; fp32 runs the same code on eight 32 x 32 x 2 each).  Every score tile is computed transposed to
 // where it is contracted next, so that its C fragment IS the B operand of the following product and never leaves the registers:
@@ -244,7 +246,7 @@ template <typename Fill, typename Use> __device__ __forceinline__ void overlap(u
 }
 
 struct Seq {  // what a sequence's queries may see
-  int len, start;  // keys 0 .. len - 1; query i sees key j <= start + i (causal)
+  int len, start;  // keys 0 .. len - 1, no query sees one behind; query i sees key j <= start + i (causal)
 };
 __device__ __forceinline__ Seq sequence(const tfpp_diff_attn_params& p, int b) {
   Seq s;
@@ -255,6 +257,7 @@ __device__ __forceinline__ Seq sequence(const tfpp_diff_attn_params& p, int b) {
   }
   const int start = p.q_start ? __builtin_amdgcn_readfirstlane(p.q_start[b]) : p.q_start_all;
   s.start = start < -p.Tq ? -p.Tq : (start < p.Tk ? start : p.Tk);  // (beyond: nothing is seen, everything is; sums with positions stay in 32 bits)
+  if (p.causal && s.start + p.Tq < s.len) s.len = s.start + p.Tq;    // (what lies behind the last query's keys may be stale: slots of a cache)
   return s;
 }
 // bit i: key j0 + i exists and is not left out

@@ -1667,8 +1667,9 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
     h // (H // Hkv)); any strides with a contiguous last dimension (slices of a fused projection, [B, H, T, ...] caches seen through permute).
     lam: fp32 [H] or [1].  norm_weight: [dv], fp32 or bf16, or None.  scale > 0, default d ** -0.5.
   Which keys a query sees: kv_len (int32 [B] on the device) leaves out keys >= kv_len[b]; key_mask (bool or uint8 [B, Tk]) those where it is 0; causal
-  those with key > q_start + query, q_start an int, int32 [B] on the device, or None for Tk - Tq.  k and v of keys left out by kv_len or key_mask may
-  hold anything; the other values have to be finite, the scaled scores below 1e30.  A query that sees no key gives zeros.
+  those with key > q_start + query, q_start an int, int32 [B] on the device, or None for Tk - Tq.  k and v of keys that no query of the sequence sees
+  (left out by kv_len or key_mask, or behind the last query's in a causal call: slots of a cache that are not filled yet) may hold anything; the other values have
+  to be finite, the scaled scores below 1e30.  A query that sees no key gives zeros.
   New tokens against a cache: q [B, 1, ...], k and v the whole cache, kv_len the tokens it holds (the new ones among them); for several new tokens
   causal=True and q_start = kv_len - Tq.
   save=True keeps what diff_attn_bwd needs.  ``out``: written in place of a new tensor, any strides that do not overlap, no memory shared
