@@ -1511,11 +1511,22 @@ bool valid(const tfpp_diff_attn_params& p, int dtype) {
          p.d >= 1 && p.d <= 128 && p.dv >= 1 && p.dv <= 256 && (p.n_lam == 1 || p.n_lam == p.H) && p.scale > 0.f && std::isfinite(p.scale) && (!p.norm || p.eps > 0.f) &&
          p.Tq < (1 << 29) && p.Tk < (1 << 29) && (long)p.B * p.H < (1l << 24);
 }
-// Can q, k, v be read 16 bytes at a time?
+// Can q, k, v be read 16 bytes at a time?  A token's stride has to hold its channels: rows that share memory (one token expanded over all, windows) would put
+// what `fill` takes for zeros, the rows behind the last one, inside its buffer.
 bool vector_rows(const tfpp_diff_attn_params& p, int vec) {
+  if (p.q_s[1] < p.d || p.k_s[1] < p.d || p.v_s[1] < p.dv) return false;
   const int64_t far = (1 << 24) * (int64_t)vec / 16;  // 16 MB from token to token: a tile's offsets fit 32 bits
   return p.d % vec == 0 && p.dv % vec == 0 && p.q_s[1] <= far && p.k_s[1] <= far && p.v_s[1] <= far && !(((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15) && strides_vec(p.q_s, 4, vec) && strides_vec(p.k_s, 4, vec) &&
          strides_vec(p.v_s, 3, vec);
+}
+// the stride of a single token can be anything: one that holds its channels and is a multiple of 16 bytes
+tfpp_diff_attn_params one_token(tfpp_diff_attn_params p) {
+  if (p.Tq == 1) p.q_s[1] = (p.d + 7) & ~7;
+  if (p.Tk == 1) {
+    p.k_s[1] = (p.d + 7) & ~7;
+    p.v_s[1] = (p.dv + 7) & ~7;
+  }
+  return p;
 }
 // Can an output be written 16 bytes at a time?
 bool out_vector(const void* ptr, const int64_t* s, int n, int vec) { return !((uintptr_t)ptr & 15) && strides_vec(s, n, vec); }
@@ -1624,7 +1635,7 @@ int64_t row_floats(const tfpp_diff_attn_params& p) { return ((int64_t)row_blocks
 
 extern "C" int tfpp_diff_attn_fwd(const tfpp_diff_attn_params* pp, int dtype, void* stream) {
   if (!pp || !valid(*pp, dtype) || !pp->out || (pp->o1 != nullptr) != (pp->o2 != nullptr)) return TFPP_EINVAL;
-  tfpp_diff_attn_params p = *pp;
+  tfpp_diff_attn_params p = one_token(*pp);
   p.out_vec = out_vector(p.out, p.o_s, 3, dtype == TFPP_F32 ? 4 : 8);
   p.splits = few_splits(p);
   if (p.splits > 1 && !p.partial) return TFPP_EINVAL;
@@ -1648,7 +1659,7 @@ extern "C" int tfpp_diff_attn_bwd_partial_floats(const tfpp_diff_attn_params* p,
 
 extern "C" int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* pp, int dtype, void* stream) {
   if (!pp || !valid(*pp, dtype)) return TFPP_EINVAL;
-  tfpp_diff_attn_params p = *pp;
+  tfpp_diff_attn_params p = one_token(*pp);
   if (!p.dout || !p.o1 || !p.o2 || !p.lse || !p.d_o || (dtype == TFPP_BF16 && !p.slope) || !p.delta || !p.partial || !p.dlam || !p.dq_out || !p.dk_out || !p.dv_out || (p.norm_w && !p.dnorm_w)) return TFPP_EINVAL;
   if (p.H > 65535 || (((uintptr_t)p.o1 | (uintptr_t)p.o2 | (uintptr_t)p.d_o | (dtype == TFPP_BF16 ? (uintptr_t)p.slope : 0)) & 15)) return TFPP_EINVAL;
   const int vec = dtype == TFPP_F32 ? 4 : 8;

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_transformer_ops_gpu import BF16, DEV, F32, attn_compare, attn_inputs, ops, randn  # noqa: F401  (ops: the fixture)
+from test_transformer_ops_gpu import BF16, DEV, F32, attn_compare, attn_inputs, attn_oracle, attn_visible, ops, randn, within  # noqa: F401  (ops: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,35 @@ def test_causal_calls_do_not_see_what_lies_behind_their_last_query(ops, Tq, d, d
       grads = ops.diff_attn_bwd(dout, q, k0, v0, lam, ctx)
       assert all(x is None or torch.equal(x, y) for x, y in zip(grads, wgrads))
       assert not grads[1][gone].any() and not grads[2][gone].any()
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('what', ['q', 'k', 'v', 'all', 'windows'])
+@pytest.mark.parametrize('d', [32, 64, 72])
+def test_tokens_that_share_memory(ops, what, d, dtype):
+  """One query, key or value expanded over all tokens, or windows of a longer row.  The scores are large, so that a row that does not exist would not go
+  unnoticed."""
+  B, Tq, Tk, H, Hkv = 2, 41, 75, 2, 1
+  q, k, v, dout, lam = attn_inputs(B, Tq, Tk, H, Hkv, d, 2 * d, dtype, seed=510)
+  q, k = q * 6, k * 6
+  if what == 'windows':  # token t has the channels 8 t ..
+    base = randn(4 * 2 * d * (Tk + 8), dtype=dtype, seed=511)
+    q = (base * 6).as_strided(q.shape, (Tq * 8 + 4 * d, 8, 2 * d, d, 1))
+    v = base.as_strided(v.shape, (Tk * 8 + 4 * d, 8, 2 * d, 1), 16)
+  else:
+    q, k, v = (t[:, :1].expand_as(t) if what in (n, 'all') else t for n, t in (('q', q), ('k', k), ('v', v)))
+  for opt in (dict(), dict(causal=True), dict(kv_len=torch.tensor([75, 33], dtype=torch.int32, device=DEV))):
+    out, ctx = ops.diff_attn_fwd(q, k, v, lam, norm_eps=1e-5, save=True, **opt)
+    grads = ops.diff_attn_bwd(dout, q, k, v, lam, ctx)
+    assert torch.isfinite(out).all() and all(torch.isfinite(g).all() for g in grads if g is not None)
+    want = attn_oracle(q, k, v, lam, attn_visible(B, Tq, Tk, **opt), dout=dout)
+    # a probability below 2^-126 is zero in 32 bits: 1.2e-38 times |dP - delta| <= 1e4, |K| or |Q| <= 1e2 and 75 tokens, 1e-30 at most, whatever the value
+    for n, g in zip(('out', 'dq', 'dk', 'dv', 'dlam'), (out, *grads)):
+      within(n, g, want[n][0], want[n][1] + 1e-30)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_single_tokens_with_any_stride(ops, dtype):
+  q, k, v, dout, lam = attn_inputs(2, 1, 1, 2, 1, 32, 64, dtype, seed=520)
+  odd = lambda t: torch.cat([t.flatten(), t.new_zeros(64)]).as_strided(t.shape, (t.stride(0), 3, *t.stride()[2:]))
+  attn_compare(ops, odd(q), odd(k), odd(v), dout, lam)
