@@ -433,7 +433,7 @@ template <typename T> void dispatch(const tfpp_block_norm_params& p, bool bwd, i
 }  // namespace
 
 extern "C" int tfpp_block_norm_fwd(const tfpp_block_norm_params* p, int dtype, void* stream) {
-  if (!p || !valid(*p, dtype) || !p->y || (p->pre && !p->h)) return TFPP_EINVAL;
+  if (!p || !valid(*p, dtype) || !p->y || (p->pre && !p->h) || ((uintptr_t)p->stat & 15)) return TFPP_EINVAL;
   if (dtype == TFPP_F32) dispatch<float>(*p, false, 0, (hipStream_t)stream);
   else dispatch<bf16_t>(*p, false, 0, (hipStream_t)stream);
   TFPP_CHECK_LAUNCH();

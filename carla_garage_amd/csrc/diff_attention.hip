@@ -1635,6 +1635,7 @@ int64_t row_floats(const tfpp_diff_attn_params& p) { return ((int64_t)row_blocks
 
 extern "C" int tfpp_diff_attn_fwd(const tfpp_diff_attn_params* pp, int dtype, void* stream) {
   if (!pp || !valid(*pp, dtype) || !pp->out || (pp->o1 != nullptr) != (pp->o2 != nullptr)) return TFPP_EINVAL;
+  if (((uintptr_t)pp->o1 | (uintptr_t)pp->o2 | (uintptr_t)pp->partial) & 15) return TFPP_EINVAL;  // (stored 16 bytes at a time)
   tfpp_diff_attn_params p = one_token(*pp);
   p.out_vec = out_vector(p.out, p.o_s, 3, dtype == TFPP_F32 ? 4 : 8);
   p.splits = few_splits(p);
@@ -1661,7 +1662,7 @@ extern "C" int tfpp_diff_attn_bwd(const tfpp_diff_attn_params* pp, int dtype, vo
   if (!pp || !valid(*pp, dtype)) return TFPP_EINVAL;
   tfpp_diff_attn_params p = one_token(*pp);
   if (!p.dout || !p.o1 || !p.o2 || !p.lse || !p.d_o || (dtype == TFPP_BF16 && !p.slope) || !p.delta || !p.partial || !p.dlam || !p.dq_out || !p.dk_out || !p.dv_out || (p.norm_w && !p.dnorm_w)) return TFPP_EINVAL;
-  if (p.H > 65535 || (((uintptr_t)p.o1 | (uintptr_t)p.o2 | (uintptr_t)p.d_o | (dtype == TFPP_BF16 ? (uintptr_t)p.slope : 0)) & 15)) return TFPP_EINVAL;
+  if (p.H > 65535 || (((uintptr_t)p.o1 | (uintptr_t)p.o2 | (uintptr_t)p.d_o | (dtype == TFPP_BF16 ? (uintptr_t)p.slope : 0) | (uintptr_t)p.partial) & 15)) return TFPP_EINVAL;
   const int vec = dtype == TFPP_F32 ? 4 : 8;
   p.dq_vec = out_vector(p.dq_out, p.dq_s, 4, vec);
   p.dk_vec = out_vector(p.dk_out, p.dk_s, 4, vec);

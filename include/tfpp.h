@@ -705,11 +705,13 @@ int tfpp_block_norm_bwd_partial_floats(const tfpp_block_norm_params* p, int64_t*
  * (norm = 0: out = out_scale * O).  Element (b, t, h, i, c) of q lies at b q_s[0] + t q_s[1] + h q_s[2] + i q_s[3] + c, and so on: strides in
  * elements, the last dimension contiguous.  H is a multiple of Hkv: query head h reads key / value head h / (H / Hkv).  d <= 128, dv <= 256.
  * lam: n_lam = H (or 1) fp32 values.  kv_len (nullable): valid keys of each sequence; key_mask (nullable, [B] rows of pitch ld_mask): 0 leaves a key
- * out; causal: key j is seen by query i when j <= q_start[b] + i (q_start null: q_start_all).  K and V of keys that
- * no query of the sequence sees (left out by kv_len or key_mask, or behind the last query's in a causal call) may hold anything.  A query without keys: out = 0.  Forward: partial is scratch of tfpp_diff_attn_fwd_partial_floats (null where that is 0).
+ * out; causal: key j is seen by query i when j <= q_start[b] + i (q_start null: q_start_all).  K and V of keys that no query of the sequence sees
+ * (left out by kv_len or key_mask, or behind the last query's in a causal call) may hold anything.  A query without keys: out = 0.  Forward: partial is
+ * 16-byte aligned scratch of tfpp_diff_attn_fwd_partial_floats (null where that is 0).
  * Forward for training also writes o1, o2 ([B, H, Tq, dv rounded up to 8]: O and P_2 V in `dtype`, 16-byte aligned) and lse ([2, B, H, Tq], log2).
- * Backward reads them, dout and the inputs, and writes d_o, slope (bf16 only; both in the layout of o1), delta (layout of lse), partial
- * (tfpp_diff_attn_bwd_partial_floats): scratch; dlam [n_lam], dnorm_w (type of norm_w), and the gradients dq_out, dk_out, dv_out with their own strides.  Fixed summation order throughout. */
+ * Backward reads them, dout and the inputs, and writes d_o, slope (bf16 only; both in the layout of o1), delta (layout of lse) and partial
+ * (tfpp_diff_attn_bwd_partial_floats), all scratch, 16-byte aligned but delta; dlam [n_lam], dnorm_w (type of norm_w), and the gradients dq_out, dk_out,
+ * dv_out with their own strides.  Fixed summation order throughout. */
 typedef struct {
   const void *q, *k, *v;
   const float* lam;
