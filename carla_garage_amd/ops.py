@@ -1673,7 +1673,7 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
   New tokens against a cache: q [B, 1, ...], k and v the whole cache, kv_len the tokens it holds (the new ones among them); for several new tokens
   causal=True and q_start = kv_len - Tq.
   save=True keeps what diff_attn_bwd needs.  ``out``: written in place of a new tensor, any strides that do not overlap, no memory shared
-  with q, k or v (slices of one buffer that do not meet are fine)."""
+  with another argument (slices of one buffer that do not meet are fine)."""
   dev, qs, ks, vs, shape = _diff_attn_check(q, k, v, lam)
   B, Tq, Tk, H, Hkv, d, dv = shape
   if norm_weight is not None and (norm_weight.dtype not in (torch.float32, torch.bfloat16) or norm_weight.numel() != dv or not norm_weight.is_contiguous() or
@@ -1703,7 +1703,7 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
       if tuple(out.shape) != (B, Tq, H, dv) or out.dtype != q.dtype or out.device != dev:
         raise ValueError(f'out: {q.dtype} {(B, Tq, H, dv)} on {dev}, got {out.dtype} {tuple(out.shape)}')
       _disjoint(out, 'out')
-      _apart(out, 'out', (('q', q), ('k', k), ('v', v)))
+      _apart(out, 'out', (('q', q), ('k', k), ('v', v), ('lam', lam), ('norm_weight', norm_weight), ('kv_len', kv_len), ('q_start', start_t), ('key_mask', key_mask)))
     os_ = _last_contiguous(out, 'out', 4)
     ctx = None
     if save:
@@ -1752,7 +1752,8 @@ def diff_attn_bwd(dout, q, k, v, lam, ctx, dq=None, dk=None, dv=None):
         if t.shape != like.shape or t.dtype != q.dtype or t.device != dev:
           raise ValueError(f'{n}: {q.dtype} {tuple(like.shape)} on {dev}, got {t.dtype} {tuple(t.shape)}')
         _disjoint(t, n)
-        _apart(t, n, (('dout', dout), ('q', q), ('k', k), ('v', v), *zip(('dq', 'dk'), outs)))
+        _apart(t, n, (('dout', dout), ('q', q), ('k', k), ('v', v), ('lam', lam), ('norm_weight', ctx.norm_weight), ('kv_len', ctx.kv_len), ('q_start', ctx.q_start),
+                      ('key_mask', ctx.key_mask), *zip(('dq', 'dk'), outs)))
       outs.append(t)
     strides = [_last_contiguous(t, n, dims) for n, t, dims in zip(('dq', 'dk', 'dv'), outs, (5, 5, 4))]
     w = ctx.norm_weight

@@ -64,3 +64,25 @@ def test_single_tokens_with_any_stride(ops, dtype):
   q, k, v, dout, lam = attn_inputs(2, 1, 1, 2, 1, 32, 64, dtype, seed=520)
   odd = lambda t: torch.cat([t.flatten(), t.new_zeros(64)]).as_strided(t.shape, (t.stride(0), 3, *t.stride()[2:]))
   attn_compare(ops, odd(q), odd(k), odd(v), dout, lam)
+
+
+def test_outputs_may_not_lie_in_the_small_arguments(ops):
+  """lambda, the norm's weights, lengths, starts and the mask are read while results are written: an output in their memory is refused."""
+  B, T, H, d = 2, 9, 2, 16
+  q, k, v, dout, _ = attn_inputs(B, T, T, H, H, d, 2 * d, F32, seed=530)
+  arena = torch.zeros(q.numel() + 64, device=DEV)
+  out, dq = arena[:dout.numel()].view(dout.shape), arena[:q.numel()].view(q.shape)
+  ints = arena.view(torch.int32)
+  small = dict(lam=arena[4:4 + H], norm_weight=arena[8:8 + 2 * d], kv_len=ints[2:2 + B], q_start=ints[2:2 + B], key_mask=arena.view(torch.uint8)[:B * T].view(B, T))
+  for n, t in small.items():
+    kw = {'lam': torch.full((H,), 0.5, device=DEV), **{n: t}}
+    lam = kw.pop('lam')
+    with pytest.raises(ValueError, match=n):
+      ops.diff_attn_fwd(q, k, v, lam, causal=True, out=out, **kw)
+    _, ctx = ops.diff_attn_fwd(q, k, v, lam, causal=True, save=True, **kw)
+    for g in (dict(dq=dq), dict(dk=dq), dict(dv=out)):
+      with pytest.raises(ValueError, match=n):
+        ops.diff_attn_bwd(dout, q, k, v, lam, ctx, **g)
+  far = {n: t.clone() for n, t in small.items() if n != 'q_start'}
+  lam = far.pop('lam')
+  ops.diff_attn_fwd(q, k, v, lam, out=arena[64:64 + dout.numel()].view(dout.shape), **far)
