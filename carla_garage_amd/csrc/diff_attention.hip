@@ -1602,8 +1602,13 @@ int padded_blocks(const tfpp_diff_attn_params& p) {  // NB of dispatch(), or mor
 // Which forward kernel, and how many splits of the keys?  0: the one for many queries.
 int few_splits(const tfpp_diff_attn_params& p) {
   const long wg = (long)p.B * p.H * ((p.Tq + QB - 1) / QB);
-  if (wg >= 512 || (p.Tq > 64 && wg > 64)) return 0;  // (12 x 4 heads x 320 queries: 27 us there, 44 us here)
-  const long rows = (long)(p.H / p.Hkv) * p.Tq, base = (long)p.B * p.Hkv * ((rows + 31) / 32);
+  const long group = p.H / p.Hkv, rows = group * p.Tq, base = (long)p.B * p.Hkv * ((rows + 31) / 32);
+  if (p.Tq > 64 && wg > 64) return 0;  // (12 x 4 heads x 320 queries: 27 us there, 44 us here)
+  // Where either kernel fills the chip, this one is for rows that fit one tile: it reads keys and values once for all heads that share them, the other one for
+  // each head, with 128 queries a workgroup however few there are.  One token each, bf16: 64 x 16 heads of 64 / 128 over 4, 320 and 4096 keys, 43 and 429 us there,
+  // 15 and 114 here; 128 x 8 heads of 32 / 64, not shared, 29 and 299, 25 and 231.  More tiles (32 tokens each): 46 there, 53 here.  Up to
+  // 64 keys that are not shared leave waves of this one without any: 13 there, 16 here.
+  if (wg >= 512 && (rows > 32 || (group == 1 && p.Tk <= 64))) return 0;
   long n = (512 + base - 1) / base, most = (p.Tk + 511) / 512;  // two workgroups a CU; at least 512 keys (4 blocks a wave) in a split
   if (n > most) n = most;
   if (n > 64) n = 64;  // (the join holds one split a lane)

@@ -86,3 +86,32 @@ def test_outputs_may_not_lie_in_the_small_arguments(ops):
   far = {n: t.clone() for n, t in small.items() if n != 'q_start'}
   lam = far.pop('lam')
   ops.diff_attn_fwd(q, k, v, lam, out=arena[64:64 + dout.numel()].view(dout.shape), **far)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('heads', [(16, 4, 64, 128), (8, 2, 32, 64), (8, 8, 27, 54), (4, 2, 128, 256)], ids=str)
+@pytest.mark.parametrize('Tq', [1, 2, 5])
+def test_answers_do_not_depend_on_how_many_sequences_there_are(ops, Tq, heads, dtype):
+  """New tokens of 512 and 1024 batch x heads take the kernel that a few sequences take: the same bits (a cache this short is not split)."""
+  H, Hkv, d, dv = heads
+  for total in (512, 1024):
+    B, Tk = total // H, 320
+    q, k, v, dout, lam = attn_inputs(B, Tq, Tk, H, Hkv, d, dv, dtype, seed=540)
+    lens = torch.randint(Tq, Tk + 1, (B,), generator=torch.Generator().manual_seed(total), dtype=torch.int32).to(DEV)
+    opt = dict(causal=True, norm_weight=randn(dv, seed=541, mean=1.0, std=0.1))
+    out, _ = ops.diff_attn_fwd(q, k, v, lam, kv_len=lens, q_start=lens - Tq, **opt)
+    for b in range(0, B, 16):
+      s = slice(b, b + 16)
+      part, _ = ops.diff_attn_fwd(q[s], k[s], v[s], lam, kv_len=lens[s].clone(), q_start=(lens - Tq)[s].clone(), **opt)
+      assert torch.equal(out[s], part)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('Tk', [1, 50, 700])
+@pytest.mark.parametrize('heads', [(8, 2, 64, 128), (8, 8, 16, 32)], ids=str)
+def test_single_tokens_of_many_sequences(ops, heads, Tk, dtype):
+  H, Hkv, d, dv = heads
+  for B in (64, 128):
+    q, k, v, dout, lam = attn_inputs(B, 1, Tk, H, Hkv, d, dv, dtype, seed=550)
+    lens = torch.randint(0, Tk + 1, (B,), generator=torch.Generator().manual_seed(B), dtype=torch.int32).to(DEV)
+    attn_compare(ops, q, k, v, dout, lam, train=B == 64, kv_len=lens)
