@@ -8,6 +8,7 @@ import ctypes
 import os
 import re
 import subprocess
+import threading
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
@@ -224,6 +225,7 @@ class _Lib:
   def __init__(self):
     self._dll = None
     self._fns = {}
+    self._loading = threading.Lock()
     self.profiler = None
 
   def raw(self, name):
@@ -232,8 +234,13 @@ class _Lib:
     return self._fns[name]
 
   def load(self):
-    if self._dll is not None:
-      return self
+    if self._dll is None:
+      with self._loading:  # (threads whose first calls come together: one loads, the others wait)
+        if self._dll is None:
+          self._load()
+    return self
+
+  def _load(self):
     if not os.path.exists(LIB_PATH):
       raise TfppError(f'{LIB_PATH} is missing: run `python -c "import __graft_entry__ as g; g.build()"` '
                       '(there is no PyTorch/CPU fallback for the HIP path)')
@@ -241,14 +248,14 @@ class _Lib:
     # reuses what is already mapped).  Loaded before torch, libtfpp_hip.so pulls in /opt/rocm's copy, the process ends up with two runtimes and
     # every launch of this library fails with hipErrorNoDevice once torch has opened the device (seen with build() and smoke() in one process).
     import torch  # noqa: F401
-    self._dll = ctypes.CDLL(LIB_PATH)
+    dll, fns = ctypes.CDLL(LIB_PATH), {}
     for name, argtypes in declared_functions().items():
-      fn = getattr(self._dll, name)  # AttributeError if the library does not export a declared symbol
+      fn = getattr(dll, name)  # AttributeError if the library does not export a declared symbol
       fn.argtypes = argtypes
       fn.restype = ctypes.c_int
-      self._fns[name] = fn
+      fns[name] = fn
     sizes = (ctypes.c_int * 8)()
-    n = self._dll.tfpp_struct_sizes(sizes, 8)
+    n = dll.tfpp_struct_sizes(sizes, 8)
     mine = [ctypes.sizeof(ConvParams), ctypes.sizeof(WgradParams), ctypes.sizeof(BgemmParams), ctypes.sizeof(PackDesc),
             ctypes.sizeof(AttnParams)]
     mine.append(ctypes.sizeof(BnRows))
@@ -256,14 +263,14 @@ class _Lib:
     mine.append(ctypes.sizeof(DiffAttnParams))
     if n != len(mine) or list(sizes[:n]) != mine:
       raise TfppError(f'struct layout mismatch: library {list(sizes[:n])} vs ctypes {mine}')
-    if self._dll.tfpp_version() != ABI_VERSION:
-      raise TfppError(f'ABI version mismatch: library {self._dll.tfpp_version()}, binding {ABI_VERSION} (include/tfpp.h TFPP_ABI_VERSION: bumped with every signature change)')
+    if dll.tfpp_version() != ABI_VERSION:
+      raise TfppError(f'ABI version mismatch: library {dll.tfpp_version()}, binding {ABI_VERSION} (include/tfpp.h TFPP_ABI_VERSION: bumped with every signature change)')
     got = ctypes.c_uint64(0)
-    self._fns['tfpp_source_hash'](ctypes.byref(got))
+    fns['tfpp_source_hash'](ctypes.byref(got))
     if os.environ.get('TFPP_SKIP_HASH_CHECK', '0') != '1' and int(got.value) != source_hash():
       raise TfppError(f'{LIB_PATH} was built from other sources (hash {int(got.value):016x}, sources {source_hash():016x}): '
                       'rebuild with `python -c "import __graft_entry__ as g; g.build()"`')
-    return self
+    self._fns, self._dll = fns, dll  # (complete and checked: a load that raised has left nothing that a second call would take for a loaded library)
 
   def __getattr__(self, name):
     if name.startswith('_'):
