@@ -1531,14 +1531,16 @@ tfpp_diff_attn_params one_token(tfpp_diff_attn_params p) {
 // Can an output be written 16 bytes at a time?
 bool out_vector(const void* ptr, const int64_t* s, int n, int vec) { return !((uintptr_t)ptr & 15) && strides_vec(s, n, vec); }
 
+// more than 64 KB of LDS: once for each device.  The mark is set behind the call, so that of two threads that come here first both make it.
 template <typename K> int lds_limit(K* kernel, int bytes, unsigned long long* done) {
-  if (bytes > 64 * 1024 && tfpp_first_use_on_this_device(done)) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) {
-      *done = 0;
-      return -(int)e;
-    }
-  }
+  if (bytes <= 64 * 1024) return 0;
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit) return 0;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return -(int)e;
+  __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
   return 0;
 }
 

@@ -115,3 +115,36 @@ def test_single_tokens_of_many_sequences(ops, heads, Tk, dtype):
     q, k, v, dout, lam = attn_inputs(B, 1, Tk, H, Hkv, d, dv, dtype, seed=550)
     lens = torch.randint(0, Tk + 1, (B,), generator=torch.Generator().manual_seed(B), dtype=torch.int32).to(DEV)
     attn_compare(ops, q, k, v, dout, lam, train=B == 64, kv_len=lens)
+
+
+def test_calls_of_several_threads(ops):
+  """Threads with streams of their own, released together: their first calls of the wide kernels and later ones give what one thread gives."""
+  import threading
+  cases = [(2, 90, 150, 2, 1, d, 2 * d) for d in (128, 96, 72, 64)]
+  start, got, errors = threading.Barrier(4), [None] * 4, []
+  data = [attn_inputs(*c, BF16, seed=560) for c in cases]
+  torch.cuda.synchronize()
+
+  def step(i):
+    q, k, v, dout, lam = data[i]
+    out, ctx = ops.diff_attn_fwd(q, k, v, lam, causal=True, save=True)
+    return [out, *ops.diff_attn_bwd(dout, q, k, v, lam, ctx)[:4]]
+
+  def work(i):
+    try:
+      with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        for n in range(8):
+          got[i] = step((i + n) % 4)
+        torch.cuda.current_stream().synchronize()
+    except Exception as e:  # noqa: BLE001
+      errors.append(e)
+
+  threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+  for t in threads:
+    t.start()
+  for t in threads:
+    t.join()
+  assert not errors, errors
+  for i in range(4):
+    assert all(torch.equal(a, b) for a, b in zip(got[i], step((i + 7) % 4)))
