@@ -148,3 +148,16 @@ def test_calls_of_several_threads(ops):
   assert not errors, errors
   for i in range(4):
     assert all(torch.equal(a, b) for a, b in zip(got[i], step((i + 7) % 4)))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('eps', [1e-30, 1e-5, 0.5])
+def test_tiny_and_large_eps_with_queries_that_see_nothing(ops, eps, dtype):
+  """r = 1 / sqrt(mean(O^2) + eps) is 1e15 for a query without keys: its powers leave 32 bits, its gradients are zeros all the same."""
+  q, k, v, dout, lam = attn_inputs(2, 9, 40, 2, 1, 32, 64, dtype, seed=570)
+  lens = torch.tensor([0, 33], dtype=torch.int32, device=DEV)
+  w = randn(64, seed=571, mean=1.0, std=0.1)
+  want = attn_oracle(q, k, v, lam, attn_visible(2, 9, 40, kv_len=lens), dout=dout, w=w, eps=eps)
+  out, ctx = ops.diff_attn_fwd(q, k, v, lam, kv_len=lens, norm_weight=w, norm_eps=eps, save=True)
+  for n, g in zip(('out', 'dq', 'dk', 'dv', 'dlam', 'dw'), (out, *ops.diff_attn_bwd(dout, q, k, v, lam, ctx))):
+    within(n, g, *want[n])
