@@ -17,10 +17,13 @@ from .engine import F32
 
 
 @torch.no_grad()
-def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
   """``torch.nn.utils.clip_grad_norm_`` (team_code/train.py:904-906) over the fused kernels: two launches for any number of gradients (ops.GradClip).
-  norm_type 1, 2 or inf.  Returns the norm before clipping (fp32 device scalar); the gradients are scaled in place.  As torch's, it reads the
-  norm on the host before it scales when ``error_if_nonfinite`` is set, and the gradients are then left as they were."""
+  Returns the norm before clipping (fp32 device scalar); the gradients are scaled in place.  As torch's, it reads the norm on the host before it
+  scales when ``error_if_nonfinite`` is set, and the gradients are then left as they were.  norm_type 1, 2 or inf, gradients fp32 or bf16, dense, on one
+  device, none of them twice: ValueError / TypeError otherwise.  ``foreach`` is taken for the signature's sake, there is one way of doing it.
+  Every call looks the gradients up and copies a table of their addresses to the device (1.0 ms for 1332 of them, 0.06 ms for 24), which a capture does not
+  allow: for gradients that stay where they are, keep an ops.GradClip."""
   grads = [p.grad for p in ([parameters] if isinstance(parameters, torch.Tensor) else parameters) if p.grad is not None]
   if not grads:
     return torch.tensor(0.0)
