@@ -11,8 +11,8 @@
 // Layout: a row belongs to TPR threads (64 .. 512, at most 8 elements each: 16 would not fit the registers beside their column sums, hence C <= 4096);
 // row sums are DPP moves plus one LDS exchange when TPR > 64.  Column sums (the parameter gradients) stay in registers over all rows of the
 // workgroup, one row of partials per workgroup, added in a fixed order by block_norm_colsum_kernel: bit-reproducible.
-// Measured, 16384 rows of 2048 in bf16 with a gate for each token: forward 72 us (336 MB, 4.7 TB/s; a large copy reaches 5.1), backward 141 us (537 MB,
-// 3.8 TB/s: 12 waves a CU is what the column sums leave) and 6 us for their sum; 3840 rows of 576, a gate for each sample: 12 + 25 + 6 us, latency.
+// Measured, 16384 rows of 2048 in bf16 with a gate for each token: forward 67 us (336 MB, 5.0 TB/s; a large copy reaches 5.1), backward 134 us (537 MB,
+// 4.0 TB/s: 12 waves a CU is what the column sums leave) and 6 us for their sum; 3840 rows of 576, a gate for each sample: 12 + 25 + 6 us, latency.
 #include "common.h"
 #include "../../include/tfpp.h"
 

@@ -274,11 +274,11 @@ template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32
 // ---------------------------------------------------------------------------------------------------------------------------------
 // forward.  A wave has 32 queries, lane l and l + 32 = one query.  S_i^T = K_i Q_i^T (keys x queries), running maximum and sum per query,
 // O_i^T += V^T P_i^T: both maps share every V operand.  O_1 and O_2 are kept apart to the end because their sums are not known before; one pass,
-// 4 d + 4 dv flop a pair.  Long sequences are bounded by the matrix unit and what stands between its products (the exponentials, the LDS reads of
-// operands), short ones by the latency of that chain in a single wave.  8100 causal tokens, 8 heads of 128 / 256: 410 us, 655 TFLOP/s (a product of
-// 8192^3 by the library: 1189); 2 x 4096 causal, 16 heads of 64 / 128: 255 us; 12 x 320, 4 heads of 72 / 144: 25 us, 10 of them launch, first loads
-// and epilogue.  Wide heads (split): O_1 and O_2 of 32 queries do not fit one wave's registers, so two waves share the queries, one map
-// each, and meet in LDS at the end.
+// 4 d + 4 dv flop a pair.  Long sequences are bounded by a wave's own chain of scores, exponentials and value products, of which two waves a SIMD overlap
+// a part: 8100 causal tokens, 8 heads of 128 / 256: 437 us (0.92 PFLOP/s of these products; one of 8192^3 by the library: 1.19), the matrix unit busy in
+// 47 % of the cycles, vector issue in 42 %, LDS in 24 %.  (Clocks that have settled; the first dozen calls after a pause take up to 570 us.)  2 x 4096 causal,
+// 16 heads of 64 / 128: 243 us; 12 x 320, 4 heads of 72 / 144: 24 us, 10 of them launch, first loads and epilogue.  Wide heads (split):
+// O_1 and O_2 of 32 queries do not fit one wave's registers, so two waves share the queries, one map each, and meet in LDS at the end.
 template <typename T, int NB> constexpr bool fwd_split() { return NB >= (sizeof(T) == 2 ? 5 : 4); }
 
 enum { Q_HELD, Q_GLOBAL, Q_LDS };  // where a wave's queries are: registers, or read again for every tile
@@ -833,7 +833,7 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_fwd_join_
 //    saved O and O_2 (whose rounding, 2^-8 relative at most, stays in delta_i), and partial sums of dw, dlambda from the unrounded dO.
 //    The forward pass saves O, not O_1: r, dO and dw are made of it, and a difference of two saved maps would hold their roundings, |O_1| / |O| times as
 //    large (64 / 128, V of mean 1, lambda 0.95: dw 1.8e-2 off, 3.4e-3 with O saved).  For bf16 also g, see dQ.
-//    Bounded by HBM: 131072 rows of 128, 168 MB in 45 us (3.8 TB/s).
+//    Bounded by HBM: 131072 rows of 128, 168 MB in 44 us (3.8 TB/s).
 // grid (blocks, H); lpr lanes a row (a power of two), 8 channels a lane: 16-byte loads, 64 / lpr rows a wave at a time.  partial: [1 + dv][blocks x H], the
 // sums of one value side by side.
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) { return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
@@ -978,15 +978,15 @@ template <typename T> __global__ __launch_bounds__(256) void diff_attn_bwd_sum_k
 }
 
 // 2. dQ.  Workgroup = (batch, head, 128 queries), wave = 32 queries, as the forward pass: S_i^T = K_i Q_i^T, dP^T = V dO^T (keys x queries),
-//    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.  2 x 4096 causal, 16 heads of 64 / 128: 354 us; 12 x 320, 4 heads
-//    of 72 / 144: 30 us.
+//    dQ_i^T += K_i^T dS_i^T.  The row's sum, delta_i and limits are one value a lane.  2 x 4096 causal, 16 heads of 64 / 128: 331 us, vector
+//    issue in 65 % of the cycles, the matrix unit in 38 %, LDS in 17 %; 12 x 320, 4 heads of 72 / 144: 28 us.
 //    bf16: dlambda = - sum f, f = dO(O) . O_2, is a sum that cancels, and the row pass has it from the saved O and O_2, which are rounded and made of
 //    rounded probabilities: percents of it where the heads are few.  Here P is at hand in 32 bits, and both are put right to first order:
 //      O_2 beside dO:  sum_j P_2 (dP - delta_2) = dO . (O_2 - saved O_2)
 //      O inside dO:    sum_j (P_1 - lambda P_2) g . V_j - g . saved O = g . (O - saved O),  g = df/dO = - r^2 / dv ((u . O_2 - 3 a b) O^ + b u + dv a O_2)
 //                      with O^ = r O, a = mean(u O^), b = O^ . O_2  (the row pass subtracts g . saved O)
 //    The product with g shares the V operand of dP: 2 dv of 8 d + 4 dv flop a pair.  What is left is of second order, 1e-5 of the terms' root
-//    (before: 2e-3 to 3e-2).  2 x 4096 causal: 273 -> 354 us; 12 x 320: 25 -> 30 us.
+//    (before: 2e-3 to 3e-2).  2 x 4096 causal: 273 -> 331 us; 12 x 320: 23 -> 28 us.
 //    Wide heads: a workgroup has one map (the grid's y), dP is computed by both, and two waves fit a SIMD in place of one
 //    (12 x 320 queries over 1280 keys, without g: 68 us, 82 us with both maps in a wave).  bf16 heads of 81 .. 128 hold q, dO, g and dQ in the registers of
 //    one wave a SIMD (8 heads of 128 / 256 over 2 x 2048: backward 456 us; with both maps in a wave 481).
@@ -1164,8 +1164,9 @@ template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (dq
 // 3. dK, dV.  Workgroup = (batch, key / value head, 128 keys), wave = 32 keys, lane l and l + 32 = one key: S_i = Q_i K_i^T and dP = dO V^T
 //    (queries x keys), dV^T += dO^T (P_1 - lambda P_2), dK_i^T += Q_i^T dS_i, over all queries of all heads that share the key / value head.
 //    Wide heads: the accumulators of all three do not fit one wave's registers, so dK_1, dK_2 (PART_DK, the map in the grid's y) and dV (PART_DV) are
-//    separate workgroups of one launch; S and dP are computed again (3 / 2 of the flop).  Bounded by the matrix unit and the registers: 2 x 4096 causal, 4
-//    heads of 64 / 128 shared by 16: 460 us and 23 us for the join; 12 x 320, 4 heads of 72 / 144: 26 us (39 us as two launches).
+//    separate workgroups of one launch; S and dP are computed again (3 / 2 of the flop).  2 x 4096 causal, 4
+//    heads of 64 / 128 shared by 16: 433 us and 24 us for the join, the matrix unit busy in 35 % of the cycles, LDS in 33 %, vector issue in 44 %, and its
+//    two waves a SIMD wait in 44 % of theirs: the registers leave no third one.  12 x 320, 4 heads of 72 / 144: 24 us (as two launches 39).
 enum { PART_ALL, PART_DK, PART_DV };
 template <typename T, int NB, bool VECTOR> constexpr bool dkv_split() { return NB >= (sizeof(T) == 2 && VECTOR ? 5 : 4); }
 // d = 33 .. 64, bf16: the 128 keys' V and the last 16 channels of their K stay in LDS instead of 40 registers, which lets two waves share a SIMD (256

@@ -161,3 +161,24 @@ def test_tiny_and_large_eps_with_queries_that_see_nothing(ops, eps, dtype):
   out, ctx = ops.diff_attn_fwd(q, k, v, lam, kv_len=lens, norm_weight=w, norm_eps=eps, save=True)
   for n, g in zip(('out', 'dq', 'dk', 'dv', 'dlam', 'dw'), (out, *ops.diff_attn_bwd(dout, q, k, v, lam, ctx))):
     within(n, g, *want[n])
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('d,pd', [(27, 32), (9, 16)])
+def test_heads_padded_with_zeros(ops, d, pd, dtype):
+  """Channels of zeros up to a multiple of 16 bytes, the scale of the narrow heads, weights and eps for the wider mean: the narrow heads' numbers."""
+  B, Tq, Tk, H, Hkv, dv = 2, 45, 83, 2, 1, 2 * d
+  pv = (dv + 7) // 8 * 8
+  q, k, v, dout, lam = attn_inputs(B, Tq, Tk, H, Hkv, d, dv, dtype, seed=580)
+  w = randn(dv, seed=581, mean=1.0, std=0.1)
+  wide = lambda t, n: torch.nn.functional.pad(t, (0, n - t.shape[-1]))
+  want = attn_oracle(q, k, v, lam, attn_visible(B, Tq, Tk, causal=True), dout=dout, w=w, eps=1e-5)
+  out, ctx = ops.diff_attn_fwd(wide(q, pd), wide(k, pd), wide(v, pv), lam, causal=True, scale=d ** -0.5, norm_weight=wide(w, pv) * math.sqrt(dv / pv), norm_eps=1e-5 * dv / pv, save=True)
+  dq, dk, dvv, dlam, dw = ops.diff_attn_bwd(wide(dout, pv), wide(q, pd), wide(k, pd), wide(v, pv), lam, ctx)
+  for n, g, m in (('out', out, dv), ('dq', dq, d), ('dk', dk, d), ('dv', dvv, dv)):
+    value, err = want[n]
+    # (the weights' square root and product round three times in 32 bits: 2^-22 of a value)
+    within(n, g[..., :m], value, err + 2.0 ** -22 * value.abs())
+    assert n == 'dq' or n == 'dk' or not g[..., m:].any()
+  within('dlam', dlam, want['dlam'][0], want['dlam'][1] * (1 + 2.0 ** -22))
+  within('dw', dw[:dv] * math.sqrt(dv / pv), want['dw'][0], want['dw'][1] + 2.0 ** -22 * want['dw'][0].abs())
