@@ -994,8 +994,8 @@ template <typename T, int NB> constexpr int dq_maps() { return NB >= (sizeof(T) 
 template <typename T, int NB, bool VECTOR> constexpr int dq_waves() { return sizeof(T) == 2 && NB == 8 && VECTOR ? 1 : 2; }  // of a SIMD
 // bf16 heads of 33 .. 64: the last fragments of a wave's g stay in LDS, which spares the registers that would go to scratch
 template <typename T, int NB, bool VECTOR> constexpr int dq_stash() { return sizeof(T) == 2 && NB == 4 && VECTOR ? 4 : 0; }
-template <typename T, int NB, bool VECTOR> constexpr int dq_images() { return 2 * 32 * (dq_maps<T, NB>() * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES); }
-template <typename T, int NB, bool VECTOR> constexpr int dq_lds() { return at_least(dq_images<T, NB, VECTOR>() + dq_stash<T, NB, VECTOR>() * 256 * 16, 4 * STRIP_BYTES); }
+template <typename T, int NB> constexpr int dq_images() { return 2 * 32 * (dq_maps<T, NB>() * Img<T, (NB + 1) / 2>::ROW_BYTES + Img<T, NB>::ROW_BYTES); }
+template <typename T, int NB, bool VECTOR> constexpr int dq_lds() { return at_least(dq_images<T, NB>() + dq_stash<T, NB, VECTOR>() * 256 * 16, 4 * STRIP_BYTES); }
 
 template <typename T, int NB, bool VECTOR> __global__ __launch_bounds__(256, (dq_waves<T, NB, VECTOR>())) void diff_attn_bwd_dq_kernel(tfpp_diff_attn_params p) {
   constexpr int KT = 32, NT = 256, CD = (NB + 1) / 2, MAPS = dq_maps<T, NB>();
