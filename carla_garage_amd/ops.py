@@ -1676,7 +1676,6 @@ def diff_attn_fwd(q, k, v, lam, *, scale=None, causal=False, q_start=None, kv_le
   with another argument (slices of one buffer that do not meet are fine)."""
   dev, qs, ks, vs, shape = _diff_attn_check(q, k, v, lam)
   B, Tq, Tk, H, Hkv, d, dv = shape
-  causal, norm = bool(causal), bool(norm)
   if norm_weight is not None and (norm_weight.dtype not in (torch.float32, torch.bfloat16) or norm_weight.numel() != dv or not norm_weight.is_contiguous() or
                                   norm_weight.device != dev or not norm):
     raise ValueError(f'norm_weight: {dv} contiguous fp32 or bf16 values on {dev}, with norm=True')

@@ -182,11 +182,3 @@ def test_heads_padded_with_zeros(ops, d, pd, dtype):
     assert n == 'dq' or n == 'dk' or not g[..., m:].any()
   within('dlam', dlam, want['dlam'][0], want['dlam'][1] * (1 + 2.0 ** -22))
   within('dw', dw[:dv] * math.sqrt(dv / pv), want['dw'][0], want['dw'][1] + 2.0 ** -22 * want['dw'][0].abs())
-
-
-def test_truth_values_of_any_kind(ops):
-  import numpy as np
-  q, k, v, dout, lam = attn_inputs(1, 9, 9, 2, 1, 32, 64, BF16, seed=590)
-  want = ops.diff_attn_fwd(q, k, v, lam, causal=True, norm=False)[0]
-  for yes, no in ((np.True_, np.False_), (1, 0), (torch.tensor(True), torch.tensor(False))):
-    assert torch.equal(ops.diff_attn_fwd(q, k, v, lam, causal=yes, norm=no)[0], want)
